@@ -321,6 +321,65 @@ int tkv_dequantize(const uint8_t *packed, const uint16_t *scale, const uint16_t 
                    int64_t rows, int32_t D, int32_t nbits, int32_t group_size, int32_t out_type,
                    void *out, tkv_stream_t stream);
 
+/* Attention of one new token over 16-bit page pools (fp16, or bf16 with
+ * is_bf16), out and lse fp32.  All strides are in elements, rows of D elements
+ * are dense, and every pointer and stride is a multiple of 16 bytes:
+ *   q          (B, HQ, D), strides batch, head
+ *   k, v       pools (num_pages, HKV, page_size, D), strides page, head, token:
+ *              token t of row b, KV head h is token t % page_size of page
+ *              block_table[b * block_table_stride + t / page_size] (entries
+ *              outside [0, num_pages) are clamped into the pool).  page_size is
+ *              a multiple of 16; D is 64, 128 or 256
+ *   seq_lens   row b attends to its first seq_lens[b] tokens, clamped to
+ *              [0, max_pages * page_size] (NULL: all of them).  A row of no
+ *              tokens gets out = 0 and lse = -inf
+ *   out        (B, HQ, D);  lse (B, HQ) or NULL: the natural logarithm of the
+ *              row's sum of exp(score)
+ *   k_new/v_new  NULL, or (B, HKV, D) in the pools' type, strides batch, head:
+ *              the token at L_b - 1 of every row, attended to and put into its
+ *              page by this call (not stored where the table entry lies outside
+ *              [0, num_pages); rows of no tokens take none)
+ * The rows' tokens are cut on the device, from their lengths: a piece holds at
+ * most max(least_chunks, ceil(sum_b ceil(L_b / 32) / target_pieces)) chunks of
+ * 32 tokens.  target_pieces == 0 keeps every row whole in one launch; otherwise
+ * a second launch joins the pieces, partials holds max_pieces * HQ * (D + 2)
+ * floats (16-byte aligned), row_pieces 2 * B int32 (8-byte aligned), and
+ * max_pieces is at least target_pieces + B (at most 65535).  waves: 4 or 8 per
+ * workgroup (0: 4).  No counterpart in the reference (its caches are contiguous). */
+typedef struct tkv_paged16_args {
+  const void *q;
+  int64_t q_strides[2];
+  void *k, *v;
+  int64_t k_strides[3], v_strides[3];
+  const int32_t *block_table, *seq_lens;
+  float *out, *lse, *partials;
+  int32_t *row_pieces;
+  const void *k_new, *v_new;
+  int64_t k_new_strides[2], v_new_strides[2];
+  int32_t is_bf16, B, HQ, HKV, D;
+  int32_t block_table_stride, max_pages, page_size, num_pages;
+  float sm_scale;
+  int32_t least_chunks, target_pieces, max_pieces, waves;
+} tkv_paged16_args;
+int tkv_paged16_decode_attention(const tkv_paged16_args *args, tkv_stream_t stream);
+
+/* K and V of N tokens per row into such pools, one launch: token n of row b, for
+ * n < counts[b] (NULL: N), goes to position positions[b] + n.  k_new, v_new
+ * (B, HKV, N, D), strides batch, head, token, in the pools' type or fp32
+ * (new_is_fp32), rounded to nearest even; bases and strides are multiples of 16
+ * bytes.  Positions outside [0, max_pages * page_size) and table entries
+ * outside [0, num_pages) are not written.  Any page_size; D a multiple of 8. */
+typedef struct tkv_paged16_append_args {
+  const void *k_new, *v_new;
+  int64_t k_new_strides[3], v_new_strides[3];
+  void *k, *v;
+  int64_t k_strides[3], v_strides[3];
+  const int32_t *block_table, *positions, *counts;
+  int32_t new_is_fp32, is_bf16, B, HKV, N, D;
+  int32_t block_table_stride, max_pages, page_size, num_pages;
+} tkv_paged16_append_args;
+int tkv_paged16_append(const tkv_paged16_append_args *args, tkv_stream_t stream);
+
 typedef struct tkv_device_info_t {
   int32_t device;
   int32_t compute_units;

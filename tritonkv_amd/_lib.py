@@ -72,6 +72,71 @@ class DecodeArgs(ctypes.Structure):
     ]
 
 
+class Paged16Args(ctypes.Structure):
+    """Mirror of ``tkv_paged16_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_strides", ctypes.c_int64 * 2),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("block_table", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("partials", ctypes.c_void_p),
+        ("row_pieces", ctypes.c_void_p),
+        ("k_new", ctypes.c_void_p),
+        ("v_new", ctypes.c_void_p),
+        ("k_new_strides", ctypes.c_int64 * 2),
+        ("v_new_strides", ctypes.c_int64 * 2),
+        ("is_bf16", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("HQ", ctypes.c_int32),
+        ("HKV", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("block_table_stride", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("sm_scale", ctypes.c_float),
+        ("least_chunks", ctypes.c_int32),
+        ("target_pieces", ctypes.c_int32),
+        ("max_pieces", ctypes.c_int32),
+        ("waves", ctypes.c_int32),
+    ]
+
+
+class Paged16AppendArgs(ctypes.Structure):
+    """Mirror of ``tkv_paged16_append_args``."""
+
+    _fields_ = [
+        ("k_new", ctypes.c_void_p),
+        ("v_new", ctypes.c_void_p),
+        ("k_new_strides", ctypes.c_int64 * 3),
+        ("v_new_strides", ctypes.c_int64 * 3),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("block_table", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("new_is_fp32", ctypes.c_int32),
+        ("is_bf16", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("HKV", ctypes.c_int32),
+        ("N", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("block_table_stride", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+    ]
+
+
 class DeviceInfo(ctypes.Structure):
     """Mirror of ``tkv_device_info_t``."""
 
@@ -114,6 +179,8 @@ SIGNATURES = {
     "tkv_pack_codes": ([_P, _I64, _I32, _I32, _P, _P], ctypes.c_int),
     "tkv_unpack_dequant": ([_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P], ctypes.c_int),
     "tkv_dequantize": ([_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P], ctypes.c_int),
+    "tkv_paged16_decode_attention": ([ctypes.POINTER(Paged16Args), _P], ctypes.c_int),
+    "tkv_paged16_append": ([ctypes.POINTER(Paged16AppendArgs), _P], ctypes.c_int),
     "tkv_device_info": ([ctypes.POINTER(DeviceInfo)], ctypes.c_int),
     "tkv_status_string": ([ctypes.c_int], ctypes.c_char_p),
     "tkv_abi_version": ([], ctypes.c_int),

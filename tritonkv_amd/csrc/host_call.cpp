@@ -28,7 +28,7 @@
 
 namespace {
 
-typedef int (*DecodeFn)(const tkv_decode_args*, tkv_stream_t);
+typedef int (*EntryFn)(const void*, tkv_stream_t);  // any entry that takes an argument block and a stream
 typedef int (*ChannelFn)(const tkv_decode_args*, const void*, const void*, const int32_t*, int32_t,
                          tkv_stream_t);
 
@@ -44,10 +44,14 @@ struct Slot {
   c10::ScalarType dtype;
   c10::Device device{c10::kCPU};
   std::vector<int64_t> sizes;
+  std::vector<int64_t> strides;  // of a tensor that is used as it is strided; else empty: contiguous
 };
 
+constexpr size_t kMaxArgs = 1024;  // bytes of an argument block
+
 struct Call {
-  tkv_decode_args args;
+  size_t size;
+  alignas(16) char args[kMaxArgs];
   void* entry;
   c10::DeviceIndex device;
   std::vector<Slot> slots;
@@ -57,14 +61,14 @@ struct Call {
   int32_t res_cap;
 };
 
-// The tensor's storage if it is an ordinary contiguous tensor, else null.
-void* plain_pointer(const at::Tensor& t) {
+// The tensor's storage if it is an ordinary tensor, contiguous or of these strides, else null.
+void* plain_pointer(const at::Tensor& t, const std::vector<int64_t>& strides) {
   const auto* impl = t.unsafeGetTensorImpl();
   if (!impl->has_storage() || impl->is_python_dispatch() || t.layout() != c10::kStrided ||
       impl->key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Functionalize,
                                                    c10::DispatchKey::FuncTorchBatched,
                                                    c10::DispatchKey::FuncTorchGradWrapper})) ||
-      !t.is_contiguous())
+      !(strides.empty() ? t.is_contiguous() : t.strides() == c10::IntArrayRef(strides)))
     return nullptr;
   return t.mutable_data_ptr();
 }
@@ -74,24 +78,30 @@ void free_call(PyObject* capsule) {
 }
 
 // prepare(args: bytes, entry: int, device: int, slots: tuple of (tensor or None,
-//   offset or -1, alignment), window: None or (k_res, v_res, res_lens, res_cap))
+//   offset or -1, alignment[, strided: the argument block holds its strides]),
+//   window: None or (k_res, v_res, res_lens, res_cap))
 PyObject* prepare(PyObject*, PyObject* const* a, Py_ssize_t n) {
   try {
     char* bytes;
     Py_ssize_t len;
-    if (n != 5 || PyBytes_AsStringAndSize(a[0], &bytes, &len) || len != sizeof(tkv_decode_args) ||
-        !PyTuple_Check(a[3])) {
+    if (n != 5 || PyBytes_AsStringAndSize(a[0], &bytes, &len) || len > (Py_ssize_t)kMaxArgs ||
+        (a[4] != Py_None && len != sizeof(tkv_decode_args)) || !PyTuple_Check(a[3])) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "prepare: wrong arguments");
       return nullptr;
     }
     auto call = std::make_unique<Call>();
-    std::memcpy(&call->args, bytes, len);
+    call->size = len;
+    std::memcpy(call->args, bytes, len);
     call->entry = PyLong_AsVoidPtr(a[1]);
     call->device = (c10::DeviceIndex)PyLong_AsLong(a[2]);
     for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[3]); ++i) {
       PyObject *t;
-      int offset, align;
-      if (!PyArg_ParseTuple(PyTuple_GET_ITEM(a[3], i), "Oii", &t, &offset, &align)) return nullptr;
+      int offset, align, strided = 0;
+      if (!PyArg_ParseTuple(PyTuple_GET_ITEM(a[3], i), "Oii|i", &t, &offset, &align, &strided)) return nullptr;
+      if (offset != kFixed && (offset < 0 || offset + (Py_ssize_t)sizeof(void*) > len)) {
+        PyErr_SetString(PyExc_ValueError, "prepare: an offset past the argument block");
+        return nullptr;
+      }
       Slot s{};
       s.present = t != Py_None;
       s.offset = offset;
@@ -102,7 +112,8 @@ PyObject* prepare(PyObject*, PyObject* const* a, Py_ssize_t n) {
           return nullptr;
         }
         const at::Tensor& v = THPVariable_Unpack(t);
-        s.ptr = plain_pointer(v);
+        if (strided && !v.is_contiguous()) s.strides = v.strides().vec();
+        s.ptr = plain_pointer(v, s.strides);
         if (!s.ptr || ((uintptr_t)s.ptr & s.align_mask)) Py_RETURN_NONE;  // not a call to keep
         s.dtype = v.scalar_type();
         s.device = v.device();
@@ -139,7 +150,8 @@ PyObject* run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!call) return nullptr;
   try {
     if ((size_t)(n - 1) != call->slots.size()) Py_RETURN_NONE;
-    tkv_decode_args args = call->args;
+    alignas(16) char args[kMaxArgs];
+    std::memcpy(args, call->args, call->size);
     for (size_t i = 0; i < call->slots.size(); ++i) {
       const Slot& s = call->slots[i];
       PyObject* o = a[i + 1];
@@ -151,9 +163,9 @@ PyObject* run(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const at::Tensor& t = THPVariable_Unpack(o);
       if (t.scalar_type() != s.dtype || t.device() != s.device || t.sizes() != c10::IntArrayRef(s.sizes))
         Py_RETURN_NONE;
-      void* p = plain_pointer(t);
+      void* p = plain_pointer(t, s.strides);
       if (!p || ((uintptr_t)p & s.align_mask) || (s.offset == kFixed && p != s.ptr)) Py_RETURN_NONE;
-      if (s.offset != kFixed) std::memcpy(reinterpret_cast<char*>(&args) + s.offset, &p, sizeof p);
+      if (s.offset != kFixed) std::memcpy(args + s.offset, &p, sizeof p);
     }
     c10::hip::OptionalHIPGuard guard;
     if (c10::hip::current_device() != call->device) guard.set_index(call->device);
@@ -161,9 +173,9 @@ PyObject* run(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int rc;
     Py_BEGIN_ALLOW_THREADS
     rc = call->channel
-             ? reinterpret_cast<ChannelFn>(call->entry)(&args, call->k_res, call->v_res, call->res_lens,
+             ? reinterpret_cast<ChannelFn>(call->entry)(reinterpret_cast<const tkv_decode_args*>(args), call->k_res, call->v_res, call->res_lens,
                                                         call->res_cap, st)
-             : reinterpret_cast<DecodeFn>(call->entry)(&args, st);
+             : reinterpret_cast<EntryFn>(call->entry)(args, st);
     Py_END_ALLOW_THREADS
     return PyLong_FromLong(rc);
   } catch (const std::exception& e) {

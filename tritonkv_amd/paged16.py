@@ -1,0 +1,339 @@
+"""16-bit paged KV cache: fp16 and bf16 page pools, their append and their decode.
+
+The unquantized counterpart of :mod:`tritonkv_amd.paged`.  A pool is a plain
+tensor ``(num_pages, HKV, page_size, D)`` of ``torch.float16`` or
+``torch.bfloat16``; logical token t of batch row b lives in page
+``block_table[b, t // page_size]`` at slot ``t % page_size``.  Pools are used
+as they are strided, as long as a token's D values are dense and rows start on
+16 bytes: a token-major pool seen as ``(num_pages, page_size, HKV,
+D).transpose(1, 2)`` or the K half of a ``(num_pages, 2, HKV, page_size, D)``
+pool is one.  ``page_size`` is a multiple of 16.
+
+The decode cuts the rows' tokens on the device, from ``seq_lens`` itself:
+tables may be as wide as the longest request can get, and a captured step
+keeps a balanced split as the rows grow.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+from .kernels.fused_decode_attn import _backend, _check_out, _PreparedCall, _prepared, compute_units
+from .paged import _check_table
+from .quantize import _require_gpu
+
+PAGE_MULTIPLE = 16
+HEAD_DIMS = (64, 128, 256)
+DTYPES = (torch.float16, torch.bfloat16)
+
+
+def empty_paged16_pool(num_pages: int, HKV: int, page_size: int, D: int,
+                       dtype: torch.dtype = torch.float16, device="cuda") -> torch.Tensor:
+    """An uninitialised 16-bit page pool of ``num_pages`` pages of ``page_size`` tokens."""
+    if page_size <= 0 or page_size % PAGE_MULTIPLE:
+        raise ValueError(f"page_size must be a positive multiple of {PAGE_MULTIPLE}, got {page_size}")
+    if num_pages <= 0 or HKV <= 0:
+        raise ValueError(f"num_pages and HKV must be positive, got {num_pages} and {HKV}")
+    if D not in HEAD_DIMS:
+        raise ValueError(f"D must be one of {HEAD_DIMS}, got {D}")
+    if dtype not in DTYPES:
+        raise TypeError(f"dtype must be float16 or bfloat16, got {dtype}")
+    return torch.empty(num_pages, HKV, page_size, D, dtype=dtype, device=device)
+
+
+def _dense_rows(t: torch.Tensor, align: int) -> bool:
+    """Whether t's last axis is dense and every row starts on 16 bytes (``align`` elements)."""
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
+        all(s % align == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1)
+
+
+def _strides(t: torch.Tensor, align: int) -> tuple:
+    """t's strides without the last axis; those of axes of one entry, which nothing
+    multiplies, as ``align``."""
+    return tuple(s if n > 1 else align for s, n in zip(t.stride()[:-1], t.shape))
+
+
+def _check_pools16(k_pool, v_pool) -> tuple:
+    for name, pool in (("k_pool", k_pool), ("v_pool", v_pool)):
+        if not isinstance(pool, torch.Tensor) or pool.dim() != 4:
+            raise ValueError(f"{name} must be a (num_pages, HKV, page_size, D) tensor")
+        if pool.dtype not in DTYPES:
+            raise TypeError(f"{name} must be float16 or bfloat16, got {pool.dtype}")
+        if pool.numel() == 0:
+            raise ValueError(f"{name} is empty")
+        if not _dense_rows(pool, 8) or any(s == 0 for s in _strides(pool, 8)):
+            raise ValueError(f"{name} must hold each token's D values densely, on 16-byte boundaries")
+    if v_pool.shape != k_pool.shape or v_pool.dtype != k_pool.dtype or v_pool.device != k_pool.device:
+        raise ValueError("K and V pools must have the same shape, dtype and device")
+    num_pages, HKV, page_size, D = k_pool.shape
+    if page_size % PAGE_MULTIPLE:
+        raise ValueError(f"page_size must be a multiple of {PAGE_MULTIPLE}, got {page_size}")
+    if D not in HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {D}")
+    return num_pages, HKV, page_size, D
+
+
+def _int32_arg(t, n: int, device, name: str, what: str):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n \
+            or t.device != device:
+        raise ValueError(f"{name} must be an int32 tensor of {what} on the pools' device")
+    return t.contiguous()
+
+
+# Workgroups the decode's pieces should come to, per compute unit, and the
+# fewest tokens a piece of a cut row holds.
+WORKGROUPS_PER_CU = 3
+LEAST_TOKENS = 256
+MAX_PIECES = 65535  # grid y-dimension limit
+
+
+def plan_pieces(B: int, HKV: int, G: int, S: int, device=None,
+                piece_tokens: int | None = None) -> tuple[int, int, int]:
+    """``(least_chunks, target_pieces, max_pieces)`` of a decode (``include/tkv.h``).
+
+    ``S`` is the tables' capacity; the rows' lengths are the device's
+    business.  ``piece_tokens`` fixes the size of the pieces instead."""
+    units = HKV * -(-G // 16)  # workgroups that share a piece
+    if B > MAX_PIECES - 1:
+        raise ValueError(f"at most {MAX_PIECES - 1} rows, got {B}")
+    if piece_tokens is not None:
+        if piece_tokens <= 0:
+            raise ValueError(f"piece_tokens must be positive, got {piece_tokens}")
+        least = -(-piece_tokens // 32)
+        pieces = B * -(-S // (32 * least))  # as many as full rows have
+        if pieces > MAX_PIECES - B:
+            raise ValueError(f"piece_tokens={piece_tokens} cuts {B} rows of up to {S} tokens into "
+                             f"more than {MAX_PIECES} pieces")
+        return (least, 0, B) if S <= 32 * least else (least, pieces, pieces + B)
+    least = LEAST_TOKENS // 32
+    if S <= LEAST_TOKENS:
+        return least, 0, B
+    cu = compute_units(device) or 256
+    target = min(max(1, WORKGROUPS_PER_CU * cu // units), B * -(-S // LEAST_TOKENS), MAX_PIECES - B)
+    return least, target, target + B
+
+
+def _buffer(ws: dict, name: str, n: int, dtype, device) -> torch.Tensor:
+    """A workspace buffer of n entries; one that is in use is never replaced, since a
+    captured graph may hold its address."""
+    key = (name, n, str(device))
+    t = ws.get(key)
+    if t is None:
+        t = ws[key] = torch.empty(n, dtype=dtype, device=device)
+    return t
+
+
+class _Prepared16(_PreparedCall):
+    """A checked call of a 16-bit entry point: the argument block's tensors are all slots."""
+
+    __slots__ = ()
+
+    def run(self, *tensors) -> bool:
+        rc = _lib.host().run(self.call, *tensors)
+        if rc is None:
+            return False
+        if rc:
+            _lib.check(rc, self.what)
+        return True
+
+
+def _keep16(ws, key, args, entry, what, device, buffers, slots):
+    if ws is None or _lib.host() is None:
+        return
+    call = _lib.host().prepare(bytes(args), _lib.address(entry), device.index, slots, None)
+    if call is not None:
+        ws["call"] = _Prepared16(key, call, what, None, device, buffers)
+
+
+def _offset(struct, field: str) -> int:
+    return getattr(struct, field).offset
+
+
+_D = {f: _offset(_lib.Paged16Args, f) for f in ("q", "out", "lse", "k_new", "v_new")}
+_A = {f: _offset(_lib.Paged16AppendArgs, f) for f in ("k_new", "v_new", "positions", "counts")}
+
+
+def _new_rows(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """New tokens as the kernels read them: in the pools' type or fp32, rows on 16 bytes."""
+    if x.dtype != dtype and x.dtype != torch.float32:
+        x = x.float()
+    return x if _dense_rows(x, 8 if x.dtype == dtype else 4) else x.contiguous().clone()
+
+
+def paged16_append(k_pool: torch.Tensor, v_pool: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
+                   block_table: torch.Tensor, positions: torch.Tensor,
+                   counts: torch.Tensor | None = None, _workspace: dict | None = None) -> None:
+    """K and V of new tokens ``(B, HKV, N, D)`` into 16-bit page pools, in one launch.
+
+    Row b's first ``counts[b]`` tokens (None: all N) take logical positions
+    ``positions[b]``, ``positions[b] + 1``, ... and land in the pages the block
+    table names, rounded to the pools' type (nearest even).  ``k_new`` and
+    ``v_new`` are float16, bfloat16 or float32 in any strides; a token-major
+    ``(B, N, HKV, D).transpose(1, 2)`` is read as it lies.  Positions outside
+    ``[0, block_table.shape[1] * page_size)`` and table entries outside ``[0,
+    num_pages)`` are not written.  Two tokens for one place leave either.
+    Allocates nothing where the tensors are used as they lie, and does not
+    synchronise.
+    """
+    key = None
+    if _workspace is not None:
+        key = ("append16",)
+        prep = _prepared(_workspace, key)
+        if prep is not None and prep.run(k_pool, v_pool, k_new, v_new, block_table, positions, counts):
+            return
+    num_pages, HKV, page_size, D = _check_pools16(k_pool, v_pool)
+    device = k_pool.device
+    for name, x in (("k_new", k_new), ("v_new", v_new)):
+        if not isinstance(x, torch.Tensor) or x.dim() != 4 or (x.shape[1], x.shape[3]) != (HKV, D):
+            raise ValueError(f"{name} must be a (B, {HKV}, N, {D}) tensor")
+        if x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+            raise TypeError(f"{name} must be float16, bfloat16 or float32, got {x.dtype}")
+        if x.device != device:
+            raise ValueError(f"{name} is on {x.device}, the pools on {device}")
+    if k_new.shape != v_new.shape or k_new.dtype != v_new.dtype:
+        raise ValueError("k_new and v_new must have the same shape and dtype")
+    B, _, N, _ = k_new.shape
+    table = _check_table(block_table, B, device)
+    pos = _int32_arg(positions, B, device, "positions", "B start positions")
+    num = None if counts is None else _int32_arg(counts, B, device, "counts", "B token counts")
+    _require_gpu(k_pool, "paged16_append")
+    if B == 0 or N == 0:
+        return
+    kn, vn = _new_rows(k_new, k_pool.dtype), _new_rows(v_new, k_pool.dtype)
+    align = 8 if kn.dtype == k_pool.dtype else 4
+    args = _lib.Paged16AppendArgs(
+        k_new=kn.data_ptr(), v_new=vn.data_ptr(), k_new_strides=_strides(kn, align),
+        v_new_strides=_strides(vn, align), k=k_pool.data_ptr(), v=v_pool.data_ptr(),
+        k_strides=_strides(k_pool, 8), v_strides=_strides(v_pool, 8), block_table=table.data_ptr(),
+        positions=pos.data_ptr(), counts=_lib.ptr(num), new_is_fp32=int(kn.dtype == torch.float32),
+        is_bf16=int(k_pool.dtype == torch.bfloat16), B=B, HKV=HKV, N=N, D=D,
+        block_table_stride=table.shape[1], max_pages=table.shape[1], page_size=page_size,
+        num_pages=num_pages)
+    _lib.check(_lib.launch(device, "tkv_paged16_append", args), "paged16_append")
+    if key is not None and kn is k_new and vn is v_new:
+        _keep16(_workspace, key, args, "tkv_paged16_append", "paged16_append", device, (),
+                ((k_pool, -1, 16, 1), (v_pool, -1, 16, 1), (k_new, _A["k_new"], 16, 1),
+                 (v_new, _A["v_new"], 16, 1), (block_table, -1, 4), (positions, _A["positions"], 4),
+                 (counts, _A["counts"], 4)))
+
+
+def paged16_decode_attention(
+    q: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor | None = None,
+    sm_scale: float | None = None,
+    out: torch.Tensor | None = None,
+    lse: torch.Tensor | None = None,
+    _workspace: dict | None = None,
+    *,
+    k_new: torch.Tensor | None = None,
+    v_new: torch.Tensor | None = None,
+    piece_tokens: int | None = None,
+) -> torch.Tensor:
+    """One decode step of attention over 16-bit page pools.
+
+    q: ``(B, HQ, D)`` in the pools' type, D 64, 128 or 256; pools as
+    :func:`empty_paged16_pool`; block_table: ``(B, max_pages)`` int32;
+    seq_lens: ``(B,)`` int32 (None: every row holds ``max_pages * page_size``
+    tokens).  Returns ``(B, HQ, D)`` float32, in ``out`` if it is given.  A row
+    of no tokens gives zeros.  ``lse``: a contiguous ``(B, HQ)`` float32 tensor
+    that receives the natural logarithm of each row's sum of exp(score), -inf
+    for a row of no tokens, so that the results over two caches can be joined.
+
+    ``k_new`` / ``v_new``, ``(B, HKV, D)`` or ``(B, HKV, 1, D)`` in the pools'
+    type, fuse the step's append into the call: the token takes position
+    ``seq_lens[b] - 1`` of its row, in the page (unless the table entry lies
+    outside the pool) and in the attention.
+
+    ``piece_tokens`` fixes how many tokens a workgroup takes of a row; by
+    default the device chooses, from the lengths.  With ``_workspace`` the
+    call allocates nothing but a missing ``out`` and keeps its checked form for
+    the next call; calls that may overlap in time must not share one.
+    """
+    key = None
+    if _workspace is not None:
+        key = ("paged16", sm_scale, piece_tokens)
+        prep = _prepared(_workspace, key)
+        if prep is not None:
+            res = out if out is not None or not isinstance(q, torch.Tensor) else \
+                torch.empty(q.shape, dtype=torch.float32, device=q.device)
+            if prep.run(q, k_pool, v_pool, block_table, seq_lens, res, lse, k_new, v_new):
+                return res
+    num_pages, HKV, page_size, D = _check_pools16(k_pool, v_pool)
+    device = k_pool.device
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.shape[2] != D:
+        raise ValueError(f"q must be a (B, HQ, {D}) tensor")
+    if q.dtype != k_pool.dtype:
+        raise TypeError(f"q must have the pools' dtype {k_pool.dtype}, got {q.dtype}")
+    if q.device != device:
+        raise ValueError("q and the pools must be on the same device")
+    B, HQ, _ = q.shape
+    if B == 0 or HQ == 0 or HQ % HKV:
+        raise ValueError(f"q of {B} rows and HQ={HQ}: HQ must be a multiple of HKV={HKV}, and neither zero")
+    table = _check_table(block_table, B, device)
+    S = table.shape[1] * page_size
+    lens = None if seq_lens is None else _int32_arg(seq_lens, B, device, "seq_lens", "B lengths")
+    if lse is not None and (lse.shape != (B, HQ) or lse.dtype != torch.float32 or not lse.is_contiguous()
+                            or lse.device != device):
+        raise ValueError(f"lse must be a contiguous float32 ({B}, {HQ}) tensor on {device}")
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new must be given together")
+    new = [None, None]
+    if k_new is not None:
+        for i, (name, x) in enumerate((("k_new", k_new), ("v_new", v_new))):
+            x = x[:, :, 0] if x.dim() == 4 and x.shape[2] == 1 else x
+            if tuple(x.shape) != (B, HKV, D):
+                raise ValueError(f"{name} must have shape ({B}, {HKV}, {D}) or ({B}, {HKV}, 1, {D}), "
+                                 f"got {tuple(x.shape)}")
+            if x.dtype != k_pool.dtype:
+                raise TypeError(f"{name} must have the pools' dtype {k_pool.dtype}, got {x.dtype}")
+            if x.device != device:
+                raise ValueError(f"{name} must be on the pools' device")
+            new[i] = x if _dense_rows(x, 8) else x.contiguous().clone()
+    out = _check_out(out, B, HQ, D, device)
+    if out.data_ptr() % 16:
+        raise ValueError("out must start on a 16-byte boundary")
+    G = HQ // HKV
+    least, target, pieces = plan_pieces(B, HKV, G, S, device, piece_tokens)
+    ok, why = _backend(q)
+    if not ok:
+        raise RuntimeError(f"paged16_decode_attention requires the tritonkv_amd HIP backend: {why}")
+    qk = q if _dense_rows(q, 8) else q.contiguous().clone()
+    partials = rows = None
+    if target:
+        ws = {} if _workspace is None else _workspace
+        partials = _buffer(ws, "partials16", pieces * HQ * (D + 2), torch.float32, device)
+        rows = _buffer(ws, "row_pieces16", 2 * B, torch.int32, device)
+    kn, vn = new
+    args = _lib.Paged16Args(
+        q=qk.data_ptr(), q_strides=_strides(qk, 8), k=k_pool.data_ptr(), v=v_pool.data_ptr(),
+        k_strides=_strides(k_pool, 8), v_strides=_strides(v_pool, 8), block_table=table.data_ptr(),
+        seq_lens=_lib.ptr(lens), out=out.data_ptr(), lse=_lib.ptr(lse), partials=_lib.ptr(partials),
+        row_pieces=_lib.ptr(rows), k_new=_lib.ptr(kn), v_new=_lib.ptr(vn),
+        k_new_strides=_strides(kn, 8) if kn is not None else (0, 0),
+        v_new_strides=_strides(vn, 8) if vn is not None else (0, 0),
+        is_bf16=int(k_pool.dtype == torch.bfloat16), B=B, HQ=HQ, HKV=HKV, D=D,
+        block_table_stride=table.shape[1], max_pages=table.shape[1], page_size=page_size,
+        num_pages=num_pages,
+        sm_scale=1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
+        least_chunks=least, target_pieces=target, max_pieces=pieces, waves=4)
+    _lib.check(_lib.launch(device, "tkv_paged16_decode_attention", args), "paged16_decode_attention")
+    if key is not None and qk is q:
+        strided = (k_new is None or kn.data_ptr() == k_new.data_ptr()) and \
+            (v_new is None or vn.data_ptr() == v_new.data_ptr())
+        if strided:  # nothing was copied: every tensor is read where it lies
+            _keep16(_workspace, key, args, "tkv_paged16_decode_attention", "paged16_decode_attention",
+                    device, (partials, rows),
+                    ((q, _D["q"], 16, 1), (k_pool, -1, 16, 1), (v_pool, -1, 16, 1), (block_table, -1, 4),
+                     (seq_lens, -1, 4), (out, _D["out"], 16), (lse, _D["lse"], 4),
+                     (k_new, _D["k_new"], 16, 1), (v_new, _D["v_new"], 16, 1)))
+    return out
+
+
+__all__ = ["PAGE_MULTIPLE", "HEAD_DIMS", "empty_paged16_pool", "paged16_append",
+           "paged16_decode_attention", "plan_pieces"]
