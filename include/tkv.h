@@ -380,6 +380,78 @@ typedef struct tkv_paged16_append_args {
 } tkv_paged16_append_args;
 int tkv_paged16_append(const tkv_paged16_append_args *args, tkv_stream_t stream);
 
+/* Page tensors that share page numbers: page p of tensor t is the `bytes[t]`
+ * bytes at src[t] + p * src_stride[t], and a copy writes them at dst[t] + q *
+ * dst_stride[t] (the same pointers and strides within one set of pools).
+ * Pointers, strides and bytes are multiples of 16. */
+#define TKV_PAGE_TENSORS 32
+typedef struct tkv_page_set {
+  const void *src[TKV_PAGE_TENSORS];
+  void *dst[TKV_PAGE_TENSORS];
+  int64_t src_stride[TKV_PAGE_TENSORS], dst_stride[TKV_PAGE_TENSORS], bytes[TKV_PAGE_TENSORS];
+  int32_t count;
+} tkv_page_set;
+
+/* Page dst[i] := page src[i] in every tensor of the set, for i < n.  A pair with a
+ * number outside [0, src_pages) or [0, dst_pages) is skipped; of several pairs
+ * with one destination the first is carried out.  Within one set of pools (same)
+ * a page that the call reads is never written: a pair whose destination is a
+ * pair's source is skipped, and (p, p) is no pair.  work: tkv_copy_pages_work()
+ * int32, 8-byte aligned (none for up to 512 pairs).  No counterpart in the
+ * reference, nor have the next two (its caches have no pages). */
+typedef struct tkv_copy_pages_args {
+  tkv_page_set set;
+  const int32_t *src, *dst;
+  int32_t *work;
+  int32_t n, src_pages, dst_pages, same;
+} tkv_copy_pages_args;
+int64_t tkv_copy_pages_work(int32_t n, int32_t src_pages, int32_t dst_pages);
+int tkv_copy_pages(const tkv_copy_pages_args *args, tkv_stream_t stream);
+
+/* New rows of a block table out of its old ones, in place, over pages counted in
+ * refs (entries of used slots, slot < ceil(seq_lens / page_size), that name a
+ * page; 0: free).  Row b becomes the first min(n_b, L_a) tokens of old row a =
+ * parents[b] (parents NULL: b; outside [0, B): an empty row), with pages for n_b
+ * = new_lens[b] tokens (NULL: L_a; below 0: 0).  Full pages are shared.  The page
+ * that a row ends in, if it is not full, is the row's own: it stays with one row
+ * where only children of the row it belonged to alone end in it (that row itself,
+ * else the lowest), and every other row gets a copy.  New pages are the lowest that
+ * were free before the call, in row order.  Then seq_lens[b] = n_b, entries past
+ * the row's pages are -1, and refs follow.  *status is TKV_ROWS_DONE, or says why
+ * nothing was changed.  set: the pools (src == dst), whose copies go with the
+ * table; work: tkv_fork_rows_work() int32, 8-byte aligned.  Two launches; at most
+ * 8192 rows. */
+enum { TKV_ROWS_DONE = 0, TKV_ROWS_NO_PAGES = 1, TKV_ROWS_PAST_TABLE = 2 };
+typedef struct tkv_fork_rows_args {
+  tkv_page_set set;
+  int32_t *block_table, *seq_lens, *refs;
+  const int32_t *parents, *new_lens;
+  int32_t *status, *work;
+  int32_t table_stride, B, max_pages, page_size, num_pages;
+} tkv_fork_rows_args;
+int64_t tkv_fork_rows_work(int32_t B, int32_t max_pages, int32_t num_pages, int32_t parents);
+int tkv_fork_rows(const tkv_fork_rows_args *args, tkv_stream_t stream);
+
+/* Live pages (refs > 0) to the low end: with n of them, the i-th live page at or
+ * past n is copied to the i-th free page below n in every tensor of the set;
+ * out_table is block_table with the moved pages' new numbers, out_refs refs with
+ * their counts at the new places, and *live (NULL: not wanted) n.  out_table and
+ * out_refs may be block_table and refs.  The old places keep their bytes.  work:
+ * tkv_compact_pages_work() int32, 8-byte aligned.  Two launches. */
+typedef struct tkv_compact_pages_args {
+  tkv_page_set set;
+  const int32_t *block_table, *refs;
+  int32_t *out_table, *out_refs, *live, *work;
+  int32_t table_stride, out_stride, B, max_pages, num_pages;
+} tkv_compact_pages_args;
+int64_t tkv_compact_pages_work(int32_t num_pages);
+int tkv_compact_pages(const tkv_compact_pages_args *args, tkv_stream_t stream);
+
+/* The copies of the tkv_fork_rows or tkv_compact_pages call that last used `work`,
+ * in the tensors of another set (a set holds 32).  most: the most pairs there can
+ * be, the call's B or num_pages / 2. */
+int tkv_copy_planned(const tkv_page_set *set, const int32_t *work, int32_t most, tkv_stream_t stream);
+
 typedef struct tkv_device_info_t {
   int32_t device;
   int32_t compute_units;

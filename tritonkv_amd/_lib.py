@@ -137,6 +137,76 @@ class Paged16AppendArgs(ctypes.Structure):
     ]
 
 
+PAGE_TENSORS = 32  # TKV_PAGE_TENSORS
+
+
+class PageSet(ctypes.Structure):
+    """Mirror of ``tkv_page_set``."""
+
+    _fields_ = [
+        ("src", ctypes.c_void_p * PAGE_TENSORS),
+        ("dst", ctypes.c_void_p * PAGE_TENSORS),
+        ("src_stride", ctypes.c_int64 * PAGE_TENSORS),
+        ("dst_stride", ctypes.c_int64 * PAGE_TENSORS),
+        ("bytes", ctypes.c_int64 * PAGE_TENSORS),
+        ("count", ctypes.c_int32),
+    ]
+
+
+class CopyPagesArgs(ctypes.Structure):
+    """Mirror of ``tkv_copy_pages_args``."""
+
+    _fields_ = [
+        ("set", PageSet),
+        ("src", ctypes.c_void_p),
+        ("dst", ctypes.c_void_p),
+        ("work", ctypes.c_void_p),
+        ("n", ctypes.c_int32),
+        ("src_pages", ctypes.c_int32),
+        ("dst_pages", ctypes.c_int32),
+        ("same", ctypes.c_int32),
+    ]
+
+
+class ForkRowsArgs(ctypes.Structure):
+    """Mirror of ``tkv_fork_rows_args``."""
+
+    _fields_ = [
+        ("set", PageSet),
+        ("block_table", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("refs", ctypes.c_void_p),
+        ("parents", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("work", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+    ]
+
+
+class CompactPagesArgs(ctypes.Structure):
+    """Mirror of ``tkv_compact_pages_args``."""
+
+    _fields_ = [
+        ("set", PageSet),
+        ("block_table", ctypes.c_void_p),
+        ("refs", ctypes.c_void_p),
+        ("out_table", ctypes.c_void_p),
+        ("out_refs", ctypes.c_void_p),
+        ("live", ctypes.c_void_p),
+        ("work", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int32),
+        ("out_stride", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+    ]
+
+
 class DeviceInfo(ctypes.Structure):
     """Mirror of ``tkv_device_info_t``."""
 
@@ -181,6 +251,13 @@ SIGNATURES = {
     "tkv_dequantize": ([_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P], ctypes.c_int),
     "tkv_paged16_decode_attention": ([ctypes.POINTER(Paged16Args), _P], ctypes.c_int),
     "tkv_paged16_append": ([ctypes.POINTER(Paged16AppendArgs), _P], ctypes.c_int),
+    "tkv_copy_pages_work": ([_I32, _I32, _I32], _I64),
+    "tkv_copy_pages": ([ctypes.POINTER(CopyPagesArgs), _P], ctypes.c_int),
+    "tkv_fork_rows_work": ([_I32, _I32, _I32, _I32], _I64),
+    "tkv_fork_rows": ([ctypes.POINTER(ForkRowsArgs), _P], ctypes.c_int),
+    "tkv_compact_pages_work": ([_I32], _I64),
+    "tkv_compact_pages": ([ctypes.POINTER(CompactPagesArgs), _P], ctypes.c_int),
+    "tkv_copy_planned": ([ctypes.POINTER(PageSet), _P, _I32, _P], ctypes.c_int),
     "tkv_device_info": ([ctypes.POINTER(DeviceInfo)], ctypes.c_int),
     "tkv_status_string": ([ctypes.c_int], ctypes.c_char_p),
     "tkv_abi_version": ([], ctypes.c_int),

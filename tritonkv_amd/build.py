@@ -40,7 +40,7 @@ CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libtkv_hip.so")
 HOSTCALL = os.path.join(PKG, "_hostcall.so")
-SOURCES = ["decode_attention.hip", "quant_pack.hip", "dequant.hip", "runtime.hip", "paged16.hip"] + [
+SOURCES = ["decode_attention.hip", "quant_pack.hip", "dequant.hip", "runtime.hip", "paged16.hip", "pages.hip"] + [
     f"quant_split_{bits}{hc}.hip" for bits in ("k4v4", "k2v2", "k4v2", "k2v4") for hc in ("", "_h4", "_h8")]
 ARCH = "gfx950"
 

@@ -47,7 +47,7 @@ struct Slot {
   std::vector<int64_t> strides;  // of a tensor that is used as it is strided; else empty: contiguous
 };
 
-constexpr size_t kMaxArgs = 1024;  // bytes of an argument block
+constexpr size_t kMaxArgs = 2048;  // bytes of an argument block
 
 struct Call {
   size_t size;

@@ -1,0 +1,589 @@
+// Bookkeeping of page pools on the device, for gfx950: copying pages, forking /
+// truncating / growing / freeing rows of a block table over reference-counted
+// pages, and moving the live pages to the low end of the pools.
+//
+// No formula here but the copies' bytes: a page that moves is read and written
+// once in every tensor.  The plans are integers; each is made by one workgroup
+// in one pass over the rows and one over the reference counts, so that a
+// call is two launches and its result does not depend on any order: pages are
+// handed out lowest first, in row order, by prefix sums, and the only atomics are
+// integer sums, maxima and minima.
+#include <hip/hip_runtime.h>
+
+#include "tkv_device.h"
+#include "../../include/tkv.h"
+
+namespace tkv {
+
+constexpr int kPlan = 1024;                  // threads of a plan's workgroup
+constexpr int kSlice = 16384;                // bytes of a page that a workgroup copies at a time
+constexpr int kMaxRows = 8192;               // rows of a fork: two LDS integers each
+constexpr int kInlinePairs = 512;            // pairs that the copy checks by itself
+constexpr int kPagesPerThread = 64;          // bits of a thread's mask of pages
+
+// A barrier behind which the workgroup's memory operations have been carried out.
+__device__ __forceinline__ void settle() {
+  __builtin_amdgcn_s_waitcnt(0);  // vmcnt(0) expcnt(0) lgkmcnt(0)
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------------------
+// The copy.  Item = one slice of one tensor's page; workgroups stride over the
+// items of the first `count` pairs.
+// ---------------------------------------------------------------------------
+struct CopyPlan {
+  tkv_page_set set;
+  int32_t first[TKV_PAGE_TENSORS];  // slices of a page before tensor t
+  int32_t slices;                   // of a page, in all tensors
+};
+
+__device__ __forceinline__ void copy_slice(const CopyPlan& c, int src, int dst, int slice) {
+  int t = 0;
+#pragma unroll
+  for (int step = TKV_PAGE_TENSORS / 2; step; step /= 2)
+    if (t + step < c.set.count && c.first[t + step] <= slice) t += step;
+  const int64_t at = (int64_t)(slice - c.first[t]) * kSlice;
+  const int64_t left = c.set.bytes[t] - at;
+  const int units = (int)((left < kSlice ? left : (int64_t)kSlice) / 16);
+  const u4* from = reinterpret_cast<const u4*>(static_cast<const char*>(c.set.src[t]) + src * c.set.src_stride[t] + at);
+  u4* to = reinterpret_cast<u4*>(static_cast<char*>(c.set.dst[t]) + dst * c.set.dst_stride[t] + at);
+  constexpr int kPer = kSlice / 16 / 256;
+  u4 x[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int u = threadIdx.x + 256 * i;
+    if (u < units) x[i] = __builtin_nontemporal_load(from + u);
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int u = threadIdx.x + 256 * i;
+    if (u < units) __builtin_nontemporal_store(x[i], to + u);
+  }
+}
+
+// Pairs (x, y) = (source, destination); a negative source is no pair.
+__device__ __forceinline__ void copy_pairs(const CopyPlan& c, const int2* pairs, int count, int group, int groups) {
+  const int64_t items = (int64_t)count * c.slices;
+  for (int64_t i = group; i < items; i += groups) {
+    const int p = (int)(i / c.slices);
+    const int2 pair = pairs[p];
+    if (pair.x >= 0) copy_slice(c, pair.x, pair.y, (int)(i - (int64_t)p * c.slices));
+  }
+}
+
+// Whether the lists name a pair at all.
+__device__ __forceinline__ bool is_pair(const tkv_copy_pages_args& a, int s, int d) {
+  return s >= 0 && s < a.src_pages && d >= 0 && d < a.dst_pages && !(a.same && s == d);
+}
+
+// A few pairs: every workgroup checks its own pair against all of them.  A pair
+// is carried out unless an earlier one has its destination or, within one set
+// of pools, any one reads it.
+__global__ void __launch_bounds__(256) copy_few_kernel(CopyPlan c, tkv_copy_pages_args a) {
+  const int64_t items = (int64_t)a.n * c.slices;
+  for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+    const int p = (int)(i / c.slices);
+    const int s = a.src[p], d = a.dst[p];
+    bool bad = !is_pair(a, s, d);
+    for (int x = threadIdx.x; x < a.n; x += 256) {
+      const int sx = a.src[x], dx = a.dst[x];
+      if (is_pair(a, sx, dx) && ((x < p && dx == d) || (a.same && sx == d))) bad = true;
+    }
+    if (!__syncthreads_or(bad)) copy_slice(c, s, d, (int)(i - (int64_t)p * c.slices));
+  }
+}
+
+// Many pairs: the same rule in three passes of one workgroup over the pages
+// that the pairs name (owner: the first pair of a destination; read: a source).
+__global__ void __launch_bounds__(kPlan) copy_check_kernel(tkv_copy_pages_args a) {
+  int* owner = a.work;
+  int* read = owner + a.dst_pages;
+  int2* pairs = reinterpret_cast<int2*>(a.work + a.dst_pages + a.src_pages + (((a.dst_pages + a.src_pages) & 1)));
+  for (int i = threadIdx.x; i < a.n; i += kPlan) {
+    const int s = a.src[i], d = a.dst[i];
+    if (is_pair(a, s, d)) {
+      owner[d] = a.n;
+      if (a.same) read[d] = 0;
+    }
+  }
+  settle();
+  for (int i = threadIdx.x; i < a.n; i += kPlan) {
+    const int s = a.src[i], d = a.dst[i];
+    if (is_pair(a, s, d)) {
+      atomicMin(owner + d, i);
+      if (a.same) atomicExch(read + s, 1);
+    }
+  }
+  settle();
+  for (int i = threadIdx.x; i < a.n; i += kPlan) {
+    const int s = a.src[i], d = a.dst[i];
+    bool ok = is_pair(a, s, d);
+    if (ok) ok = atomicAdd(owner + d, 0) == i && !(a.same && atomicAdd(read + d, 0) != 0);
+    pairs[i] = make_int2(ok ? s : -1, d);
+  }
+}
+
+__global__ void __launch_bounds__(256) copy_pairs_kernel(CopyPlan c, const int2* pairs, const int* count, int n) {
+  copy_pairs(c, pairs, count ? *count : n, blockIdx.x, gridDim.x);
+}
+
+// ---------------------------------------------------------------------------
+// Sums over a plan's workgroup.
+// ---------------------------------------------------------------------------
+struct ScanLds {
+  int2 wave[kPlan / 64];
+};
+
+// Exclusive sums of (x, y) over the threads before this one; total of both.
+__device__ __forceinline__ int2 block_scan(ScanLds& lds, int x, int y, int2& total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int sx = x, sy = y;
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) {
+    const int ox = __shfl_up(sx, off, 64), oy = __shfl_up(sy, off, 64);
+    if (lane >= off) {
+      sx += ox;
+      sy += oy;
+    }
+  }
+  __syncthreads();  // the previous scan's sums have been read
+  if (lane == 63) lds.wave[w] = make_int2(sx, sy);
+  __syncthreads();
+  int2 before = make_int2(0, 0);
+  total = make_int2(0, 0);
+#pragma unroll
+  for (int i = 0; i < kPlan / 64; ++i) {
+    const int2 v = lds.wave[i];
+    if (i < w) {
+      before.x += v.x;
+      before.y += v.y;
+    }
+    total.x += v.x;
+    total.y += v.y;
+  }
+  return make_int2(before.x + sx - x, before.y + sy - y);
+}
+
+// Bits of the pages p0 .. p0 + per - 1 (per <= 64) that are in use.
+__device__ __forceinline__ uint64_t used_mask(const int32_t* __restrict__ refs, int64_t p0, int per, int N) {
+  uint64_t m = 0;
+  if (p0 + per <= N && per % 4 == 0 && (reinterpret_cast<uintptr_t>(refs + p0) & 15) == 0) {
+#pragma unroll 4
+    for (int i = 0; i < per; i += 4) {
+      const int4 v = *reinterpret_cast<const int4*>(refs + p0 + i);
+      m |= (uint64_t)((v.x > 0) | (v.y > 0) << 1 | (v.z > 0) << 2 | (v.w > 0) << 3) << i;
+    }
+  } else {
+    for (int i = 0; i < per; ++i)
+      if (p0 + i < N && refs[p0 + i] > 0) m |= uint64_t(1) << i;
+  }
+  return m;
+}
+__device__ __forceinline__ uint64_t first_bits(int64_t n) {
+  return n <= 0 ? 0 : n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1;
+}
+// Pages a thread takes of N in one round of the workgroup.
+__device__ __forceinline__ int pages_per_thread(int N) {
+  const int per = ((N + kPlan - 1) / kPlan + 3) & ~3;
+  return per < kPagesPerThread ? per : kPagesPerThread;
+}
+
+// ---------------------------------------------------------------------------
+// Rows: row b becomes the first min(want_b, L_a) tokens of old row a =
+// parents[b], with pages for want_b.  keep = min(want_b, L_a) has f = keep /
+// page full pages, which are shared, and perhaps a partial one.  That page stays
+// with one row (`heir`) if nobody else keeps it: it was a's alone, no other
+// child of a keeps it as a full page, and of the children that end in it the heir
+// is a itself or the lowest; every other child copies it to its first new page.
+// ---------------------------------------------------------------------------
+struct RowsWork {  // a.work, in int32
+  int* head;       // status, copies, new pages
+  int *old_len, *kept, *first, *pages;
+  int2* pairs;
+  int *fresh, *staged;
+};
+
+__host__ __device__ inline int64_t rows_work_ints(int64_t B, int64_t P, int64_t N, bool staged) {
+  return 16 + 6 * B + N + (staged ? B * P : 0);
+}
+
+__device__ __forceinline__ RowsWork rows_work(const tkv_fork_rows_args& a) {
+  RowsWork w;
+  int* p = a.work;
+  w.head = p;
+  w.pairs = reinterpret_cast<int2*>(p + 16);
+  w.old_len = p + 16 + 2 * a.B;
+  w.kept = w.old_len + a.B;
+  w.first = w.kept + a.B;
+  w.pages = w.first + a.B;
+  w.fresh = w.pages + a.B;
+  w.staged = w.fresh + a.num_pages;
+  return w;
+}
+
+struct Row {
+  int a, want, f, last;  // parent (-1: none), tokens, full pages kept, pool page after them
+  bool rest;             // ... of which some tokens are kept
+};
+
+__device__ __forceinline__ int table_tokens(const tkv_fork_rows_args& a) { return a.max_pages * a.page_size; }
+
+__device__ __forceinline__ Row row_of(const tkv_fork_rows_args& a, int b) {
+  Row r;
+  r.a = a.parents ? a.parents[b] : b;
+  if (r.a < 0 || r.a >= a.B) r.a = -1;
+  const int have = r.a < 0 ? 0 : max(0, min(a.seq_lens[r.a], table_tokens(a)));
+  r.want = r.a < 0 ? 0 : a.new_lens ? max(0, a.new_lens[b]) : have;
+  const int keep = min(have, r.want);
+  r.f = keep / a.page_size;
+  r.rest = keep % a.page_size != 0;
+  r.last = r.rest ? a.block_table[(int64_t)r.a * a.table_stride + r.f] : -1;
+  return r;
+}
+
+__global__ void __launch_bounds__(kPlan) rows_plan_kernel(tkv_fork_rows_args a) {
+  extern __shared__ int lds[];
+  __shared__ ScanLds scan;
+  __shared__ int past;
+  const RowsWork w = rows_work(a);
+  const int tid = threadIdx.x, B = a.B, P = a.max_pages, N = a.num_pages;
+  if (blockIdx.x > 0) {
+    // The rows' old pages, which the second launch reads while it writes the table.
+    for (int64_t i = (int64_t)(blockIdx.x - 1) * kPlan + tid; i < (int64_t)B * P; i += (int64_t)(gridDim.x - 1) * kPlan) {
+      const int b = (int)(i / P);
+      w.staged[i] = a.block_table[(int64_t)b * a.table_stride + (i - (int64_t)b * P)];
+    }
+    return;
+  }
+  int *most = lds, *best = lds + B;
+  for (int b = tid; b < B; b += kPlan) {
+    most[b] = -1;
+    best[b] = B;
+  }
+  if (tid == 0) past = 0;
+  __syncthreads();
+  for (int b = tid; b < B; b += kPlan) {
+    const Row r = row_of(a, b);
+    if (r.a >= 0) atomicMax(most + r.a, r.f);
+    if (r.want > table_tokens(a)) past = 1;
+  }
+  __syncthreads();
+  auto may_inherit = [&](const Row& r) {
+    return r.rest && r.f == most[r.a] && r.last >= 0 && r.last < N && a.refs[r.last] == 1;
+  };
+  for (int b = tid; b < B; b += kPlan) {
+    const Row r = row_of(a, b);
+    if (may_inherit(r)) atomicMin(best + r.a, r.a == b ? -1 : b);
+  }
+  __syncthreads();
+  const bool too_long = past != 0;
+  int2 done = make_int2(0, 0);  // new pages and copies of the rows before this round's
+  for (int b0 = 0; b0 < B; b0 += kPlan) {
+    const int b = b0 + tid;
+    Row r;
+    int need = 0, pages = 0;
+    bool heir = false, copy = false;
+    if (b < B) {
+      r = row_of(a, b);
+      heir = may_inherit(r) && best[r.a] == (r.a == b ? -1 : b);
+      pages = (int)(((int64_t)r.want + a.page_size - 1) / a.page_size);
+      // (a row that does not fit its table asks for nothing: the call fails)
+      need = too_long ? 0 : pages - r.f - (heir ? 1 : 0);
+      copy = !too_long && r.rest && !heir;
+    }
+    int2 total;
+    const int2 at = block_scan(scan, need, copy ? 1 : 0, total);
+    if (b < B) {
+      w.old_len[b] = max(0, min(a.seq_lens[b], table_tokens(a)));
+      w.kept[b] = r.f + (heir ? 1 : 0);
+      w.first[b] = done.x + at.x;
+      w.pages[b] = pages;
+      if (copy) w.pairs[done.y + at.y] = make_int2(r.last, done.x + at.x);
+    }
+    done.x += total.x;
+    done.y += total.y;
+  }
+  // The lowest free pages.
+  int found = 0;
+  const int per = pages_per_thread(N);
+  for (int64_t p0 = 0; p0 < N && found < done.x; p0 += (int64_t)per * kPlan) {
+    const int64_t mine = p0 + (int64_t)tid * per;
+    uint64_t m = ~used_mask(a.refs, mine, per, N) & first_bits(N - mine) & first_bits(per);
+    int2 total;
+    int at = found + block_scan(scan, __popcll(m), 0, total).x;
+    for (; m && at < done.x; m &= m - 1) w.fresh[at++] = (int)(mine + __builtin_ctzll(m));
+    found += total.x;
+  }
+  const int status = too_long ? TKV_ROWS_PAST_TABLE : found < done.x ? TKV_ROWS_NO_PAGES : TKV_ROWS_DONE;
+  settle();
+  const int copies = status ? 0 : done.y;
+  for (int i = tid; i < copies; i += kPlan) {
+    int2 p = w.pairs[i];
+    p.y = w.fresh[p.y];
+    if (p.x >= N) p.x = -1;  // the table names no page there
+    w.pairs[i] = p;
+  }
+  if (tid == 0) {
+    w.head[0] = status;
+    w.head[1] = copies;
+    *a.status = status;
+  }
+}
+
+// Workgroups [0, tables): the table, lengths and counts; the others: the copies.
+__global__ void __launch_bounds__(256) rows_apply_kernel(tkv_fork_rows_args a, CopyPlan c, int tables) {
+  const RowsWork w = rows_work(a);
+  if (w.head[0] != TKV_ROWS_DONE) return;
+  if ((int)blockIdx.x >= tables) {
+    copy_pairs(c, w.pairs, w.head[1], blockIdx.x - tables, gridDim.x - tables);
+    return;
+  }
+  const int P = a.max_pages, N = a.num_pages;
+  const int64_t entries = (int64_t)a.B * P;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)tables * 256) {
+    const int b = (int)(i / P), slot = (int)(i - (int64_t)b * P);
+    int* at = a.block_table + (int64_t)b * a.table_stride + slot;
+    const int old = *at, kept = w.kept[b], pages = w.pages[b];
+    int now = -1;
+    if (slot < kept) {
+      const int from = a.parents ? a.parents[b] : b;
+      now = a.parents ? w.staged[(int64_t)from * P + slot] : old;
+    } else if (slot < pages) {
+      now = w.fresh[w.first[b] + slot - kept];
+    }
+    const int was = (w.old_len[b] + a.page_size - 1) / a.page_size;
+    const int dec = slot < was && old >= 0 && old < N ? old : -1;
+    const int inc = slot < pages && now >= 0 && now < N ? now : -1;
+    if (dec != inc) {
+      if (dec >= 0) atomicSub(a.refs + dec, 1);
+      if (inc >= 0) atomicAdd(a.refs + inc, 1);
+    }
+    if (now != old) *at = now;
+    if (slot == 0) {
+      const bool none = a.parents && (a.parents[b] < 0 || a.parents[b] >= a.B);
+      const int len = a.new_lens ? (none ? 0 : max(0, a.new_lens[b]))
+                      : a.parents ? (none ? 0 : w.old_len[a.parents[b]]) : w.old_len[b];
+      a.seq_lens[b] = len;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Compaction: with n live pages (refs > 0), the i-th live page at or past n moves
+// to the i-th free page below n.
+// ---------------------------------------------------------------------------
+struct CompactWork {
+  int* head;   // live pages, moves
+  int2* pairs;
+  int *rank;   // of a page that moves or is moved onto; -1 for the others
+  int *count;  // references of the i-th page that moves
+};
+
+__host__ __device__ inline int64_t compact_work_ints(int64_t N) { return 16 + (N + 2) + N + N / 2 + 1; }
+
+__device__ __forceinline__ CompactWork compact_work(const tkv_compact_pages_args& a) {
+  CompactWork w;
+  w.head = a.work;
+  w.pairs = reinterpret_cast<int2*>(a.work + 16);  // at most N / 2 moves
+  w.rank = a.work + 16 + (a.num_pages + 2);
+  w.count = w.rank + a.num_pages;
+  return w;
+}
+
+__global__ void __launch_bounds__(kPlan) compact_plan_kernel(tkv_compact_pages_args a) {
+  __shared__ ScanLds scan;
+  const CompactWork w = compact_work(a);
+  const int tid = threadIdx.x, N = a.num_pages, per = pages_per_thread(N);
+  const int64_t round = (int64_t)per * kPlan;
+  int live = 0;
+  uint64_t m = 0;
+  for (int64_t p0 = 0; p0 < N; p0 += round) {
+    m = used_mask(a.refs, p0 + (int64_t)tid * per, per, N);
+    int2 total;
+    block_scan(scan, __popcll(m), 0, total);
+    live += total.x;
+  }
+  int2 done = make_int2(0, 0);
+  for (int64_t p0 = 0; p0 < N; p0 += round) {
+    const int64_t mine = p0 + (int64_t)tid * per;
+    if (N > round) m = used_mask(a.refs, mine, per, N);
+    const uint64_t low = first_bits(live - mine), in = first_bits(N - mine) & first_bits(per);
+    const uint64_t from = m & ~low, to = ~m & low & in;
+    int2 total;
+    const int2 at = block_scan(scan, __popcll(from), __popcll(to), total);
+    int s = done.x + at.x, d = done.y + at.y;
+    for (int i = 0; i < per && mine + i < N; ++i) {
+      const uint64_t bit = uint64_t(1) << i;
+      int rank = -1;
+      if (from & bit) {
+        w.pairs[s].x = (int)(mine + i);
+        w.count[s] = a.refs[mine + i];
+        rank = s++;
+      } else if (to & bit) {
+        w.pairs[d].y = (int)(mine + i);
+        rank = d++;
+      }
+      w.rank[mine + i] = rank;
+    }
+    done.x += total.x;
+    done.y += total.y;
+  }
+  if (tid == 0) {
+    w.head[0] = live;
+    w.head[1] = done.x;
+    if (a.live) *a.live = live;
+  }
+}
+
+// Workgroups [0, tables): the table and the counts; the others: the copies.
+__global__ void __launch_bounds__(256) compact_apply_kernel(tkv_compact_pages_args a, CopyPlan c, int tables) {
+  const CompactWork w = compact_work(a);
+  const int live = w.head[0];
+  if ((int)blockIdx.x >= tables) {
+    copy_pairs(c, w.pairs, w.head[1], blockIdx.x - tables, gridDim.x - tables);
+    return;
+  }
+  const int P = a.max_pages, N = a.num_pages;
+  const int64_t entries = (int64_t)a.B * P;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries + N; i += (int64_t)tables * 256) {
+    if (i < entries) {
+      const int b = (int)(i / P), slot = (int)(i - (int64_t)b * P);
+      int page = a.block_table[(int64_t)b * a.table_stride + slot];
+      if (page >= live && page < N && w.rank[page] >= 0) page = w.pairs[w.rank[page]].y;
+      a.out_table[(int64_t)b * a.out_stride + slot] = page;
+    } else {
+      const int p = (int)(i - entries);
+      const int rank = w.rank[p];
+      a.out_refs[p] = p >= live ? 0 : rank >= 0 ? w.count[rank] : a.refs[p];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+static int make_plan(const tkv_page_set& s, CopyPlan& c) {
+  if (s.count < 0 || s.count > TKV_PAGE_TENSORS) return TKV_EINVAL;
+  c.set = s;
+  int64_t slices = 0;
+  for (int t = 0; t < s.count; ++t) {
+    if (!s.src[t] || !s.dst[t] || s.bytes[t] <= 0) return TKV_EINVAL;
+    if (((uintptr_t)s.src[t] | (uintptr_t)s.dst[t] | (uint64_t)s.bytes[t] | (uint64_t)s.src_stride[t] |
+         (uint64_t)s.dst_stride[t]) & 15)
+      return TKV_EINVAL;
+    if (s.src_stride[t] < s.bytes[t] || s.dst_stride[t] < s.bytes[t]) return TKV_EINVAL;
+    c.first[t] = (int32_t)slices;
+    slices += (s.bytes[t] + kSlice - 1) / kSlice;
+    if (slices > INT32_MAX) return TKV_EUNSUPPORTED;
+  }
+  for (int t = s.count; t < TKV_PAGE_TENSORS; ++t) c.first[t] = INT32_MAX;
+  c.slices = (int32_t)slices;
+  return TKV_OK;
+}
+
+constexpr int kCopyGroups = 4096;  // workgroups that stride over the copies
+
+static unsigned copy_groups(int64_t pairs, const CopyPlan& c) {
+  const int64_t items = pairs * c.slices;
+  return (unsigned)(items < kCopyGroups ? items : kCopyGroups);
+}
+
+static int launched() {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? TKV_OK : (int)e;
+}
+
+}  // namespace tkv
+
+extern "C" int64_t tkv_copy_pages_work(int32_t n, int32_t src_pages, int32_t dst_pages) {
+  if (n < 0 || src_pages < 0 || dst_pages < 0) return -1;
+  return n <= tkv::kInlinePairs ? 0 : (int64_t)src_pages + dst_pages + 1 + 2 * (int64_t)n;
+}
+
+extern "C" int tkv_copy_pages(const tkv_copy_pages_args* a, tkv_stream_t stream) {
+  using namespace tkv;
+  if (!a || !a->src || !a->dst || a->n <= 0 || a->src_pages <= 0 || a->dst_pages <= 0) return TKV_EINVAL;
+  if (a->same && a->src_pages != a->dst_pages) return TKV_EINVAL;
+  CopyPlan c;
+  const int rc = make_plan(a->set, c);
+  if (rc) return rc;
+  if (!c.slices) return TKV_OK;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  (void)hipGetLastError();
+  const dim3 grid(copy_groups(a->n, c));
+  if (a->n <= kInlinePairs) {
+    copy_few_kernel<<<grid, dim3(256), 0, st>>>(c, *a);
+  } else {
+    if (!a->work || (uintptr_t)a->work & 7) return TKV_EINVAL;
+    const int pages = a->dst_pages + a->src_pages;
+    const int2* pairs = reinterpret_cast<const int2*>(a->work + pages + (pages & 1));
+    copy_check_kernel<<<dim3(1), dim3(kPlan), 0, st>>>(*a);
+    copy_pairs_kernel<<<grid, dim3(256), 0, st>>>(c, pairs, nullptr, a->n);
+  }
+  return launched();
+}
+
+extern "C" int64_t tkv_fork_rows_work(int32_t B, int32_t max_pages, int32_t num_pages, int32_t parents) {
+  if (B <= 0 || max_pages <= 0 || num_pages <= 0) return -1;
+  return tkv::rows_work_ints(B, max_pages, num_pages, parents != 0);
+}
+
+extern "C" int tkv_fork_rows(const tkv_fork_rows_args* a, tkv_stream_t stream) {
+  using namespace tkv;
+  if (!a || !a->block_table || !a->seq_lens || !a->refs || !a->status || !a->work || (uintptr_t)a->work & 7)
+    return TKV_EINVAL;
+  if (a->B <= 0 || a->max_pages <= 0 || a->num_pages <= 0 || a->page_size <= 0 || a->table_stride < a->max_pages)
+    return TKV_EINVAL;
+  if (a->B > kMaxRows) return TKV_EUNSUPPORTED;
+  if ((int64_t)a->max_pages * a->page_size > INT32_MAX || (int64_t)a->B * a->max_pages > INT32_MAX) return TKV_EINVAL;
+  CopyPlan c;
+  const int rc = make_plan(a->set, c);
+  if (rc) return rc;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  (void)hipGetLastError();
+  const int64_t entries = (int64_t)a->B * a->max_pages;
+  const unsigned staging = a->parents ? (unsigned)((entries + 4 * kPlan - 1) / (4 * kPlan)) : 0;
+  rows_plan_kernel<<<dim3(1 + (staging < 512 ? staging : 512)), dim3(kPlan), 2 * sizeof(int) * a->B, st>>>(*a);
+  const int64_t tables = (entries + 255) / 256;
+  const int t = (int)(tables < 2048 ? tables : 2048);
+  rows_apply_kernel<<<dim3(t + copy_groups(a->B, c)), dim3(256), 0, st>>>(*a, c, t);
+  return launched();
+}
+
+extern "C" int64_t tkv_compact_pages_work(int32_t num_pages) {
+  return num_pages <= 0 ? -1 : tkv::compact_work_ints(num_pages);
+}
+
+extern "C" int tkv_compact_pages(const tkv_compact_pages_args* a, tkv_stream_t stream) {
+  using namespace tkv;
+  if (!a || !a->block_table || !a->refs || !a->out_table || !a->out_refs || !a->work || (uintptr_t)a->work & 7)
+    return TKV_EINVAL;
+  if (a->B <= 0 || a->max_pages <= 0 || a->num_pages <= 0 || a->table_stride < a->max_pages ||
+      a->out_stride < a->max_pages)
+    return TKV_EINVAL;
+  CopyPlan c;
+  const int rc = make_plan(a->set, c);
+  if (rc) return rc;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  (void)hipGetLastError();
+  compact_plan_kernel<<<dim3(1), dim3(kPlan), 0, st>>>(*a);
+  const int64_t tables = ((int64_t)a->B * a->max_pages + a->num_pages + 255) / 256;
+  const int t = (int)(tables < 2048 ? tables : 2048);
+  compact_apply_kernel<<<dim3(t + copy_groups(a->num_pages / 2, c)), dim3(256), 0, st>>>(*a, c, t);
+  return launched();
+}
+
+// The copies of a plan in further tensors: pairs and their count as the plan left them.
+extern "C" int tkv_copy_planned(const tkv_page_set* set, const int32_t* work, int32_t most, tkv_stream_t stream) {
+  using namespace tkv;
+  if (!set || !work || (uintptr_t)work & 7 || most < 0) return TKV_EINVAL;
+  CopyPlan c;
+  const int rc = make_plan(*set, c);
+  if (rc) return rc;
+  const unsigned groups = copy_groups(most, c);
+  if (!groups) return TKV_OK;
+  (void)hipGetLastError();
+  copy_pairs_kernel<<<dim3(groups), dim3(256), 0, reinterpret_cast<hipStream_t>(stream)>>>(
+      c, reinterpret_cast<const int2*>(work + 16), work + 1, 0);
+  return launched();
+}

@@ -1,0 +1,349 @@
+"""Pages of a cache on the device: copied, forked, handed out, taken back, compacted.
+
+A paged cache is page pools (of any layer, K and V; 2/4-bit
+:class:`~tritonkv_amd.quantize.QuantizedTensor` pools of
+:mod:`tritonkv_amd.paged` or 16-bit tensors of :mod:`tritonkv_amd.paged16`)
+that share page numbers, and three int32 tensors that say which row owns what:
+
+* ``block_table`` ``(B, max_pages)``: row b's pages in order, -1 after them;
+* ``seq_lens`` ``(B,)``: its tokens; it uses ``ceil(seq_lens[b] / page_size)`` pages;
+* ``refs`` ``(num_pages,)``: how many used table entries name each page, 0 for
+  a free one.  (A caller may add counts of its own to keep pages alive.)
+
+An empty cache is a table of -1 and two tensors of zeros.  From there
+:func:`resize_rows` makes room, truncates and frees, :func:`fork_rows` makes
+rows out of other rows (parallel samples, beams, a shared prefix), sharing
+their full pages, and :func:`compact_pages` moves the live pages to the low end
+of the pools.  A page that is not full belongs to one row alone, so the appends
+(:func:`~tritonkv_amd.paged.paged_append`, ``paged16_append`` and the decodes'
+fused ones) never write into another row's tokens.
+
+Everything runs on the current stream, in two launches, from device tensors
+alone: nothing is copied to the host and no call synchronises.  Calls that may
+overlap in time must not share a ``_workspace``.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .paged16 import _buffer, _int32_arg, _keep16, _offset
+from .kernels.fused_decode_attn import _prepared
+from .quantize import QuantizedTensor, _require_gpu
+
+MAX_ROWS = 8192
+
+
+def _tensors(pools) -> list:
+    """The page tensors of pools, in order."""
+    if isinstance(pools, (QuantizedTensor, torch.Tensor)):
+        raise TypeError("pools must be a list or tuple of page pools")
+    found = []
+    for p in pools:
+        if isinstance(p, QuantizedTensor):
+            found += [p.packed, p.scale, p.zero]
+        elif isinstance(p, torch.Tensor):
+            found.append(p)
+        else:
+            raise TypeError(f"a page pool is a QuantizedTensor or a tensor, got {type(p).__name__}")
+    return found
+
+
+def _page_size(pools) -> int:
+    sizes = {(p.packed if isinstance(p, QuantizedTensor) else p).shape[2] for p in pools
+             if (p.packed if isinstance(p, QuantizedTensor) else p).dim() == 4}
+    if len(sizes) != 1:
+        raise ValueError(f"the pools must be (num_pages, HKV, page_size, ...) of one page_size, got {sorted(sizes)}")
+    return sizes.pop()
+
+
+def _check_pages(tensors: list, num_pages: int | None, device, what: str) -> list:
+    """``(address, page stride in bytes, bytes of a page)`` of every page tensor."""
+    found = []
+    for t in tensors:
+        if t.dim() != 4 or t.numel() == 0 or (num_pages is not None and t.shape[0] != num_pages):
+            raise ValueError(f"{what} must hold (num_pages, HKV, page_size, ...) tensors"
+                             + ("" if num_pages is None else f" of {num_pages} pages") + f", got {tuple(t.shape)}")
+        if t.device != device:
+            raise ValueError(f"{what} must be on {device}, got a tensor on {t.device}")
+        dense = 1  # a page is one block of memory, in whatever order of its axes
+        for stride, n in sorted((s, n) for s, n in zip(t.stride()[1:], t.shape[1:]) if n > 1):
+            if stride != dense:
+                raise ValueError(f"{what}: a page must be one dense block, got strides {tuple(t.stride())}")
+            dense *= n
+        size = dense * t.element_size()
+        stride = t.stride(0) * t.element_size() if t.shape[0] > 1 else size
+        if stride < size:
+            raise ValueError(f"{what}: pages overlap, got strides {tuple(t.stride())}")
+        if size % 16 or stride % 16 or t.data_ptr() % 16:
+            raise ValueError(f"{what}: pages must start on 16 bytes and be a multiple of them, got {size} bytes "
+                             f"every {stride}")
+        found.append((t.data_ptr(), stride, size))
+    return found
+
+
+def _page_sets(src: list, dst: list) -> list:
+    """The tensors as sets of at most ``PAGE_TENSORS``; one empty set without any."""
+    n = _lib.PAGE_TENSORS
+    sets = []
+    for i in range(0, max(1, len(src)), n):
+        s, d = src[i:i + n], dst[i:i + n]
+        sets.append(_lib.PageSet(src=tuple(x[0] for x in s), dst=tuple(x[0] for x in d),
+                                 src_stride=tuple(x[1] for x in s), dst_stride=tuple(x[1] for x in d),
+                                 bytes=tuple(x[2] for x in s), count=len(s)))
+    return sets
+
+
+def _work(ws: dict | None, name: str, n: int, device) -> torch.Tensor:
+    return _buffer({} if ws is None else ws, name, n, torch.int32, device)
+
+
+def _check_rows(block_table, refs) -> tuple:
+    """B and max_pages of a table that is written in place, and the pages of refs."""
+    if not isinstance(refs, torch.Tensor) or refs.dtype != torch.int32 or refs.dim() != 1 or refs.numel() == 0 \
+            or not refs.is_contiguous():
+        raise ValueError("refs must be a contiguous int32 (num_pages,) tensor")
+    if not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32 or block_table.dim() != 2 \
+            or block_table.numel() == 0 or block_table.device != refs.device or _row_stride(block_table) is None:
+        raise ValueError("block_table must be an int32 (B, max_pages) tensor with dense rows on refs' device")
+    return block_table.shape
+
+
+def _row_stride(t: torch.Tensor) -> int | None:
+    """Entries between the rows of a table, None if its rows are not dense or overlap."""
+    B, P = t.shape
+    if P > 1 and t.stride(1) != 1:
+        return None
+    stride = t.stride(0) if B > 1 else P
+    return stride if stride >= P else None
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.untyped_storage().data_ptr() == b.untyped_storage().data_ptr()
+
+
+_C = {f: _offset(_lib.CopyPagesArgs, f) for f in ("src", "dst")}
+_F = {f: _offset(_lib.ForkRowsArgs, f) for f in ("parents", "new_lens", "status")}
+_P = {f: _offset(_lib.CompactPagesArgs, f) for f in ("live",)}
+
+
+def copy_pages(pools, src: torch.Tensor, dst: torch.Tensor, dst_pools=None, _workspace: dict | None = None) -> None:
+    """Page ``dst[i]`` := page ``src[i]`` in every one of ``pools``, for all pairs of one call.
+
+    pools: a list of page pools that share page numbers; ``src`` and ``dst``:
+    int32 ``(n,)`` tensors on their device.  With ``dst_pools``, a list of
+    pools of the same pages in other memory, pages go from ``pools`` to
+    those.  A pair with a number outside the pools is skipped (-1 marks one
+    that is not wanted).  Of several pairs with one destination the first is
+    carried out.  Within one set of pools a page that the call reads is
+    never written: a pair whose destination is a pair's source is skipped.
+    """
+    tensors = _tensors(pools)
+    others = None if dst_pools is None else _tensors(dst_pools)
+    key = None
+    if _workspace is not None:
+        key = ("copy_pages", len(tensors), others is None)
+        prep = _prepared(_workspace, key)
+        if prep is not None and prep.run(src, dst, *tensors, *(others or ())):
+            return
+    if not tensors:
+        raise ValueError("pools is empty")
+    device = tensors[0].device
+    from_ = _check_pages(tensors, tensors[0].shape[0], device, "pools")
+    to = from_
+    src_pages = dst_pages = tensors[0].shape[0]
+    if others is not None:
+        if len(others) != len(tensors):
+            raise ValueError(f"dst_pools must hold as many tensors as pools: {len(others)} and {len(tensors)}")
+        dst_pages = others[0].shape[0] if others[0].dim() else 0
+        to = _check_pages(others, dst_pages, device, "dst_pools")
+        for a, b in zip(tensors, others):
+            order = [sorted(range(1, 4), key=lambda i: (t.stride(i), t.shape[i])) for t in (a, b)]
+            if a.shape[1:] != b.shape[1:] or a.dtype != b.dtype or order[0] != order[1]:
+                raise ValueError(f"dst_pools must have pools' page shapes, order and dtypes: {tuple(a.shape)} "
+                                 f"{a.dtype} and {tuple(b.shape)} {b.dtype}")
+        if any(_overlap(a, b) for a in tensors for b in others):
+            raise ValueError("dst_pools must not share memory with pools")
+    if not isinstance(src, torch.Tensor):
+        raise ValueError("src must be an int32 tensor of page numbers")
+    n = src.numel()
+    s, d = (_int32_arg(x, n, device, name, "page numbers, as many as the other")
+            for name, x in (("src", src), ("dst", dst)))
+    _require_gpu(tensors[0], "copy_pages")
+    if n == 0:
+        return
+    words = _lib.load().tkv_copy_pages_work(n, src_pages, dst_pages)
+    work = _work(_workspace, "copy_pages", words, device) if words else None
+    sets = _page_sets(from_, to)
+    for one in sets:
+        args = _lib.CopyPagesArgs(set=one, src=s.data_ptr(), dst=d.data_ptr(), work=_lib.ptr(work), n=n,
+                                  src_pages=src_pages, dst_pages=dst_pages, same=int(others is None))
+        _lib.check(_lib.launch(device, "tkv_copy_pages", args), "copy_pages")
+    if key is not None and len(sets) == 1:
+        _keep16(_workspace, key, args, "tkv_copy_pages", "copy_pages", device, (work,),
+                ((src, _C["src"], 4), (dst, _C["dst"], 4),
+                 *((t, -1, 16, 1) for t in (*tensors, *(others or ())))))
+
+
+def fork_rows(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor,
+              parents: torch.Tensor | None, new_lens: torch.Tensor | None = None,
+              status: torch.Tensor | None = None, _workspace: dict | None = None) -> torch.Tensor:
+    """Make every row of a block table out of an old row, in place.
+
+    Row b becomes the first ``min(new_lens[b], seq_lens[a])`` tokens of old
+    row ``a = parents[b]``, with pages for ``new_lens[b]`` tokens;
+    ``new_lens=None`` keeps ``a``'s length, ``parents=None`` every row's own
+    tokens, and a parent outside ``[0, B)`` (say -1) empties the row.  So
+
+    * ``parents = arange(B)`` with some entries changed forks rows into empty
+      or finished ones, a beam search's choice of beams reorders them;
+    * a smaller ``new_lens`` truncates, 0 or a parent of -1 frees;
+    * a larger one makes room: tokens from the old length on are whatever the
+      new pages hold until they are written.
+
+    Full pages are shared (``refs`` counts the rows).  The page that a row ends
+    in, if not full, stays with one row -- the parent itself, else its first
+    child -- if no other row keeps it, and is copied for every other one, in
+    all of ``pools``, by the same launch that rewrites the table.  New pages are
+    the lowest that were free before the call, in row order, whatever runs
+    in parallel.  At most 8192 rows.
+
+    Returns ``status``, an int32 ``(1,)`` tensor: 0, or 1 where the free
+    pages, or 2 where a row's table entries, do not suffice; then nothing was
+    changed.  It is on the device, so reading it is what waits for the call.
+    """
+    tensors = _tensors(pools)
+    key = None
+    if _workspace is not None:
+        key = ("fork_rows", len(tensors))
+        prep = _prepared(_workspace, key)
+        if prep is not None:
+            got = status
+            if got is None and isinstance(refs, torch.Tensor):
+                got = torch.empty(1, dtype=torch.int32, device=refs.device)
+            if prep.run(block_table, seq_lens, refs, parents, new_lens, got, *tensors):
+                return got
+    B, max_pages = _check_rows(block_table, refs)
+    device, num_pages = refs.device, refs.numel()
+    if B > MAX_ROWS:
+        raise ValueError(f"at most {MAX_ROWS} rows, got {B}")
+    if not tensors:
+        raise ValueError("pools is empty")
+    pages = _check_pages(tensors, num_pages, device, "pools")
+    page_size = _page_size(pools)
+    if max_pages * page_size > 2 ** 31 - 1:
+        raise ValueError(f"{max_pages} pages of {page_size} tokens a row: at most 2**31 - 1 tokens")
+    if not isinstance(seq_lens, torch.Tensor) or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be a contiguous int32 tensor of B lengths: it is written in place")
+    _int32_arg(seq_lens, B, device, "seq_lens", "B lengths")
+    par = None if parents is None else _int32_arg(parents, B, device, "parents", "B rows")
+    new = None if new_lens is None else _int32_arg(new_lens, B, device, "new_lens", "B lengths")
+    written = [block_table, seq_lens, refs]
+    if status is None:
+        status_given = torch.empty(1, dtype=torch.int32, device=device)
+    else:
+        status_given = _int32_arg(status, 1, device, "status", "one entry")
+        written.append(status)
+    for i, a in enumerate(written):
+        if any(_overlap(a, b) for b in written[i + 1:] + [x for x in (parents, new_lens) if x is not None]):
+            raise ValueError("block_table, seq_lens, refs and status are written: they must not share memory "
+                             "with each other, parents or new_lens")
+    _require_gpu(refs, "fork_rows")
+    words = _lib.load().tkv_fork_rows_work(B, max_pages, num_pages, int(par is not None))
+    work = _work(_workspace, "fork_rows", words, device)
+    sets = _page_sets(pages, pages)
+    args = _lib.ForkRowsArgs(
+        set=sets[0], block_table=block_table.data_ptr(), seq_lens=seq_lens.data_ptr(), refs=refs.data_ptr(),
+        parents=_lib.ptr(par), new_lens=_lib.ptr(new), status=status_given.data_ptr(), work=work.data_ptr(),
+        table_stride=_row_stride(block_table), B=B, max_pages=max_pages, page_size=page_size, num_pages=num_pages)
+    _lib.check(_lib.launch(device, "tkv_fork_rows", args), "fork_rows")
+    for one in sets[1:]:
+        _lib.check(_lib.launch(device, "tkv_copy_planned", one, work.data_ptr(), B), "fork_rows")
+    if key is not None and len(sets) == 1:
+        _keep16(_workspace, key, args, "tkv_fork_rows", "fork_rows", device, (work,),
+                ((block_table, -1, 4, 1), (seq_lens, -1, 4), (refs, -1, 4), (parents, _F["parents"], 4),
+                 (new_lens, _F["new_lens"], 4), (status_given, _F["status"], 4),
+                 *((t, -1, 16, 1) for t in tensors)))
+    return status_given
+
+
+def resize_rows(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor,
+                new_lens: torch.Tensor, status: torch.Tensor | None = None,
+                _workspace: dict | None = None) -> torch.Tensor:
+    """Give every row ``new_lens[b]`` tokens: :func:`fork_rows` with every row its own parent.
+
+    Rows that grow get pages, rows that shrink return theirs, a length of 0
+    frees the row.  A row cut inside a page that it shares gets its own
+    copy of that page.
+    """
+    if new_lens is None:
+        raise ValueError("new_lens must be an int32 tensor of B lengths")
+    return fork_rows(pools, block_table, seq_lens, refs, None, new_lens, status, _workspace)
+
+
+def compact_pages(pools, block_table: torch.Tensor, refs: torch.Tensor, out=None,
+                  live: torch.Tensor | None = None, _workspace: dict | None = None) -> tuple:
+    """Move the live pages (``refs > 0``) to the low end of the pools.
+
+    With n of them, the i-th live page at or past n is copied to the i-th free
+    page below n in every one of ``pools``; afterwards pages n and up are free,
+    and the pools' tails may be given back or lent out.  Returns
+    ``(block_table, refs, live)`` with the new numbers and counts, ``live`` an
+    int32 ``(1,)`` tensor holding n.  ``out``: a table and counts to write
+    instead of the given ones, which then stay valid, as do the pages they
+    name, until something is written to the pools: readers may go on with the
+    old table and be switched over later.
+    """
+    tensors = _tensors(pools)
+    out_table, out_refs = (block_table, refs) if out is None else out
+    key = None
+    if _workspace is not None:
+        key = ("compact_pages", len(tensors))
+        prep = _prepared(_workspace, key)
+        if prep is not None:
+            got = live
+            if got is None and isinstance(refs, torch.Tensor):
+                got = torch.empty(1, dtype=torch.int32, device=refs.device)
+            if prep.run(block_table, refs, out_table, out_refs, got, *tensors):
+                return out_table, out_refs, got
+    B, max_pages = _check_rows(block_table, refs)
+    device, num_pages = refs.device, refs.numel()
+    if out is not None:
+        _check_rows(out_table, out_refs)
+        if out_table.shape != block_table.shape or out_refs.shape != refs.shape or out_refs.device != device:
+            raise ValueError("out must be a table and counts of the given ones' shapes on their device")
+        if _overlap(out_table, block_table) or _overlap(out_refs, refs) or _overlap(out_table, refs) \
+                or _overlap(out_refs, block_table):
+            raise ValueError("out must not share memory with block_table or refs")
+    if _overlap(out_table, out_refs):
+        raise ValueError("block_table and refs must not share memory")
+    if not tensors:
+        raise ValueError("pools is empty")
+    pages = _check_pages(tensors, num_pages, device, "pools")
+    if live is None:
+        live_given = torch.empty(1, dtype=torch.int32, device=device)
+    else:
+        live_given = _int32_arg(live, 1, device, "live", "one entry")
+        if any(_overlap(live, t) for t in (block_table, refs, out_table, out_refs)):
+            raise ValueError("live must not share memory with the tables or counts")
+    _require_gpu(refs, "compact_pages")
+    words = _lib.load().tkv_compact_pages_work(num_pages)
+    work = _work(_workspace, "compact_pages", words, device)
+    sets = _page_sets(pages, pages)
+    args = _lib.CompactPagesArgs(
+        set=sets[0], block_table=block_table.data_ptr(), refs=refs.data_ptr(), out_table=out_table.data_ptr(),
+        out_refs=out_refs.data_ptr(), live=live_given.data_ptr(), work=work.data_ptr(),
+        table_stride=_row_stride(block_table), out_stride=_row_stride(out_table), B=B, max_pages=max_pages,
+        num_pages=num_pages)
+    _lib.check(_lib.launch(device, "tkv_compact_pages", args), "compact_pages")
+    for one in sets[1:]:
+        _lib.check(_lib.launch(device, "tkv_copy_planned", one, work.data_ptr(), num_pages // 2), "compact_pages")
+    if key is not None and len(sets) == 1:
+        _keep16(_workspace, key, args, "tkv_compact_pages", "compact_pages", device, (work,),
+                ((block_table, -1, 4, 1), (refs, -1, 4), (out_table, -1, 4, 1), (out_refs, -1, 4),
+                 (live_given, _P["live"], 4), *((t, -1, 16, 1) for t in tensors)))
+    return out_table, out_refs, live_given
+
+
+__all__ = ["MAX_ROWS", "copy_pages", "fork_rows", "resize_rows", "compact_pages"]
