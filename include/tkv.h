@@ -339,13 +339,14 @@ int tkv_dequantize(const uint8_t *packed, const uint16_t *scale, const uint16_t 
  *              the token at L_b - 1 of every row, attended to and put into its
  *              page by this call (not stored where the table entry lies outside
  *              [0, num_pages); rows of no tokens take none)
- * The rows' tokens are cut on the device, from their lengths: a piece holds at
- * most max(least_chunks, ceil(sum_b ceil(L_b / 32) / target_pieces)) chunks of
- * 32 tokens.  target_pieces == 0 keeps every row whole in one launch; otherwise
- * a second launch joins the pieces, partials holds max_pieces * HQ * (D + 2)
- * floats (16-byte aligned), row_pieces 2 * B int32 (8-byte aligned), and
- * max_pieces is at least target_pieces + B (at most 65535).  waves: 4 or 8 per
- * workgroup (0: 4).  No counterpart in the reference (its caches are contiguous). */
+ * The rows are cut on the device, from their lengths: their chunks of 32 tokens
+ * (an empty row counts as one), laid end to end, are shared out evenly over at
+ * most `workgroups` workgroups (1 to 65535) per KV head and 16 query heads, of at
+ * least least_chunks chunks each, and a second launch joins the rows that were
+ * cut: partials holds 2 * workgroups * HQ * (D + 2) floats (16-byte aligned),
+ * row_pieces 2 * B int32 (8-byte aligned).  workgroups == 0 keeps every row
+ * whole, in one launch (at most 65535 rows).  waves: 4 or 8 per workgroup
+ * (0: 4).  No counterpart in the reference (its caches are contiguous). */
 typedef struct tkv_paged16_args {
   const void *q;
   int64_t q_strides[2];
@@ -359,7 +360,7 @@ typedef struct tkv_paged16_args {
   int32_t is_bf16, B, HQ, HKV, D;
   int32_t block_table_stride, max_pages, page_size, num_pages;
   float sm_scale;
-  int32_t least_chunks, target_pieces, max_pieces, waves;
+  int32_t least_chunks, workgroups, waves;
 } tkv_paged16_args;
 int tkv_paged16_decode_attention(const tkv_paged16_args *args, tkv_stream_t stream);
 

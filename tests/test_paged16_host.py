@@ -108,32 +108,40 @@ def test_append_refuses(kw, error, match):
 @pytest.mark.parametrize("B", [1, 7, 256, 60000])
 @pytest.mark.parametrize("HKV,G", [(1, 1), (8, 4), (2, 40)])
 @pytest.mark.parametrize("S", [16, 512, 4096, 1 << 20])
-def test_the_plan_has_room_for_every_piece(B, HKV, G, S):
-    """Whatever the lengths, sum_b n_b <= max_pieces (the device's arithmetic, restated)."""
+def test_the_shares_cover_every_chunk_once(B, HKV, G, S):
+    """Whatever the lengths: shares follow each other, none is empty, and the share that a
+    chunk is looked up in holds it (the device's arithmetic, restated)."""
     import random
 
-    from tritonkv_amd.paged16 import MAX_PIECES, plan_pieces
+    from tritonkv_amd.paged16 import MAX_WORKGROUPS, plan_shares
 
     rng = random.Random(B * S)
     for piece in (None, 48, S):
         try:
-            least, target, most = plan_pieces(B, HKV, G, S, "cpu", piece)
+            least, groups = plan_shares(B, HKV, G, S, "cpu", piece)
         except ValueError:
-            assert piece is not None and B * -(-S // piece) > MAX_PIECES - 2 * B
+            assert piece is not None and -(-B * -(-S // 32) // -(-piece // 32)) > MAX_WORKGROUPS
             continue
-        assert B <= most <= MAX_PIECES and least > 0 and (target == 0 or target + B <= most)
-        if target == 0:
+        assert 0 <= groups <= MAX_WORKGROUPS and least > 0
+        if groups == 0:
+            assert S <= 32 * least
             continue
         for lens in ([S] * B, [0] * B, [S] + [0] * (B - 1), [rng.randint(0, S) for _ in range(B)]):
-            chunks = [-(-n // 32) for n in lens]
-            c = max(least, -(-sum(chunks) // target))
-            pieces = 0
-            for l in chunks:
-                n = -(-l // c) if l > c else 1
-                each = -(-l // n)
-                pieces += -(-l // each) if l > c else 1
-                assert each <= c
-            assert pieces <= most
+            total = sum(max(1, -(-n // 32)) for n in lens)
+            W = min(groups, -(-total // least))
+            each, more = divmod(total, W)
+            assert each > 0
+
+            def start(i):
+                return i * each + min(i, more)
+
+            def of(chunk):
+                big = more * (each + 1)
+                return chunk // (each + 1) if chunk < big else more + (chunk - big) // each
+
+            assert start(0) == 0 and start(W) == total
+            for i in rng.sample(range(W), min(W, 50)):
+                assert of(start(i)) == of(start(i + 1) - 1) == i
 
 
 def test_argument_blocks_match_the_header():
@@ -158,15 +166,15 @@ def _decode_args():
     return _lib.Paged16Args(q=d, q_strides=(1024, 128), k=d, v=d, k_strides=(8192, 4096, 128),
                             v_strides=(8192, 4096, 128), block_table=d, out=d, partials=d, row_pieces=d, B=2,
                             HQ=8, HKV=2, D=128, block_table_stride=4, max_pages=4, page_size=32, num_pages=4,
-                            sm_scale=0.1, least_chunks=2, target_pieces=4, max_pieces=6, waves=4)
+                            sm_scale=0.1, least_chunks=2, workgroups=4, waves=4)
 
 
 @pytest.mark.parametrize("field,value", [
     ("q", None), ("q", 0x1008), ("k", None), ("v", 0x1008), ("out", 0x1004), ("block_table", None),
     ("partials", None), ("partials", 0x1008), ("row_pieces", 0x1004), ("k_new", 0x1000), ("B", 0), ("HQ", 7),
     ("HKV", 0), ("page_size", 24), ("page_size", 0), ("max_pages", 0), ("num_pages", 0),
-    ("block_table_stride", 3), ("max_pages", 1 << 27), ("least_chunks", 0), ("target_pieces", -1),
-    ("max_pieces", 5), ("max_pieces", 65536), ("waves", 5), ("k_strides", (8192, 4096, 132)),
+    ("block_table_stride", 3), ("max_pages", 1 << 27), ("least_chunks", 0), ("workgroups", -1),
+    ("workgroups", 65536), ("waves", 5), ("k_strides", (8192, 4096, 132)),
     ("v_strides", (8192, 4096, 0)), ("k_strides", (8192, 4096, 1 << 26)), ("k_strides", (-8, 4096, 128)),
     ("q_strides", (1024, 4))])
 def test_c_entry_refuses(field, value):

@@ -103,8 +103,7 @@ class Paged16Args(ctypes.Structure):
         ("num_pages", ctypes.c_int32),
         ("sm_scale", ctypes.c_float),
         ("least_chunks", ctypes.c_int32),
-        ("target_pieces", ctypes.c_int32),
-        ("max_pieces", ctypes.c_int32),
+        ("workgroups", ctypes.c_int32),
         ("waves", ctypes.c_int32),
     ]
 

@@ -63,118 +63,161 @@ struct Bf16 {
 };
 
 // ---------------------------------------------------------------------------
-// The plan of the pieces, made on the device from the rows' lengths.
+// The split, made on the device from the rows' lengths.
 //
 // A serving loop's table is as wide as its longest request may get, and the
 // lengths live on the device, so a split of the table's capacity would leave
-// most pieces empty.  Instead every workgroup derives the same plan from the
-// lengths: with l_b = ceil(L_b / 32) chunks, a piece holds at most
-//   c = max(least, ceil(sum_b l_b / target))
-// chunks, row b is cut evenly into n_b = ceil(l_b / c) pieces (an empty row
-// keeps one, which writes its zeros), and workgroup `slot` takes the slot-th
-// piece in row order: sum_b n_b <= target + B pieces.  target == 0: one piece
-// per row.
+// most pieces empty and the others uneven.  Instead the rows' chunks (32 tokens;
+// an empty row counts as one, which writes its zeros) are laid end to end, and the
+// W = min(workgroups, ceil(chunks / least_chunks)) workgroups of a KV head
+// take equal shares of that line: workgroup i the chunks from share_start(i) on.
+// A share covers the end of one row, whole rows, and the start of another; each
+// such segment is attended by itself.  Whole rows are written out; the others
+// leave a partial in slot 2i (the row began in an earlier share) or 2i + 1, and
+// the join kernel merges a row's partials, which lie in consecutive shares.
+// workgroups == 0: one workgroup per row.
+//
+// Measured on 32 rows of 200-16184 tokens (HKV 8, D 128): pieces of one row each,
+// cut evenly, 184-194 us; shares 172 us, as fast as 32 equal rows of that sum.
 // ---------------------------------------------------------------------------
 struct Paged16Params {
   tkv_paged16_args a;
   int G, page_tiles, S;
   float qk_scale;  // sm_scale * log2(e)
-};
-
-struct Piece {
-  int b, L, lo, hi;   // tokens [lo, hi) of row b, which holds L
-  int base, count;    // the row's first piece and how many it has
-  bool live;
+  uint32_t k16[3], v16[3];  // the pools' strides in 16 bytes: products of 32 bits by 32
 };
 
 __device__ __forceinline__ int clamp_len(int L, int S) { return max(0, min(L, S)); }
+__device__ __forceinline__ uint32_t chunks_of(int L) { return max(1u, ((uint32_t)L + 31) / 32); }
 
-// Pieces of a row of l chunks, and how many chunks each holds.
-__device__ __forceinline__ void cut_row(uint32_t l, uint32_t c, uint32_t& count, uint32_t& chunks) {
-  if (l <= c) {
-    count = 1;
-    chunks = l;
-  } else {
-    const uint32_t n = (l + c - 1) / c;
-    chunks = (l + n - 1) / n;
-    count = (l + chunks - 1) / chunks;
-  }
+// Inclusive sum over the wave's lanes, on the VALU: four shifts within rows of 16
+// lanes, then the rows' totals passed on.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t add_dpp(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = add_dpp<0x111, 0xF>(v);  // row_shr:1
+  v = add_dpp<0x112, 0xF>(v);
+  v = add_dpp<0x114, 0xF>(v);
+  v = add_dpp<0x118, 0xF>(v);
+  v = add_dpp<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  return add_dpp<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
 }
 
-__device__ __forceinline__ Piece find_piece(const Paged16Params& prm, int slot) {
-  const int32_t* __restrict__ lens = prm.a.seq_lens;
-  const int B = prm.a.B, S = prm.S, lane = threadIdx.x & 63;
-  const uint32_t least = prm.a.least_chunks, target = prm.a.target_pieces;
-  Piece p;
-  uint32_t count, chunks, s;
-  if (target == 0) {  // one piece per row
-    p.live = slot < B;
-    if (!p.live) return p;
-    p.b = slot;
-    p.L = lens ? clamp_len(__builtin_amdgcn_readfirstlane(lens[slot]), S) : S;
-    p.base = slot;
-    count = 1;
-    chunks = ((uint32_t)p.L + 31) / 32;
-    s = 0;
-  } else if (!lens || B == 1) {  // every row alike
-    p.L = lens ? clamp_len(__builtin_amdgcn_readfirstlane(lens[0]), S) : S;
-    const uint32_t l = ((uint32_t)p.L + 31) / 32;
-    const uint32_t c = max(least, (l * B + target - 1) / target);
-    cut_row(l, c, count, chunks);
-    p.b = (uint32_t)slot / count;
-    p.live = p.b < B;
-    if (!p.live) return p;
-    p.base = p.b * count;
-    s = slot - p.base;
-  } else {
-    uint32_t sum = 0;
-    for (int b0 = 0; b0 < B; b0 += 64)
-      if (b0 + lane < B) sum += ((uint32_t)clamp_len(lens[b0 + lane], S) + 31) / 32;
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) sum += __shfl_xor((int)sum, off, 64);
-    const uint32_t c = max(least, (sum + target - 1) / target);
-    uint32_t before = 0;
-    p.live = false;
-    for (int b0 = 0; b0 < B; b0 += 64) {
-      const bool in = b0 + lane < B;
-      const int L = in ? clamp_len(lens[b0 + lane], S) : 0;
-      uint32_t n, m;
-      cut_row(((uint32_t)L + 31) / 32, c, n, m);
-      n = in ? n : 0;
-      uint32_t end = n;  // inclusive sum over the lanes
-#pragma unroll
-      for (int off = 1; off < 64; off *= 2) {
-        const uint32_t o = __shfl_up((int)end, off, 64);
-        end += lane >= off ? o : 0;
-      }
-      const uint64_t past = __builtin_amdgcn_ballot_w64(before + end > (uint32_t)slot);
-      if (past) {
-        const int at = __builtin_ctzll(past);
-        p.live = true;
-        p.b = b0 + at;
-        p.L = __builtin_amdgcn_readlane(L, at);
-        count = __builtin_amdgcn_readlane((int)n, at);
-        chunks = __builtin_amdgcn_readlane((int)m, at);
-        p.base = before + __builtin_amdgcn_readlane((int)end, at) - count;
-        s = slot - p.base;
-        break;
-      }
-      before += __builtin_amdgcn_readlane((int)end, 63);
+struct Shares {
+  uint32_t each, more;  // the first `more` shares hold each + 1 chunks
+  __device__ __forceinline__ uint32_t start(uint32_t i) const { return i * each + min(i, more); }
+  __device__ __forceinline__ uint32_t of(uint32_t chunk) const {
+    const uint32_t big = more * (each + 1);
+    return chunk < big ? chunk / (each + 1) : more + (chunk - big) / each;
+  }
+};
+
+// The rows' lengths, 64 of them in a wave's lanes at a time.
+struct RowLens {
+  const int32_t* lens;
+  int B, S, lane, first, L;
+  __device__ __forceinline__ void load(int b0) {
+    first = b0;
+    L = lens ? (b0 + lane < B ? clamp_len(lens[b0 + lane], S) : 0) : S;
+  }
+  __device__ __forceinline__ int of(int b) {  // b uniform
+    if (b >= first + 64) load(b);
+    return __builtin_amdgcn_readlane(L, b - first);
+  }
+};
+
+struct Segment {
+  int b, L;             // a row and its length
+  uint32_t begin, end;  // its chunks of this segment
+  uint32_t at;          // the row's first chunk on the line
+};
+
+// Chunks from which on every workgroup has its least (saturated).
+__device__ __forceinline__ uint32_t full_at(const tkv_paged16_args& a) {
+  const uint64_t n = (uint64_t)(uint32_t)a.workgroups * (uint32_t)a.least_chunks;
+  return n > 0xffffffffu ? 0xffffffffu : (uint32_t)n;
+}
+
+__device__ __forceinline__ Shares make_shares(uint32_t total, const tkv_paged16_args& a, uint32_t& W) {
+  W = a.workgroups;
+  if (total < full_at(a)) W = min(W, (total + a.least_chunks - 1) / (uint32_t)a.least_chunks);
+  Shares s;
+  s.each = total / W;
+  s.more = total - s.each * W;
+  return s;
+}
+
+// This workgroup's first segment and the end of its share; false: it has none.
+__device__ __forceinline__ bool first_segment(const Paged16Params& prm, int i, RowLens& rows, Shares& sh,
+                                              Segment& g, uint32_t& share_end) {
+  const int B = prm.a.B, lane = rows.lane;
+  if (prm.a.workgroups == 0) {
+    rows.load(i & ~63);
+    g.b = i;
+    g.L = rows.of(i);
+    g.begin = g.at = 0;
+    g.end = share_end = chunks_of(g.L);
+    sh.each = sh.more = 0;
+    return true;
+  }
+  rows.load(0);
+  uint32_t W;
+  if (!rows.lens || B == 1) {  // every row alike
+    const int L = rows.of(0);
+    const uint32_t l = chunks_of(L);
+    sh = make_shares(l * B, prm.a, W);
+    if ((uint32_t)i >= W) return false;
+    const uint32_t from = sh.start(i);
+    share_end = sh.start(i + 1);
+    g.b = from / l;
+    g.L = L;
+    g.at = g.b * l;
+    g.begin = from - g.at;
+    g.end = min(share_end - g.at, l);
+    return true;
+  }
+  // Up to 64 rows, which is most batches, one scan serves the sum and the search.
+  uint32_t l = lane < B ? chunks_of(rows.L) : 0, past = wave_scan(l);
+  uint32_t sum = __builtin_amdgcn_readlane((int)past, 63);
+  for (int b0 = 64; b0 < B; b0 += 64) {
+    rows.load(b0);
+    sum += __builtin_amdgcn_readlane((int)wave_scan(b0 + lane < B ? chunks_of(rows.L) : 0), 63);
+  }
+  sh = make_shares(sum, prm.a, W);
+  if ((uint32_t)i >= W) return false;
+  const uint32_t from = sh.start(i);
+  share_end = sh.start(i + 1);
+  uint32_t before = 0;
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    if (B > 64) {
+      rows.load(b0);
+      l = b0 + lane < B ? chunks_of(rows.L) : 0;
+      past = wave_scan(l);
     }
-    if (!p.live) return p;
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(before + past > from);
+    if (hit) {
+      const int at = __builtin_ctzll(hit);
+      const uint32_t n = __builtin_amdgcn_readlane((int)l, at);
+      g.b = b0 + at;
+      g.L = __builtin_amdgcn_readlane(rows.L, at);
+      g.at = before + __builtin_amdgcn_readlane((int)past, at) - n;
+      g.begin = from - g.at;
+      g.end = min(share_end - g.at, n);
+      return true;
+    }
+    before += __builtin_amdgcn_readlane((int)past, 63);
   }
-  p.count = count;
-  p.lo = (int)(32 * s * chunks);
-  p.hi = s + 1 == count ? p.L : (int)(32 * (s + 1) * chunks);
-  return p;
+  return false;  // not reached: from < sum
 }
 
-// Where the partial of head h of piece `slot` lives.
-__device__ __forceinline__ int64_t partial_row(const tkv_paged16_args& a, int slot, int h) {
+// Where the partial of head h in a slot lives; maxima and sums after all rows.
+__device__ __forceinline__ int64_t partial_row(const tkv_paged16_args& a, uint32_t slot, int h) {
   return (int64_t)slot * a.HQ + h;
 }
 __device__ __forceinline__ float* partial_ml(const tkv_paged16_args& a) {
-  return a.partials + (int64_t)a.max_pieces * a.HQ * a.D;
+  return a.partials + (int64_t)2 * a.workgroups * a.HQ * a.D;
 }
 
 __device__ __forceinline__ void store_row4(const tkv_paged16_args& a, float shift, int64_t row, int d, f4 o,
@@ -190,51 +233,58 @@ __device__ __forceinline__ void store_row4(const tkv_paged16_args& a, float shif
 // The split kernel.
 // ---------------------------------------------------------------------------
 template <class T, int D, int NW, bool APPEND>
-__global__ void __launch_bounds__(NW * 64) paged16_split_kernel(Paged16Params prm) {
+__global__ void __launch_bounds__(NW * 64, D == 256 ? 2 : D == 128 ? 3 : 4) paged16_split_kernel(Paged16Params prm) {
   constexpr int NKM = D / 32;  // 16x16x32 steps over the head dim
   constexpr int EPL = D / 16;  // V dims per lane (and V MFMAs)
   constexpr int VW = EPL / 2;  // dwords of them
   const tkv_paged16_args& a = prm.a;
-  extern __shared__ float lds[];  // per wave: rows of D + 1 floats, then max and sum of each row
-
-  const int slot = blockIdx.y;
-  const Piece pc = find_piece(prm, slot);
-  if (!pc.live) return;
-  const int hk = blockIdx.x % a.HKV, hb0 = (blockIdx.x / a.HKV) * 16;
-  const int nh = min(16, prm.G - hb0), h0 = hk * prm.G + hb0;
-  const int b = pc.b, lo = pc.lo, hi = pc.hi, last = hi - 1;
+  constexpr int QROW = D + 8;  // elements of a query row in LDS: 16 rows meet no bank twice
+  // The queries of the 16 heads, the new token's K and V rows (APPEND), then per wave
+  // of the merge: rows of D + 1 floats, maximum and sum of each.
+  extern __shared__ float lds_all[];
+  uint16_t* const lds_q = reinterpret_cast<uint16_t*>(lds_all);
+  uint16_t* const lds_new = lds_q + 16 * QROW;
+  float* const lds = lds_all + 8 * QROW + (APPEND ? D : 0);
 
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, j = lane >> 4;
-  // The row's last piece takes the new token in place of the page's row.
-  const bool app = APPEND && hi == pc.L && hi > lo;
+  RowLens rows{a.seq_lens, a.B, prm.S, lane, 0, 0};
+  Shares sh;
+  Segment g;
+  uint32_t share_end;
+  if (!first_segment(prm, blockIdx.y, rows, sh, g, share_end)) return;
+  const int hk = blockIdx.x % a.HKV, hb0 = (blockIdx.x / a.HKV) * 16;
+  const int nh = min(16, prm.G - hb0), h0 = hk * prm.G + hb0;
 
-  // Addresses.  Lane l looks up tile l % 2 of the wave's chunk l / 2: the
-  // table entries and 64-bit tile addresses of 32 chunks come from one load.
   const int64_t kts = a.k_strides[2], vts = a.v_strides[2];
-  uint64_t kt = 0, vt = 0;  // this lane's tile
-  auto tiles = [&](int c0) {
-    const int t = lo + 32 * (w + NW * (c0 + (lane >> 1))) + 16 * (lane & 1);
-    uint32_t page = 0, at = 0;  // past the piece: the pool's first tile, whose rows are masked
-    if (t < hi) {
-      const uint32_t t16 = (uint32_t)t / 16, pg = t16 / (uint32_t)prm.page_tiles;
-      at = 16 * (t16 - pg * prm.page_tiles);
-      page = min(max(a.block_table[(int64_t)b * a.block_table_stride + pg], 0), a.num_pages - 1);
-    }
-    kt = (uint64_t)a.k + 2 * (page * a.k_strides[0] + hk * a.k_strides[1] + at * kts);
-    vt = (uint64_t)a.v + 2 * (page * a.v_strides[0] + hk * a.v_strides[1] + at * vts);
-  };
-  auto lane_ptr = [&](uint64_t x, int l) {
-    const uint32_t x0 = __builtin_amdgcn_readlane((int)(uint32_t)x, l);
-    const uint32_t x1 = __builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), l);
-    return reinterpret_cast<const void*>(((uint64_t)x1 << 32) | x0);
-  };
   const uint32_t kspan = (uint32_t)(15 * kts + D) * 2, vspan = (uint32_t)(15 * vts + D) * 2;
   const uint32_t klane = (uint32_t)(r * kts + 8 * j) * 2;
   uint32_t vlane[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) vlane[i] = (uint32_t)((4 * j + i) * vts + EPL * r) * 2;
 
+  // Addresses.  Lane l looks up tile l % 2 of the wave's chunk l / 2: the
+  // table entries and 64-bit tile addresses of 32 chunks come from one load.
+  const uint64_t khead = (uint64_t)a.k + 16 * ((uint64_t)hk * prm.k16[1]);
+  const uint64_t vhead = (uint64_t)a.v + 16 * ((uint64_t)hk * prm.v16[1]);
+  uint64_t kt = 0, vt = 0;  // this lane's tile
+  int lo, hi;               // tokens of the segment
+  auto tiles = [&](int c0) {
+    const int t = lo + 32 * (w + NW * (c0 + (lane >> 1))) + 16 * (lane & 1);
+    uint32_t page = 0, at = 0;  // past the segment: the pool's first tile, whose rows are masked
+    if (t < hi) {
+      const uint32_t t16 = (uint32_t)t / 16, pg = t16 / (uint32_t)prm.page_tiles;
+      at = 16 * (t16 - pg * prm.page_tiles);
+      page = min(max(a.block_table[(int64_t)g.b * a.block_table_stride + pg], 0), a.num_pages - 1);
+    }
+    kt = khead + 16 * ((uint64_t)page * prm.k16[0] + (uint64_t)at * prm.k16[2]);
+    vt = vhead + 16 * ((uint64_t)page * prm.v16[0] + (uint64_t)at * prm.v16[2]);
+  };
+  auto lane_ptr = [&](uint64_t x, int l) {
+    const uint32_t x0 = __builtin_amdgcn_readlane((int)(uint32_t)x, l);
+    const uint32_t x1 = __builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), l);
+    return reinterpret_cast<const void*>(((uint64_t)x1 << 32) | x0);
+  };
   u4 kx[2][NKM];
   uint32_t vx[8][VW];
   auto load_k = [&](int c) {
@@ -267,208 +317,235 @@ __global__ void __launch_bounds__(NW * 64) paged16_split_kernel(Paged16Params pr
     }
   };
 
-  tiles(0);
-  const int cb0 = lo + 32 * w;
-  if (cb0 < hi) {
-    load_k(0);
-    load_v(0);
-  }
-
-  u4 knew[NKM];
-  uint32_t vnew[VW];
-  const bool owner = app && w == ((last - lo) / 32) % NW;
-  if (APPEND && owner) {
-    const uint16_t* kn = static_cast<const uint16_t*>(a.k_new) + b * a.k_new_strides[0] + hk * a.k_new_strides[1];
-    const uint16_t* vn = static_cast<const uint16_t*>(a.v_new) + b * a.v_new_strides[0] + hk * a.v_new_strides[1];
-#pragma unroll
-    for (int m = 0; m < NKM; ++m) knew[m] = *reinterpret_cast<const u4*>(kn + 32 * m + 8 * j);
-#pragma unroll
-    for (int e = 0; e < VW; e += 2) {
-      const u2 x = *reinterpret_cast<const u2*>(vn + EPL * r + 2 * e);
-      vnew[e] = x[0];
-      vnew[e + 1] = x[1];
+  bool app, owner;  // the segment takes the new token; in this wave
+  // Starts segment g: what its first chunk needs is on its way afterwards.
+  auto begin_segment = [&] {
+    const int bt = (int)opaque(tid), bl = bt & 63;
+    lo = 32 * (int)g.begin;
+    hi = min(g.L, 32 * (int)g.end);
+    app = APPEND && hi == g.L && hi > lo;
+    owner = app && w == ((hi - 1 - lo) / 32) % NW;
+    u4 new8 = {0u, 0u, 0u, 0u};  // lanes 0 .. D / 8 - 1: 8 dims of the new key; then of the value
+    const bool mine = APPEND && owner && bl < D / 4;
+    if (APPEND && mine) {
+      const bool isv = bl >= D / 8;
+      const int64_t* st = isv ? a.v_new_strides : a.k_new_strides;
+      new8 = *reinterpret_cast<const u4*>(static_cast<const uint16_t*>(isv ? a.v_new : a.k_new) + g.b * st[0] +
+                                          hk * st[1] + 8 * (bl & (D / 8 - 1)));
     }
-  }
-
-  u4 qf[NKM];
-  {
-    const bool hv = r < nh;
-    const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.q_strides[0] + (h0 + (hv ? r : 0)) * a.q_strides[1];
+    // The queries: 8 dims of a head per thread and round, zero past the group.  They and
+    // the new rows wait in LDS, which leaves the registers to K and V.
+    constexpr int QV = 16 * (D / 8), QR = (QV + NW * 64 - 1) / (NW * 64);
+    u4 q8[QR];
 #pragma unroll
-    for (int m = 0; m < NKM; ++m) {
-      const u4 x = *reinterpret_cast<const u4*>(q + 32 * m + 8 * j);
-      qf[m] = hv ? x : u4{0u, 0u, 0u, 0u};
+    for (int i = 0; i < QR; ++i) {
+      const int u = bt + NW * 64 * i, head = u / (D / 8);
+      q8[i] = u4{0u, 0u, 0u, 0u};
+      if (head < nh)
+        q8[i] = *reinterpret_cast<const u4*>(static_cast<const uint16_t*>(a.q) + g.b * a.q_strides[0] +
+                                             (h0 + head) * a.q_strides[1] + 8 * (u % (D / 8)));
     }
-  }
-
-  f4 accv[EPL];
+    tiles(0);
 #pragma unroll
-  for (int mv = 0; mv < EPL; ++mv) accv[mv] = f4{0.f, 0.f, 0.f, 0.f};
-  float m_run = -INFINITY, l_run = 0.0f;
-
-  auto step = [&](int c, int cb, auto tail) {
-    constexpr bool TAIL = decltype(tail)::value;
-    const bool more = cb + 32 * NW < hi;
-    if constexpr (TAIL && APPEND) {
-      if (owner && cb + 32 >= hi) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (cb + 16 * t + r == last)
-#pragma unroll
-            for (int m = 0; m < NKM; ++m) kx[t][m] = knew[m];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (cb + slot_token(j, i) == last)
-#pragma unroll
-            for (int e = 0; e < VW; ++e) vx[i][e] = vnew[e];
-      }
+    for (int i = 0; i < QR; ++i) {
+      const int u = bt + NW * 64 * i, head = u / (D / 8);
+      if (u < QV) *reinterpret_cast<u4*>(lds_q + head * QROW + 8 * (u % (D / 8))) = q8[i];
     }
-    float x[8];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      f4 s = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int m = 0; m < NKM; ++m) s = T::mfma(kx[t][m], qf[m], s);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * t + i] = s[i] * prm.qk_scale;
+    if (APPEND && mine) *reinterpret_cast<u4*>(lds_new + 8 * bl) = new8;
+    if (lo + 32 * w < hi) {
+      load_k(0);
+      load_v(0);
     }
-    if constexpr (TAIL) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (cb + slot_token(j, i) > last) x[i] = -INFINITY;
-    }
-    if (!TAIL && more) {
-      if (((c + 1) & 31) == 0) {
-        // V of chunk c is in registers already: its loads were issued from the old tiles.
-        tiles(c + 1);
-      }
-      load_k(c + 1);
-    }
-    // Online softmax in base 2; the accumulators are rescaled only in chunks
-    // where a head's maximum rose.
-    float top = x[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
-    if (__builtin_amdgcn_ballot_w64(top > m_run) != 0) {
-      const float mn = vmax(m_run, xor_max16_32(top));
-      const float alpha = safe_exp2_diff(m_run, mn);
-      m_run = mn;
-      l_run *= alpha;
-#pragma unroll
-      for (int mv = 0; mv < EPL; ++mv) accv[mv] *= alpha;
-    }
-    // scores of -inf under a maximum of -inf give p = 0, not NaN
-    const float off = T::kShift - (m_run == -INFINITY ? 0.0f : m_run);
-    float p[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(x[i] + off);
-      l_run += p[i];
-    }
-    u4 pt[T::kTerms];
-#pragma unroll
-    for (int n = 0; n < T::kTerms; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t wd = T::pack(p[2 * i], p[2 * i + 1]);
-        pt[n][i] = wd;
-        p[2 * i] -= T::lo(wd);
-        p[2 * i + 1] -= T::hi(wd);
-      }
-    if constexpr (TAIL) {
-      // Rows past the sequence are whatever the page holds there (possibly
-      // NaN or Inf); p = 0 alone would not cancel them in the MFMA.
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (cb + slot_token(j, i) > last)
-#pragma unroll
-          for (int e = 0; e < VW; ++e) vx[i][e] = 0u;
-    }
-#pragma unroll
-    for (int mv = 0; mv < EPL; ++mv) {
-      const uint32_t sel = (mv & 1) ? 0x07060302u : 0x05040100u;
-      u4 av;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) av[i] = perm(vx[2 * i + 1][mv / 2], vx[2 * i][mv / 2], sel);
-#pragma unroll
-      for (int n = T::kTerms - 1; n >= 0; --n) accv[mv] = T::mfma(av, pt[n], accv[mv]);
-    }
-    if (!TAIL && more) load_v(c + 1);
+    __syncthreads();
   };
 
-  // Full chunks, then the partial last one, or the one that takes the new token.
-  const int full = app ? last : hi;
-  int c = 0, cb = cb0;
-  for (; cb + 32 <= full; cb += 32 * NW, ++c) step(c, cb, std::false_type{});
-  if (cb < hi) step(c, cb, std::true_type{});
+  begin_segment();
+  for (;;) {
+    const int last = hi - 1;
+    f4 accv[EPL];
+#pragma unroll
+    for (int mv = 0; mv < EPL; ++mv) accv[mv] = f4{0.f, 0.f, 0.f, 0.f};
+    float m_run = -INFINITY, l_run = 0.0f;
 
-  if (APPEND && owner && hb0 == 0) {
-    const uint32_t t16 = (uint32_t)last / 16, pg = t16 / (uint32_t)prm.page_tiles;
-    const int page = a.block_table[(int64_t)b * a.block_table_stride + pg];
-    if (page >= 0 && page < a.num_pages) {
-      const int64_t at = last - (int64_t)pg * prm.page_tiles * 16;
-      uint16_t* kd = static_cast<uint16_t*>(a.k) + page * a.k_strides[0] + hk * a.k_strides[1] + at * kts;
-      uint16_t* vd = static_cast<uint16_t*>(a.v) + page * a.v_strides[0] + hk * a.v_strides[1] + at * vts;
-      if (r == 0)
+    auto step = [&](int c, int cb, auto tail) {
+      constexpr bool TAIL = decltype(tail)::value;
+      const bool more = cb + 32 * NW < hi;
+      if constexpr (TAIL && APPEND) {
+        if (owner) {
 #pragma unroll
-        for (int m = 0; m < NKM; ++m) *reinterpret_cast<u4*>(kd + 32 * m + 8 * j) = knew[m];
-      if (j == 0)
+          for (int t = 0; t < 2; ++t)
+            if (cb + 16 * t + r == last)
 #pragma unroll
-        for (int e = 0; e < VW; e += 2) *reinterpret_cast<u2*>(vd + EPL * r + 2 * e) = u2{vnew[e], vnew[e + 1]};
-    }
-  }
+              for (int m = 0; m < NKM; ++m) kx[t][m] = *reinterpret_cast<const u4*>(lds_new + 32 * m + 8 * j);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (cb + slot_token(j, i) == last)
+#pragma unroll
+              for (int e = 0; e < VW; ++e) vx[i][e] = reinterpret_cast<const uint32_t*>(lds_new + D + EPL * r)[e];
+        }
+      }
+      float x[8];
+      {
+        // (opaque: read again in every chunk, not kept in registers)
+        const uint16_t* ql = lds_q + (int)opaque((uint32_t)(r * QROW + 8 * j));
+        f4 s[2] = {f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int m = 0; m < NKM; ++m) {
+          const u4 qf = *reinterpret_cast<const u4*>(ql + 32 * m);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) s[t] = T::mfma(kx[t][m], qf, s[t]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = s[i / 4][i % 4] * prm.qk_scale;
+      }
+      if constexpr (TAIL) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (cb + slot_token(j, i) > last) x[i] = -INFINITY;
+      }
+      if (!TAIL && more) {
+        if (((c + 1) & 31) == 0) tiles(c + 1);  // V of chunk c is on its way already
+        load_k(c + 1);
+      }
+      // Online softmax in base 2; the accumulators are rescaled only in chunks
+      // where a head's maximum rose.
+      float top = x[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
+      if (__builtin_amdgcn_ballot_w64(top > m_run) != 0) {
+        const float mn = vmax(m_run, xor_max16_32(top));
+        const float alpha = safe_exp2_diff(m_run, mn);
+        m_run = mn;
+        l_run *= alpha;
+#pragma unroll
+        for (int mv = 0; mv < EPL; ++mv) accv[mv] *= alpha;
+      }
+      // scores of -inf under a maximum of -inf give p = 0, not NaN
+      const float off = T::kShift - (m_run == -INFINITY ? 0.0f : m_run);
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(x[i] + off);
+        l_run += p[i];
+      }
+      u4 pt[T::kTerms];
+#pragma unroll
+      for (int n = 0; n < T::kTerms; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t wd = T::pack(p[2 * i], p[2 * i + 1]);
+          pt[n][i] = wd;
+          p[2 * i] -= T::lo(wd);
+          p[2 * i + 1] -= T::hi(wd);
+        }
+      if constexpr (TAIL) {
+        // Rows past the sequence are whatever the page holds there (possibly
+        // NaN or Inf); p = 0 alone would not cancel them in the MFMA.
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (cb + slot_token(j, i) > last)
+#pragma unroll
+            for (int e = 0; e < VW; ++e) vx[i][e] = 0u;
+      }
+#pragma unroll
+      for (int mv = 0; mv < EPL; ++mv) {
+        const uint32_t sel = (mv & 1) ? 0x07060302u : 0x05040100u;
+        u4 av;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) av[i] = perm(vx[2 * i + 1][mv / 2], vx[2 * i][mv / 2], sel);
+#pragma unroll
+        for (int n = T::kTerms - 1; n >= 0; --n) accv[mv] = T::mfma(av, pt[n], accv[mv]);
+      }
+      if (!TAIL && more) load_v(c + 1);
+    };
 
-  // Merge of the waves.
-  const int rows = min(16, prm.G);
-  const int stride = rows * (D + 1) + 2 * rows;
-  float* mine = lds + w * stride;
-  const float lt = xor_sum16_32(l_run);
-  if (r < nh) {
-#pragma unroll
-    for (int mv = 0; mv < EPL; ++mv)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mine[r * (D + 1) + EPL * (4 * j + i) + mv] = accv[mv][i];
-    if (j == 0) {
-      mine[rows * (D + 1) + r] = m_run;
-      mine[rows * (D + 2) + r] = lt;
+    // Full chunks, then the row's partial last one, or the one that takes the new token.
+    const int full = app ? last : hi;
+    int c = 0, cb = lo + 32 * w;
+    for (; cb + 32 <= full; cb += 32 * NW, ++c) step(c, cb, std::false_type{});
+    if (cb < hi) step(c, cb, std::true_type{});
+
+    if (APPEND && owner && hb0 == 0) {
+      const uint32_t t16 = (uint32_t)last / 16, pg = t16 / (uint32_t)prm.page_tiles;
+      const int page = a.block_table[(int64_t)g.b * a.block_table_stride + pg];
+      if (page >= 0 && page < a.num_pages) {
+        const int64_t at = last - (int64_t)pg * prm.page_tiles * 16;
+        uint16_t* kd = static_cast<uint16_t*>(a.k) + page * a.k_strides[0] + hk * a.k_strides[1] + at * kts;
+        uint16_t* vd = static_cast<uint16_t*>(a.v) + page * a.v_strides[0] + hk * a.v_strides[1] + at * vts;
+        if (lane < D / 8) {
+          *reinterpret_cast<u4*>(kd + 8 * lane) = *reinterpret_cast<const u4*>(lds_new + 8 * lane);
+          *reinterpret_cast<u4*>(vd + 8 * lane) = *reinterpret_cast<const u4*>(lds_new + D + 8 * lane);
+        }
+      }
     }
+
+    // Merge of the waves.  (opaque: the addresses of this part would else be kept in
+    // registers over the whole loop.)
+    const int mr = (int)opaque(r), mj = (int)opaque(j), mt = (int)opaque(tid);
+    const int b = g.b, mine_rows = min(16, prm.G);
+    const int stride = mine_rows * (D + 1) + 2 * mine_rows;
+    const float lt = xor_sum16_32(l_run);
+    if (mr < nh) {
+      float* mine = lds + w * stride;
+#pragma unroll
+      for (int mv = 0; mv < EPL; ++mv)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine[mr * (D + 1) + EPL * (4 * mj + i) + mv] = accv[mv][i];
+      if (mj == 0) {
+        mine[mine_rows * (D + 1) + mr] = m_run;
+        mine[mine_rows * (D + 2) + mr] = lt;
+      }
+    }
+    __syncthreads();
+    // Where this segment goes.
+    const uint32_t l = chunks_of(g.L);
+    const bool whole = g.begin == 0 && g.end == l;
+    const uint32_t slot = 2 * blockIdx.y + (g.begin == 0 ? 1 : 0);
+    if (a.workgroups && g.begin == 0 && blockIdx.x == 0 && mt == 0)
+      reinterpret_cast<int2*>(a.row_pieces)[b] =
+          make_int2(blockIdx.y, whole ? 1 : (int)(sh.of(g.at + l - 1) - blockIdx.y + 1));
+    for (int idx = mt; idx < nh * (D / 4); idx += NW * 64) {
+      const int n = idx / (D / 4), d = 4 * (idx % (D / 4));
+      float mw[NW], mstar = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < NW; ++x) {
+        mw[x] = lds[x * stride + mine_rows * (D + 1) + n];
+        mstar = fmaxf(mstar, mw[x]);
+      }
+      f4 o = f4{0.f, 0.f, 0.f, 0.f};
+      float ls = 0.0f;
+#pragma unroll
+      for (int x = 0; x < NW; ++x) {
+        // A wave whose scores were all NaN keeps a maximum of -inf and a sum of
+        // NaN, which the factor 0 hands on.
+        const float f = safe_exp2_diff(mw[x], mstar);
+        const float* ow = lds + x * stride + n * (D + 1) + d;
+        o += f4{ow[0], ow[1], ow[2], ow[3]} * f;
+        ls = fmaf(f, lds[x * stride + mine_rows * (D + 2) + n], ls);
+      }
+      if (whole) {
+        store_row4(a, T::kShift, (int64_t)b * a.HQ + h0 + n, d, o, mstar, ls);
+      } else {
+        const int64_t row = partial_row(a, slot, h0 + n);
+        *reinterpret_cast<f4*>(a.partials + row * D + d) = o;
+        if (d == 0) *reinterpret_cast<float2*>(partial_ml(a) + 2 * row) = make_float2(mstar, ls);
+      }
+    }
+    if (g.at + g.end >= share_end) break;
+    __syncthreads();  // the partials in LDS have been read
+    g.at += l;
+    ++g.b;
+    g.L = rows.of(g.b);
+    g.begin = 0;
+    g.end = min(share_end - g.at, chunks_of(g.L));
+    begin_segment();
   }
-  __syncthreads();
-  for (int idx = tid; idx < nh * (D / 4); idx += NW * 64) {
-    const int n = idx / (D / 4), d = 4 * (idx % (D / 4));
-    float mw[NW], mstar = -INFINITY;
-#pragma unroll
-    for (int x = 0; x < NW; ++x) {
-      mw[x] = lds[x * stride + rows * (D + 1) + n];
-      mstar = fmaxf(mstar, mw[x]);
-    }
-    f4 o = f4{0.f, 0.f, 0.f, 0.f};
-    float l = 0.0f;
-#pragma unroll
-    for (int x = 0; x < NW; ++x) {
-      // A wave whose scores were all NaN keeps a maximum of -inf and a sum of
-      // NaN, which the factor 0 hands on.
-      const float f = safe_exp2_diff(mw[x], mstar);
-      const float* ow = lds + x * stride + n * (D + 1) + d;
-      o += f4{ow[0], ow[1], ow[2], ow[3]} * f;
-      l = fmaf(f, lds[x * stride + rows * (D + 2) + n], l);
-    }
-    if (pc.count == 1) {
-      store_row4(a, T::kShift, (int64_t)b * a.HQ + h0 + n, d, o, mstar, l);
-    } else {
-      const int64_t row = partial_row(a, slot, h0 + n);
-      *reinterpret_cast<f4*>(a.partials + row * D + d) = o;
-      if (d == 0) *reinterpret_cast<float2*>(partial_ml(a) + 2 * row) = make_float2(mstar, l);
-    }
-  }
-  if (a.target_pieces && slot == pc.base && blockIdx.x == 0 && tid == 0)
-    reinterpret_cast<int2*>(a.row_pieces)[b] = make_int2(pc.base, pc.count);
 }
 
 // ---------------------------------------------------------------------------
-// The join of rows cut into pieces: one 256-thread workgroup per (b, h); rows
-// of one piece were written by the split kernel.  Thread (g, dq) merges float4
-// column dq of pieces g, g + SG, ...; the SG groups meet in LDS.
+// The join of rows that several workgroups shared: one 256-thread workgroup per
+// (b, h); whole rows were written by the split kernel.  Thread (g, dq) merges
+// float4 column dq of pieces g, g + SG, ...; the SG groups meet in LDS.
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ void __launch_bounds__(256) paged16_join_kernel(Paged16Params prm, float shift) {
@@ -485,7 +562,7 @@ __global__ void __launch_bounds__(256) paged16_join_kernel(Paged16Params prm, fl
   f4 o = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int s = g; s < pieces.y; s += SG) {
-    const int64_t row = partial_row(a, pieces.x + s, h);
+    const int64_t row = partial_row(a, 2 * (pieces.x + s) + (s == 0 ? 1 : 0), h);
     const float2 x = *reinterpret_cast<const float2*>(ml + 2 * row);
     const f4 os = *reinterpret_cast<const f4*>(a.partials + row * D + 4 * dq);
     const float mn = fmaxf(m, x.x);
@@ -568,7 +645,7 @@ constexpr int kMaxPageTokens = 1 << 24;
 static bool pool_ok(const void* p, const int64_t* strides) {
   if (!p || (uintptr_t)p & 15) return false;
   for (int i = 0; i < 3; ++i)
-    if (strides[i] < 0 || strides[i] % 8) return false;
+    if (strides[i] < 0 || strides[i] % 8 || strides[i] / 8 > UINT32_MAX) return false;
   return strides[2] > 0 && strides[2] < (int64_t(1) << 26);
 }
 static bool rows_ok(const void* p, const int64_t* strides, int n, int align) {
@@ -586,7 +663,7 @@ static int check_paged16(const tkv_paged16_args* a) {
       a->num_pages <= 0 || a->block_table_stride < a->max_pages)
     return TKV_EINVAL;
   if ((int64_t)a->max_pages * a->page_size > INT32_MAX - 65536) return TKV_EINVAL;
-  // the plan sums the rows' chunks in 32 bits
+  // the rows' chunks are summed in 32 bits
   if ((int64_t)a->B * ((int64_t)a->max_pages * a->page_size / 32 + 1) > INT32_MAX) return TKV_EINVAL;
   if (!pool_ok(a->k, a->k_strides) || !pool_ok(a->v, a->v_strides)) return TKV_EINVAL;
   if (!rows_ok(a->q, a->q_strides, 2, 8)) return TKV_EINVAL;
@@ -596,11 +673,10 @@ static int check_paged16(const tkv_paged16_args* a) {
         !rows_ok(a->v_new, a->v_new_strides, 2, 8))
       return TKV_EINVAL;
   }
-  if (a->least_chunks <= 0 || a->target_pieces < 0) return TKV_EINVAL;
-  if (a->max_pieces <= 0 || a->max_pieces > 65535) return TKV_EINVAL;
-  if ((int64_t)a->target_pieces + a->B > a->max_pieces) return TKV_EINVAL;
-  if (a->target_pieces && (!a->partials || (uintptr_t)a->partials & 15 || !a->row_pieces ||
-                           (uintptr_t)a->row_pieces & 7))
+  if (a->least_chunks <= 0 || a->workgroups < 0 || a->workgroups > 65535) return TKV_EINVAL;
+  if (!a->workgroups && a->B > 65535) return TKV_EINVAL;
+  if (a->workgroups && (!a->partials || (uintptr_t)a->partials & 15 || !a->row_pieces ||
+                        (uintptr_t)a->row_pieces & 7))
     return TKV_EINVAL;
   if (a->waves != 0 && a->waves != 4 && a->waves != 8) return TKV_EINVAL;
   if (a->D != 64 && a->D != 128 && a->D != 256) return TKV_EUNSUPPORTED;
@@ -610,16 +686,16 @@ static int check_paged16(const tkv_paged16_args* a) {
 template <class T, int D, int NW>
 static void launch_paged16(const Paged16Params& p, dim3 grid, hipStream_t st) {
   const int rows = p.G < 16 ? p.G : 16;
-  const size_t lds = sizeof(float) * NW * (rows * (D + 1) + 2 * rows);
+  const size_t lds = 32 * (D + 8) + sizeof(float) * NW * (rows * (D + 1) + 2 * rows);
   if (p.a.k_new)
-    paged16_split_kernel<T, D, NW, true><<<grid, dim3(NW * 64), lds, st>>>(p);
+    paged16_split_kernel<T, D, NW, true><<<grid, dim3(NW * 64), lds + 4 * D, st>>>(p);
   else
     paged16_split_kernel<T, D, NW, false><<<grid, dim3(NW * 64), lds, st>>>(p);
 }
 
 template <class T>
 static void dispatch_paged16(const Paged16Params& p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.a.HKV * ((p.G + 15) / 16)), (unsigned)p.a.max_pieces);
+  const dim3 grid((unsigned)(p.a.HKV * ((p.G + 15) / 16)), (unsigned)(p.a.workgroups ? p.a.workgroups : p.a.B));
   const bool wide = p.a.waves == 8;
   if (p.a.D == 64) {
     if (wide) launch_paged16<T, 64, 8>(p, grid, st);
@@ -630,7 +706,7 @@ static void dispatch_paged16(const Paged16Params& p, hipStream_t st) {
   } else {
     launch_paged16<T, 256, 4>(p, grid, st);  // 8 waves' partials would not fit the LDS
   }
-  if (!p.a.target_pieces) return;
+  if (!p.a.workgroups) return;
   const dim3 rows((unsigned)(p.a.B * p.a.HQ));
   if (p.a.D == 64) paged16_join_kernel<64><<<rows, dim3(256), 0, st>>>(p, T::kShift);
   else if (p.a.D == 128) paged16_join_kernel<128><<<rows, dim3(256), 0, st>>>(p, T::kShift);
@@ -649,6 +725,10 @@ extern "C" int tkv_paged16_decode_attention(const tkv_paged16_args* a, tkv_strea
   p.page_tiles = a->page_size / 16;
   p.S = a->max_pages * a->page_size;
   p.qk_scale = a->sm_scale * kLog2e;
+  for (int i = 0; i < 3; ++i) {
+    p.k16[i] = (uint32_t)(a->k_strides[i] / 8);
+    p.v16[i] = (uint32_t)(a->v_strides[i] / 8);
+  }
   (void)hipGetLastError();
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (a->is_bf16) dispatch_paged16<Bf16>(p, st);

@@ -83,37 +83,38 @@ def _int32_arg(t, n: int, device, name: str, what: str):
     return t.contiguous()
 
 
-# Workgroups the decode's pieces should come to, per compute unit, and the
-# fewest tokens a piece of a cut row holds.
+# Workgroups of the decode per compute unit, and the fewest tokens each takes.
 WORKGROUPS_PER_CU = 3
 LEAST_TOKENS = 256
-MAX_PIECES = 65535  # grid y-dimension limit
+WAVES = 4
+MAX_WORKGROUPS = 65535  # grid y-dimension limit
 
 
-def plan_pieces(B: int, HKV: int, G: int, S: int, device=None,
-                piece_tokens: int | None = None) -> tuple[int, int, int]:
-    """``(least_chunks, target_pieces, max_pieces)`` of a decode (``include/tkv.h``).
+def plan_shares(B: int, HKV: int, G: int, S: int, device=None,
+                piece_tokens: int | None = None) -> tuple[int, int]:
+    """``(least_chunks, workgroups)`` of a decode (``include/tkv.h``).
 
     ``S`` is the tables' capacity; the rows' lengths are the device's
-    business.  ``piece_tokens`` fixes the size of the pieces instead."""
-    units = HKV * -(-G // 16)  # workgroups that share a piece
-    if B > MAX_PIECES - 1:
-        raise ValueError(f"at most {MAX_PIECES - 1} rows, got {B}")
+    business.  ``piece_tokens`` fixes a workgroup's tokens instead."""
+    units = HKV * -(-G // 16)  # workgroups that attend to the same tokens
+    if B > MAX_WORKGROUPS:
+        raise ValueError(f"at most {MAX_WORKGROUPS} rows, got {B}")
     if piece_tokens is not None:
         if piece_tokens <= 0:
             raise ValueError(f"piece_tokens must be positive, got {piece_tokens}")
         least = -(-piece_tokens // 32)
-        pieces = B * -(-S // (32 * least))  # as many as full rows have
-        if pieces > MAX_PIECES - B:
+        if S <= 32 * least:
+            return least, 0
+        most = -(-B * -(-S // 32) // least)  # where every row fills its table
+        if most > MAX_WORKGROUPS:
             raise ValueError(f"piece_tokens={piece_tokens} cuts {B} rows of up to {S} tokens into "
-                             f"more than {MAX_PIECES} pieces")
-        return (least, 0, B) if S <= 32 * least else (least, pieces, pieces + B)
+                             f"more than {MAX_WORKGROUPS} pieces")
+        return least, most
     least = LEAST_TOKENS // 32
     if S <= LEAST_TOKENS:
-        return least, 0, B
+        return least, 0
     cu = compute_units(device) or 256
-    target = min(max(1, WORKGROUPS_PER_CU * cu // units), B * -(-S // LEAST_TOKENS), MAX_PIECES - B)
-    return least, target, target + B
+    return least, min(max(1, int(WORKGROUPS_PER_CU * cu) // units), -(-B * -(-S // 32) // least), MAX_WORKGROUPS)
 
 
 def _buffer(ws: dict, name: str, n: int, dtype, device) -> torch.Tensor:
@@ -299,15 +300,15 @@ def paged16_decode_attention(
     if out.data_ptr() % 16:
         raise ValueError("out must start on a 16-byte boundary")
     G = HQ // HKV
-    least, target, pieces = plan_pieces(B, HKV, G, S, device, piece_tokens)
+    least, groups = plan_shares(B, HKV, G, S, device, piece_tokens)
     ok, why = _backend(q)
     if not ok:
         raise RuntimeError(f"paged16_decode_attention requires the tritonkv_amd HIP backend: {why}")
     qk = q if _dense_rows(q, 8) else q.contiguous().clone()
     partials = rows = None
-    if target:
+    if groups:
         ws = {} if _workspace is None else _workspace
-        partials = _buffer(ws, "partials16", pieces * HQ * (D + 2), torch.float32, device)
+        partials = _buffer(ws, "partials16", 2 * groups * HQ * (D + 2), torch.float32, device)
         rows = _buffer(ws, "row_pieces16", 2 * B, torch.int32, device)
     kn, vn = new
     args = _lib.Paged16Args(
@@ -321,7 +322,7 @@ def paged16_decode_attention(
         block_table_stride=table.shape[1], max_pages=table.shape[1], page_size=page_size,
         num_pages=num_pages,
         sm_scale=1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
-        least_chunks=least, target_pieces=target, max_pieces=pieces, waves=4)
+        least_chunks=least, workgroups=groups, waves=WAVES)
     _lib.check(_lib.launch(device, "tkv_paged16_decode_attention", args), "paged16_decode_attention")
     if key is not None and qk is q:
         strided = (k_new is None or kn.data_ptr() == k_new.data_ptr()) and \
@@ -336,4 +337,4 @@ def paged16_decode_attention(
 
 
 __all__ = ["PAGE_MULTIPLE", "HEAD_DIMS", "empty_paged16_pool", "paged16_append",
-           "paged16_decode_attention", "plan_pieces"]
+           "paged16_decode_attention", "plan_shares"]
