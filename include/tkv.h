@@ -342,11 +342,12 @@ int tkv_dequantize(const uint8_t *packed, const uint16_t *scale, const uint16_t 
  * The rows are cut on the device, from their lengths: their chunks of 32 tokens
  * (an empty row counts as one), laid end to end, are shared out evenly over at
  * most `workgroups` workgroups (1 to 65535) per KV head and 16 query heads, of at
- * least least_chunks chunks each, and a second launch joins the rows that were
+ * least least_chunks chunks each -- or over long_workgroups (at most workgroups;
+ * 0: never) where the batch has no more rows and each gets at least long_chunks --
+ * and a second launch joins the rows that were
  * cut: partials holds 2 * workgroups * HQ * (D + 2) floats (16-byte aligned),
  * row_pieces 2 * B int32 (8-byte aligned).  workgroups == 0 keeps every row
- * whole, in one launch (at most 65535 rows).  waves: 4 or 8 per workgroup
- * (0: 4).  No counterpart in the reference (its caches are contiguous). */
+ * whole, in one launch (at most 65535 rows).  No counterpart in the reference (its caches are contiguous). */
 typedef struct tkv_paged16_args {
   const void *q;
   int64_t q_strides[2];
@@ -360,7 +361,7 @@ typedef struct tkv_paged16_args {
   int32_t is_bf16, B, HQ, HKV, D;
   int32_t block_table_stride, max_pages, page_size, num_pages;
   float sm_scale;
-  int32_t least_chunks, workgroups, waves;
+  int32_t least_chunks, workgroups, long_workgroups, long_chunks;
 } tkv_paged16_args;
 int tkv_paged16_decode_attention(const tkv_paged16_args *args, tkv_stream_t stream);
 

@@ -118,17 +118,18 @@ def test_the_shares_cover_every_chunk_once(B, HKV, G, S):
     rng = random.Random(B * S)
     for piece in (None, 48, S):
         try:
-            least, groups = plan_shares(B, HKV, G, S, "cpu", piece)
+            least, groups, few, long = plan_shares(B, HKV, G, S, 128, "cpu", piece)
         except ValueError:
             assert piece is not None and -(-B * -(-S // 32) // -(-piece // 32)) > MAX_WORKGROUPS
             continue
         assert 0 <= groups <= MAX_WORKGROUPS and least > 0
         if groups == 0:
-            assert S <= 32 * least
+            assert S <= 1024 if piece is None else S <= 32 * least
             continue
+        assert 0 <= few <= groups and (few == 0 or long > 0)
         for lens in ([S] * B, [0] * B, [S] + [0] * (B - 1), [rng.randint(0, S) for _ in range(B)]):
             total = sum(max(1, -(-n // 32)) for n in lens)
-            W = min(groups, -(-total // least))
+            W = few if B <= few and total >= few * long else min(groups, -(-total // least))
             each, more = divmod(total, W)
             assert each > 0
 
@@ -166,7 +167,7 @@ def _decode_args():
     return _lib.Paged16Args(q=d, q_strides=(1024, 128), k=d, v=d, k_strides=(8192, 4096, 128),
                             v_strides=(8192, 4096, 128), block_table=d, out=d, partials=d, row_pieces=d, B=2,
                             HQ=8, HKV=2, D=128, block_table_stride=4, max_pages=4, page_size=32, num_pages=4,
-                            sm_scale=0.1, least_chunks=2, workgroups=4, waves=4)
+                            sm_scale=0.1, least_chunks=2, workgroups=4)
 
 
 @pytest.mark.parametrize("field,value", [
@@ -174,7 +175,8 @@ def _decode_args():
     ("partials", None), ("partials", 0x1008), ("row_pieces", 0x1004), ("k_new", 0x1000), ("B", 0), ("HQ", 7),
     ("HKV", 0), ("page_size", 24), ("page_size", 0), ("max_pages", 0), ("num_pages", 0),
     ("block_table_stride", 3), ("max_pages", 1 << 27), ("least_chunks", 0), ("workgroups", -1),
-    ("workgroups", 65536), ("waves", 5), ("k_strides", (8192, 4096, 132)),
+    ("workgroups", 65536), ("long_workgroups", 5), ("long_workgroups", -1), ("long_chunks", -1),
+    ("long_workgroups", 2),  ("k_strides", (8192, 4096, 132)),
     ("v_strides", (8192, 4096, 0)), ("k_strides", (8192, 4096, 1 << 26)), ("k_strides", (-8, 4096, 128)),
     ("q_strides", (1024, 4))])
 def test_c_entry_refuses(field, value):

@@ -104,7 +104,8 @@ class Paged16Args(ctypes.Structure):
         ("sm_scale", ctypes.c_float),
         ("least_chunks", ctypes.c_int32),
         ("workgroups", ctypes.c_int32),
-        ("waves", ctypes.c_int32),
+        ("long_workgroups", ctypes.c_int32),
+        ("long_chunks", ctypes.c_int32),
     ]
 
 

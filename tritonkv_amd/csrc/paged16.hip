@@ -70,7 +70,9 @@ struct Bf16 {
 // most pieces empty and the others uneven.  Instead the rows' chunks (32 tokens;
 // an empty row counts as one, which writes its zeros) are laid end to end, and the
 // W = min(workgroups, ceil(chunks / least_chunks)) workgroups of a KV head
-// take equal shares of that line: workgroup i the chunks from share_start(i) on.
+// take equal shares of that line, workgroup i the chunks from Shares::start(i) on.
+// (long_workgroups of them where that gives each long_chunks at least, in batches of
+// no more rows: fewer, longer streams then read faster; paged16.py has the figures.)
 // A share covers the end of one row, whole rows, and the start of another; each
 // such segment is attended by itself.  Whole rows are written out; the others
 // leave a partial in slot 2i (the row began in an earlier share) or 2i + 1, and
@@ -142,7 +144,8 @@ __device__ __forceinline__ uint32_t full_at(const tkv_paged16_args& a) {
 
 __device__ __forceinline__ Shares make_shares(uint32_t total, const tkv_paged16_args& a, uint32_t& W) {
   W = a.workgroups;
-  if (total < full_at(a)) W = min(W, (total + a.least_chunks - 1) / (uint32_t)a.least_chunks);
+  if (a.B <= a.long_workgroups && total >= (uint32_t)a.long_workgroups * (uint32_t)a.long_chunks) W = a.long_workgroups;
+  else if (total < full_at(a)) W = min(W, (total + a.least_chunks - 1) / (uint32_t)a.least_chunks);
   Shares s;
   s.each = total / W;
   s.more = total - s.each * W;
@@ -233,7 +236,7 @@ __device__ __forceinline__ void store_row4(const tkv_paged16_args& a, float shif
 // The split kernel.
 // ---------------------------------------------------------------------------
 template <class T, int D, int NW, bool APPEND>
-__global__ void __launch_bounds__(NW * 64, D == 256 ? 2 : D == 128 ? 3 : 4) paged16_split_kernel(Paged16Params prm) {
+__global__ void __launch_bounds__(NW * 64, D == 256 ? 1 : D == 128 ? 3 : 4) paged16_split_kernel(Paged16Params prm) {
   constexpr int NKM = D / 32;  // 16x16x32 steps over the head dim
   constexpr int EPL = D / 16;  // V dims per lane (and V MFMAs)
   constexpr int VW = EPL / 2;  // dwords of them
@@ -504,6 +507,16 @@ __global__ void __launch_bounds__(NW * 64, D == 256 ? 2 : D == 128 ? 3 : 4) page
     if (a.workgroups && g.begin == 0 && blockIdx.x == 0 && mt == 0)
       reinterpret_cast<int2*>(a.row_pieces)[b] =
           make_int2(blockIdx.y, whole ? 1 : (int)(sh.of(g.at + l - 1) - blockIdx.y + 1));
+    // The next segment, whose first loads run behind this one's merge.
+    const bool again = g.at + g.end < share_end;
+    if (again) {
+      g.at += l;
+      ++g.b;
+      g.L = rows.of(g.b);
+      g.begin = 0;
+      g.end = min(share_end - g.at, chunks_of(g.L));
+      begin_segment();
+    }
     for (int idx = mt; idx < nh * (D / 4); idx += NW * 64) {
       const int n = idx / (D / 4), d = 4 * (idx % (D / 4));
       float mw[NW], mstar = -INFINITY;
@@ -531,37 +544,36 @@ __global__ void __launch_bounds__(NW * 64, D == 256 ? 2 : D == 128 ? 3 : 4) page
         if (d == 0) *reinterpret_cast<float2*>(partial_ml(a) + 2 * row) = make_float2(mstar, ls);
       }
     }
-    if (g.at + g.end >= share_end) break;
+    if (!again) break;
     __syncthreads();  // the partials in LDS have been read
-    g.at += l;
-    ++g.b;
-    g.L = rows.of(g.b);
-    g.begin = 0;
-    g.end = min(share_end - g.at, chunks_of(g.L));
-    begin_segment();
   }
 }
 
 // ---------------------------------------------------------------------------
-// The join of rows that several workgroups shared: one 256-thread workgroup per
-// (b, h); whole rows were written by the split kernel.  Thread (g, dq) merges
-// float4 column dq of pieces g, g + SG, ...; the SG groups meet in LDS.
+// The join of rows that several workgroups shared; whole rows were written by the
+// split kernel.  LANES lanes take a (b, h): lane (g, dq) merges float4 column dq of
+// pieces g, g + SG, ..., and the SG groups meet in LDS.
+// Few rows have many pieces and take 256 lanes each; many rows have one to three
+// pieces each, and four of them share a workgroup.
 // ---------------------------------------------------------------------------
-template <int D>
+template <int D, int LANES>
 __global__ void __launch_bounds__(256) paged16_join_kernel(Paged16Params prm, float shift) {
-  constexpr int DQ = D / 4, SG = 256 / DQ;
-  __shared__ float sm_m[SG], sm_l[SG];
-  __shared__ f4 sm_a[SG][DQ];
+  constexpr int DQ = D / 4, SG = LANES / DQ, ROWS = 256 / LANES;
+  __shared__ float sm_m[ROWS][SG], sm_l[ROWS][SG];
+  __shared__ f4 sm_a[ROWS][SG][DQ];
   const tkv_paged16_args& a = prm.a;
-  const int b = blockIdx.x / a.HQ, h = blockIdx.x % a.HQ;
-  const int2 pieces = reinterpret_cast<const int2*>(a.row_pieces)[b];
-  if (pieces.y <= 1) return;
-  const int t = threadIdx.x, dq = t % DQ, g = t / DQ;
+  const int in = threadIdx.x / LANES, row0 = blockIdx.x * ROWS + in;
+  const bool live = row0 < a.B * a.HQ;
+  const int b = live ? row0 / a.HQ : 0, h = row0 - b * a.HQ;
+  const int2 pieces = live ? reinterpret_cast<const int2*>(a.row_pieces)[b] : make_int2(0, 0);
+  if (ROWS == 1 && pieces.y <= 1) return;
+  const int t = threadIdx.x % LANES, dq = t % DQ, g = t / DQ;
   const float* ml = partial_ml(a);
   float m = -INFINITY, l = 0.0f;
   f4 o = f4{0.f, 0.f, 0.f, 0.f};
+  const int n = pieces.y > 1 ? pieces.y : 0;
 #pragma unroll 4
-  for (int s = g; s < pieces.y; s += SG) {
+  for (int s = g; s < n; s += SG) {
     const int64_t row = partial_row(a, 2 * (pieces.x + s) + (s == 0 ? 1 : 0), h);
     const float2 x = *reinterpret_cast<const float2*>(ml + 2 * row);
     const f4 os = *reinterpret_cast<const f4*>(a.partials + row * D + 4 * dq);
@@ -572,21 +584,21 @@ __global__ void __launch_bounds__(256) paged16_join_kernel(Paged16Params prm, fl
     m = mn;
   }
   if (dq == 0) {
-    sm_m[g] = m;
-    sm_l[g] = l;
+    sm_m[in][g] = m;
+    sm_l[in][g] = l;
   }
-  sm_a[g][dq] = o;
+  sm_a[in][g][dq] = o;
   __syncthreads();
-  if (g == 0) {
+  if (g == 0 && n) {
     float mstar = -INFINITY, lt = 0.0f;
 #pragma unroll
-    for (int x = 0; x < SG; ++x) mstar = fmaxf(mstar, sm_m[x]);
+    for (int x = 0; x < SG; ++x) mstar = fmaxf(mstar, sm_m[in][x]);
     f4 ot = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < SG; ++x) {
-      const float f = safe_exp2_diff(sm_m[x], mstar);
-      ot += sm_a[x][dq] * f;
-      lt += sm_l[x] * f;
+      const float f = safe_exp2_diff(sm_m[in][x], mstar);
+      ot += sm_a[in][x][dq] * f;
+      lt += sm_l[in][x] * f;
     }
     store_row4(a, shift, (int64_t)b * a.HQ + h, 4 * dq, ot, mstar, lt);
   }
@@ -640,6 +652,7 @@ __global__ void __launch_bounds__(256) paged16_append_kernel(AppendParams prm) {
 // Host side: validation and dispatch.
 // ---------------------------------------------------------------------------
 constexpr int kMaxPageTokens = 1 << 24;
+constexpr int kJoinRows = 512;  // (b, h) rows from which on the join takes a wave for each
 
 // Pool rows are read and written 16 bytes at a time; one 16-row tile spans 32 bits.
 static bool pool_ok(const void* p, const int64_t* strides) {
@@ -674,18 +687,21 @@ static int check_paged16(const tkv_paged16_args* a) {
       return TKV_EINVAL;
   }
   if (a->least_chunks <= 0 || a->workgroups < 0 || a->workgroups > 65535) return TKV_EINVAL;
+  if (a->long_workgroups < 0 || a->long_workgroups > a->workgroups || a->long_chunks < 0 ||
+      (int64_t)a->long_workgroups * a->long_chunks > INT32_MAX || (a->long_workgroups && !a->long_chunks))
+    return TKV_EINVAL;
   if (!a->workgroups && a->B > 65535) return TKV_EINVAL;
   if (a->workgroups && (!a->partials || (uintptr_t)a->partials & 15 || !a->row_pieces ||
                         (uintptr_t)a->row_pieces & 7))
     return TKV_EINVAL;
-  if (a->waves != 0 && a->waves != 4 && a->waves != 8) return TKV_EINVAL;
   if (a->D != 64 && a->D != 128 && a->D != 256) return TKV_EUNSUPPORTED;
   return TKV_OK;
 }
 
 template <class T, int D, int NW>
-static void launch_paged16(const Paged16Params& p, dim3 grid, hipStream_t st) {
+static void launch_paged16(const Paged16Params& p, hipStream_t st) {
   const int rows = p.G < 16 ? p.G : 16;
+  const dim3 grid((unsigned)(p.a.HKV * ((p.G + 15) / 16)), (unsigned)(p.a.workgroups ? p.a.workgroups : p.a.B));
   const size_t lds = 32 * (D + 8) + sizeof(float) * NW * (rows * (D + 1) + 2 * rows);
   if (p.a.k_new)
     paged16_split_kernel<T, D, NW, true><<<grid, dim3(NW * 64), lds + 4 * D, st>>>(p);
@@ -693,24 +709,24 @@ static void launch_paged16(const Paged16Params& p, dim3 grid, hipStream_t st) {
     paged16_split_kernel<T, D, NW, false><<<grid, dim3(NW * 64), lds, st>>>(p);
 }
 
+template <int D>
+static void launch_join(const Paged16Params& p, float shift, hipStream_t st) {
+  const int rows = p.a.B * p.a.HQ;
+  if (rows >= kJoinRows) paged16_join_kernel<D, 64><<<dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st>>>(p, shift);
+  else paged16_join_kernel<D, 256><<<dim3((unsigned)rows), dim3(256), 0, st>>>(p, shift);
+}
+
+template <class T, int D>
+static void dispatch_paged16(const Paged16Params& p, hipStream_t st) {
+  launch_paged16<T, D, 4>(p, st);
+  if (p.a.workgroups) launch_join<D>(p, T::kShift, st);
+}
+
 template <class T>
 static void dispatch_paged16(const Paged16Params& p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.a.HKV * ((p.G + 15) / 16)), (unsigned)(p.a.workgroups ? p.a.workgroups : p.a.B));
-  const bool wide = p.a.waves == 8;
-  if (p.a.D == 64) {
-    if (wide) launch_paged16<T, 64, 8>(p, grid, st);
-    else launch_paged16<T, 64, 4>(p, grid, st);
-  } else if (p.a.D == 128) {
-    if (wide) launch_paged16<T, 128, 8>(p, grid, st);
-    else launch_paged16<T, 128, 4>(p, grid, st);
-  } else {
-    launch_paged16<T, 256, 4>(p, grid, st);  // 8 waves' partials would not fit the LDS
-  }
-  if (!p.a.workgroups) return;
-  const dim3 rows((unsigned)(p.a.B * p.a.HQ));
-  if (p.a.D == 64) paged16_join_kernel<64><<<rows, dim3(256), 0, st>>>(p, T::kShift);
-  else if (p.a.D == 128) paged16_join_kernel<128><<<rows, dim3(256), 0, st>>>(p, T::kShift);
-  else paged16_join_kernel<256><<<rows, dim3(256), 0, st>>>(p, T::kShift);
+  if (p.a.D == 64) dispatch_paged16<T, 64>(p, st);
+  else if (p.a.D == 128) dispatch_paged16<T, 128>(p, st);
+  else dispatch_paged16<T, 256>(p, st);
 }
 
 }  // namespace tkv

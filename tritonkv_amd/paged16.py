@@ -83,20 +83,36 @@ def _int32_arg(t, n: int, device, name: str, what: str):
     return t.contiguous()
 
 
-# Workgroups of the decode per compute unit, and the fewest tokens each takes.
-WORKGROUPS_PER_CU = 3
-LEAST_TOKENS = 256
-WAVES = 4
 MAX_WORKGROUPS = 65535  # grid y-dimension limit
 
 
-def plan_shares(B: int, HKV: int, G: int, S: int, device=None,
-                piece_tokens: int | None = None) -> tuple[int, int]:
-    """``(least_chunks, workgroups)`` of a decode (``include/tkv.h``).
+def plan_shares(B: int, HKV: int, G: int, S: int, D: int = 128, device=None,
+                piece_tokens: int | None = None) -> tuple[int, int, int, int]:
+    """``(least_chunks, workgroups, long_workgroups, long_chunks)`` of a decode (``include/tkv.h``).
 
-    ``S`` is the tables' capacity; the rows' lengths are the device's
-    business.  ``piece_tokens`` fixes a workgroup's tokens instead."""
-    units = HKV * -(-G // 16)  # workgroups that attend to the same tokens
+    ``S`` is the tables' capacity; the rows' lengths are the device's business.
+    ``piece_tokens`` fixes a workgroup's tokens instead.  The rules, with
+    what was measured on MI355X (us of a captured step; U = HKV times the
+    blocks of 16 query heads, the workgroups that attend to the same tokens):
+
+    * Rows stay whole, in one launch, where that is faster than cutting them
+      and joining (a second launch, 2.4 us and more): one CU reads at most
+      38 GB/s, so only short rows, or many.  Up to 256 tokens of 128 dims (250
+      tokens, D 128: B * U = 2 5.8 whole, 7.0 cut; 32 6.6, 8.5; D 256 9.4, 8.9),
+      twice that from 64 row units on (505 tokens: B * U = 2 8.0, 6.9; 32 10.2,
+      8.7; 128 10.6, 12.1), four times from 512 (up to 512 of 1024: 512 units
+      20.6, 24.3).
+    * Otherwise two workgroups per CU (four at head dim 64, whose chunks are half
+      as large: 8 rows of up to 2999, 16 KV heads, w = 1 / 2 / 4 17.1 / 16.3 /
+      15.2), of at least 128 tokens of 128 dims, half of that in tables of
+      at most 512 tokens (one row of 505: 6.9, with 128 7.4; of 4000: 9.0, 8.1).
+    * One per CU where the batch has no more rows than that and every workgroup
+      gets a long stream, 16 chunks (32 rows of 8192: 2 per CU 169, 1 157;
+      32 of 1000-16384 185, 179; one of 32768 27.3, 26.2; but 16 of up to 1024,
+      9 chunks each, 13.6, 14.3, and 64 of up to 2048, two rows each, 55.9, 60.5);
+      128 chunks at head dim 64 (32 rows of up to 16384 132, 126; 8 rows 38.5, 39.4).
+    """
+    units = HKV * -(-G // 16)
     if B > MAX_WORKGROUPS:
         raise ValueError(f"at most {MAX_WORKGROUPS} rows, got {B}")
     if piece_tokens is not None:
@@ -104,17 +120,19 @@ def plan_shares(B: int, HKV: int, G: int, S: int, device=None,
             raise ValueError(f"piece_tokens must be positive, got {piece_tokens}")
         least = -(-piece_tokens // 32)
         if S <= 32 * least:
-            return least, 0
+            return least, 0, 0, 0
         most = -(-B * -(-S // 32) // least)  # where every row fills its table
         if most > MAX_WORKGROUPS:
             raise ValueError(f"piece_tokens={piece_tokens} cuts {B} rows of up to {S} tokens into "
                              f"more than {MAX_WORKGROUPS} pieces")
-        return least, most
-    least = LEAST_TOKENS // 32
-    if S <= LEAST_TOKENS:
-        return least, 0
+        return least, most, 0, 0
+    row = S * D
+    if row <= 32768 * (4 if B * units >= 512 else 2 if B * units >= 64 else 1):
+        return 1, 0, 0, 0
+    least = (256 if S <= 512 else 512) // D or 1
     cu = compute_units(device) or 256
-    return least, min(max(1, int(WORKGROUPS_PER_CU * cu) // units), -(-B * -(-S // 32) // least), MAX_WORKGROUPS)
+    groups = min(max(1, (4 if D == 64 else 2) * cu // units), -(-B * -(-S // 32) // least), MAX_WORKGROUPS)
+    return least, groups, min(groups, max(1, cu // units)), 128 if D == 64 else 16
 
 
 def _buffer(ws: dict, name: str, n: int, dtype, device) -> torch.Tensor:
@@ -300,7 +318,7 @@ def paged16_decode_attention(
     if out.data_ptr() % 16:
         raise ValueError("out must start on a 16-byte boundary")
     G = HQ // HKV
-    least, groups = plan_shares(B, HKV, G, S, device, piece_tokens)
+    least, groups, few, long = plan_shares(B, HKV, G, S, D, device, piece_tokens)
     ok, why = _backend(q)
     if not ok:
         raise RuntimeError(f"paged16_decode_attention requires the tritonkv_amd HIP backend: {why}")
@@ -322,7 +340,7 @@ def paged16_decode_attention(
         block_table_stride=table.shape[1], max_pages=table.shape[1], page_size=page_size,
         num_pages=num_pages,
         sm_scale=1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
-        least_chunks=least, workgroups=groups, waves=WAVES)
+        least_chunks=least, workgroups=groups, long_workgroups=few, long_chunks=long)
     _lib.check(_lib.launch(device, "tkv_paged16_decode_attention", args), "paged16_decode_attention")
     if key is not None and qk is q:
         strided = (k_new is None or kn.data_ptr() == k_new.data_ptr()) and \
