@@ -370,7 +370,8 @@ int tkv_paged16_decode_attention(const tkv_paged16_args *args, tkv_stream_t stre
  * (B, HKV, N, D), strides batch, head, token, in the pools' type or fp32
  * (new_is_fp32), rounded to nearest even; bases and strides are multiples of 16
  * bytes.  Positions outside [0, max_pages * page_size) and table entries
- * outside [0, num_pages) are not written.  Any page_size; D a multiple of 8. */
+ * outside [0, num_pages) are not written.  Any page_size; D a multiple of 8; at most
+ * 65535 rows and 2^31 - 1 groups of 8 values in each (N * HKV * D / 8). */
 typedef struct tkv_paged16_append_args {
   const void *k_new, *v_new;
   int64_t k_new_strides[3], v_new_strides[3];
@@ -399,7 +400,7 @@ typedef struct tkv_page_set {
  * with one destination the first is carried out.  Within one set of pools (same)
  * a page that the call reads is never written: a pair whose destination is a
  * pair's source is skipped, and (p, p) is no pair.  work: tkv_copy_pages_work()
- * int32, 8-byte aligned (none for up to 512 pairs).  No counterpart in the
+ * int32, 8-byte aligned (none for up to 1024 pairs).  No counterpart in the
  * reference, nor have the next two (its caches have no pages). */
 typedef struct tkv_copy_pages_args {
   tkv_page_set set;

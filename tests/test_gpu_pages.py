@@ -58,7 +58,7 @@ def _copied(src, dst, src_pages, dst_pages, same):
     return done
 
 
-@pytest.mark.parametrize("n", [1, 3, 256, 257, 512, 513, 2000])
+@pytest.mark.parametrize("n", [1, 3, 256, 257, 512, 513, 1024, 1025, 2000])
 @pytest.mark.parametrize("kind", ["clean", "wild"])
 @pytest.mark.parametrize("other", [False, True])
 def test_copy_pairs(n, kind, other):

@@ -154,8 +154,8 @@ def test_work_sizes():
     from tritonkv_amd import _lib
 
     lib = _lib.load()
-    assert lib.tkv_copy_pages_work(512, 100, 100) == 0
-    assert lib.tkv_copy_pages_work(513, 100, 7) >= 107 + 2 * 513
+    assert lib.tkv_copy_pages_work(1024, 100, 100) == 0
+    assert lib.tkv_copy_pages_work(1025, 100, 7) >= 107 + 2 * 1025
     assert lib.tkv_fork_rows_work(4, 10, 100, 1) - lib.tkv_fork_rows_work(4, 10, 100, 0) == 40
     assert lib.tkv_fork_rows_work(4, 10, 100, 0) >= 6 * 4 + 100
     assert lib.tkv_compact_pages_work(100) >= 250
@@ -196,7 +196,7 @@ def test_c_entries_refuse_page_sets(change):
 
 @pytest.mark.parametrize("kind,field,value", [
     ("copy", "src", None), ("copy", "dst", None), ("copy", "n", 0), ("copy", "src_pages", 0),
-    ("copy", "dst_pages", 7), ("copy", "n", 513),
+    ("copy", "dst_pages", 7), ("copy", "n", 1025),
     ("fork", "block_table", None), ("fork", "seq_lens", None), ("fork", "refs", None), ("fork", "status", None),
     ("fork", "work", None), ("fork", "work", 0x1004), ("fork", "B", 0), ("fork", "max_pages", 0),
     ("fork", "num_pages", 0), ("fork", "page_size", 0), ("fork", "table_stride", 2),

@@ -16,9 +16,9 @@
 namespace tkv {
 
 constexpr int kPlan = 1024;                  // threads of a plan's workgroup
-constexpr int kSlice = 16384;                // bytes of a page that a workgroup copies at a time
+constexpr int kCopy = 1024;                  // threads of a copy's workgroup
 constexpr int kMaxRows = 8192;               // rows of a fork: two LDS integers each
-constexpr int kInlinePairs = 512;            // pairs that the copy checks by itself
+constexpr int kInlinePairs = 1024;           // pairs that the copy checks by itself
 constexpr int kPagesPerThread = 64;          // bits of a thread's mask of pages
 
 // A barrier behind which the workgroup's memory operations have been carried out.
@@ -30,72 +30,97 @@ __device__ __forceinline__ void settle() {
 // ---------------------------------------------------------------------------
 // The copy.  Item = one slice of one tensor's page; workgroups stride over the
 // items of the first `count` pairs.
+//
+// Bound by HBM.  A slice of 64 KiB, read whole by 1024 threads before any of it is
+// written, copies 4000 scattered pages of 128 KiB at 5.9 TB/s; 16 KiB by 256
+// threads 5.1, 64 KiB by 256 threads 5.2, torch's copy_ of 2 GiB 4.9.  Where the
+// call copies less than 32 MiB, slices of 16 KiB reach more CUs.  Both without
+// keeping the bytes in the caches (non-temporal; 4% on the large ones).
 // ---------------------------------------------------------------------------
+constexpr int kSlices[2] = {16384, 65536};
+constexpr int64_t kLongCopy = 32 << 20;
+
 struct CopyPlan {
   tkv_page_set set;
-  int32_t first[TKV_PAGE_TENSORS];  // slices of a page before tensor t
-  int32_t slices;                   // of a page, in all tensors
+  int32_t first[2][TKV_PAGE_TENSORS];  // slices of a page before tensor t, of either size
+  int32_t slices[2];                   // of a page, in all tensors
+  int64_t bytes;                       // of a page, in all tensors
 };
 
+template <int LONG>
 __device__ __forceinline__ void copy_slice(const CopyPlan& c, int src, int dst, int slice) {
+  constexpr int kSize = kSlices[LONG];
   int t = 0;
 #pragma unroll
   for (int step = TKV_PAGE_TENSORS / 2; step; step /= 2)
-    if (t + step < c.set.count && c.first[t + step] <= slice) t += step;
-  const int64_t at = (int64_t)(slice - c.first[t]) * kSlice;
+    if (t + step < c.set.count && c.first[LONG][t + step] <= slice) t += step;
+  const int64_t at = (int64_t)(slice - c.first[LONG][t]) * kSize;
   const int64_t left = c.set.bytes[t] - at;
-  const int units = (int)((left < kSlice ? left : (int64_t)kSlice) / 16);
+  const int units = (int)((left < kSize ? left : (int64_t)kSize) / 16);
   const u4* from = reinterpret_cast<const u4*>(static_cast<const char*>(c.set.src[t]) + src * c.set.src_stride[t] + at);
   u4* to = reinterpret_cast<u4*>(static_cast<char*>(c.set.dst[t]) + dst * c.set.dst_stride[t] + at);
-  constexpr int kPer = kSlice / 16 / 256;
+  constexpr int kPer = kSize / 16 / kCopy;
   u4 x[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int u = threadIdx.x + 256 * i;
+    const int u = threadIdx.x + kCopy * i;
     if (u < units) x[i] = __builtin_nontemporal_load(from + u);
   }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int u = threadIdx.x + 256 * i;
+    const int u = threadIdx.x + kCopy * i;
     if (u < units) __builtin_nontemporal_store(x[i], to + u);
   }
 }
 
 // Pairs (x, y) = (source, destination); a negative source is no pair.
+template <int LONG>
 __device__ __forceinline__ void copy_pairs(const CopyPlan& c, const int2* pairs, int count, int group, int groups) {
-  const int64_t items = (int64_t)count * c.slices;
+  const int64_t items = (int64_t)count * c.slices[LONG];
   for (int64_t i = group; i < items; i += groups) {
-    const int p = (int)(i / c.slices);
+    const int p = (int)(i / c.slices[LONG]);
     const int2 pair = pairs[p];
-    if (pair.x >= 0) copy_slice(c, pair.x, pair.y, (int)(i - (int64_t)p * c.slices));
+    if (pair.x >= 0) copy_slice<LONG>(c, pair.x, pair.y, (int)(i - (int64_t)p * c.slices[LONG]));
   }
 }
+__device__ __forceinline__ void copy_pairs(const CopyPlan& c, const int2* pairs, int count, int group, int groups) {
+  if (count * c.bytes >= kLongCopy) copy_pairs<1>(c, pairs, count, group, groups);
+  else copy_pairs<0>(c, pairs, count, group, groups);
+}
+
+// tkv_copy_pages_args without its set.
+struct PairLists {
+  const int32_t *src, *dst;
+  int32_t* work;
+  int32_t n, src_pages, dst_pages, same;
+};
 
 // Whether the lists name a pair at all.
-__device__ __forceinline__ bool is_pair(const tkv_copy_pages_args& a, int s, int d) {
+__device__ __forceinline__ bool is_pair(const PairLists& a, int s, int d) {
   return s >= 0 && s < a.src_pages && d >= 0 && d < a.dst_pages && !(a.same && s == d);
 }
 
 // A few pairs: every workgroup checks its own pair against all of them.  A pair
 // is carried out unless an earlier one has its destination or, within one set
 // of pools, any one reads it.
-__global__ void __launch_bounds__(256) copy_few_kernel(CopyPlan c, tkv_copy_pages_args a) {
-  const int64_t items = (int64_t)a.n * c.slices;
+template <int LONG>
+__global__ void __launch_bounds__(kCopy) copy_few_kernel(CopyPlan c, PairLists a) {
+  const int64_t items = (int64_t)a.n * c.slices[LONG];
   for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
-    const int p = (int)(i / c.slices);
+    const int p = (int)(i / c.slices[LONG]);
     const int s = a.src[p], d = a.dst[p];
     bool bad = !is_pair(a, s, d);
-    for (int x = threadIdx.x; x < a.n; x += 256) {
+    for (int x = threadIdx.x; x < a.n; x += kCopy) {
       const int sx = a.src[x], dx = a.dst[x];
       if (is_pair(a, sx, dx) && ((x < p && dx == d) || (a.same && sx == d))) bad = true;
     }
-    if (!__syncthreads_or(bad)) copy_slice(c, s, d, (int)(i - (int64_t)p * c.slices));
+    if (!__syncthreads_or(bad)) copy_slice<LONG>(c, s, d, (int)(i - (int64_t)p * c.slices[LONG]));
   }
 }
 
 // Many pairs: the same rule in three passes of one workgroup over the pages
 // that the pairs name (owner: the first pair of a destination; read: a source).
-__global__ void __launch_bounds__(kPlan) copy_check_kernel(tkv_copy_pages_args a) {
+__global__ void __launch_bounds__(kPlan) copy_check_kernel(PairLists a) {
   int* owner = a.work;
   int* read = owner + a.dst_pages;
   int2* pairs = reinterpret_cast<int2*>(a.work + a.dst_pages + a.src_pages + (((a.dst_pages + a.src_pages) & 1)));
@@ -123,7 +148,7 @@ __global__ void __launch_bounds__(kPlan) copy_check_kernel(tkv_copy_pages_args a
   }
 }
 
-__global__ void __launch_bounds__(256) copy_pairs_kernel(CopyPlan c, const int2* pairs, const int* count, int n) {
+__global__ void __launch_bounds__(kCopy) copy_pairs_kernel(CopyPlan c, const int2* pairs, const int* count, int n) {
   copy_pairs(c, pairs, count ? *count : n, blockIdx.x, gridDim.x);
 }
 
@@ -196,6 +221,14 @@ __device__ __forceinline__ int pages_per_thread(int N) {
 // child of a keeps it as a full page, and of the children that end in it the heir
 // is a itself or the lowest; every other child copies it to its first new page.
 // ---------------------------------------------------------------------------
+// tkv_fork_rows_args without its set.
+struct RowsParams {
+  int32_t *block_table, *seq_lens, *refs;
+  const int32_t *parents, *new_lens;
+  int32_t *status, *work;
+  int32_t table_stride, B, max_pages, page_size, num_pages;
+};
+
 struct RowsWork {  // a.work, in int32
   int* head;       // status, copies, new pages
   int *old_len, *kept, *first, *pages;
@@ -207,7 +240,7 @@ __host__ __device__ inline int64_t rows_work_ints(int64_t B, int64_t P, int64_t 
   return 16 + 6 * B + N + (staged ? B * P : 0);
 }
 
-__device__ __forceinline__ RowsWork rows_work(const tkv_fork_rows_args& a) {
+__device__ __forceinline__ RowsWork rows_work(const RowsParams& a) {
   RowsWork w;
   int* p = a.work;
   w.head = p;
@@ -226,9 +259,9 @@ struct Row {
   bool rest;             // ... of which some tokens are kept
 };
 
-__device__ __forceinline__ int table_tokens(const tkv_fork_rows_args& a) { return a.max_pages * a.page_size; }
+__device__ __forceinline__ int table_tokens(const RowsParams& a) { return a.max_pages * a.page_size; }
 
-__device__ __forceinline__ Row row_of(const tkv_fork_rows_args& a, int b) {
+__device__ __forceinline__ Row row_of(const RowsParams& a, int b) {
   Row r;
   r.a = a.parents ? a.parents[b] : b;
   if (r.a < 0 || r.a >= a.B) r.a = -1;
@@ -241,7 +274,7 @@ __device__ __forceinline__ Row row_of(const tkv_fork_rows_args& a, int b) {
   return r;
 }
 
-__global__ void __launch_bounds__(kPlan) rows_plan_kernel(tkv_fork_rows_args a) {
+__global__ void __launch_bounds__(kPlan) rows_plan_kernel(RowsParams a) {
   extern __shared__ int lds[];
   __shared__ ScanLds scan;
   __shared__ int past;
@@ -261,19 +294,29 @@ __global__ void __launch_bounds__(kPlan) rows_plan_kernel(tkv_fork_rows_args a) 
     best[b] = B;
   }
   if (tid == 0) past = 0;
+  // This thread's first row and first pages stay in registers: most plans need no others.
+  const int per = pages_per_thread(N);
+  const uint64_t mask0 = used_mask(a.refs, (int64_t)tid * per, per, N);
+  Row row0{-1, 0, 0, -1, false};
+  int owners0 = 0;  // references of the page that it ends in
+  if (tid < B) {
+    row0 = row_of(a, tid);
+    if (row0.last >= 0 && row0.last < N) owners0 = a.refs[row0.last];
+  }
   __syncthreads();
   for (int b = tid; b < B; b += kPlan) {
-    const Row r = row_of(a, b);
+    const Row r = b == tid ? row0 : row_of(a, b);
     if (r.a >= 0) atomicMax(most + r.a, r.f);
     if (r.want > table_tokens(a)) past = 1;
   }
   __syncthreads();
-  auto may_inherit = [&](const Row& r) {
-    return r.rest && r.f == most[r.a] && r.last >= 0 && r.last < N && a.refs[r.last] == 1;
+  auto may_inherit = [&](const Row& r, int b) {
+    if (!r.rest || r.f != most[r.a] || r.last < 0 || r.last >= N) return false;
+    return (b == tid ? owners0 : a.refs[r.last]) == 1;
   };
   for (int b = tid; b < B; b += kPlan) {
-    const Row r = row_of(a, b);
-    if (may_inherit(r)) atomicMin(best + r.a, r.a == b ? -1 : b);
+    const Row r = b == tid ? row0 : row_of(a, b);
+    if (may_inherit(r, b)) atomicMin(best + r.a, r.a == b ? -1 : b);
   }
   __syncthreads();
   const bool too_long = past != 0;
@@ -284,8 +327,8 @@ __global__ void __launch_bounds__(kPlan) rows_plan_kernel(tkv_fork_rows_args a) 
     int need = 0, pages = 0;
     bool heir = false, copy = false;
     if (b < B) {
-      r = row_of(a, b);
-      heir = may_inherit(r) && best[r.a] == (r.a == b ? -1 : b);
+      r = b == tid ? row0 : row_of(a, b);
+      heir = may_inherit(r, b) && best[r.a] == (r.a == b ? -1 : b);
       pages = (int)(((int64_t)r.want + a.page_size - 1) / a.page_size);
       // (a row that does not fit its table asks for nothing: the call fails)
       need = too_long ? 0 : pages - r.f - (heir ? 1 : 0);
@@ -305,10 +348,9 @@ __global__ void __launch_bounds__(kPlan) rows_plan_kernel(tkv_fork_rows_args a) 
   }
   // The lowest free pages.
   int found = 0;
-  const int per = pages_per_thread(N);
   for (int64_t p0 = 0; p0 < N && found < done.x; p0 += (int64_t)per * kPlan) {
     const int64_t mine = p0 + (int64_t)tid * per;
-    uint64_t m = ~used_mask(a.refs, mine, per, N) & first_bits(N - mine) & first_bits(per);
+    uint64_t m = ~(p0 ? used_mask(a.refs, mine, per, N) : mask0) & first_bits(N - mine) & first_bits(per);
     int2 total;
     int at = found + block_scan(scan, __popcll(m), 0, total).x;
     for (; m && at < done.x; m &= m - 1) w.fresh[at++] = (int)(mine + __builtin_ctzll(m));
@@ -331,7 +373,7 @@ __global__ void __launch_bounds__(kPlan) rows_plan_kernel(tkv_fork_rows_args a) 
 }
 
 // Workgroups [0, tables): the table, lengths and counts; the others: the copies.
-__global__ void __launch_bounds__(256) rows_apply_kernel(tkv_fork_rows_args a, CopyPlan c, int tables) {
+__global__ void __launch_bounds__(kCopy) rows_apply_kernel(RowsParams a, CopyPlan c, int tables) {
   const RowsWork w = rows_work(a);
   if (w.head[0] != TKV_ROWS_DONE) return;
   if ((int)blockIdx.x >= tables) {
@@ -340,7 +382,7 @@ __global__ void __launch_bounds__(256) rows_apply_kernel(tkv_fork_rows_args a, C
   }
   const int P = a.max_pages, N = a.num_pages;
   const int64_t entries = (int64_t)a.B * P;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)tables * 256) {
+  for (int64_t i = (int64_t)blockIdx.x * kCopy + threadIdx.x; i < entries; i += (int64_t)tables * kCopy) {
     const int b = (int)(i / P), slot = (int)(i - (int64_t)b * P);
     int* at = a.block_table + (int64_t)b * a.table_stride + slot;
     const int old = *at, kept = w.kept[b], pages = w.pages[b];
@@ -372,6 +414,13 @@ __global__ void __launch_bounds__(256) rows_apply_kernel(tkv_fork_rows_args a, C
 // Compaction: with n live pages (refs > 0), the i-th live page at or past n moves
 // to the i-th free page below n.
 // ---------------------------------------------------------------------------
+// tkv_compact_pages_args without its set.
+struct CompactParams {
+  const int32_t *block_table, *refs;
+  int32_t *out_table, *out_refs, *live, *work;
+  int32_t table_stride, out_stride, B, max_pages, num_pages;
+};
+
 struct CompactWork {
   int* head;   // live pages, moves
   int2* pairs;
@@ -381,7 +430,7 @@ struct CompactWork {
 
 __host__ __device__ inline int64_t compact_work_ints(int64_t N) { return 16 + (N + 2) + N + N / 2 + 1; }
 
-__device__ __forceinline__ CompactWork compact_work(const tkv_compact_pages_args& a) {
+__device__ __forceinline__ CompactWork compact_work(const CompactParams& a) {
   CompactWork w;
   w.head = a.work;
   w.pairs = reinterpret_cast<int2*>(a.work + 16);  // at most N / 2 moves
@@ -390,7 +439,7 @@ __device__ __forceinline__ CompactWork compact_work(const tkv_compact_pages_args
   return w;
 }
 
-__global__ void __launch_bounds__(kPlan) compact_plan_kernel(tkv_compact_pages_args a) {
+__global__ void __launch_bounds__(kPlan) compact_plan_kernel(CompactParams a) {
   __shared__ ScanLds scan;
   const CompactWork w = compact_work(a);
   const int tid = threadIdx.x, N = a.num_pages, per = pages_per_thread(N);
@@ -436,7 +485,7 @@ __global__ void __launch_bounds__(kPlan) compact_plan_kernel(tkv_compact_pages_a
 }
 
 // Workgroups [0, tables): the table and the counts; the others: the copies.
-__global__ void __launch_bounds__(256) compact_apply_kernel(tkv_compact_pages_args a, CopyPlan c, int tables) {
+__global__ void __launch_bounds__(kCopy) compact_apply_kernel(CompactParams a, CopyPlan c, int tables) {
   const CompactWork w = compact_work(a);
   const int live = w.head[0];
   if ((int)blockIdx.x >= tables) {
@@ -445,7 +494,7 @@ __global__ void __launch_bounds__(256) compact_apply_kernel(tkv_compact_pages_ar
   }
   const int P = a.max_pages, N = a.num_pages;
   const int64_t entries = (int64_t)a.B * P;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries + N; i += (int64_t)tables * 256) {
+  for (int64_t i = (int64_t)blockIdx.x * kCopy + threadIdx.x; i < entries + N; i += (int64_t)tables * kCopy) {
     if (i < entries) {
       const int b = (int)(i / P), slot = (int)(i - (int64_t)b * P);
       int page = a.block_table[(int64_t)b * a.table_stride + slot];
@@ -465,26 +514,33 @@ __global__ void __launch_bounds__(256) compact_apply_kernel(tkv_compact_pages_ar
 static int make_plan(const tkv_page_set& s, CopyPlan& c) {
   if (s.count < 0 || s.count > TKV_PAGE_TENSORS) return TKV_EINVAL;
   c.set = s;
-  int64_t slices = 0;
+  c.bytes = 0;
+  int64_t slices[2] = {0, 0};
   for (int t = 0; t < s.count; ++t) {
     if (!s.src[t] || !s.dst[t] || s.bytes[t] <= 0) return TKV_EINVAL;
     if (((uintptr_t)s.src[t] | (uintptr_t)s.dst[t] | (uint64_t)s.bytes[t] | (uint64_t)s.src_stride[t] |
          (uint64_t)s.dst_stride[t]) & 15)
       return TKV_EINVAL;
     if (s.src_stride[t] < s.bytes[t] || s.dst_stride[t] < s.bytes[t]) return TKV_EINVAL;
-    c.first[t] = (int32_t)slices;
-    slices += (s.bytes[t] + kSlice - 1) / kSlice;
-    if (slices > INT32_MAX) return TKV_EUNSUPPORTED;
+    for (int k = 0; k < 2; ++k) {
+      c.first[k][t] = (int32_t)slices[k];
+      slices[k] += (s.bytes[t] + kSlices[k] - 1) / kSlices[k];
+      if (slices[k] > INT32_MAX) return TKV_EUNSUPPORTED;
+    }
+    c.bytes += s.bytes[t];
   }
-  for (int t = s.count; t < TKV_PAGE_TENSORS; ++t) c.first[t] = INT32_MAX;
-  c.slices = (int32_t)slices;
+  for (int k = 0; k < 2; ++k) {
+    for (int t = s.count; t < TKV_PAGE_TENSORS; ++t) c.first[k][t] = INT32_MAX;
+    c.slices[k] = (int32_t)slices[k];
+  }
   return TKV_OK;
 }
 
-constexpr int kCopyGroups = 4096;  // workgroups that stride over the copies
+constexpr int kCopyGroups = 8192;  // workgroups that stride over the copies
 
+// Workgroups for at most `pairs` copies.
 static unsigned copy_groups(int64_t pairs, const CopyPlan& c) {
-  const int64_t items = pairs * c.slices;
+  const int64_t items = pairs * c.slices[0];
   return (unsigned)(items < kCopyGroups ? items : kCopyGroups);
 }
 
@@ -507,18 +563,21 @@ extern "C" int tkv_copy_pages(const tkv_copy_pages_args* a, tkv_stream_t stream)
   CopyPlan c;
   const int rc = make_plan(a->set, c);
   if (rc) return rc;
-  if (!c.slices) return TKV_OK;
+  if (!c.slices[0]) return TKV_OK;
+  if (a->n > kInlinePairs && (!a->work || (uintptr_t)a->work & 7)) return TKV_EINVAL;
+  const PairLists p{a->src, a->dst, a->work, a->n, a->src_pages, a->dst_pages, a->same};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   (void)hipGetLastError();
   const dim3 grid(copy_groups(a->n, c));
-  if (a->n <= kInlinePairs) {
-    copy_few_kernel<<<grid, dim3(256), 0, st>>>(c, *a);
-  } else {
-    if (!a->work || (uintptr_t)a->work & 7) return TKV_EINVAL;
+  if (a->n > kInlinePairs) {
     const int pages = a->dst_pages + a->src_pages;
     const int2* pairs = reinterpret_cast<const int2*>(a->work + pages + (pages & 1));
-    copy_check_kernel<<<dim3(1), dim3(kPlan), 0, st>>>(*a);
-    copy_pairs_kernel<<<grid, dim3(256), 0, st>>>(c, pairs, nullptr, a->n);
+    copy_check_kernel<<<dim3(1), dim3(kPlan), 0, st>>>(p);
+    copy_pairs_kernel<<<grid, dim3(kCopy), 0, st>>>(c, pairs, nullptr, a->n);
+  } else if (a->n * c.bytes >= kLongCopy) {
+    copy_few_kernel<1><<<grid, dim3(kCopy), 0, st>>>(c, p);
+  } else {
+    copy_few_kernel<0><<<grid, dim3(kCopy), 0, st>>>(c, p);
   }
   return launched();
 }
@@ -543,10 +602,12 @@ extern "C" int tkv_fork_rows(const tkv_fork_rows_args* a, tkv_stream_t stream) {
   (void)hipGetLastError();
   const int64_t entries = (int64_t)a->B * a->max_pages;
   const unsigned staging = a->parents ? (unsigned)((entries + 4 * kPlan - 1) / (4 * kPlan)) : 0;
-  rows_plan_kernel<<<dim3(1 + (staging < 512 ? staging : 512)), dim3(kPlan), 2 * sizeof(int) * a->B, st>>>(*a);
-  const int64_t tables = (entries + 255) / 256;
-  const int t = (int)(tables < 2048 ? tables : 2048);
-  rows_apply_kernel<<<dim3(t + copy_groups(a->B, c)), dim3(256), 0, st>>>(*a, c, t);
+  const RowsParams p{a->block_table, a->seq_lens, a->refs, a->parents, a->new_lens, a->status, a->work,
+                     a->table_stride, a->B, a->max_pages, a->page_size, a->num_pages};
+  rows_plan_kernel<<<dim3(1 + (staging < 512 ? staging : 512)), dim3(kPlan), 2 * sizeof(int) * a->B, st>>>(p);
+  const int64_t tables = (entries + kCopy - 1) / kCopy;
+  const int t = (int)(tables < 512 ? tables : 512);
+  rows_apply_kernel<<<dim3(t + copy_groups(a->B, c)), dim3(kCopy), 0, st>>>(p, c, t);
   return launched();
 }
 
@@ -566,10 +627,12 @@ extern "C" int tkv_compact_pages(const tkv_compact_pages_args* a, tkv_stream_t s
   if (rc) return rc;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   (void)hipGetLastError();
-  compact_plan_kernel<<<dim3(1), dim3(kPlan), 0, st>>>(*a);
-  const int64_t tables = ((int64_t)a->B * a->max_pages + a->num_pages + 255) / 256;
-  const int t = (int)(tables < 2048 ? tables : 2048);
-  compact_apply_kernel<<<dim3(t + copy_groups(a->num_pages / 2, c)), dim3(256), 0, st>>>(*a, c, t);
+  const CompactParams p{a->block_table, a->refs, a->out_table, a->out_refs, a->live, a->work,
+                        a->table_stride, a->out_stride, a->B, a->max_pages, a->num_pages};
+  compact_plan_kernel<<<dim3(1), dim3(kPlan), 0, st>>>(p);
+  const int64_t tables = ((int64_t)a->B * a->max_pages + a->num_pages + kCopy - 1) / kCopy;
+  const int t = (int)(tables < 512 ? tables : 512);
+  compact_apply_kernel<<<dim3(t + copy_groups(a->num_pages / 2, c)), dim3(kCopy), 0, st>>>(p, c, t);
   return launched();
 }
 
@@ -583,7 +646,7 @@ extern "C" int tkv_copy_planned(const tkv_page_set* set, const int32_t* work, in
   const unsigned groups = copy_groups(most, c);
   if (!groups) return TKV_OK;
   (void)hipGetLastError();
-  copy_pairs_kernel<<<dim3(groups), dim3(256), 0, reinterpret_cast<hipStream_t>(stream)>>>(
+  copy_pairs_kernel<<<dim3(groups), dim3(kCopy), 0, reinterpret_cast<hipStream_t>(stream)>>>(
       c, reinterpret_cast<const int2*>(work + 16), work + 1, 0);
   return launched();
 }

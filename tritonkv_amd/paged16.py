@@ -83,7 +83,7 @@ def _int32_arg(t, n: int, device, name: str, what: str):
     return t.contiguous()
 
 
-MAX_WORKGROUPS = 65535  # grid y-dimension limit
+MAX_ROWS = MAX_WORKGROUPS = 65535  # grid y-dimension limit
 
 
 def plan_shares(B: int, HKV: int, G: int, S: int, D: int = 128, device=None,
@@ -113,8 +113,8 @@ def plan_shares(B: int, HKV: int, G: int, S: int, D: int = 128, device=None,
       128 chunks at head dim 64 (32 rows of up to 16384 132, 126; 8 rows 38.5, 39.4).
     """
     units = HKV * -(-G // 16)
-    if B > MAX_WORKGROUPS:
-        raise ValueError(f"at most {MAX_WORKGROUPS} rows, got {B}")
+    if B > MAX_ROWS:
+        raise ValueError(f"at most {MAX_ROWS} rows, got {B}")
     if piece_tokens is not None:
         if piece_tokens <= 0:
             raise ValueError(f"piece_tokens must be positive, got {piece_tokens}")
@@ -215,6 +215,8 @@ def paged16_append(k_pool: torch.Tensor, v_pool: torch.Tensor, k_new: torch.Tens
     if k_new.shape != v_new.shape or k_new.dtype != v_new.dtype:
         raise ValueError("k_new and v_new must have the same shape and dtype")
     B, _, N, _ = k_new.shape
+    if B > MAX_ROWS or N * HKV * D // 8 > 2 ** 31 - 1:
+        raise ValueError(f"k_new and v_new: at most {MAX_ROWS} rows of 2**34 values, got {tuple(k_new.shape)}")
     table = _check_table(block_table, B, device)
     pos = _int32_arg(positions, B, device, "positions", "B start positions")
     num = None if counts is None else _int32_arg(counts, B, device, "counts", "B token counts")
