@@ -17,6 +17,7 @@
 // the output would be 2e-4 (fp16) or 2e-3 (bf16) off, and the extra MFMAs
 // run in the shadow of the loads.
 #include "decode_common.h"
+#include "launch.h"
 
 namespace tkv {
 
@@ -709,34 +710,33 @@ static int check_paged16(const tkv_paged16_args* a) {
 }
 
 template <class T, int D, int NW>
-static void launch_paged16(const Paged16Params& p, hipStream_t st) {
+static int launch_paged16(const Paged16Params& p, hipStream_t st) {
   const int rows = p.G < 16 ? p.G : 16;
   const dim3 grid((unsigned)(p.a.HKV * ((p.G + 15) / 16)), (unsigned)(p.a.workgroups ? p.a.workgroups : p.a.B));
   const size_t lds = 32 * (D + 8) + sizeof(float) * NW * (rows * (D + 1) + 2 * rows);
-  if (p.a.k_new)
-    paged16_split_kernel<T, D, NW, true><<<grid, dim3(NW * 64), lds + 4 * D, st>>>(p);
-  else
-    paged16_split_kernel<T, D, NW, false><<<grid, dim3(NW * 64), lds, st>>>(p);
+  return p.a.k_new ? launch(paged16_split_kernel<T, D, NW, true>, grid, dim3(NW * 64), lds + 4 * D, st, p)
+                   : launch(paged16_split_kernel<T, D, NW, false>, grid, dim3(NW * 64), lds, st, p);
 }
 
 template <int D>
-static void launch_join(const Paged16Params& p, float shift, hipStream_t st) {
+static int launch_join(const Paged16Params& p, float shift, hipStream_t st) {
   const int rows = p.a.B * p.a.HQ;
-  if (rows >= kJoinRows) paged16_join_kernel<D, 64><<<dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st>>>(p, shift);
-  else paged16_join_kernel<D, 256><<<dim3((unsigned)rows), dim3(256), 0, st>>>(p, shift);
+  return rows >= kJoinRows
+             ? launch(paged16_join_kernel<D, 64>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, shift)
+             : launch(paged16_join_kernel<D, 256>, dim3((unsigned)rows), dim3(256), 0, st, p, shift);
 }
 
 template <class T, int D>
-static void dispatch_paged16(const Paged16Params& p, hipStream_t st) {
-  launch_paged16<T, D, 4>(p, st);
-  if (p.a.workgroups) launch_join<D>(p, T::kShift, st);
+static int dispatch_paged16(const Paged16Params& p, hipStream_t st) {
+  const int rc = launch_paged16<T, D, 4>(p, st);
+  return rc || !p.a.workgroups ? rc : launch_join<D>(p, T::kShift, st);
 }
 
 template <class T>
-static void dispatch_paged16(const Paged16Params& p, hipStream_t st) {
-  if (p.a.D == 64) dispatch_paged16<T, 64>(p, st);
-  else if (p.a.D == 128) dispatch_paged16<T, 128>(p, st);
-  else dispatch_paged16<T, 256>(p, st);
+static int dispatch_paged16(const Paged16Params& p, hipStream_t st) {
+  if (p.a.D == 64) return dispatch_paged16<T, 64>(p, st);
+  if (p.a.D == 128) return dispatch_paged16<T, 128>(p, st);
+  return dispatch_paged16<T, 256>(p, st);
 }
 
 }  // namespace tkv
@@ -755,12 +755,8 @@ extern "C" int tkv_paged16_decode_attention(const tkv_paged16_args* a, tkv_strea
     p.k16[i] = (uint32_t)(a->k_strides[i] / 8);
     p.v16[i] = (uint32_t)(a->v_strides[i] / 8);
   }
-  (void)hipGetLastError();
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (a->is_bf16) dispatch_paged16<Bf16>(p, st);
-  else dispatch_paged16<Half>(p, st);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? TKV_OK : (int)e;
+  return a->is_bf16 ? dispatch_paged16<Bf16>(p, st) : dispatch_paged16<Half>(p, st);
 }
 
 extern "C" int tkv_paged16_append(const tkv_paged16_append_args* a, tkv_stream_t stream) {
@@ -780,14 +776,9 @@ extern "C" int tkv_paged16_append(const tkv_paged16_append_args* a, tkv_stream_t
   const dim3 grid((unsigned)(2 * blocks), (unsigned)a->B);
   const uint32_t n = (uint32_t)items;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  (void)hipGetLastError();
-  if (a->is_bf16) {
-    if (a->new_is_fp32) paged16_append_kernel<Bf16, true><<<grid, dim3(256), 0, st>>>(*a, n);
-    else paged16_append_kernel<Bf16, false><<<grid, dim3(256), 0, st>>>(*a, n);
-  } else {
-    if (a->new_is_fp32) paged16_append_kernel<Half, true><<<grid, dim3(256), 0, st>>>(*a, n);
-    else paged16_append_kernel<Half, false><<<grid, dim3(256), 0, st>>>(*a, n);
-  }
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? TKV_OK : (int)e;
+  if (a->is_bf16)
+    return a->new_is_fp32 ? launch(paged16_append_kernel<Bf16, true>, grid, dim3(256), 0, st, *a, n)
+                          : launch(paged16_append_kernel<Bf16, false>, grid, dim3(256), 0, st, *a, n);
+  return a->new_is_fp32 ? launch(paged16_append_kernel<Half, true>, grid, dim3(256), 0, st, *a, n)
+                        : launch(paged16_append_kernel<Half, false>, grid, dim3(256), 0, st, *a, n);
 }

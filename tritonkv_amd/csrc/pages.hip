@@ -10,6 +10,7 @@
 // integer sums, maxima and minima.
 #include <hip/hip_runtime.h>
 
+#include "launch.h"
 #include "tkv_device.h"
 #include "../../include/tkv.h"
 
@@ -544,11 +545,6 @@ static unsigned copy_groups(int64_t pairs, const CopyPlan& c) {
   return (unsigned)(items < kCopyGroups ? items : kCopyGroups);
 }
 
-static int launched() {
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? TKV_OK : (int)e;
-}
-
 }  // namespace tkv
 
 extern "C" int64_t tkv_copy_pages_work(int32_t n, int32_t src_pages, int32_t dst_pages) {
@@ -567,19 +563,14 @@ extern "C" int tkv_copy_pages(const tkv_copy_pages_args* a, tkv_stream_t stream)
   if (a->n > kInlinePairs && (!a->work || (uintptr_t)a->work & 7)) return TKV_EINVAL;
   const PairLists p{a->src, a->dst, a->work, a->n, a->src_pages, a->dst_pages, a->same};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  (void)hipGetLastError();
-  const dim3 grid(copy_groups(a->n, c));
-  if (a->n > kInlinePairs) {
-    const int pages = a->dst_pages + a->src_pages;
-    const int2* pairs = reinterpret_cast<const int2*>(a->work + pages + (pages & 1));
-    copy_check_kernel<<<dim3(1), dim3(kPlan), 0, st>>>(p);
-    copy_pairs_kernel<<<grid, dim3(kCopy), 0, st>>>(c, pairs, nullptr, a->n);
-  } else if (a->n * c.bytes >= kLongCopy) {
-    copy_few_kernel<1><<<grid, dim3(kCopy), 0, st>>>(c, p);
-  } else {
-    copy_few_kernel<0><<<grid, dim3(kCopy), 0, st>>>(c, p);
-  }
-  return launched();
+  const dim3 grid(copy_groups(a->n, c)), block(kCopy);
+  if (a->n <= kInlinePairs)
+    return a->n * c.bytes >= kLongCopy ? launch(copy_few_kernel<1>, grid, block, 0, st, c, p)
+                                       : launch(copy_few_kernel<0>, grid, block, 0, st, c, p);
+  const int pages = a->dst_pages + a->src_pages;
+  const int2* pairs = reinterpret_cast<const int2*>(a->work + pages + (pages & 1));
+  const int bad = launch(copy_check_kernel, dim3(1), dim3(kPlan), 0, st, p);
+  return bad ? bad : launch(copy_pairs_kernel, grid, block, 0, st, c, pairs, (const int*)nullptr, (int)a->n);
 }
 
 extern "C" int64_t tkv_fork_rows_work(int32_t B, int32_t max_pages, int32_t num_pages, int32_t parents) {
@@ -599,16 +590,16 @@ extern "C" int tkv_fork_rows(const tkv_fork_rows_args* a, tkv_stream_t stream) {
   const int rc = make_plan(a->set, c);
   if (rc) return rc;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  (void)hipGetLastError();
   const int64_t entries = (int64_t)a->B * a->max_pages;
   const unsigned staging = a->parents ? (unsigned)((entries + 4 * kPlan - 1) / (4 * kPlan)) : 0;
   const RowsParams p{a->block_table, a->seq_lens, a->refs, a->parents, a->new_lens, a->status, a->work,
                      a->table_stride, a->B, a->max_pages, a->page_size, a->num_pages};
-  rows_plan_kernel<<<dim3(1 + (staging < 512 ? staging : 512)), dim3(kPlan), 2 * sizeof(int) * a->B, st>>>(p);
+  const int bad = launch(rows_plan_kernel, dim3(1 + (staging < 512 ? staging : 512)), dim3(kPlan),
+                         2 * sizeof(int) * a->B, st, p);
+  if (bad) return bad;
   const int64_t tables = (entries + kCopy - 1) / kCopy;
   const int t = (int)(tables < 512 ? tables : 512);
-  rows_apply_kernel<<<dim3(t + copy_groups(a->B, c)), dim3(kCopy), 0, st>>>(p, c, t);
-  return launched();
+  return launch(rows_apply_kernel, dim3(t + copy_groups(a->B, c)), dim3(kCopy), 0, st, p, c, t);
 }
 
 extern "C" int64_t tkv_compact_pages_work(int32_t num_pages) {
@@ -626,14 +617,13 @@ extern "C" int tkv_compact_pages(const tkv_compact_pages_args* a, tkv_stream_t s
   const int rc = make_plan(a->set, c);
   if (rc) return rc;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  (void)hipGetLastError();
   const CompactParams p{a->block_table, a->refs, a->out_table, a->out_refs, a->live, a->work,
                         a->table_stride, a->out_stride, a->B, a->max_pages, a->num_pages};
-  compact_plan_kernel<<<dim3(1), dim3(kPlan), 0, st>>>(p);
+  const int bad = launch(compact_plan_kernel, dim3(1), dim3(kPlan), 0, st, p);
+  if (bad) return bad;
   const int64_t tables = ((int64_t)a->B * a->max_pages + a->num_pages + kCopy - 1) / kCopy;
   const int t = (int)(tables < 512 ? tables : 512);
-  compact_apply_kernel<<<dim3(t + copy_groups(a->num_pages / 2, c)), dim3(kCopy), 0, st>>>(p, c, t);
-  return launched();
+  return launch(compact_apply_kernel, dim3(t + copy_groups(a->num_pages / 2, c)), dim3(kCopy), 0, st, p, c, t);
 }
 
 // The copies of a plan in further tensors: pairs and their count as the plan left them.
@@ -645,8 +635,6 @@ extern "C" int tkv_copy_planned(const tkv_page_set* set, const int32_t* work, in
   if (rc) return rc;
   const unsigned groups = copy_groups(most, c);
   if (!groups) return TKV_OK;
-  (void)hipGetLastError();
-  copy_pairs_kernel<<<dim3(groups), dim3(kCopy), 0, reinterpret_cast<hipStream_t>(stream)>>>(
-      c, reinterpret_cast<const int2*>(work + 16), work + 1, 0);
-  return launched();
+  return launch(copy_pairs_kernel, dim3(groups), dim3(kCopy), 0, reinterpret_cast<hipStream_t>(stream), c,
+                reinterpret_cast<const int2*>(work + 16), (const int*)(work + 1), 0);
 }

@@ -136,9 +136,11 @@ def plan_shares(B: int, HKV: int, G: int, S: int, D: int = 128, device=None,
 
 
 def _buffer(ws: dict, name: str, n: int, dtype, device) -> torch.Tensor:
-    """A workspace buffer of n entries; one that is in use is never replaced, since a
-    captured graph may hold its address."""
-    key = (name, n, str(device))
+    """A workspace buffer of at least n entries.  One that was handed out is never
+    dropped, since a captured graph may hold its address; sizes are powers of two, so
+    that those of a varying batch come to twice the largest at most."""
+    n = 1 << max(0, n - 1).bit_length()
+    key = (name, n, device)
     t = ws.get(key)
     if t is None:
         t = ws[key] = torch.empty(n, dtype=dtype, device=device)
