@@ -29,64 +29,70 @@ __device__ __forceinline__ void settle() {
 }
 
 // ---------------------------------------------------------------------------
-// The copy.  Item = one slice of one tensor's page; workgroups stride over the
-// items of the first `count` pairs.
+// The copy.  Item = one 16 KiB slice of one tensor's page (the last of a page may be
+// less); the items of all pairs lie in a row, and workgroups stride over them RUN at
+// a time: they read RUN slices whole before they write any of them.
 //
-// Bound by HBM.  A slice of 64 KiB, read whole by 1024 threads before any of it is
-// written, copies 4000 scattered pages of 128 KiB at 5.9 TB/s; 16 KiB by 256
-// threads 5.1, 64 KiB by 256 threads 5.2, torch's copy_ of 2 GiB 4.9.  Where the
-// call copies less than 32 MiB, slices of 16 KiB reach more CUs.  Both without
-// keeping the bytes in the caches (non-temporal; 4% on the large ones).
+// Bound by HBM, and by how its reads and writes alternate: 4000 scattered pages of 128
+// KiB go at 5.9 TB/s in runs of 64 KiB by 1024 threads, at 5.1 in 16 KiB by 256 threads,
+// at 5.2 in 64 KiB by 256; torch's copy_ of 2 GiB at 4.9.  Where a call copies less
+// than 32 MiB, runs of one slice reach more CUs.  The bytes pass by the caches
+// (non-temporal loads and stores: 4% on the large ones).
 // ---------------------------------------------------------------------------
-constexpr int kSlices[2] = {16384, 65536};
+constexpr int kSlice = kCopy * 16;
+constexpr int kRun = 4;
 constexpr int64_t kLongCopy = 32 << 20;
 
 struct CopyPlan {
   tkv_page_set set;
-  int32_t first[2][TKV_PAGE_TENSORS];  // slices of a page before tensor t, of either size
-  int32_t slices[2];                   // of a page, in all tensors
-  int64_t bytes;                       // of a page, in all tensors
+  int32_t first[TKV_PAGE_TENSORS];  // slices of a page before tensor t
+  int32_t slices;                   // of a page, in all tensors
+  int64_t bytes;                    // of a page, in all tensors
 };
 
-template <int LONG>
-__device__ __forceinline__ void copy_slice(const CopyPlan& c, int src, int dst, int slice) {
-  constexpr int kSize = kSlices[LONG];
-  int t = 0;
+// Pair p of the copies as (source, destination); a negative source is no pair.
+// pair_of(p) may hold barriers: it is called by all threads alike.
+template <int RUN, class PairOf>
+__device__ __forceinline__ void copy_run(const CopyPlan& c, int64_t items, int group, int groups, PairOf pair_of) {
+  for (int64_t base = (int64_t)group * RUN; base < items; base += (int64_t)groups * RUN) {
+    int p = items <= UINT32_MAX ? (int)((uint32_t)base / (uint32_t)c.slices) : (int)(base / c.slices);
+    int s = (int)(base - (int64_t)p * c.slices);
+    int2 pair = pair_of(p);
+    u4 x[RUN];
+    u4* to[RUN];
 #pragma unroll
-  for (int step = TKV_PAGE_TENSORS / 2; step; step /= 2)
-    if (t + step < c.set.count && c.first[LONG][t + step] <= slice) t += step;
-  const int64_t at = (int64_t)(slice - c.first[LONG][t]) * kSize;
-  const int64_t left = c.set.bytes[t] - at;
-  const int units = (int)((left < kSize ? left : (int64_t)kSize) / 16);
-  const u4* from = reinterpret_cast<const u4*>(static_cast<const char*>(c.set.src[t]) + src * c.set.src_stride[t] + at);
-  u4* to = reinterpret_cast<u4*>(static_cast<char*>(c.set.dst[t]) + dst * c.set.dst_stride[t] + at);
-  constexpr int kPer = kSize / 16 / kCopy;
-  u4 x[kPer];
+    for (int i = 0; i < RUN; ++i) {
+      to[i] = nullptr;
+      if (base + i >= items) continue;
+      if (i) {
+        if (++s == c.slices) {
+          s = 0;
+          pair = pair_of(++p);
+        }
+      }
+      if (pair.x < 0) continue;
+      int t = 0;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int u = threadIdx.x + kCopy * i;
-    if (u < units) x[i] = __builtin_nontemporal_load(from + u);
-  }
+      for (int step = TKV_PAGE_TENSORS / 2; step; step /= 2)
+        if (t + step < c.set.count && c.first[t + step] <= s) t += step;
+      const int64_t at = (int64_t)(s - c.first[t]) * kSlice + threadIdx.x * 16;
+      if (at >= c.set.bytes[t]) continue;
+      x[i] = __builtin_nontemporal_load(
+          reinterpret_cast<const u4*>(static_cast<const char*>(c.set.src[t]) + pair.x * c.set.src_stride[t] + at));
+      to[i] = reinterpret_cast<u4*>(static_cast<char*>(c.set.dst[t]) + pair.y * c.set.dst_stride[t] + at);
+    }
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int u = threadIdx.x + kCopy * i;
-    if (u < units) __builtin_nontemporal_store(x[i], to + u);
+    for (int i = 0; i < RUN; ++i)
+      if (to[i]) __builtin_nontemporal_store(x[i], to[i]);
   }
 }
 
-// Pairs (x, y) = (source, destination); a negative source is no pair.
-template <int LONG>
+// The first `count` of a plan's pairs.
 __device__ __forceinline__ void copy_pairs(const CopyPlan& c, const int2* pairs, int count, int group, int groups) {
-  const int64_t items = (int64_t)count * c.slices[LONG];
-  for (int64_t i = group; i < items; i += groups) {
-    const int p = (int)(i / c.slices[LONG]);
-    const int2 pair = pairs[p];
-    if (pair.x >= 0) copy_slice<LONG>(c, pair.x, pair.y, (int)(i - (int64_t)p * c.slices[LONG]));
-  }
-}
-__device__ __forceinline__ void copy_pairs(const CopyPlan& c, const int2* pairs, int count, int group, int groups) {
-  if (count * c.bytes >= kLongCopy) copy_pairs<1>(c, pairs, count, group, groups);
-  else copy_pairs<0>(c, pairs, count, group, groups);
+  const int64_t items = (int64_t)count * c.slices;
+  auto pair_of = [&](int p) { return pairs[p]; };
+  if (count * c.bytes >= kLongCopy) copy_run<kRun>(c, items, group, groups, pair_of);
+  else copy_run<1>(c, items, group, groups, pair_of);
 }
 
 // tkv_copy_pages_args without its set.
@@ -104,19 +110,17 @@ __device__ __forceinline__ bool is_pair(const PairLists& a, int s, int d) {
 // A few pairs: every workgroup checks its own pair against all of them.  A pair
 // is carried out unless an earlier one has its destination or, within one set
 // of pools, any one reads it.
-template <int LONG>
+template <int RUN>
 __global__ void __launch_bounds__(kCopy) copy_few_kernel(CopyPlan c, PairLists a) {
-  const int64_t items = (int64_t)a.n * c.slices[LONG];
-  for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
-    const int p = (int)(i / c.slices[LONG]);
+  copy_run<RUN>(c, (int64_t)a.n * c.slices, blockIdx.x, gridDim.x, [&](int p) {
     const int s = a.src[p], d = a.dst[p];
     bool bad = !is_pair(a, s, d);
     for (int x = threadIdx.x; x < a.n; x += kCopy) {
       const int sx = a.src[x], dx = a.dst[x];
       if (is_pair(a, sx, dx) && ((x < p && dx == d) || (a.same && sx == d))) bad = true;
     }
-    if (!__syncthreads_or(bad)) copy_slice<LONG>(c, s, d, (int)(i - (int64_t)p * c.slices[LONG]));
-  }
+    return make_int2(__syncthreads_or(bad) ? -1 : s, d);
+  });
 }
 
 // Many pairs: the same rule in three passes of one workgroup over the pages
@@ -516,24 +520,20 @@ static int make_plan(const tkv_page_set& s, CopyPlan& c) {
   if (s.count < 0 || s.count > TKV_PAGE_TENSORS) return TKV_EINVAL;
   c.set = s;
   c.bytes = 0;
-  int64_t slices[2] = {0, 0};
+  int64_t slices = 0;
   for (int t = 0; t < s.count; ++t) {
     if (!s.src[t] || !s.dst[t] || s.bytes[t] <= 0) return TKV_EINVAL;
     if (((uintptr_t)s.src[t] | (uintptr_t)s.dst[t] | (uint64_t)s.bytes[t] | (uint64_t)s.src_stride[t] |
          (uint64_t)s.dst_stride[t]) & 15)
       return TKV_EINVAL;
     if (s.src_stride[t] < s.bytes[t] || s.dst_stride[t] < s.bytes[t]) return TKV_EINVAL;
-    for (int k = 0; k < 2; ++k) {
-      c.first[k][t] = (int32_t)slices[k];
-      slices[k] += (s.bytes[t] + kSlices[k] - 1) / kSlices[k];
-      if (slices[k] > INT32_MAX) return TKV_EUNSUPPORTED;
-    }
+    c.first[t] = (int32_t)slices;
+    slices += (s.bytes[t] + kSlice - 1) / kSlice;
+    if (slices > INT32_MAX) return TKV_EUNSUPPORTED;
     c.bytes += s.bytes[t];
   }
-  for (int k = 0; k < 2; ++k) {
-    for (int t = s.count; t < TKV_PAGE_TENSORS; ++t) c.first[k][t] = INT32_MAX;
-    c.slices[k] = (int32_t)slices[k];
-  }
+  for (int t = s.count; t < TKV_PAGE_TENSORS; ++t) c.first[t] = INT32_MAX;
+  c.slices = (int32_t)slices;
   return TKV_OK;
 }
 
@@ -541,7 +541,7 @@ constexpr int kCopyGroups = 8192;  // workgroups that stride over the copies
 
 // Workgroups for at most `pairs` copies.
 static unsigned copy_groups(int64_t pairs, const CopyPlan& c) {
-  const int64_t items = pairs * c.slices[0];
+  const int64_t items = pairs * c.slices;
   return (unsigned)(items < kCopyGroups ? items : kCopyGroups);
 }
 
@@ -559,14 +559,14 @@ extern "C" int tkv_copy_pages(const tkv_copy_pages_args* a, tkv_stream_t stream)
   CopyPlan c;
   const int rc = make_plan(a->set, c);
   if (rc) return rc;
-  if (!c.slices[0]) return TKV_OK;
+  if (!c.slices) return TKV_OK;
   if (a->n > kInlinePairs && (!a->work || (uintptr_t)a->work & 7)) return TKV_EINVAL;
   const PairLists p{a->src, a->dst, a->work, a->n, a->src_pages, a->dst_pages, a->same};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(copy_groups(a->n, c)), block(kCopy);
   if (a->n <= kInlinePairs)
-    return a->n * c.bytes >= kLongCopy ? launch(copy_few_kernel<1>, grid, block, 0, st, c, p)
-                                       : launch(copy_few_kernel<0>, grid, block, 0, st, c, p);
+    return a->n * c.bytes >= kLongCopy ? launch(copy_few_kernel<kRun>, grid, block, 0, st, c, p)
+                                       : launch(copy_few_kernel<1>, grid, block, 0, st, c, p);
   const int pages = a->dst_pages + a->src_pages;
   const int2* pairs = reinterpret_cast<const int2*>(a->work + pages + (pages & 1));
   const int bad = launch(copy_check_kernel, dim3(1), dim3(kPlan), 0, st, p);
