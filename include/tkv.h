@@ -341,7 +341,8 @@ int tkv_dequantize(const uint8_t *packed, const uint16_t *scale, const uint16_t 
  *              [0, num_pages); rows of no tokens take none)
  * The rows are cut on the device, from their lengths: their chunks of 32 tokens
  * (an empty row counts as one), laid end to end, are shared out evenly over at
- * most `workgroups` workgroups (1 to 65535) per KV head and 16 query heads, of at
+ * most `workgroups` workgroups (1 to 65535) per KV head and 16 query heads (32 where
+ * a KV head has more than 16), of at
  * least least_chunks chunks each -- or over long_workgroups (at most workgroups;
  * 0: never) where the batch has no more rows and each gets at least long_chunks --
  * and a second launch joins the rows that were

@@ -138,6 +138,70 @@ def test_head_layouts(dtype, HQ, HKV):
     _check(*_decode(*case), *case)
 
 
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("G", [16, 17, 31, 32, 33, 64])
+def test_head_blocks_of_other_head_dims(D, G):
+    case = _case([1, 300, 65], 2 * G, 2, D, 16, 20, BF16, seed=G)
+    _check(*_decode(*case), *case)
+    _check(*_decode(*case, piece_tokens=64), *case)
+
+
+def test_thousands_of_rows_and_large_pages():
+    g = torch.Generator().manual_seed(22)
+    lens = torch.randint(0, 90, (5000,), generator=g).tolist()
+    case = _case(lens, 2, 1, 64, 16, 40, F16, seed=22)  # tables of 640 tokens: cut, and joined
+    out, lse = _decode(*case)
+    at = list(range(0, 5000, 97)) + [4999]
+    q, kp, vp, table, lens = case
+    _check(out[at], lse[at], q[at], kp, vp, table[at], lens[at])
+    case = _case([5000, 1, 4096, 4097], 4, 2, 128, 4096, 2, BF16, seed=23)
+    _check(*_decode(*case), *case)
+
+
+def test_one_workspace_for_every_layer():
+    from tritonkv_amd.paged16 import paged16_append, paged16_decode_attention
+
+    ws, wa = {}, {}
+    for seed in range(3):
+        q, kp, vp, table, lens = _case([300, 5, 64], 8, 2, 128, 64, 8, BF16, seed=seed)
+        new = torch.randn(2, 3, 2, 1, 128, device=DEV).to(BF16)
+        want_k, want_v = kp.clone(), vp.clone()
+        paged16_append(want_k, want_v, new[0], new[1], table, lens - 1)
+        paged16_append(kp, vp, new[0], new[1], table, lens - 1, _workspace=wa)
+        assert torch.equal(kp.view(torch.int16), want_k.view(torch.int16))
+        assert torch.equal(vp.view(torch.int16), want_v.view(torch.int16))
+        out = paged16_decode_attention(q, kp, vp, table, lens, _workspace=ws)
+        _check(out, None, q, kp, vp, table, lens)
+        prep = (ws["call"], wa["call"]) if seed == 0 else prep
+        assert (ws["call"], wa["call"]) == prep
+
+
+def test_two_calls_at_once():
+    from tritonkv_amd.paged16 import paged16_decode_attention
+
+    cases = [_case([9000, 20, 400], 8, 2, 128, 64, 160, BF16, seed=s) for s in (30, 31)]
+    want = [paged16_decode_attention(*c) for c in cases]
+    streams, ws = [torch.cuda.Stream() for _ in cases], [{} for _ in cases]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(paged16_decode_attention(*cases[i], _workspace=ws[i]))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(o, w) for o in outs)
+
+
+def test_expanded_queries_and_one_pool_for_both():
+    q, kp, vp, table, lens = _case([300, 5, 64], 8, 2, 128, 64, 8, F16, seed=32)
+    one = q[:1].expand(3, 8, 128)
+    _check(*_decode(one, kp, kp.clone(), table, lens), one, kp, kp, table, lens)
+    got, _ = _decode(one, kp, kp, table, lens)
+    assert torch.equal(got, _decode(one.contiguous(), kp, kp.clone(), table, lens)[0])
+
+
 @pytest.mark.parametrize("D,dtype", [(64, F16), (128, BF16), (256, F16)])
 def test_a_long_row_among_short_ones(D, dtype):
     case = _case([20011, 3, 0, 1000, 64], 8, 2, D, 64, 400, dtype, seed=3)

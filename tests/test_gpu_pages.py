@@ -285,6 +285,28 @@ def test_strided_table_shared_counts_and_quantized_pools():
         assert torch.equal(_bits(t), _bits(w))
 
 
+def test_state_in_one_buffer_off_16_bytes():
+    """Counts that start anywhere are read one by one."""
+    from tritonkv_amd.pages import compact_pages, fork_rows, resize_rows
+
+    m = Model(3, 4, 37, 16)
+    pool = _pool(37)
+    state = torch.full((1 + 12 + 3 + 37 + 1,), -1, dtype=torch.int32, device=DEV)
+    table, lens, refs = state[1:13].view(3, 4), state[13:16], state[17:54]
+    lens.zero_()
+    refs.zero_()
+    assert refs.data_ptr() % 16
+    for new in ([20, 64, 5], [33, 0, 17]):
+        m.fork(None, new)
+        assert resize_rows([pool], table, lens, refs, _i32(new)).tolist() == [0]
+        assert m.same_as(table, lens, refs)
+    m.fork([0, 0, 2])
+    fork_rows([pool], table, lens, refs, _i32([0, 0, 2]))
+    _compacted(m)
+    compact_pages([pool], table, refs)
+    assert m.same_as(table, lens, refs) and state[0] == -1 and state[16] == -1
+
+
 def test_more_tensors_than_a_launch_takes():
     from tritonkv_amd.pages import compact_pages, fork_rows
 

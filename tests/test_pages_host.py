@@ -64,7 +64,13 @@ def test_copy_between_pools_of_one_memory_is_refused():
 
     p = _pool(8)
     with pytest.raises(ValueError, match="share memory"):
+        copy_pages([p[:5]], Z(1), Z(1), [p[4:]])
+    with pytest.raises(ValueError, match="share memory"):
+        copy_pages([p, p.clone()], Z(1), Z(1), [p.clone(), p])
+    with pytest.raises(RuntimeError, match="GPU"):  # parts of one allocation that do not meet
         copy_pages([p[:4]], Z(1), Z(1), [p[4:]])
+    with pytest.raises(RuntimeError, match="GPU"):  # one KV head: its stride says nothing
+        copy_pages([_pool(6, 1)], Z(1), Z(1), [_pool(6, 16, 1).transpose(1, 2)])
 
 
 BIG = Z(2, 3)
@@ -101,6 +107,16 @@ def test_fork_refuses(kw, error, match):
     a.update(kw)
     with pytest.raises(error, match=match):
         fork_rows(**a)
+
+
+def test_state_may_lie_in_one_buffer():
+    from tritonkv_amd.pages import fork_rows
+
+    state = Z(20)
+    with pytest.raises(RuntimeError, match="GPU"):
+        fork_rows([_pool()], state[:6].view(2, 3), state[6:8], state[8:14], state[14:16], state[16:18], state[18:19])
+    with pytest.raises(ValueError, match="share memory"):
+        fork_rows([_pool()], state[:6].view(2, 3), state[5:7], state[8:14], state[14:16])
 
 
 def test_resize_needs_lengths():

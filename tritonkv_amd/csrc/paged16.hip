@@ -7,7 +7,7 @@
 // The decode reads every live token's K and V row once (2 * D * 2 bytes per
 // token and KV head) for 4 * D * G flops: it is bound by HBM for every GQA
 // group.  One workgroup = one piece of one row's tokens for one KV head and up
-// to 16 of its query heads; each wave walks 32-token chunks, two 16-row MFMA
+// to 32 of its query heads; each wave walks 32-token chunks, two 16-row MFMA
 // tiles.  Scores are S^T = K Q^T (tokens as rows, heads as columns), whose
 // accumulator layout is the B operand layout of O^T = V^T P^T, so the
 // probabilities stay in registers (as in the contiguous fp16 kernel).
@@ -236,19 +236,23 @@ __device__ __forceinline__ void store_row4(const tkv_paged16_args& a, float shif
 // ---------------------------------------------------------------------------
 // The split kernel.
 // ---------------------------------------------------------------------------
-template <class T, int D, int NW, bool APPEND>
-__global__ void __launch_bounds__(NW * 64, D == 256 ? 1 : D == 128 ? 3 : 4) paged16_split_kernel(Paged16Params prm) {
+// HT: tiles of 16 query heads per workgroup, 1 or (G > 16) 2.  A second workgroup for
+// heads 16 to 31 would read all of K and V again: 16 rows of up to 8192, HKV 8, G 24
+// took 82 us with one tile and 54 at G 16.
+template <class T, int D, int HT, int NW, bool APPEND>
+__global__ void __launch_bounds__(NW * 64, D == 256 ? 1 : D == 128 ? 4 - HT : 5 - HT)
+paged16_split_kernel(Paged16Params prm) {
   constexpr int NKM = D / 32;  // 16x16x32 steps over the head dim
   constexpr int EPL = D / 16;  // V dims per lane (and V MFMAs)
   constexpr int VW = EPL / 2;  // dwords of them
   const tkv_paged16_args& a = prm.a;
   constexpr int QROW = D + 8;  // elements of a query row in LDS: 16 rows meet no bank twice
-  // The queries of the 16 heads, the new token's K and V rows (APPEND), then per wave
+  // The queries of the heads, the new token's K and V rows (APPEND), then per wave
   // of the merge: rows of D + 1 floats, maximum and sum of each.
   extern __shared__ float lds_all[];
   uint16_t* const lds_q = reinterpret_cast<uint16_t*>(lds_all);
-  uint16_t* const lds_new = lds_q + 16 * QROW;
-  float* const lds = lds_all + 8 * QROW + (APPEND ? D : 0);
+  uint16_t* const lds_new = lds_q + 16 * HT * QROW;
+  float* const lds = lds_all + 8 * HT * QROW + (APPEND ? D : 0);
 
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, j = lane >> 4;
@@ -257,8 +261,8 @@ __global__ void __launch_bounds__(NW * 64, D == 256 ? 1 : D == 128 ? 3 : 4) page
   Segment g;
   uint32_t share_end;
   if (!first_segment(prm, blockIdx.y, rows, sh, g, share_end)) return;
-  const int hk = blockIdx.x % a.HKV, hb0 = (blockIdx.x / a.HKV) * 16;
-  const int nh = min(16, prm.G - hb0), h0 = hk * prm.G + hb0;
+  const int hk = blockIdx.x % a.HKV, hb0 = (blockIdx.x / a.HKV) * 16 * HT;
+  const int nh = min(16 * HT, prm.G - hb0), h0 = hk * prm.G + hb0;
 
   const int64_t kts = a.k_strides[2], vts = a.v_strides[2];
   const uint32_t kspan = (uint32_t)(15 * kts + D) * 2, vspan = (uint32_t)(15 * vts + D) * 2;
@@ -339,7 +343,7 @@ __global__ void __launch_bounds__(NW * 64, D == 256 ? 1 : D == 128 ? 3 : 4) page
     }
     // The queries: 8 dims of a head per thread and round, zero past the group.  They and
     // the new rows wait in LDS, which leaves the registers to K and V.
-    constexpr int QV = 16 * (D / 8), QR = (QV + NW * 64 - 1) / (NW * 64);
+    constexpr int QV = 16 * HT * (D / 8), QR = (QV + NW * 64 - 1) / (NW * 64);
     u4 q8[QR];
 #pragma unroll
     for (int i = 0; i < QR; ++i) {
@@ -366,10 +370,15 @@ __global__ void __launch_bounds__(NW * 64, D == 256 ? 1 : D == 128 ? 3 : 4) page
   begin_segment();
   for (;;) {
     const int last = hi - 1;
-    f4 accv[EPL];
+    f4 accv[HT][EPL];
+    float m_run[HT], l_run[HT];
 #pragma unroll
-    for (int mv = 0; mv < EPL; ++mv) accv[mv] = f4{0.f, 0.f, 0.f, 0.f};
-    float m_run = -INFINITY, l_run = 0.0f;
+    for (int ht = 0; ht < HT; ++ht) {
+#pragma unroll
+      for (int mv = 0; mv < EPL; ++mv) accv[ht][mv] = f4{0.f, 0.f, 0.f, 0.f};
+      m_run[ht] = -INFINITY;
+      l_run[ht] = 0.0f;
+    }
 
     auto step = [&](int c, int cb, auto tail) {
       constexpr bool TAIL = decltype(tail)::value;
@@ -388,24 +397,32 @@ __global__ void __launch_bounds__(NW * 64, D == 256 ? 1 : D == 128 ? 3 : 4) page
               for (int e = 0; e < VW; ++e) vx[i][e] = reinterpret_cast<const uint32_t*>(lds_new + D + EPL * r)[e];
         }
       }
-      float x[8];
+      float x[HT][8];
       {
         // (opaque: read again in every chunk, not kept in registers)
         const uint16_t* ql = lds_q + (int)opaque((uint32_t)(r * QROW + 8 * j));
-        f4 s[2] = {f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}};
+        f4 s[HT][2];
 #pragma unroll
-        for (int m = 0; m < NKM; ++m) {
-          const u4 qf = *reinterpret_cast<const u4*>(ql + 32 * m);
+        for (int ht = 0; ht < HT; ++ht) s[ht][0] = s[ht][1] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int t = 0; t < 2; ++t) s[t] = T::mfma(kx[t][m], qf, s[t]);
-        }
+        for (int m = 0; m < NKM; ++m)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = s[i / 4][i % 4] * prm.qk_scale;
+          for (int ht = 0; ht < HT; ++ht) {
+            const u4 qf = *reinterpret_cast<const u4*>(ql + 16 * ht * QROW + 32 * m);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) s[ht][t] = T::mfma(kx[t][m], qf, s[ht][t]);
+          }
+#pragma unroll
+        for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[ht][i] = s[ht][i / 4][i % 4] * prm.qk_scale;
       }
       if constexpr (TAIL) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (cb + slot_token(j, i) > last) x[i] = -INFINITY;
+        for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (cb + slot_token(j, i) > last) x[ht][i] = -INFINITY;
       }
       if (!TAIL && more) {
         if (((c + 1) & 31) == 0) tiles(c + 1);  // V of chunk c is on its way already
@@ -413,35 +430,38 @@ __global__ void __launch_bounds__(NW * 64, D == 256 ? 1 : D == 128 ? 3 : 4) page
       }
       // Online softmax in base 2; the accumulators are rescaled only in chunks
       // where a head's maximum rose.
-      float top = x[0];
+      u4 pt[HT][T::kTerms];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
-      if (__builtin_amdgcn_ballot_w64(top > m_run) != 0) {
-        const float mn = vmax(m_run, xor_max16_32(top));
-        const float alpha = safe_exp2_diff(m_run, mn);
-        m_run = mn;
-        l_run *= alpha;
+      for (int ht = 0; ht < HT; ++ht) {
+        float top = x[ht][0];
 #pragma unroll
-        for (int mv = 0; mv < EPL; ++mv) accv[mv] *= alpha;
-      }
-      // scores of -inf under a maximum of -inf give p = 0, not NaN
-      const float off = T::kShift - (m_run == -INFINITY ? 0.0f : m_run);
-      float p[8];
+        for (int i = 1; i < 8; ++i) top = fmaxf(top, x[ht][i]);
+        if (__builtin_amdgcn_ballot_w64(top > m_run[ht]) != 0) {
+          const float mn = vmax(m_run[ht], xor_max16_32(top));
+          const float alpha = safe_exp2_diff(m_run[ht], mn);
+          m_run[ht] = mn;
+          l_run[ht] *= alpha;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(x[i] + off);
-        l_run += p[i];
-      }
-      u4 pt[T::kTerms];
-#pragma unroll
-      for (int n = 0; n < T::kTerms; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t wd = T::pack(p[2 * i], p[2 * i + 1]);
-          pt[n][i] = wd;
-          p[2 * i] -= T::lo(wd);
-          p[2 * i + 1] -= T::hi(wd);
+          for (int mv = 0; mv < EPL; ++mv) accv[ht][mv] *= alpha;
         }
+        // scores of -inf under a maximum of -inf give p = 0, not NaN
+        const float off = T::kShift - (m_run[ht] == -INFINITY ? 0.0f : m_run[ht]);
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(x[ht][i] + off);
+          l_run[ht] += p[i];
+        }
+#pragma unroll
+        for (int n = 0; n < T::kTerms; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t wd = T::pack(p[2 * i], p[2 * i + 1]);
+            pt[ht][n][i] = wd;
+            p[2 * i] -= T::lo(wd);
+            p[2 * i + 1] -= T::hi(wd);
+          }
+      }
       if constexpr (TAIL) {
         // Rows past the sequence are whatever the page holds there (possibly
         // NaN or Inf); p = 0 alone would not cancel them in the MFMA.
@@ -458,7 +478,9 @@ __global__ void __launch_bounds__(NW * 64, D == 256 ? 1 : D == 128 ? 3 : 4) page
 #pragma unroll
         for (int i = 0; i < 4; ++i) av[i] = perm(vx[2 * i + 1][mv / 2], vx[2 * i][mv / 2], sel);
 #pragma unroll
-        for (int n = T::kTerms - 1; n >= 0; --n) accv[mv] = T::mfma(av, pt[n], accv[mv]);
+        for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+          for (int n = T::kTerms - 1; n >= 0; --n) accv[ht][mv] = T::mfma(av, pt[ht][n], accv[ht][mv]);
       }
       if (!TAIL && more) load_v(c + 1);
     };
@@ -486,18 +508,21 @@ __global__ void __launch_bounds__(NW * 64, D == 256 ? 1 : D == 128 ? 3 : 4) page
     // Merge of the waves.  (opaque: the addresses of this part would else be kept in
     // registers over the whole loop.)
     const int mr = (int)opaque(r), mj = (int)opaque(j), mt = (int)opaque(tid);
-    const int b = g.b, mine_rows = min(16, prm.G);
+    const int b = g.b, mine_rows = min(16 * HT, prm.G);
     const int stride = mine_rows * (D + 1) + 2 * mine_rows;
-    const float lt = xor_sum16_32(l_run);
-    if (mr < nh) {
+#pragma unroll
+    for (int ht = 0; ht < HT; ++ht) {
+      const float lt = xor_sum16_32(l_run[ht]);
+      const int n = mr + 16 * ht;
+      if (n >= nh) continue;
       float* mine = lds + w * stride;
 #pragma unroll
       for (int mv = 0; mv < EPL; ++mv)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mine[mr * (D + 1) + EPL * (4 * mj + i) + mv] = accv[mv][i];
+        for (int i = 0; i < 4; ++i) mine[n * (D + 1) + EPL * (4 * mj + i) + mv] = accv[ht][mv][i];
       if (mj == 0) {
-        mine[mine_rows * (D + 1) + mr] = m_run;
-        mine[mine_rows * (D + 2) + mr] = lt;
+        mine[mine_rows * (D + 1) + n] = m_run[ht];
+        mine[mine_rows * (D + 2) + n] = lt;
       }
     }
     __syncthreads();
@@ -709,13 +734,14 @@ static int check_paged16(const tkv_paged16_args* a) {
   return TKV_OK;
 }
 
-template <class T, int D, int NW>
+template <class T, int D, int HT>
 static int launch_paged16(const Paged16Params& p, hipStream_t st) {
-  const int rows = p.G < 16 ? p.G : 16;
-  const dim3 grid((unsigned)(p.a.HKV * ((p.G + 15) / 16)), (unsigned)(p.a.workgroups ? p.a.workgroups : p.a.B));
-  const size_t lds = 32 * (D + 8) + sizeof(float) * NW * (rows * (D + 1) + 2 * rows);
-  return p.a.k_new ? launch(paged16_split_kernel<T, D, NW, true>, grid, dim3(NW * 64), lds + 4 * D, st, p)
-                   : launch(paged16_split_kernel<T, D, NW, false>, grid, dim3(NW * 64), lds, st, p);
+  constexpr int NW = 4;
+  const int rows = p.G < 16 * HT ? p.G : 16 * HT, blocks = (p.G + 16 * HT - 1) / (16 * HT);
+  const dim3 grid((unsigned)(p.a.HKV * blocks), (unsigned)(p.a.workgroups ? p.a.workgroups : p.a.B));
+  const size_t lds = 32 * HT * (D + 8) + sizeof(float) * NW * (rows * (D + 1) + 2 * rows);
+  return p.a.k_new ? launch(paged16_split_kernel<T, D, HT, NW, true>, grid, dim3(NW * 64), lds + 4 * D, st, p)
+                   : launch(paged16_split_kernel<T, D, HT, NW, false>, grid, dim3(NW * 64), lds, st, p);
 }
 
 template <int D>
@@ -728,7 +754,7 @@ static int launch_join(const Paged16Params& p, float shift, hipStream_t st) {
 
 template <class T, int D>
 static int dispatch_paged16(const Paged16Params& p, hipStream_t st) {
-  const int rc = launch_paged16<T, D, 4>(p, st);
+  const int rc = p.G <= 16 ? launch_paged16<T, D, 1>(p, st) : launch_paged16<T, D, 2>(p, st);
   return rc || !p.a.workgroups ? rc : launch_join<D>(p, T::kShift, st);
 }
 

@@ -93,7 +93,7 @@ def plan_shares(B: int, HKV: int, G: int, S: int, D: int = 128, device=None,
     ``S`` is the tables' capacity; the rows' lengths are the device's business.
     ``piece_tokens`` fixes a workgroup's tokens instead.  The rules, with
     what was measured on MI355X (us of a captured step; U = HKV times the
-    blocks of 16 query heads, the workgroups that attend to the same tokens):
+    blocks of query heads, 16 or for more 32, the workgroups that attend to the same tokens):
 
     * Rows stay whole, in one launch, where that is faster than cutting them
       and joining (a second launch, 2.4 us and more): one CU reads at most
@@ -112,7 +112,7 @@ def plan_shares(B: int, HKV: int, G: int, S: int, D: int = 128, device=None,
       9 chunks each, 13.6, 14.3, and 64 of up to 2048, two rows each, 55.9, 60.5);
       128 chunks at head dim 64 (32 rows of up to 16384 132, 126; 8 rows 38.5, 39.4).
     """
-    units = HKV * -(-G // 16)
+    units = HKV * -(-G // (16 if G <= 16 else 32))
     if B > MAX_ROWS:
         raise ValueError(f"at most {MAX_ROWS} rows, got {B}")
     if piece_tokens is not None:
@@ -148,7 +148,9 @@ def _buffer(ws: dict, name: str, n: int, dtype, device) -> torch.Tensor:
 
 
 class _Prepared16(_PreparedCall):
-    """A checked call of a 16-bit entry point: the argument block's tensors are all slots."""
+    """A checked call of this module or of ``pages``, kept as a decode's is.  Here
+    every tensor may be another one of the same form, so that one workspace serves
+    all layers of a model."""
 
     __slots__ = ()
 
@@ -173,8 +175,10 @@ def _offset(struct, field: str) -> int:
     return getattr(struct, field).offset
 
 
-_D = {f: _offset(_lib.Paged16Args, f) for f in ("q", "out", "lse", "k_new", "v_new")}
-_A = {f: _offset(_lib.Paged16AppendArgs, f) for f in ("k_new", "v_new", "positions", "counts")}
+_D = {f: _offset(_lib.Paged16Args, f) for f in ("q", "k", "v", "block_table", "seq_lens", "out", "lse", "k_new",
+                                                "v_new")}
+_A = {f: _offset(_lib.Paged16AppendArgs, f) for f in ("k", "v", "k_new", "v_new", "block_table", "positions",
+                                                      "counts")}
 
 
 def _new_rows(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
@@ -238,8 +242,8 @@ def paged16_append(k_pool: torch.Tensor, v_pool: torch.Tensor, k_new: torch.Tens
     _lib.check(_lib.launch(device, "tkv_paged16_append", args), "paged16_append")
     if key is not None and kn is k_new and vn is v_new:
         _keep16(_workspace, key, args, "tkv_paged16_append", "paged16_append", device, (),
-                ((k_pool, -1, 16, 1), (v_pool, -1, 16, 1), (k_new, _A["k_new"], 16, 1),
-                 (v_new, _A["v_new"], 16, 1), (block_table, -1, 4), (positions, _A["positions"], 4),
+                ((k_pool, _A["k"], 16, 1), (v_pool, _A["v"], 16, 1), (k_new, _A["k_new"], 16, 1),
+                 (v_new, _A["v_new"], 16, 1), (block_table, _A["block_table"], 4), (positions, _A["positions"], 4),
                  (counts, _A["counts"], 4)))
 
 
@@ -275,8 +279,10 @@ def paged16_decode_attention(
 
     ``piece_tokens`` fixes how many tokens a workgroup takes of a row; by
     default the device chooses, from the lengths.  With ``_workspace`` the
-    call allocates nothing but a missing ``out`` and keeps its checked form for
-    the next call; calls that may overlap in time must not share one.
+    call allocates nothing but a missing ``out`` and keeps its checked form: a
+    call like the previous one, on any tensors of the same shapes, strides and
+    dtypes (every layer's pools), is checked and launched natively.  Calls that
+    may overlap in time must not share a workspace.
     """
     key = None
     if _workspace is not None:
@@ -352,8 +358,8 @@ def paged16_decode_attention(
         if strided:  # nothing was copied: every tensor is read where it lies
             _keep16(_workspace, key, args, "tkv_paged16_decode_attention", "paged16_decode_attention",
                     device, (partials, rows),
-                    ((q, _D["q"], 16, 1), (k_pool, -1, 16, 1), (v_pool, -1, 16, 1), (block_table, -1, 4),
-                     (seq_lens, -1, 4), (out, _D["out"], 16), (lse, _D["lse"], 4),
+                    ((q, _D["q"], 16, 1), (k_pool, _D["k"], 16, 1), (v_pool, _D["v"], 16, 1),
+                     (block_table, _D["block_table"], 4), (seq_lens, _D["seq_lens"], 4), (out, _D["out"], 16), (lse, _D["lse"], 4),
                      (k_new, _D["k_new"], 16, 1), (v_new, _D["v_new"], 16, 1)))
     return out
 

@@ -119,8 +119,15 @@ def _row_stride(t: torch.Tensor) -> int | None:
     return stride if stride >= P else None
 
 
+def _span(t: torch.Tensor) -> tuple:
+    """First and last address of t's entries."""
+    first = t.data_ptr()
+    return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() - 1
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    return a.untyped_storage().data_ptr() == b.untyped_storage().data_ptr()
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 <= b1 and b0 <= a1
 
 
 _C = {f: _offset(_lib.CopyPagesArgs, f) for f in ("src", "dst")}
@@ -159,7 +166,7 @@ def copy_pages(pools, src: torch.Tensor, dst: torch.Tensor, dst_pools=None, _wor
         dst_pages = others[0].shape[0] if others[0].dim() else 0
         to = _check_pages(others, dst_pages, device, "dst_pools")
         for a, b in zip(tensors, others):
-            order = [sorted(range(1, 4), key=lambda i: (t.stride(i), t.shape[i])) for t in (a, b)]
+            order = [sorted((i for i in range(1, 4) if t.shape[i] > 1), key=t.stride) for t in (a, b)]
             if a.shape[1:] != b.shape[1:] or a.dtype != b.dtype or order[0] != order[1]:
                 raise ValueError(f"dst_pools must have pools' page shapes, order and dtypes: {tuple(a.shape)} "
                                  f"{a.dtype} and {tuple(b.shape)} {b.dtype}")
