@@ -401,8 +401,8 @@ typedef struct tkv_page_set {
  * with one destination the first is carried out.  Within one set of pools (same)
  * a page that the call reads is never written: a pair whose destination is a
  * pair's source is skipped, and (p, p) is no pair.  work: tkv_copy_pages_work()
- * int32, 8-byte aligned (none for up to 1024 pairs).  No counterpart in the
- * reference, nor have the next two (its caches have no pages). */
+ * int32, 8-byte aligned.  No counterpart in the reference, nor have the next two
+ * (its caches have no pages). */
 typedef struct tkv_copy_pages_args {
   tkv_page_set set;
   const int32_t *src, *dst;
@@ -441,7 +441,7 @@ int tkv_fork_rows(const tkv_fork_rows_args *args, tkv_stream_t stream);
  * out_table is block_table with the moved pages' new numbers, out_refs refs with
  * their counts at the new places, and *live (NULL: not wanted) n.  out_table and
  * out_refs may be block_table and refs.  The old places keep their bytes.  work:
- * tkv_compact_pages_work() int32, 8-byte aligned.  Two launches. */
+ * tkv_compact_pages_work() int32, 16-byte aligned.  Two launches. */
 typedef struct tkv_compact_pages_args {
   tkv_page_set set;
   const int32_t *block_table, *refs;

@@ -58,21 +58,22 @@ def _copied(src, dst, src_pages, dst_pages, same):
     return done
 
 
-@pytest.mark.parametrize("n", [1, 3, 256, 257, 512, 513, 1024, 1025, 2000])
+@pytest.mark.parametrize("n", [1, 3, 1024, 1025, 2000, 4096, 4097, 10000])
 @pytest.mark.parametrize("kind", ["clean", "wild"])
 @pytest.mark.parametrize("other", [False, True])
 def test_copy_pairs(n, kind, other):
     from tritonkv_amd.pages import copy_pages
 
     rng = random.Random(n)
-    num, to_num = 4100, 2100 if other else 4100
+    num = max(4100, 2 * n + 4)
+    to_num = num // 2 if other else num
     if kind == "clean":
         order = rng.sample(range(num), num)
         src, dst = order[:n], order[n:2 * n] if not other else rng.sample(range(to_num), n)
     else:  # numbers outside, the same page twice, pages both read and written, pairs of one page
         src = [rng.choice([rng.randrange(-3, num + 3), rng.randrange(max(1, n))]) for _ in range(n)]
         dst = [rng.choice([rng.randrange(-3, to_num + 3), rng.randrange(max(1, n)), src[i]]) for i in range(n)]
-    pools = [_pool(num, seed=1), _pool(num, HKV=1, page=16, D=8, seed=2)]
+    pools = [_pool(num, HKV=1, page=16, D=32, seed=1), _pool(num, HKV=1, page=16, D=8, seed=2)]
     to = [torch.zeros_like(p[:to_num]) for p in pools] if other else None
     want = [p.clone() for p in (to or pools)]
     done = _copied(src, dst, num, to_num, not other)
@@ -86,6 +87,29 @@ def test_copy_pairs(n, kind, other):
         copy_pages(pools, _i32(src), _i32(dst), to, _workspace=ws)
         for w, p in zip(want, to or pools):
             assert torch.equal(_bits(p), _bits(w))
+
+
+@pytest.mark.parametrize("same", [False, True])
+def test_long_copies_check_their_pairs_beforehand(same):
+    """Over 32 MiB, with every kind of pair that is skipped, and pages of no whole slices."""
+    from tritonkv_amd.pages import copy_pages
+
+    rng = random.Random(5)
+    num, n = 300, 200
+    src = [rng.randrange(-2, num + 2) for _ in range(n)]
+    dst = [rng.choice([rng.randrange(-2, num + 2), src[i]]) for i in range(n)]
+    pools = [_pool(num, HKV=4, page=48, D=256, seed=1), _pool(num, HKV=3, page=16, D=64, seed=2),
+             _pool(num, HKV=8, page=64, D=128, seed=3)]
+    assert n * sum(p[0].numel() * 2 for p in pools) > 32 << 20
+    to = pools if same else [torch.zeros_like(p) for p in pools]
+    want = [p.clone() for p in to]
+    done = _copied(src, dst, num, num, same)
+    s, d = (torch.tensor(x, device=DEV) for x in zip(*done))
+    for w, p in zip(want, pools):
+        w[d] = p[s]
+    copy_pages(pools, _i32(src), _i32(dst), None if same else to)
+    for w, p in zip(want, to):
+        assert torch.equal(_bits(p), _bits(w))
 
 
 def test_copy_quantized_strided_and_many_tensors():

@@ -170,8 +170,7 @@ def test_work_sizes():
     from tritonkv_amd import _lib
 
     lib = _lib.load()
-    assert lib.tkv_copy_pages_work(1024, 100, 100) == 0
-    assert lib.tkv_copy_pages_work(1025, 100, 7) >= 107 + 2 * 1025
+    assert lib.tkv_copy_pages_work(4097, 100, 7) >= 107 + 2 * 4097
     assert lib.tkv_fork_rows_work(4, 10, 100, 1) - lib.tkv_fork_rows_work(4, 10, 100, 0) == 40
     assert lib.tkv_fork_rows_work(4, 10, 100, 0) >= 6 * 4 + 100
     assert lib.tkv_compact_pages_work(100) >= 250
@@ -199,7 +198,7 @@ def test_c_entries_refuse_page_sets(change):
             s.count = value
         else:
             getattr(s, name)[0] = value
-    c = _lib.CopyPagesArgs(set=s, src=d, dst=d, n=3, src_pages=6, dst_pages=6, same=1)
+    c = _lib.CopyPagesArgs(set=s, src=d, dst=d, work=d, n=3, src_pages=6, dst_pages=6, same=1)
     f = _lib.ForkRowsArgs(set=s, block_table=d, seq_lens=d, refs=d, status=d, work=d, table_stride=3, B=2,
                           max_pages=3, page_size=16, num_pages=6)
     p = _lib.CompactPagesArgs(set=s, block_table=d, refs=d, out_table=d, out_refs=d, work=d, table_stride=3,
@@ -212,12 +211,12 @@ def test_c_entries_refuse_page_sets(change):
 
 @pytest.mark.parametrize("kind,field,value", [
     ("copy", "src", None), ("copy", "dst", None), ("copy", "n", 0), ("copy", "src_pages", 0),
-    ("copy", "dst_pages", 7), ("copy", "n", 1025),
+    ("copy", "dst_pages", 7), ("copy", "work", None), ("copy", "work", 0x1004),
     ("fork", "block_table", None), ("fork", "seq_lens", None), ("fork", "refs", None), ("fork", "status", None),
     ("fork", "work", None), ("fork", "work", 0x1004), ("fork", "B", 0), ("fork", "max_pages", 0),
     ("fork", "num_pages", 0), ("fork", "page_size", 0), ("fork", "table_stride", 2),
     ("fork", "page_size", 1 << 30),
-    ("compact", "block_table", None), ("compact", "out_refs", None), ("compact", "work", 0x1004),
+    ("compact", "block_table", None), ("compact", "out_refs", None), ("compact", "work", 0x1008),
     ("compact", "out_stride", 2), ("compact", "num_pages", 0)])
 def test_c_entries_refuse(kind, field, value):
     from tritonkv_amd import _lib
@@ -225,7 +224,7 @@ def test_c_entries_refuse(kind, field, value):
     lib, d = _lib.load(), 0x1000
     s = _set(_lib)
     a, fn = {
-        "copy": (_lib.CopyPagesArgs(set=s, src=d, dst=d, n=3, src_pages=6, dst_pages=6, same=1), lib.tkv_copy_pages),
+        "copy": (_lib.CopyPagesArgs(set=s, src=d, dst=d, work=d, n=3, src_pages=6, dst_pages=6, same=1), lib.tkv_copy_pages),
         "fork": (_lib.ForkRowsArgs(set=s, block_table=d, seq_lens=d, refs=d, status=d, work=d, table_stride=3, B=2,
                                    max_pages=3, page_size=16, num_pages=6), lib.tkv_fork_rows),
         "compact": (_lib.CompactPagesArgs(set=s, block_table=d, refs=d, out_table=d, out_refs=d, work=d,

@@ -19,7 +19,7 @@ namespace tkv {
 constexpr int kPlan = 1024;                  // threads of a plan's workgroup
 constexpr int kCopy = 1024;                  // threads of a copy's workgroup
 constexpr int kMaxRows = 8192;               // rows of a fork: two LDS integers each
-constexpr int kInlinePairs = 1024;           // pairs that the copy checks by itself
+constexpr int kInlinePairs = 4096;           // pairs that the copy checks by itself
 constexpr int kPagesPerThread = 64;          // bits of a thread's mask of pages
 
 // A barrier behind which the workgroup's memory operations have been carried out.
@@ -107,12 +107,14 @@ __device__ __forceinline__ bool is_pair(const PairLists& a, int s, int d) {
   return s >= 0 && s < a.src_pages && d >= 0 && d < a.dst_pages && !(a.same && s == d);
 }
 
-// A few pairs: every workgroup checks its own pair against all of them.  A pair
-// is carried out unless an earlier one has its destination or, within one set
-// of pools, any one reads it.
-template <int RUN>
+// A short copy: every workgroup checks its own pair against all of them, which saves
+// the launch that checks them beforehand (below) and slows the copies down.  Pages of
+// 128 KiB, inline / beforehand: 8 pairs 3.7 / 5.8 us, 64 5.8 / 8.4, 256 17.9 / 19.7, 1024
+// 64 / 65; of 512 KiB: 8 4.4 / 6.6, 64 17.2 / 17.1, 256 60 / 56, 1024 213 / 196.  So
+// inline below 32 MiB.  A pair is carried out unless an earlier one has its
+// destination or, within one set of pools, any one reads it.
 __global__ void __launch_bounds__(kCopy) copy_few_kernel(CopyPlan c, PairLists a) {
-  copy_run<RUN>(c, (int64_t)a.n * c.slices, blockIdx.x, gridDim.x, [&](int p) {
+  copy_run<1>(c, (int64_t)a.n * c.slices, blockIdx.x, gridDim.x, [&](int p) {
     const int s = a.src[p], d = a.dst[p];
     bool bad = !is_pair(a, s, d);
     for (int x = threadIdx.x; x < a.n; x += kCopy) {
@@ -426,21 +428,31 @@ struct CompactParams {
   int32_t table_stride, out_stride, B, max_pages, num_pages;
 };
 
-struct CompactWork {
-  int* head;   // live pages, moves
-  int2* pairs;
-  int *rank;   // of a page that moves or is moved onto; -1 for the others
-  int *count;  // references of the i-th page that moves
+// The plan's blocks: the pages of one thread in one round.
+struct PageBlock {
+  uint64_t used;  // bit i: page i of the block has references
+  int from, to;   // pages before the block that move, and that are moved onto
 };
 
-__host__ __device__ inline int64_t compact_work_ints(int64_t N) { return 16 + (N + 2) + N + N / 2 + 1; }
+struct CompactWork {
+  int* head;          // live pages, moves
+  int2* pairs;        // at most N / 2 moves
+  int* count;         // references of the i-th page that moves
+  PageBlock* blocks;  // of pages_per_thread(N) >= 4 pages each
+};
+
+__host__ __device__ inline int64_t compact_work_ints(int64_t N) {
+  const int64_t pairs = 16 + (N + 2) / 2 * 2, counts = (N / 2 + 4) / 4 * 4;
+  return (pairs + counts + 3) / 4 * 4 + 4 * (N / 4 + kPlan);
+}
 
 __device__ __forceinline__ CompactWork compact_work(const CompactParams& a) {
   CompactWork w;
+  const int64_t N = a.num_pages, pairs = 16 + (N + 2) / 2 * 2, counts = (N / 2 + 4) / 4 * 4;
   w.head = a.work;
-  w.pairs = reinterpret_cast<int2*>(a.work + 16);  // at most N / 2 moves
-  w.rank = a.work + 16 + (a.num_pages + 2);
-  w.count = w.rank + a.num_pages;
+  w.pairs = reinterpret_cast<int2*>(a.work + 16);
+  w.count = a.work + pairs;
+  w.blocks = reinterpret_cast<PageBlock*>(a.work + (pairs + counts + 3) / 4 * 4);
   return w;
 }
 
@@ -462,23 +474,17 @@ __global__ void __launch_bounds__(kPlan) compact_plan_kernel(CompactParams a) {
     const int64_t mine = p0 + (int64_t)tid * per;
     if (N > round) m = used_mask(a.refs, mine, per, N);
     const uint64_t low = first_bits(live - mine), in = first_bits(N - mine) & first_bits(per);
-    const uint64_t from = m & ~low, to = ~m & low & in;
+    uint64_t from = m & ~low, to = ~m & low & in;
     int2 total;
     const int2 at = block_scan(scan, __popcll(from), __popcll(to), total);
     int s = done.x + at.x, d = done.y + at.y;
-    for (int i = 0; i < per && mine + i < N; ++i) {
-      const uint64_t bit = uint64_t(1) << i;
-      int rank = -1;
-      if (from & bit) {
-        w.pairs[s].x = (int)(mine + i);
-        w.count[s] = a.refs[mine + i];
-        rank = s++;
-      } else if (to & bit) {
-        w.pairs[d].y = (int)(mine + i);
-        rank = d++;
-      }
-      w.rank[mine + i] = rank;
+    if (mine < N) w.blocks[p0 / per + tid] = PageBlock{m, s, d};
+    for (; from; from &= from - 1, ++s) {
+      const int page = (int)mine + __builtin_ctzll(from);
+      w.pairs[s].x = page;
+      w.count[s] = a.refs[page];
     }
+    for (; to; to &= to - 1, ++d) w.pairs[d].y = (int)mine + __builtin_ctzll(to);
     done.x += total.x;
     done.y += total.y;
   }
@@ -489,6 +495,17 @@ __global__ void __launch_bounds__(kPlan) compact_plan_kernel(CompactParams a) {
   }
 }
 
+// Which move a page takes part in, -1 for none: as the source of one at or past
+// `live` pages, as the destination of one below.
+__device__ __forceinline__ int move_of(const CompactWork& w, int page, int per, int live) {
+  const int block = page / per, bit = page - block * per;
+  const PageBlock b = w.blocks[block];
+  const uint64_t below = first_bits(bit), low = first_bits((int64_t)live - (int64_t)block * per);
+  const bool used = b.used >> bit & 1;
+  if (page >= live) return used ? b.from + __popcll(b.used & ~low & below) : -1;
+  return used ? -1 : b.to + __popcll(~b.used & low & below);
+}
+
 // Workgroups [0, tables): the table and the counts; the others: the copies.
 __global__ void __launch_bounds__(kCopy) compact_apply_kernel(CompactParams a, CopyPlan c, int tables) {
   const CompactWork w = compact_work(a);
@@ -497,18 +514,19 @@ __global__ void __launch_bounds__(kCopy) compact_apply_kernel(CompactParams a, C
     copy_pairs(c, w.pairs, w.head[1], blockIdx.x - tables, gridDim.x - tables);
     return;
   }
-  const int P = a.max_pages, N = a.num_pages;
+  const int P = a.max_pages, N = a.num_pages, per = pages_per_thread(N);
   const int64_t entries = (int64_t)a.B * P;
   for (int64_t i = (int64_t)blockIdx.x * kCopy + threadIdx.x; i < entries + N; i += (int64_t)tables * kCopy) {
     if (i < entries) {
       const int b = (int)(i / P), slot = (int)(i - (int64_t)b * P);
       int page = a.block_table[(int64_t)b * a.table_stride + slot];
-      if (page >= live && page < N && w.rank[page] >= 0) page = w.pairs[w.rank[page]].y;
+      const int move = page >= live && page < N ? move_of(w, page, per, live) : -1;
+      if (move >= 0) page = w.pairs[move].y;
       a.out_table[(int64_t)b * a.out_stride + slot] = page;
     } else {
       const int p = (int)(i - entries);
-      const int rank = w.rank[p];
-      a.out_refs[p] = p >= live ? 0 : rank >= 0 ? w.count[rank] : a.refs[p];
+      const int move = p < live ? move_of(w, p, per, live) : -1;
+      a.out_refs[p] = p >= live ? 0 : move >= 0 ? w.count[move] : a.refs[p];
     }
   }
 }
@@ -549,7 +567,7 @@ static unsigned copy_groups(int64_t pairs, const CopyPlan& c) {
 
 extern "C" int64_t tkv_copy_pages_work(int32_t n, int32_t src_pages, int32_t dst_pages) {
   if (n < 0 || src_pages < 0 || dst_pages < 0) return -1;
-  return n <= tkv::kInlinePairs ? 0 : (int64_t)src_pages + dst_pages + 1 + 2 * (int64_t)n;
+  return (int64_t)src_pages + dst_pages + 1 + 2 * (int64_t)n;
 }
 
 extern "C" int tkv_copy_pages(const tkv_copy_pages_args* a, tkv_stream_t stream) {
@@ -559,14 +577,12 @@ extern "C" int tkv_copy_pages(const tkv_copy_pages_args* a, tkv_stream_t stream)
   CopyPlan c;
   const int rc = make_plan(a->set, c);
   if (rc) return rc;
+  if (!a->work || (uintptr_t)a->work & 7) return TKV_EINVAL;
   if (!c.slices) return TKV_OK;
-  if (a->n > kInlinePairs && (!a->work || (uintptr_t)a->work & 7)) return TKV_EINVAL;
   const PairLists p{a->src, a->dst, a->work, a->n, a->src_pages, a->dst_pages, a->same};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(copy_groups(a->n, c)), block(kCopy);
-  if (a->n <= kInlinePairs)
-    return a->n * c.bytes >= kLongCopy ? launch(copy_few_kernel<kRun>, grid, block, 0, st, c, p)
-                                       : launch(copy_few_kernel<1>, grid, block, 0, st, c, p);
+  if (a->n <= kInlinePairs && a->n * c.bytes < kLongCopy) return launch(copy_few_kernel, grid, block, 0, st, c, p);
   const int pages = a->dst_pages + a->src_pages;
   const int2* pairs = reinterpret_cast<const int2*>(a->work + pages + (pages & 1));
   const int bad = launch(copy_check_kernel, dim3(1), dim3(kPlan), 0, st, p);
@@ -608,7 +624,7 @@ extern "C" int64_t tkv_compact_pages_work(int32_t num_pages) {
 
 extern "C" int tkv_compact_pages(const tkv_compact_pages_args* a, tkv_stream_t stream) {
   using namespace tkv;
-  if (!a || !a->block_table || !a->refs || !a->out_table || !a->out_refs || !a->work || (uintptr_t)a->work & 7)
+  if (!a || !a->block_table || !a->refs || !a->out_table || !a->out_refs || !a->work || (uintptr_t)a->work & 15)
     return TKV_EINVAL;
   if (a->B <= 0 || a->max_pages <= 0 || a->num_pages <= 0 || a->table_stride < a->max_pages ||
       a->out_stride < a->max_pages)

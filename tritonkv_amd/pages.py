@@ -181,10 +181,10 @@ def copy_pages(pools, src: torch.Tensor, dst: torch.Tensor, dst_pools=None, _wor
     if n == 0:
         return
     words = _lib.load().tkv_copy_pages_work(n, src_pages, dst_pages)
-    work = _work(_workspace, "copy_pages", words, device) if words else None
+    work = _work(_workspace, "copy_pages", words, device)
     sets = _page_sets(from_, to)
     for one in sets:
-        args = _lib.CopyPagesArgs(set=one, src=s.data_ptr(), dst=d.data_ptr(), work=_lib.ptr(work), n=n,
+        args = _lib.CopyPagesArgs(set=one, src=s.data_ptr(), dst=d.data_ptr(), work=work.data_ptr(), n=n,
                                   src_pages=src_pages, dst_pages=dst_pages, same=int(others is None))
         _lib.check(_lib.launch(device, "tkv_copy_pages", args), "copy_pages")
     if key is not None and len(sets) == 1:
