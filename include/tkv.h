@@ -400,8 +400,8 @@ typedef struct tkv_page_set {
  * number outside [0, src_pages) or [0, dst_pages) is skipped; of several pairs
  * with one destination the first is carried out.  Within one set of pools (same)
  * a page that the call reads is never written: a pair whose destination is a
- * pair's source is skipped, and (p, p) is no pair.  work: tkv_copy_pages_work()
- * int32, 8-byte aligned.  No counterpart in the reference, nor have the next two
+ * pair's source is skipped, and (p, p) is no pair.  work: tkv_copy_pages_work(args)
+ * int32, 8-byte aligned (0: none, NULL will do; below 0: wrong arguments).  No counterpart in the reference, nor have the next two
  * (its caches have no pages). */
 typedef struct tkv_copy_pages_args {
   tkv_page_set set;
@@ -409,7 +409,7 @@ typedef struct tkv_copy_pages_args {
   int32_t *work;
   int32_t n, src_pages, dst_pages, same;
 } tkv_copy_pages_args;
-int64_t tkv_copy_pages_work(int32_t n, int32_t src_pages, int32_t dst_pages);
+int64_t tkv_copy_pages_work(const tkv_copy_pages_args *args);
 int tkv_copy_pages(const tkv_copy_pages_args *args, tkv_stream_t stream);
 
 /* New rows of a block table out of its old ones, in place, over pages counted in

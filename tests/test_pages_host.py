@@ -170,11 +170,17 @@ def test_work_sizes():
     from tritonkv_amd import _lib
 
     lib = _lib.load()
-    assert lib.tkv_copy_pages_work(4097, 100, 7) >= 107 + 2 * 4097
+    c = _lib.CopyPagesArgs(set=_set(_lib), src=0x1000, dst=0x1000, n=4096, src_pages=100, dst_pages=7)
+    assert lib.tkv_copy_pages_work(c) == 0  # 4096 pages of 4 KiB
+    c.n = 4097
+    assert lib.tkv_copy_pages_work(c) >= 107 + 2 * 4097
+    c.n, c.set.bytes[0], c.set.src_stride[0], c.set.dst_stride[0] = 32, 1 << 20, 1 << 20, 1 << 20
+    assert lib.tkv_copy_pages_work(c) >= 107 + 2 * 32
     assert lib.tkv_fork_rows_work(4, 10, 100, 1) - lib.tkv_fork_rows_work(4, 10, 100, 0) == 40
     assert lib.tkv_fork_rows_work(4, 10, 100, 0) >= 6 * 4 + 100
     assert lib.tkv_compact_pages_work(100) >= 250
-    for bad in (lib.tkv_copy_pages_work(-1, 1, 1), lib.tkv_fork_rows_work(0, 1, 1, 0),
+    c.n = 0
+    for bad in (lib.tkv_copy_pages_work(c), lib.tkv_fork_rows_work(0, 1, 1, 0),
                 lib.tkv_compact_pages_work(0)):
         assert bad == -1
 
@@ -211,7 +217,7 @@ def test_c_entries_refuse_page_sets(change):
 
 @pytest.mark.parametrize("kind,field,value", [
     ("copy", "src", None), ("copy", "dst", None), ("copy", "n", 0), ("copy", "src_pages", 0),
-    ("copy", "dst_pages", 7), ("copy", "work", None), ("copy", "work", 0x1004),
+    ("copy", "dst_pages", 0), ("copy", "dst_pages", 7), ("copy", "n", 8193), ("copy", "n", -1),
     ("fork", "block_table", None), ("fork", "seq_lens", None), ("fork", "refs", None), ("fork", "status", None),
     ("fork", "work", None), ("fork", "work", 0x1004), ("fork", "B", 0), ("fork", "max_pages", 0),
     ("fork", "num_pages", 0), ("fork", "page_size", 0), ("fork", "table_stride", 2),
@@ -224,7 +230,8 @@ def test_c_entries_refuse(kind, field, value):
     lib, d = _lib.load(), 0x1000
     s = _set(_lib)
     a, fn = {
-        "copy": (_lib.CopyPagesArgs(set=s, src=d, dst=d, work=d, n=3, src_pages=6, dst_pages=6, same=1), lib.tkv_copy_pages),
+        "copy": (_lib.CopyPagesArgs(set=s, src=d, dst=d, n=3, src_pages=6, dst_pages=6, same=1),
+                 lib.tkv_copy_pages),
         "fork": (_lib.ForkRowsArgs(set=s, block_table=d, seq_lens=d, refs=d, status=d, work=d, table_stride=3, B=2,
                                    max_pages=3, page_size=16, num_pages=6), lib.tkv_fork_rows),
         "compact": (_lib.CompactPagesArgs(set=s, block_table=d, refs=d, out_table=d, out_refs=d, work=d,

@@ -251,7 +251,7 @@ SIGNATURES = {
     "tkv_dequantize": ([_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P], ctypes.c_int),
     "tkv_paged16_decode_attention": ([ctypes.POINTER(Paged16Args), _P], ctypes.c_int),
     "tkv_paged16_append": ([ctypes.POINTER(Paged16AppendArgs), _P], ctypes.c_int),
-    "tkv_copy_pages_work": ([_I32, _I32, _I32], _I64),
+    "tkv_copy_pages_work": ([ctypes.POINTER(CopyPagesArgs)], _I64),
     "tkv_copy_pages": ([ctypes.POINTER(CopyPagesArgs), _P], ctypes.c_int),
     "tkv_fork_rows_work": ([_I32, _I32, _I32, _I32], _I64),
     "tkv_fork_rows": ([ctypes.POINTER(ForkRowsArgs), _P], ctypes.c_int),

@@ -565,24 +565,40 @@ static unsigned copy_groups(int64_t pairs, const CopyPlan& c) {
 
 }  // namespace tkv
 
-extern "C" int64_t tkv_copy_pages_work(int32_t n, int32_t src_pages, int32_t dst_pages) {
-  if (n < 0 || src_pages < 0 || dst_pages < 0) return -1;
-  return (int64_t)src_pages + dst_pages + 1 + 2 * (int64_t)n;
+namespace tkv {
+
+static int check_copy(const tkv_copy_pages_args* a, CopyPlan& c) {
+  if (!a || !a->src || !a->dst || a->n <= 0 || a->src_pages <= 0 || a->dst_pages <= 0) return TKV_EINVAL;
+  if (a->same && a->src_pages != a->dst_pages) return TKV_EINVAL;
+  return make_plan(a->set, c);
+}
+
+static bool checked_inline(const tkv_copy_pages_args* a, const CopyPlan& c) {
+  return a->n <= kInlinePairs && a->n * c.bytes < kLongCopy;
+}
+
+}  // namespace tkv
+
+extern "C" int64_t tkv_copy_pages_work(const tkv_copy_pages_args* a) {
+  using namespace tkv;
+  CopyPlan c;
+  const int rc = check_copy(a, c);
+  if (rc) return rc;
+  return checked_inline(a, c) ? 0 : (int64_t)a->src_pages + a->dst_pages + 1 + 2 * (int64_t)a->n;
 }
 
 extern "C" int tkv_copy_pages(const tkv_copy_pages_args* a, tkv_stream_t stream) {
   using namespace tkv;
-  if (!a || !a->src || !a->dst || a->n <= 0 || a->src_pages <= 0 || a->dst_pages <= 0) return TKV_EINVAL;
-  if (a->same && a->src_pages != a->dst_pages) return TKV_EINVAL;
   CopyPlan c;
-  const int rc = make_plan(a->set, c);
+  const int rc = check_copy(a, c);
   if (rc) return rc;
-  if (!a->work || (uintptr_t)a->work & 7) return TKV_EINVAL;
+  const bool in_line = checked_inline(a, c);
+  if (!in_line && (!a->work || (uintptr_t)a->work & 7)) return TKV_EINVAL;
   if (!c.slices) return TKV_OK;
   const PairLists p{a->src, a->dst, a->work, a->n, a->src_pages, a->dst_pages, a->same};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(copy_groups(a->n, c)), block(kCopy);
-  if (a->n <= kInlinePairs && a->n * c.bytes < kLongCopy) return launch(copy_few_kernel, grid, block, 0, st, c, p);
+  if (in_line) return launch(copy_few_kernel, grid, block, 0, st, c, p);
   const int pages = a->dst_pages + a->src_pages;
   const int2* pairs = reinterpret_cast<const int2*>(a->work + pages + (pages & 1));
   const int bad = launch(copy_check_kernel, dim3(1), dim3(kPlan), 0, st, p);

@@ -67,13 +67,16 @@ def _check_pages(tensors: list, num_pages: int | None, device, what: str) -> lis
                              + ("" if num_pages is None else f" of {num_pages} pages") + f", got {tuple(t.shape)}")
         if t.device != device:
             raise ValueError(f"{what} must be on {device}, got a tensor on {t.device}")
-        dense = 1  # a page is one block of memory, in whatever order of its axes
-        for stride, n in sorted((s, n) for s, n in zip(t.stride()[1:], t.shape[1:]) if n > 1):
-            if stride != dense:
-                raise ValueError(f"{what}: a page must be one dense block, got strides {tuple(t.stride())}")
-            dense *= n
-        size = dense * t.element_size()
-        stride = t.stride(0) * t.element_size() if t.shape[0] > 1 else size
+        if t.is_contiguous():
+            size = stride = t.numel() // t.shape[0] * t.element_size()
+        else:
+            dense = 1  # a page is one block of memory, in whatever order of its axes
+            for stride, n in sorted((s, n) for s, n in zip(t.stride()[1:], t.shape[1:]) if n > 1):
+                if stride != dense:
+                    raise ValueError(f"{what}: a page must be one dense block, got strides {tuple(t.stride())}")
+                dense *= n
+            size = dense * t.element_size()
+            stride = t.stride(0) * t.element_size() if t.shape[0] > 1 else size
         if stride < size:
             raise ValueError(f"{what}: pages overlap, got strides {tuple(t.stride())}")
         if size % 16 or stride % 16 or t.data_ptr() % 16:
@@ -87,11 +90,13 @@ def _page_sets(src: list, dst: list) -> list:
     """The tensors as sets of at most ``PAGE_TENSORS``; one empty set without any."""
     n = _lib.PAGE_TENSORS
     sets = []
-    for i in range(0, max(1, len(src)), n):
-        s, d = src[i:i + n], dst[i:i + n]
-        sets.append(_lib.PageSet(src=tuple(x[0] for x in s), dst=tuple(x[0] for x in d),
-                                 src_stride=tuple(x[1] for x in s), dst_stride=tuple(x[1] for x in d),
-                                 bytes=tuple(x[2] for x in s), count=len(s)))
+    for first in range(0, max(1, len(src)), n):
+        one = _lib.PageSet(count=len(src[first:first + n]))
+        from_, to, from_stride, to_stride, size = one.src, one.dst, one.src_stride, one.dst_stride, one.bytes
+        for i, (s, d) in enumerate(zip(src[first:first + n], dst[first:first + n])):
+            from_[i], from_stride[i], size[i] = s
+            to[i], to_stride[i], _ = d
+        sets.append(one)
     return sets
 
 
@@ -180,12 +185,15 @@ def copy_pages(pools, src: torch.Tensor, dst: torch.Tensor, dst_pools=None, _wor
     _require_gpu(tensors[0], "copy_pages")
     if n == 0:
         return
-    words = _lib.load().tkv_copy_pages_work(n, src_pages, dst_pages)
-    work = _work(_workspace, "copy_pages", words, device)
     sets = _page_sets(from_, to)
+    work = None
     for one in sets:
-        args = _lib.CopyPagesArgs(set=one, src=s.data_ptr(), dst=d.data_ptr(), work=work.data_ptr(), n=n,
-                                  src_pages=src_pages, dst_pages=dst_pages, same=int(others is None))
+        args = _lib.CopyPagesArgs(set=one, src=s.data_ptr(), dst=d.data_ptr(), n=n, src_pages=src_pages,
+                                  dst_pages=dst_pages, same=int(others is None))
+        words = _lib.load().tkv_copy_pages_work(args)
+        if words > 0:
+            work = _work(_workspace, "copy_pages", words, device)
+            args.work = work.data_ptr()
         _lib.check(_lib.launch(device, "tkv_copy_pages", args), "copy_pages")
     if key is not None and len(sets) == 1:
         _keep16(_workspace, key, args, "tkv_copy_pages", "copy_pages", device, (work,),
