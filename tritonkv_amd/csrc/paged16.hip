@@ -81,9 +81,16 @@ struct Bf16 {
 // each, cut evenly, 184-194 us; shares 172 / 176.  8 rows of 300-4000 take 21.7 us in
 // tables of 131072 tokens and 21.3 in tables of 4032.
 // ---------------------------------------------------------------------------
+// What finds a workgroup's first segment: scalar arguments of the kernel, which are in
+// registers when a wave starts (a struct is not), so that the lengths are asked for at once.
+struct SharePlan {
+  const int32_t* lens;
+  int B, S, workgroups, least_chunks, long_workgroups, long_chunks;
+};
+
 struct Paged16Params {
   tkv_paged16_args a;
-  int G, page_tiles, S;
+  int G, page_tiles;
   float qk_scale;  // sm_scale * log2(e)
   uint32_t k16[3], v16[3];  // the pools' strides in 16 bytes: products of 32 bits by 32
 };
@@ -136,12 +143,12 @@ struct Segment {
 };
 
 // Chunks from which on every workgroup has its least (saturated).
-__device__ __forceinline__ uint32_t full_at(const tkv_paged16_args& a) {
+__device__ __forceinline__ uint32_t full_at(const SharePlan& a) {
   const uint64_t n = (uint64_t)(uint32_t)a.workgroups * (uint32_t)a.least_chunks;
   return n > 0xffffffffu ? 0xffffffffu : (uint32_t)n;
 }
 
-__device__ __forceinline__ Shares make_shares(uint32_t total, const tkv_paged16_args& a, uint32_t& W) {
+__device__ __forceinline__ Shares make_shares(uint32_t total, const SharePlan& a, uint32_t& W) {
   W = a.workgroups;
   if (a.B <= a.long_workgroups && total >= (uint32_t)a.long_workgroups * (uint32_t)a.long_chunks) W = a.long_workgroups;
   else if (total < full_at(a)) W = min(W, (total + a.least_chunks - 1) / (uint32_t)a.least_chunks);
@@ -152,10 +159,10 @@ __device__ __forceinline__ Shares make_shares(uint32_t total, const tkv_paged16_
 }
 
 // This workgroup's first segment and the end of its share; false: it has none.
-__device__ __forceinline__ bool first_segment(const Paged16Params& prm, int i, RowLens& rows, Shares& sh,
+__device__ __forceinline__ bool first_segment(const SharePlan& plan, int i, RowLens& rows, Shares& sh,
                                               Segment& g, uint32_t& share_end) {
-  const int B = prm.a.B, lane = rows.lane;
-  if (prm.a.workgroups == 0) {
+  const int B = plan.B, lane = rows.lane;
+  if (plan.workgroups == 0) {
     rows.load(i & ~63);
     g.b = i;
     g.L = rows.of(i);
@@ -169,7 +176,7 @@ __device__ __forceinline__ bool first_segment(const Paged16Params& prm, int i, R
   if (!rows.lens || B == 1) {  // every row alike
     const int L = rows.of(0);
     const uint32_t l = chunks_of(L);
-    sh = make_shares(l * B, prm.a, W);
+    sh = make_shares(l * B, plan, W);
     if ((uint32_t)i >= W) return false;
     const uint32_t from = sh.start(i);
     share_end = sh.start(i + 1);
@@ -187,7 +194,7 @@ __device__ __forceinline__ bool first_segment(const Paged16Params& prm, int i, R
     rows.load(b0);
     sum += __builtin_amdgcn_readlane((int)wave_scan(b0 + lane < B ? chunks_of(rows.L) : 0), 63);
   }
-  sh = make_shares(sum, prm.a, W);
+  sh = make_shares(sum, plan, W);
   if ((uint32_t)i >= W) return false;
   const uint32_t from = sh.start(i);
   share_end = sh.start(i + 1);
@@ -215,20 +222,18 @@ __device__ __forceinline__ bool first_segment(const Paged16Params& prm, int i, R
 }
 
 // Where the partial of head h in a slot lives; maxima and sums after all rows.
-__device__ __forceinline__ int64_t partial_row(const tkv_paged16_args& a, uint32_t slot, int h) {
-  return (int64_t)slot * a.HQ + h;
-}
-__device__ __forceinline__ float* partial_ml(const tkv_paged16_args& a) {
-  return a.partials + (int64_t)2 * a.workgroups * a.HQ * a.D;
+__device__ __forceinline__ int64_t partial_row(int HQ, uint32_t slot, int h) { return (int64_t)slot * HQ + h; }
+__device__ __forceinline__ float* partial_ml(float* partials, int workgroups, int HQ, int D) {
+  return partials + (int64_t)2 * workgroups * HQ * D;
 }
 
-__device__ __forceinline__ void store_row4(const tkv_paged16_args& a, float shift, int64_t row, int d, f4 o,
+__device__ __forceinline__ void store_row4(float* out, float* lse, int D, float shift, int64_t row, int d, f4 o,
                                            float m, float l) {
   // A row that saw nothing (no tokens, or scores of -inf alone) is zero.
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  *reinterpret_cast<f4*>(a.out + row * a.D + d) = o * inv;
-  if (a.lse && d == 0)
-    a.lse[row] = l == 0.0f ? -INFINITY : (m - shift + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+  *reinterpret_cast<f4*>(out + row * D + d) = o * inv;
+  if (lse && d == 0)
+    lse[row] = l == 0.0f ? -INFINITY : (m - shift + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
 // ---------------------------------------------------------------------------
@@ -239,14 +244,16 @@ __device__ __forceinline__ void store_row4(const tkv_paged16_args& a, float shif
 // took 82 us with one tile and 60 with two (G 16: 56).
 template <class T, int D, int HT, int NW, bool APPEND>
 __global__ void __launch_bounds__(NW * 64, D == 256 ? 1 : D == 128 ? 4 - HT : 5 - HT)
-paged16_split_kernel(Paged16Params prm) {
+paged16_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least_chunks, int long_workgroups,
+                     int long_chunks, Paged16Params prm) {
   constexpr int NKM = D / 32;  // 16x16x32 steps over the head dim
   constexpr int EPL = D / 16;  // V dims per lane (and V MFMAs)
   constexpr int VW = EPL / 2;  // dwords of them
   const tkv_paged16_args& a = prm.a;
   constexpr int QROW = D + 8;  // elements of a query row in LDS: 16 rows meet no bank twice
+  constexpr int OROW = D + 4;  // floats of an output row there: 16-byte pieces
   // The queries of the heads, the new token's K and V rows (APPEND), then per wave
-  // of the merge: rows of D + 1 floats, maximum and sum of each.
+  // of the merge: rows of OROW floats, maximum and sum of each.
   extern __shared__ float lds_all[];
   uint16_t* const lds_q = reinterpret_cast<uint16_t*>(lds_all);
   uint16_t* const lds_new = lds_q + 16 * HT * QROW;
@@ -254,11 +261,13 @@ paged16_split_kernel(Paged16Params prm) {
 
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, j = lane >> 4;
-  RowLens rows{a.seq_lens, a.B, prm.S, lane, 0, 0};
+  RowLens rows{lens, B, S, lane, 0, 0};
   Shares sh;
   Segment g;
   uint32_t share_end;
-  if (!first_segment(prm, blockIdx.y, rows, sh, g, share_end)) return;
+  if (!first_segment(SharePlan{lens, B, S, workgroups, least_chunks, long_workgroups, long_chunks}, blockIdx.y, rows, sh,
+                     g, share_end))
+    return;
   const int hk = blockIdx.x % a.HKV, hb0 = (blockIdx.x / a.HKV) * 16 * HT;
   const int nh = min(16 * HT, prm.G - hb0), h0 = hk * prm.G + hb0;
 
@@ -507,7 +516,7 @@ paged16_split_kernel(Paged16Params prm) {
     // registers over the whole loop.)
     const int mr = (int)opaque(r), mj = (int)opaque(j), mt = (int)opaque(tid);
     const int b = g.b, mine_rows = min(16 * HT, prm.G);
-    const int stride = mine_rows * (D + 1) + 2 * mine_rows;
+    const int stride = (mine_rows * (OROW + 2) + 3) / 4 * 4;
 #pragma unroll
     for (int ht = 0; ht < HT; ++ht) {
       const float lt = xor_sum16_32(l_run[ht]);
@@ -515,12 +524,14 @@ paged16_split_kernel(Paged16Params prm) {
       if (n >= nh) continue;
       float* mine = lds + w * stride;
 #pragma unroll
-      for (int mv = 0; mv < EPL; ++mv)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mine[n * (D + 1) + EPL * (4 * mj + i) + mv] = accv[ht][mv][i];
+        for (int mv = 0; mv < EPL; mv += 4)
+          *reinterpret_cast<f4*>(mine + n * OROW + EPL * (4 * mj + i) + mv) =
+              f4{accv[ht][mv][i], accv[ht][mv + 1][i], accv[ht][mv + 2][i], accv[ht][mv + 3][i]};
       if (mj == 0) {
-        mine[mine_rows * (D + 1) + n] = m_run[ht];
-        mine[mine_rows * (D + 2) + n] = lt;
+        mine[mine_rows * OROW + n] = m_run[ht];
+        mine[mine_rows * (OROW + 1) + n] = lt;
       }
     }
     __syncthreads();
@@ -528,7 +539,7 @@ paged16_split_kernel(Paged16Params prm) {
     const uint32_t l = chunks_of(g.L);
     const bool whole = g.begin == 0 && g.end == l;
     const uint32_t slot = 2 * blockIdx.y + (g.begin == 0 ? 1 : 0);
-    if (a.workgroups && g.begin == 0 && blockIdx.x == 0 && mt == 0)
+    if (workgroups && g.begin == 0 && blockIdx.x == 0 && mt == 0)
       reinterpret_cast<int2*>(a.row_pieces)[b] =
           make_int2(blockIdx.y, whole ? 1 : (int)(sh.of(g.at + l - 1) - blockIdx.y + 1));
     // The next segment, whose first loads run behind this one's merge.
@@ -546,7 +557,7 @@ paged16_split_kernel(Paged16Params prm) {
       float mw[NW], mstar = -INFINITY;
 #pragma unroll
       for (int x = 0; x < NW; ++x) {
-        mw[x] = lds[x * stride + mine_rows * (D + 1) + n];
+        mw[x] = lds[x * stride + mine_rows * OROW + n];
         mstar = fmaxf(mstar, mw[x]);
       }
       f4 o = f4{0.f, 0.f, 0.f, 0.f};
@@ -556,16 +567,16 @@ paged16_split_kernel(Paged16Params prm) {
         // A wave whose scores were all NaN keeps a maximum of -inf and a sum of
         // NaN, which the factor 0 hands on.
         const float f = safe_exp2_diff(mw[x], mstar);
-        const float* ow = lds + x * stride + n * (D + 1) + d;
-        o += f4{ow[0], ow[1], ow[2], ow[3]} * f;
-        ls = fmaf(f, lds[x * stride + mine_rows * (D + 2) + n], ls);
+        o += *reinterpret_cast<const f4*>(lds + x * stride + n * OROW + d) * f;
+        ls = fmaf(f, lds[x * stride + mine_rows * (OROW + 1) + n], ls);
       }
       if (whole) {
-        store_row4(a, T::kShift, (int64_t)b * a.HQ + h0 + n, d, o, mstar, ls);
+        store_row4(a.out, a.lse, D, T::kShift, (int64_t)b * a.HQ + h0 + n, d, o, mstar, ls);
       } else {
-        const int64_t row = partial_row(a, slot, h0 + n);
+        const int64_t row = partial_row(a.HQ, slot, h0 + n);
         *reinterpret_cast<f4*>(a.partials + row * D + d) = o;
-        if (d == 0) *reinterpret_cast<float2*>(partial_ml(a) + 2 * row) = make_float2(mstar, ls);
+        if (d == 0)
+          *reinterpret_cast<float2*>(partial_ml(a.partials, workgroups, a.HQ, D) + 2 * row) = make_float2(mstar, ls);
       }
     }
     if (!again) break;
@@ -581,26 +592,26 @@ paged16_split_kernel(Paged16Params prm) {
 // pieces each, and four of them share a workgroup.
 // ---------------------------------------------------------------------------
 template <int D, int LANES>
-__global__ void __launch_bounds__(256) paged16_join_kernel(Paged16Params prm, float shift) {
+__global__ void __launch_bounds__(256) paged16_join_kernel(const int2* row_pieces, float* partials, float* out,
+                                                           float* lse, int HQ, int rows, int workgroups, float shift) {
   constexpr int DQ = D / 4, SG = LANES / DQ, ROWS = 256 / LANES;
   __shared__ float sm_m[ROWS][SG], sm_l[ROWS][SG];
   __shared__ f4 sm_a[ROWS][SG][DQ];
-  const tkv_paged16_args& a = prm.a;
   const int in = threadIdx.x / LANES, row0 = blockIdx.x * ROWS + in;
-  const bool live = row0 < a.B * a.HQ;
-  const int b = live ? row0 / a.HQ : 0, h = row0 - b * a.HQ;
-  const int2 pieces = live ? reinterpret_cast<const int2*>(a.row_pieces)[b] : make_int2(0, 0);
+  const bool live = row0 < rows;
+  const int b = live ? row0 / HQ : 0, h = row0 - b * HQ;
+  const int2 pieces = live ? row_pieces[b] : make_int2(0, 0);
   if (ROWS == 1 && pieces.y <= 1) return;
   const int t = threadIdx.x % LANES, dq = t % DQ, g = t / DQ;
-  const float* ml = partial_ml(a);
+  const float* ml = partial_ml(partials, workgroups, HQ, D);
   float m = -INFINITY, l = 0.0f;
   f4 o = f4{0.f, 0.f, 0.f, 0.f};
   const int n = pieces.y > 1 ? pieces.y : 0;
 #pragma unroll 4
   for (int s = g; s < n; s += SG) {
-    const int64_t row = partial_row(a, 2 * (pieces.x + s) + (s == 0 ? 1 : 0), h);
+    const int64_t row = partial_row(HQ, 2 * (pieces.x + s) + (s == 0 ? 1 : 0), h);
     const float2 x = *reinterpret_cast<const float2*>(ml + 2 * row);
-    const f4 os = *reinterpret_cast<const f4*>(a.partials + row * D + 4 * dq);
+    const f4 os = *reinterpret_cast<const f4*>(partials + row * D + 4 * dq);
     const float mn = fmaxf(m, x.x);
     const float al = safe_exp2_diff(m, mn), be = safe_exp2_diff(x.x, mn);
     o = o * al + os * be;
@@ -624,7 +635,7 @@ __global__ void __launch_bounds__(256) paged16_join_kernel(Paged16Params prm, fl
       ot += sm_a[in][x][dq] * f;
       lt += sm_l[in][x] * f;
     }
-    store_row4(a, shift, (int64_t)b * a.HQ + h, 4 * dq, ot, mstar, lt);
+    store_row4(out, lse, D, shift, row0, 4 * dq, ot, mstar, lt);
   }
 }
 
@@ -737,17 +748,21 @@ static int launch_paged16(const Paged16Params& p, hipStream_t st) {
   constexpr int NW = 4;
   const int rows = p.G < 16 * HT ? p.G : 16 * HT, blocks = (p.G + 16 * HT - 1) / (16 * HT);
   const dim3 grid((unsigned)(p.a.HKV * blocks), (unsigned)(p.a.workgroups ? p.a.workgroups : p.a.B));
-  const size_t lds = 32 * HT * (D + 8) + sizeof(float) * NW * (rows * (D + 1) + 2 * rows);
-  return p.a.k_new ? launch(paged16_split_kernel<T, D, HT, NW, true>, grid, dim3(NW * 64), lds + 4 * D, st, p)
-                   : launch(paged16_split_kernel<T, D, HT, NW, false>, grid, dim3(NW * 64), lds, st, p);
+  const int wave = (rows * (D + 6) + 3) / 4 * 4;  // floats of a wave's partial
+  const size_t lds = 32 * HT * (D + 8) + sizeof(float) * NW * wave;
+  const auto kernel = p.a.k_new ? paged16_split_kernel<T, D, HT, NW, true> : paged16_split_kernel<T, D, HT, NW, false>;
+  return launch(kernel, grid, dim3(NW * 64), p.a.k_new ? lds + 4 * D : lds, st, p.a.seq_lens, p.a.B,
+                p.a.max_pages * p.a.page_size, p.a.workgroups, p.a.least_chunks, p.a.long_workgroups, p.a.long_chunks, p);
 }
 
 template <int D>
 static int launch_join(const Paged16Params& p, float shift, hipStream_t st) {
   const int rows = p.a.B * p.a.HQ;
-  return rows >= kJoinRows
-             ? launch(paged16_join_kernel<D, 64>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, shift)
-             : launch(paged16_join_kernel<D, 256>, dim3((unsigned)rows), dim3(256), 0, st, p, shift);
+  const bool many = rows >= kJoinRows;
+  return launch(many ? paged16_join_kernel<D, 64> : paged16_join_kernel<D, 256>,
+                dim3((unsigned)(many ? (rows + 3) / 4 : rows)), dim3(256), 0, st,
+                reinterpret_cast<const int2*>(p.a.row_pieces), p.a.partials, p.a.out, p.a.lse, p.a.HQ, rows,
+                p.a.workgroups, shift);
 }
 
 template <class T, int D>
@@ -773,7 +788,6 @@ extern "C" int tkv_paged16_decode_attention(const tkv_paged16_args* a, tkv_strea
   p.a = *a;
   p.G = a->HQ / a->HKV;
   p.page_tiles = a->page_size / 16;
-  p.S = a->max_pages * a->page_size;
   p.qk_scale = a->sm_scale * kLog2e;
   for (int i = 0; i < 3; ++i) {
     p.k16[i] = (uint32_t)(a->k_strides[i] / 8);
