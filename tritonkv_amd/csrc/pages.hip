@@ -16,7 +16,8 @@
 
 namespace tkv {
 
-constexpr int kPlan = 1024;                  // threads of a plan's workgroup
+constexpr int kPlan = 1024;                  // most threads of a plan's workgroup
+constexpr int kSmallPlan = 256;              // ... where its rows and pages fit them
 constexpr int kCopy = 1024;                  // threads of a copy's workgroup
 constexpr int kMaxRows = 8192;               // rows of a fork: two LDS integers each
 constexpr int kInlinePairs = 4096;           // pairs that the copy checks by itself
@@ -162,12 +163,14 @@ __global__ void __launch_bounds__(kCopy) copy_pairs_kernel(CopyPlan c, const int
 // ---------------------------------------------------------------------------
 // Sums over a plan's workgroup.
 // ---------------------------------------------------------------------------
+template <int T>
 struct ScanLds {
-  int2 wave[kPlan / 64];
+  int2 wave[T / 64];
 };
 
 // Exclusive sums of (x, y) over the threads before this one; total of both.
-__device__ __forceinline__ int2 block_scan(ScanLds& lds, int x, int y, int2& total) {
+template <int T>
+__device__ __forceinline__ int2 block_scan(ScanLds<T>& lds, int x, int y, int2& total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int sx = x, sy = y;
 #pragma unroll
@@ -184,7 +187,7 @@ __device__ __forceinline__ int2 block_scan(ScanLds& lds, int x, int y, int2& tot
   int2 before = make_int2(0, 0);
   total = make_int2(0, 0);
 #pragma unroll
-  for (int i = 0; i < kPlan / 64; ++i) {
+  for (int i = 0; i < T / 64; ++i) {
     const int2 v = lds.wave[i];
     if (i < w) {
       before.x += v.x;
@@ -214,9 +217,9 @@ __device__ __forceinline__ uint64_t used_mask(const int32_t* __restrict__ refs, 
 __device__ __forceinline__ uint64_t first_bits(int64_t n) {
   return n <= 0 ? 0 : n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1;
 }
-// Pages a thread takes of N in one round of the workgroup.
-__device__ __forceinline__ int pages_per_thread(int N) {
-  const int per = ((N + kPlan - 1) / kPlan + 3) & ~3;
+// Pages that one of `threads` takes of N in one round of the workgroup.
+__host__ __device__ inline int pages_per_thread(int N, int threads) {
+  const int per = ((N + threads - 1) / threads + 3) & ~3;
   return per < kPagesPerThread ? per : kPagesPerThread;
 }
 
@@ -281,28 +284,29 @@ __device__ __forceinline__ Row row_of(const RowsParams& a, int b) {
   return r;
 }
 
-__global__ void __launch_bounds__(kPlan) rows_plan_kernel(RowsParams a) {
+template <int T>
+__global__ void __launch_bounds__(T) rows_plan_kernel(RowsParams a) {
   extern __shared__ int lds[];
-  __shared__ ScanLds scan;
+  __shared__ ScanLds<T> scan;
   __shared__ int past;
   const RowsWork w = rows_work(a);
   const int tid = threadIdx.x, B = a.B, P = a.max_pages, N = a.num_pages;
   if (blockIdx.x > 0) {
     // The rows' old pages, which the second launch reads while it writes the table.
-    for (int64_t i = (int64_t)(blockIdx.x - 1) * kPlan + tid; i < (int64_t)B * P; i += (int64_t)(gridDim.x - 1) * kPlan) {
+    for (int64_t i = (int64_t)(blockIdx.x - 1) * T + tid; i < (int64_t)B * P; i += (int64_t)(gridDim.x - 1) * T) {
       const int b = (int)(i / P);
       w.staged[i] = a.block_table[(int64_t)b * a.table_stride + (i - (int64_t)b * P)];
     }
     return;
   }
   int *most = lds, *best = lds + B;
-  for (int b = tid; b < B; b += kPlan) {
+  for (int b = tid; b < B; b += T) {
     most[b] = -1;
     best[b] = B;
   }
   if (tid == 0) past = 0;
   // This thread's first row and first pages stay in registers: most plans need no others.
-  const int per = pages_per_thread(N);
+  const int per = pages_per_thread(N, T);
   const uint64_t mask0 = used_mask(a.refs, (int64_t)tid * per, per, N);
   Row row0{-1, 0, 0, -1, false};
   int owners0 = 0;  // references of the page that it ends in
@@ -311,7 +315,7 @@ __global__ void __launch_bounds__(kPlan) rows_plan_kernel(RowsParams a) {
     if (row0.last >= 0 && row0.last < N) owners0 = a.refs[row0.last];
   }
   __syncthreads();
-  for (int b = tid; b < B; b += kPlan) {
+  for (int b = tid; b < B; b += T) {
     const Row r = b == tid ? row0 : row_of(a, b);
     if (r.a >= 0) atomicMax(most + r.a, r.f);
     if (r.want > table_tokens(a)) past = 1;
@@ -321,14 +325,14 @@ __global__ void __launch_bounds__(kPlan) rows_plan_kernel(RowsParams a) {
     if (!r.rest || r.f != most[r.a] || r.last < 0 || r.last >= N) return false;
     return (b == tid ? owners0 : a.refs[r.last]) == 1;
   };
-  for (int b = tid; b < B; b += kPlan) {
+  for (int b = tid; b < B; b += T) {
     const Row r = b == tid ? row0 : row_of(a, b);
     if (may_inherit(r, b)) atomicMin(best + r.a, r.a == b ? -1 : b);
   }
   __syncthreads();
   const bool too_long = past != 0;
   int2 done = make_int2(0, 0);  // new pages and copies of the rows before this round's
-  for (int b0 = 0; b0 < B; b0 += kPlan) {
+  for (int b0 = 0; b0 < B; b0 += T) {
     const int b = b0 + tid;
     Row r;
     int need = 0, pages = 0;
@@ -355,7 +359,7 @@ __global__ void __launch_bounds__(kPlan) rows_plan_kernel(RowsParams a) {
   }
   // The lowest free pages.
   int found = 0;
-  for (int64_t p0 = 0; p0 < N && found < done.x; p0 += (int64_t)per * kPlan) {
+  for (int64_t p0 = 0; p0 < N && found < done.x; p0 += (int64_t)per * T) {
     const int64_t mine = p0 + (int64_t)tid * per;
     uint64_t m = ~(p0 ? used_mask(a.refs, mine, per, N) : mask0) & first_bits(N - mine) & first_bits(per);
     int2 total;
@@ -366,7 +370,7 @@ __global__ void __launch_bounds__(kPlan) rows_plan_kernel(RowsParams a) {
   const int status = too_long ? TKV_ROWS_PAST_TABLE : found < done.x ? TKV_ROWS_NO_PAGES : TKV_ROWS_DONE;
   settle();
   const int copies = status ? 0 : done.y;
-  for (int i = tid; i < copies; i += kPlan) {
+  for (int i = tid; i < copies; i += T) {
     int2 p = w.pairs[i];
     p.y = w.fresh[p.y];
     if (p.x >= N) p.x = -1;  // the table names no page there
@@ -425,7 +429,7 @@ __global__ void __launch_bounds__(kCopy) rows_apply_kernel(RowsParams a, CopyPla
 struct CompactParams {
   const int32_t *block_table, *refs;
   int32_t *out_table, *out_refs, *live, *work;
-  int32_t table_stride, out_stride, B, max_pages, num_pages;
+  int32_t table_stride, out_stride, B, max_pages, num_pages, per;  // per: pages of a thread's block
 };
 
 // The plan's blocks: the pages of one thread in one round.
@@ -438,7 +442,7 @@ struct CompactWork {
   int* head;          // live pages, moves
   int2* pairs;        // at most N / 2 moves
   int* count;         // references of the i-th page that moves
-  PageBlock* blocks;  // of pages_per_thread(N) >= 4 pages each
+  PageBlock* blocks;  // of per >= 4 pages each
 };
 
 __host__ __device__ inline int64_t compact_work_ints(int64_t N) {
@@ -456,11 +460,12 @@ __device__ __forceinline__ CompactWork compact_work(const CompactParams& a) {
   return w;
 }
 
-__global__ void __launch_bounds__(kPlan) compact_plan_kernel(CompactParams a) {
-  __shared__ ScanLds scan;
+template <int T>
+__global__ void __launch_bounds__(T) compact_plan_kernel(CompactParams a) {
+  __shared__ ScanLds<T> scan;
   const CompactWork w = compact_work(a);
-  const int tid = threadIdx.x, N = a.num_pages, per = pages_per_thread(N);
-  const int64_t round = (int64_t)per * kPlan;
+  const int tid = threadIdx.x, N = a.num_pages, per = a.per;
+  const int64_t round = (int64_t)per * T;
   int live = 0;
   uint64_t m = 0;
   for (int64_t p0 = 0; p0 < N; p0 += round) {
@@ -514,7 +519,7 @@ __global__ void __launch_bounds__(kCopy) compact_apply_kernel(CompactParams a, C
     copy_pairs(c, w.pairs, w.head[1], blockIdx.x - tables, gridDim.x - tables);
     return;
   }
-  const int P = a.max_pages, N = a.num_pages, per = pages_per_thread(N);
+  const int P = a.max_pages, N = a.num_pages, per = a.per;
   const int64_t entries = (int64_t)a.B * P;
   for (int64_t i = (int64_t)blockIdx.x * kCopy + threadIdx.x; i < entries + N; i += (int64_t)tables * kCopy) {
     if (i < entries) {
@@ -623,11 +628,14 @@ extern "C" int tkv_fork_rows(const tkv_fork_rows_args* a, tkv_stream_t stream) {
   if (rc) return rc;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int64_t entries = (int64_t)a->B * a->max_pages;
-  const unsigned staging = a->parents ? (unsigned)((entries + 4 * kPlan - 1) / (4 * kPlan)) : 0;
+  // Small plans take 4 waves: barriers and prefix sums over 16 cost 1 us more.
+  const bool small = a->B <= kSmallPlan && a->num_pages <= 16 * kSmallPlan;
+  const int threads = small ? kSmallPlan : kPlan;
+  const unsigned staging = a->parents ? (unsigned)((entries + 4 * threads - 1) / (4 * threads)) : 0;
   const RowsParams p{a->block_table, a->seq_lens, a->refs, a->parents, a->new_lens, a->status, a->work,
                      a->table_stride, a->B, a->max_pages, a->page_size, a->num_pages};
-  const int bad = launch(rows_plan_kernel, dim3(1 + (staging < 512 ? staging : 512)), dim3(kPlan),
-                         2 * sizeof(int) * a->B, st, p);
+  const int bad = launch(small ? rows_plan_kernel<kSmallPlan> : rows_plan_kernel<kPlan>,
+                         dim3(1 + (staging < 512 ? staging : 512)), dim3(threads), 2 * sizeof(int) * a->B, st, p);
   if (bad) return bad;
   const int64_t tables = (entries + kCopy - 1) / kCopy;
   const int t = (int)(tables < 512 ? tables : 512);
@@ -649,9 +657,13 @@ extern "C" int tkv_compact_pages(const tkv_compact_pages_args* a, tkv_stream_t s
   const int rc = make_plan(a->set, c);
   if (rc) return rc;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const bool small = a->num_pages <= 16 * kSmallPlan;  // (more pages: more threads to share them)
+  const int threads = small ? kSmallPlan : kPlan;
   const CompactParams p{a->block_table, a->refs, a->out_table, a->out_refs, a->live, a->work,
-                        a->table_stride, a->out_stride, a->B, a->max_pages, a->num_pages};
-  const int bad = launch(compact_plan_kernel, dim3(1), dim3(kPlan), 0, st, p);
+                        a->table_stride, a->out_stride, a->B, a->max_pages, a->num_pages,
+                        pages_per_thread(a->num_pages, threads)};
+  const int bad = launch(small ? compact_plan_kernel<kSmallPlan> : compact_plan_kernel<kPlan>, dim3(1), dim3(threads),
+                         0, st, p);
   if (bad) return bad;
   const int64_t tables = ((int64_t)a->B * a->max_pages + a->num_pages + kCopy - 1) / kCopy;
   const int t = (int)(tables < 512 ? tables : 512);
