@@ -537,3 +537,32 @@ def test_another_stream_and_repeated_calls():
     assert m.same_as(table, lens, refs)
     with pytest.raises(ValueError):
         fork_rows(pools, table, lens.long(), refs, parents, _workspace=ws)
+
+
+def test_a_kept_call_checks_that_its_tensors_lie_apart():
+    from tritonkv_amd.pages import compact_pages, fork_rows
+
+    m = Model(2, 4, 30, 16)
+    pools = [_pool(30, seed=2)]
+    table, lens, refs = _state(m)
+    ws = {}
+    for new in ([20, 40], [40, 20]):
+        assert fork_rows(pools, table, lens, refs, _i32([0, 1]), _i32(new), _workspace=ws).tolist() == [0]
+        m.fork([0, 1], new)
+    prep = ws["call"]
+    with pytest.raises(ValueError, match="share memory"):
+        fork_rows(pools, table, lens, refs, _i32([0, 1]), lens, _workspace=ws)
+    with pytest.raises(ValueError, match="share memory"):
+        fork_rows(pools, table, lens, refs, _i32([0, 1]), _i32([9, 9]), status=refs[5:6], _workspace=ws)
+    both = _i32([0, 1, 9, 9])
+    with pytest.raises(ValueError, match="share memory"):
+        fork_rows(pools, table, lens, refs, both[:2], both[2:], status=both[1:2], _workspace=ws)
+    same = _i32([1, 0])  # read twice: no fault
+    assert fork_rows(pools, table, lens, refs, same, same, _workspace=ws).tolist() == [0]
+    m.fork([1, 0], [1, 0])
+    assert ws["call"] is prep and m.same_as(table, lens, refs)
+    ws = {}
+    for _ in range(2):  # in place: the tables are read and written
+        compact_pages(pools, table, refs, _workspace=ws)
+    with pytest.raises(ValueError, match="share memory"):
+        compact_pages(pools, table, refs, live=refs[3:4], _workspace=ws)

@@ -65,10 +65,12 @@ Z = torch.zeros
     (dict(out=Z(2 * 8 * 128 + 1)[1:].view(2, 8, 128)), ValueError, "16-byte"),
     (dict(lse=Z(2, 7)), ValueError, "lse"),
     (dict(lse=Z(2, 8, dtype=F16)), ValueError, "lse"),
+    (dict(lse=[0.0]), ValueError, "lse"),
     (dict(k_new=Z(2, 2, 128, dtype=F16)), ValueError, "together"),
     (dict(k_new=Z(2, 2, 128, dtype=F16), v_new=Z(2, 2, 64, dtype=F16)), ValueError, "v_new must have shape"),
     (dict(k_new=Z(2, 2, 128), v_new=Z(2, 2, 128)), TypeError, "pools' dtype"),
     (dict(piece_tokens=0), ValueError, "piece_tokens"),
+    (dict(piece_tokens=1 << 60), RuntimeError, "HIP"),
 ])
 def test_decode_refuses_before_the_backend(kw, error, match):
     with pytest.raises(error, match=match):

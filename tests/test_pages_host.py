@@ -249,3 +249,47 @@ def test_too_many_rows_for_the_c_entry():
     f = _lib.ForkRowsArgs(set=_set(_lib), block_table=d, seq_lens=d, refs=d, status=d, work=d, table_stride=3,
                           B=8193, max_pages=3, page_size=16, num_pages=6)
     assert _lib.load().tkv_fork_rows(ctypes.byref(f), None) == _lib.TKV_EUNSUPPORTED
+
+
+def test_too_many_pages():
+    from tritonkv_amd import _lib
+    from tritonkv_amd.pages import copy_pages, fork_rows
+
+    lib, d, n = _lib.load(), 0x1000, 2 ** 30 + 1
+    s = _set(_lib)
+    for kw in (dict(n=n), dict(src_pages=n, dst_pages=n, same=1), dict(src_pages=n)):
+        c = _lib.CopyPagesArgs(set=s, src=d, dst=d, work=d, **(dict(n=3, src_pages=6, dst_pages=6) | kw))
+        assert lib.tkv_copy_pages(ctypes.byref(c), None) == _lib.TKV_EUNSUPPORTED
+        assert lib.tkv_copy_pages_work(ctypes.byref(c)) == _lib.TKV_EUNSUPPORTED
+    f = _lib.ForkRowsArgs(set=s, block_table=d, seq_lens=d, refs=d, status=d, work=d, table_stride=3, B=2,
+                          max_pages=3, page_size=16, num_pages=n)
+    p = _lib.CompactPagesArgs(set=s, block_table=d, refs=d, out_table=d, out_refs=d, work=d, table_stride=3,
+                              out_stride=3, B=2, max_pages=3, num_pages=n)
+    assert lib.tkv_fork_rows(ctypes.byref(f), None) == _lib.TKV_EUNSUPPORTED
+    assert lib.tkv_compact_pages(ctypes.byref(p), None) == _lib.TKV_EUNSUPPORTED
+    many = torch.empty(1, dtype=torch.uint8).expand(n, 1, 16, 16)
+    with pytest.raises(ValueError, match="at most"):
+        copy_pages([many], Z(1), Z(1))
+    with pytest.raises(ValueError, match="at most"):
+        copy_pages([_pool()], Z(1).expand(n), Z(1).expand(n))
+    wide = torch.empty(2, 2 ** 30, dtype=torch.int32)  # (never touched)
+    with pytest.raises(ValueError, match="at most"):
+        fork_rows([_pool()], wide, Z(2), Z(6), Z(2))
+
+
+def test_a_kept_call_refuses_what_shares_memory():
+    from tritonkv_amd import _lib
+    from tritonkv_amd.pages import _APART, _WRITTEN
+
+    b = Z(64)
+    table, status, parents = b[:8].view(2, 4), b[8:9], b[16:18]
+    call = _lib.host().prepare(bytes(_lib.ForkRowsArgs()), _lib.address("tkv_fork_rows"), 0,
+                               ((table, -1, 4, 1 | _WRITTEN), (status, 0, 4, _WRITTEN), (parents, 8, 4, _APART),
+                                (parents, 16, 4, _APART)), None)
+    run = _lib.host().run
+    # (a call without these faults would ask for the device's stream)
+    for s, p0, p1 in ((b[7:8], parents, parents), (status, b[7:9], parents), (status, parents, b[6:8]),
+                      (b[17:18], parents, parents), (b[20:21], parents, b[19:21])):
+        assert run(call, table, s, p0, p1) is None
+    with pytest.raises(ValueError, match="too many"):
+        _lib.host().prepare(b"", 0, 0, ((table, -1, 4, _APART),) * 17, None)

@@ -45,7 +45,12 @@ struct Slot {
   c10::Device device{c10::kCPU};
   std::vector<int64_t> sizes;
   std::vector<int64_t> strides;  // of a tensor that is used as it is strided; else empty: contiguous
+  uintptr_t span;                // bytes from its first entry to the end of its last
+  bool apart, written;           // shares no memory with other such slots if one of the two is written
 };
+
+constexpr int kStrided = 1, kApart = 2, kWritten = 4;  // a slot's flags
+constexpr size_t kMaxApart = 16;                       // such slots of a call
 
 constexpr size_t kMaxArgs = 2048;  // bytes of an argument block
 
@@ -78,7 +83,8 @@ void free_call(PyObject* capsule) {
 }
 
 // prepare(args: bytes, entry: int, device: int, slots: tuple of (tensor or None,
-//   offset or -1, alignment[, strided: the argument block holds its strides]),
+//   offset or -1, alignment[, flags: 1 the argument block holds its strides, 2 it must
+//   not share memory with a slot of flag 4, 4 it is written]),
 //   window: None or (k_res, v_res, res_lens, res_cap))
 PyObject* prepare(PyObject*, PyObject* const* a, Py_ssize_t n) {
   try {
@@ -94,10 +100,11 @@ PyObject* prepare(PyObject*, PyObject* const* a, Py_ssize_t n) {
     std::memcpy(call->args, bytes, len);
     call->entry = PyLong_AsVoidPtr(a[1]);
     call->device = (c10::DeviceIndex)PyLong_AsLong(a[2]);
+    size_t apart = 0;
     for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[3]); ++i) {
       PyObject *t;
-      int offset, align, strided = 0;
-      if (!PyArg_ParseTuple(PyTuple_GET_ITEM(a[3], i), "Oii|i", &t, &offset, &align, &strided)) return nullptr;
+      int offset, align, flags = 0;
+      if (!PyArg_ParseTuple(PyTuple_GET_ITEM(a[3], i), "Oii|i", &t, &offset, &align, &flags)) return nullptr;
       if (offset != kFixed && (offset < 0 || offset + (Py_ssize_t)sizeof(void*) > len)) {
         PyErr_SetString(PyExc_ValueError, "prepare: an offset past the argument block");
         return nullptr;
@@ -112,12 +119,20 @@ PyObject* prepare(PyObject*, PyObject* const* a, Py_ssize_t n) {
           return nullptr;
         }
         const at::Tensor& v = THPVariable_Unpack(t);
-        if (strided && !v.is_contiguous()) s.strides = v.strides().vec();
+        if (flags & kStrided && !v.is_contiguous()) s.strides = v.strides().vec();
         s.ptr = plain_pointer(v, s.strides);
         if (!s.ptr || ((uintptr_t)s.ptr & s.align_mask)) Py_RETURN_NONE;  // not a call to keep
         s.dtype = v.scalar_type();
         s.device = v.device();
         s.sizes = v.sizes().vec();
+        s.written = flags & kWritten;
+        s.apart = s.written || flags & kApart;
+        s.span = v.element_size();
+        for (int64_t d = 0; d < v.dim(); ++d) s.span += v.element_size() * (v.size(d) - 1) * v.stride(d);
+        if (s.apart && ++apart > kMaxApart) {
+          PyErr_SetString(PyExc_ValueError, "prepare: too many slots that must lie apart");
+          return nullptr;
+        }
       }
       call->slots.push_back(std::move(s));
     }
@@ -152,6 +167,11 @@ PyObject* run(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if ((size_t)(n - 1) != call->slots.size()) Py_RETURN_NONE;
     alignas(16) char args[kMaxArgs];
     std::memcpy(args, call->args, call->size);
+    struct {
+      uintptr_t begin, end;
+      bool written;
+    } apart[kMaxApart];
+    size_t spans = 0;
     for (size_t i = 0; i < call->slots.size(); ++i) {
       const Slot& s = call->slots[i];
       PyObject* o = a[i + 1];
@@ -166,6 +186,12 @@ PyObject* run(PyObject*, PyObject* const* a, Py_ssize_t n) {
       void* p = plain_pointer(t, s.strides);
       if (!p || ((uintptr_t)p & s.align_mask) || (s.offset == kFixed && p != s.ptr)) Py_RETURN_NONE;
       if (s.offset != kFixed) std::memcpy(args + s.offset, &p, sizeof p);
+      if (s.apart) {
+        const uintptr_t begin = (uintptr_t)p, end = begin + s.span;
+        for (size_t x = 0; x < spans; ++x)
+          if ((s.written || apart[x].written) && begin < apart[x].end && apart[x].begin < end) Py_RETURN_NONE;
+        apart[spans++] = {begin, end, s.written};
+      }
     }
     c10::hip::OptionalHIPGuard guard;
     if (c10::hip::current_device() != call->device) guard.set_index(call->device);

@@ -22,6 +22,7 @@ constexpr int kCopy = 1024;                  // threads of a copy's workgroup
 constexpr int kMaxRows = 8192;               // rows of a fork: two LDS integers each
 constexpr int kInlinePairs = 4096;           // pairs that the copy checks by itself
 constexpr int kPagesPerThread = 64;          // bits of a thread's mask of pages
+constexpr int kMaxPages = 1 << 30;           // of a pool, and pairs of a call: sums of two fit an integer
 
 // A barrier behind which the workgroup's memory operations have been carried out.
 __device__ __forceinline__ void settle() {
@@ -131,7 +132,8 @@ __global__ void __launch_bounds__(kCopy) copy_few_kernel(CopyPlan c, PairLists a
 __global__ void __launch_bounds__(kPlan) copy_check_kernel(PairLists a) {
   int* owner = a.work;
   int* read = owner + a.dst_pages;
-  int2* pairs = reinterpret_cast<int2*>(a.work + a.dst_pages + a.src_pages + (((a.dst_pages + a.src_pages) & 1)));
+  const int64_t pages = (int64_t)a.dst_pages + a.src_pages;
+  int2* pairs = reinterpret_cast<int2*>(a.work + pages + (pages & 1));
   for (int i = threadIdx.x; i < a.n; i += kPlan) {
     const int s = a.src[i], d = a.dst[i];
     if (is_pair(a, s, d)) {
@@ -568,12 +570,9 @@ static unsigned copy_groups(int64_t pairs, const CopyPlan& c) {
   return (unsigned)(items < kCopyGroups ? items : kCopyGroups);
 }
 
-}  // namespace tkv
-
-namespace tkv {
-
 static int check_copy(const tkv_copy_pages_args* a, CopyPlan& c) {
   if (!a || !a->src || !a->dst || a->n <= 0 || a->src_pages <= 0 || a->dst_pages <= 0) return TKV_EINVAL;
+  if (a->n > kMaxPages || a->src_pages > kMaxPages || a->dst_pages > kMaxPages) return TKV_EUNSUPPORTED;
   if (a->same && a->src_pages != a->dst_pages) return TKV_EINVAL;
   return make_plan(a->set, c);
 }
@@ -604,7 +603,7 @@ extern "C" int tkv_copy_pages(const tkv_copy_pages_args* a, tkv_stream_t stream)
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(copy_groups(a->n, c)), block(kCopy);
   if (in_line) return launch(copy_few_kernel, grid, block, 0, st, c, p);
-  const int pages = a->dst_pages + a->src_pages;
+  const int64_t pages = (int64_t)a->dst_pages + a->src_pages;
   const int2* pairs = reinterpret_cast<const int2*>(a->work + pages + (pages & 1));
   const int bad = launch(copy_check_kernel, dim3(1), dim3(kPlan), 0, st, p);
   return bad ? bad : launch(copy_pairs_kernel, grid, block, 0, st, c, pairs, (const int*)nullptr, (int)a->n);
@@ -621,7 +620,7 @@ extern "C" int tkv_fork_rows(const tkv_fork_rows_args* a, tkv_stream_t stream) {
     return TKV_EINVAL;
   if (a->B <= 0 || a->max_pages <= 0 || a->num_pages <= 0 || a->page_size <= 0 || a->table_stride < a->max_pages)
     return TKV_EINVAL;
-  if (a->B > kMaxRows) return TKV_EUNSUPPORTED;
+  if (a->B > kMaxRows || a->num_pages > kMaxPages) return TKV_EUNSUPPORTED;
   if ((int64_t)a->max_pages * a->page_size > INT32_MAX || (int64_t)a->B * a->max_pages > INT32_MAX) return TKV_EINVAL;
   CopyPlan c;
   const int rc = make_plan(a->set, c);
@@ -653,6 +652,7 @@ extern "C" int tkv_compact_pages(const tkv_compact_pages_args* a, tkv_stream_t s
   if (a->B <= 0 || a->max_pages <= 0 || a->num_pages <= 0 || a->table_stride < a->max_pages ||
       a->out_stride < a->max_pages)
     return TKV_EINVAL;
+  if (a->num_pages > kMaxPages) return TKV_EUNSUPPORTED;
   CopyPlan c;
   const int rc = make_plan(a->set, c);
   if (rc) return rc;

@@ -118,7 +118,7 @@ def plan_shares(B: int, HKV: int, G: int, S: int, D: int = 128, device=None,
     if piece_tokens is not None:
         if piece_tokens <= 0:
             raise ValueError(f"piece_tokens must be positive, got {piece_tokens}")
-        least = -(-piece_tokens // 32)
+        least = min(-(-piece_tokens // 32), 1 << 26)  # more than any table holds
         if S <= 32 * least:
             return least, 0, 0, 0
         most = -(-B * -(-S // 32) // least)  # where every row fills its table
@@ -271,6 +271,8 @@ def paged16_decode_attention(
     of no tokens gives zeros.  ``lse``: a contiguous ``(B, HQ)`` float32 tensor
     that receives the natural logarithm of each row's sum of exp(score), -inf
     for a row of no tokens, so that the results over two caches can be joined.
+    Nothing past a row's length reaches them, NaN and infinities included; an
+    infinite V value of a live token gives an infinity or NaN.
 
     ``k_new`` / ``v_new``, ``(B, HKV, D)`` or ``(B, HKV, 1, D)`` in the pools'
     type, fuse the step's append into the call: the token takes position
@@ -307,8 +309,8 @@ def paged16_decode_attention(
     table = _check_table(block_table, B, device)
     S = table.shape[1] * page_size
     lens = None if seq_lens is None else _int32_arg(seq_lens, B, device, "seq_lens", "B lengths")
-    if lse is not None and (lse.shape != (B, HQ) or lse.dtype != torch.float32 or not lse.is_contiguous()
-                            or lse.device != device):
+    if lse is not None and (not isinstance(lse, torch.Tensor) or lse.shape != (B, HQ) or lse.dtype != torch.float32
+                            or not lse.is_contiguous() or lse.device != device):
         raise ValueError(f"lse must be a contiguous float32 ({B}, {HQ}) tensor on {device}")
     if (k_new is None) != (v_new is None):
         raise ValueError("k_new and v_new must be given together")

@@ -33,6 +33,7 @@ from .kernels.fused_decode_attn import _prepared
 from .quantize import QuantizedTensor, _require_gpu
 
 MAX_ROWS = 8192
+MAX_PAGES = 2 ** 30
 
 
 def _tensors(pools) -> list:
@@ -65,6 +66,8 @@ def _check_pages(tensors: list, num_pages: int | None, device, what: str) -> lis
         if t.dim() != 4 or t.numel() == 0 or (num_pages is not None and t.shape[0] != num_pages):
             raise ValueError(f"{what} must hold (num_pages, HKV, page_size, ...) tensors"
                              + ("" if num_pages is None else f" of {num_pages} pages") + f", got {tuple(t.shape)}")
+        if t.shape[0] > MAX_PAGES:
+            raise ValueError(f"{what}: at most {MAX_PAGES} pages, got {t.shape[0]}")
         if t.device != device:
             raise ValueError(f"{what} must be on {device}, got a tensor on {t.device}")
         if t.is_contiguous():
@@ -112,6 +115,9 @@ def _check_rows(block_table, refs) -> tuple:
     if not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32 or block_table.dim() != 2 \
             or block_table.numel() == 0 or block_table.device != refs.device or _row_stride(block_table) is None:
         raise ValueError("block_table must be an int32 (B, max_pages) tensor with dense rows on refs' device")
+    if refs.numel() > MAX_PAGES or block_table.numel() > 2 ** 31 - 1:
+        raise ValueError(f"at most {MAX_PAGES} pages and 2**31 - 1 table entries, got {refs.numel()} and "
+                         f"{block_table.numel()}")
     return block_table.shape
 
 
@@ -138,6 +144,7 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 _C = {f: _offset(_lib.CopyPagesArgs, f) for f in ("src", "dst")}
 _F = {f: _offset(_lib.ForkRowsArgs, f) for f in ("parents", "new_lens", "status")}
 _P = {f: _offset(_lib.CompactPagesArgs, f) for f in ("live",)}
+_APART, _WRITTEN = 2, 4  # flags of a kept call's tensors: apart from written ones; written
 
 
 def copy_pages(pools, src: torch.Tensor, dst: torch.Tensor, dst_pools=None, _workspace: dict | None = None) -> None:
@@ -180,6 +187,8 @@ def copy_pages(pools, src: torch.Tensor, dst: torch.Tensor, dst_pools=None, _wor
     if not isinstance(src, torch.Tensor):
         raise ValueError("src must be an int32 tensor of page numbers")
     n = src.numel()
+    if n > MAX_PAGES:
+        raise ValueError(f"at most {MAX_PAGES} pairs, got {n}")
     s, d = (_int32_arg(x, n, device, name, "page numbers, as many as the other")
             for name, x in (("src", src), ("dst", dst)))
     _require_gpu(tensors[0], "copy_pages")
@@ -277,9 +286,9 @@ def fork_rows(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, refs: to
         _lib.check(_lib.launch(device, "tkv_copy_planned", one, work.data_ptr(), B), "fork_rows")
     if key is not None and len(sets) == 1:
         _keep16(_workspace, key, args, "tkv_fork_rows", "fork_rows", device, (work,),
-                ((block_table, -1, 4, 1), (seq_lens, -1, 4), (refs, -1, 4), (parents, _F["parents"], 4),
-                 (new_lens, _F["new_lens"], 4), (status_given, _F["status"], 4),
-                 *((t, -1, 16, 1) for t in tensors)))
+                ((block_table, -1, 4, 1 | _WRITTEN), (seq_lens, -1, 4, _WRITTEN), (refs, -1, 4, _WRITTEN),
+                 (parents, _F["parents"], 4, _APART), (new_lens, _F["new_lens"], 4, _APART),
+                 (status_given, _F["status"], 4, _WRITTEN), *((t, -1, 16, 1) for t in tensors)))
     return status_given
 
 
@@ -356,8 +365,9 @@ def compact_pages(pools, block_table: torch.Tensor, refs: torch.Tensor, out=None
         _lib.check(_lib.launch(device, "tkv_copy_planned", one, work.data_ptr(), num_pages // 2), "compact_pages")
     if key is not None and len(sets) == 1:
         _keep16(_workspace, key, args, "tkv_compact_pages", "compact_pages", device, (work,),
-                ((block_table, -1, 4, 1), (refs, -1, 4), (out_table, -1, 4, 1), (out_refs, -1, 4),
-                 (live_given, _P["live"], 4), *((t, -1, 16, 1) for t in tensors)))
+                ((block_table, -1, 4, 1 | _APART), (refs, -1, 4, _APART), (out_table, -1, 4, 1 | _APART),
+                 (out_refs, -1, 4, _APART), (live_given, _P["live"], 4, _WRITTEN),
+                 *((t, -1, 16, 1) for t in tensors)))
     return out_table, out_refs, live_given
 
 
