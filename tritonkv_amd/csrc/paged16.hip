@@ -20,9 +20,9 @@
 // Measured, at steps of the sizes that a serving loop has (bytes of K, V, q and out
 // over the time of both launches): 32 rows of 32768, HKV 8, G 4, fp16, pages of 256:
 // 607 us, 7.1 TB/s; 32 rows of 1000-16384, HKV 8, G 8, bf16, pages of 64, with the
-// append: 175 us, 6.5 TB/s.  Pages of 64 and 16 tokens cost 3% and 7% over 256, rows of
-// different lengths 6% over equal ones (32 rows of 8192: 162 us, 6.6 TB/s).  Small
-// steps are bound by the two launches and the chain of lengths, table, K and V.
+// append: 175 us, 6.5 TB/s.  32 rows of 8192 in pages of 256, 64 and 16: 165, 166 and
+// 172 us.  Small steps are bound by the two launches and the chain of lengths, table, K
+// and V: one row of 505 tokens (12 / 2 heads) takes 6.7 us.
 #include "decode_common.h"
 #include "launch.h"
 
@@ -78,8 +78,8 @@ struct Bf16 {
 // workgroups == 0: one workgroup per row.
 //
 // Measured on 32 rows of 200-16184 tokens (HKV 8, G 4 / 8, D 128): pieces of one row
-// each, cut evenly, 184-194 us; shares 172 / 176.  8 rows of 300-4000 take 21.7 us in
-// tables of 131072 tokens and 21.3 in tables of 4032.
+// each, cut evenly, 184-194 us; shares 172 / 176.  8 rows of 300-4000 take 18.9 us in
+// tables of 131072 tokens and of 4032.
 // ---------------------------------------------------------------------------
 // What finds a workgroup's first segment: scalar arguments of the kernel, which are in
 // registers when a wave starts (a struct is not), so that the lengths are asked for at once.
@@ -241,7 +241,7 @@ __device__ __forceinline__ void store_row4(float* out, float* lse, int D, float 
 // ---------------------------------------------------------------------------
 // HT: tiles of 16 query heads per workgroup, 1 or (G > 16) 2.  A second workgroup for
 // heads 16 to 31 would read all of K and V again: 16 rows of up to 8192, HKV 8, G 24
-// took 82 us with one tile and 60 with two (G 16: 56).
+// took 82 us with one tile and 62 with two (G 16: 56).
 template <class T, int D, int HT, int NW, bool APPEND>
 __global__ void __launch_bounds__(NW * 64, D == 256 ? 1 : D == 128 ? 4 - HT : 5 - HT)
 paged16_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least_chunks, int long_workgroups,

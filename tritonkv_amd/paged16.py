@@ -97,20 +97,21 @@ def plan_shares(B: int, HKV: int, G: int, S: int, D: int = 128, device=None,
 
     * Rows stay whole, in one launch, where that is faster than cutting them
       and joining (a second launch, 2.4 us and more): one CU reads at most
-      38 GB/s, so only short rows, or many.  Up to 256 tokens of 128 dims (250
-      tokens, D 128: B * U = 2 5.8 whole, 7.0 cut; 32 6.6, 8.5; D 256 9.4, 8.9),
-      twice that from 64 row units on (505 tokens: B * U = 2 8.0, 6.9; 32 10.2,
-      8.7; 128 10.6, 12.1), four times from 512 (up to 512 of 1024: 512 units
-      20.6, 24.3).
+      38 GB/s, so only in narrow tables, or with many rows.  Up to 256 tokens of 128 dims
+      (250 tokens, D 128: B * U = 2 5.8 whole, 6.8 cut; 32 6.3, 7.1; D 256 10.7,
+      7.9), twice that from 64 row units on (505 tokens: B * U = 2 10.1, 7.0; 32 10.5,
+      7.6; 128 11.3, 11.0), four times from 512 (up to 512 of 1024: 512 units
+      19.9, 23.7).
     * Otherwise two workgroups per CU (four at head dim 64, whose chunks are half
-      as large: 8 rows of up to 2999, 16 KV heads, w = 1 / 2 / 4 17.1 / 16.3 /
-      15.2), of at least 128 tokens of 128 dims, half of that in tables of
-      at most 512 tokens (one row of 505: 6.9, with 128 7.4; of 4000: 9.0, 8.1).
+      as large: 8 rows of up to 2999, 16 KV heads, w = 1 / 2 / 4 16.9 / 15.7 /
+      15.5), of at least 128 tokens of 128 dims, half of that in tables of
+      at most 512 tokens (one row of 505: 6.7, with 128 7.2; of 4000: 8.8, 8.0).
     * One per CU where the batch has no more rows than that and every workgroup
-      gets a long stream, 16 chunks (32 rows of 8192: 2 per CU 169, 1 157;
-      32 of 1000-16384 185, 179; one of 32768 27.3, 26.2; but 16 of up to 1024,
-      9 chunks each, 13.6, 14.3, and 64 of up to 2048, two rows each, 55.9, 60.5);
-      128 chunks at head dim 64 (32 rows of up to 16384 132, 126; 8 rows 38.5, 39.4).
+      gets a long stream, 16 chunks (2 per CU, 1, in turn: 32 rows of 32768 648, 637; of
+      8192 169, 165; one of 32768 26.8, 25.9; 16 of 8000-16384 at D 256 143, 138;
+      but 16 of up to 1024, 9 chunks each, 14.0, 14.4, and 64 of up to 2048, two rows
+      each, 55.5, 58.4); 128 chunks at head dim 64 (32 rows of 30000-32768 323, 319; of
+      8000-16384 131, 130).
     """
     units = HKV * -(-G // (16 if G <= 16 else 32))
     if B > MAX_ROWS:
