@@ -19,7 +19,7 @@ namespace tkv {
 constexpr int kPlan = 1024;                  // most threads of a plan's workgroup
 constexpr int kSmallPlan = 256;              // ... where its rows and pages fit them
 constexpr int kCopy = 1024;                  // threads of a copy's workgroup
-constexpr int kMaxRows = 8192;               // rows of a fork: two LDS integers each
+constexpr int kMaxRows = 8192;               // rows of a fork: three LDS integers each
 constexpr int kInlinePairs = 4096;           // pairs that the copy checks by itself
 constexpr int kPagesPerThread = 64;          // bits of a thread's mask of pages
 constexpr int kMaxPages = 1 << 30;           // of a pool, and pairs of a call: sums of two fit an integer
@@ -39,10 +39,15 @@ __device__ __forceinline__ void settle() {
 // KiB go at 5.9 TB/s in runs of 64 KiB by 1024 threads, at 5.1 in 16 KiB by 256 threads,
 // at 5.2 in 64 KiB by 256; torch's copy_ of 2 GiB at 4.9.  Where a call copies less
 // than 32 MiB, runs of one slice reach more CUs.  The bytes pass by the caches
-// (non-temporal loads and stores: 4% on the large ones).
+// (non-temporal loads and stores: 4% on the large ones), except where a fork's rows
+// share what they read: from three copies of a page on its loads keep it, in runs of
+// 48 KiB.  126 MB from 16 rows to 15 others each take 38 us, 51 with non-temporal
+// loads; 472 MB 89 and 158; with 7 copies of a page 108 and 139; with 3 the two are alike, with 2 the cached ones
+// are 4% slower.
 // ---------------------------------------------------------------------------
 constexpr int kSlice = kCopy * 16;
 constexpr int kRun = 4;
+constexpr int kSharedRun = 3;
 constexpr int64_t kLongCopy = 32 << 20;
 
 struct CopyPlan {
@@ -53,8 +58,9 @@ struct CopyPlan {
 };
 
 // Pair p of the copies as (source, destination); a negative source is no pair.
-// pair_of(p) may hold barriers: it is called by all threads alike.
-template <int RUN, class PairOf>
+// pair_of(p) may hold barriers: it is called by all threads alike.  CACHED: the loads
+// keep what they read.
+template <int RUN, bool CACHED, class PairOf>
 __device__ __forceinline__ void copy_run(const CopyPlan& c, int64_t items, int group, int groups, PairOf pair_of) {
   for (int64_t base = (int64_t)group * RUN; base < items; base += (int64_t)groups * RUN) {
     int p = items <= UINT32_MAX ? (int)((uint32_t)base / (uint32_t)c.slices) : (int)(base / c.slices);
@@ -79,8 +85,9 @@ __device__ __forceinline__ void copy_run(const CopyPlan& c, int64_t items, int g
         if (t + step < c.set.count && c.first[t + step] <= s) t += step;
       const int64_t at = (int64_t)(s - c.first[t]) * kSlice + threadIdx.x * 16;
       if (at >= c.set.bytes[t]) continue;
-      x[i] = __builtin_nontemporal_load(
-          reinterpret_cast<const u4*>(static_cast<const char*>(c.set.src[t]) + pair.x * c.set.src_stride[t] + at));
+      const u4* from =
+          reinterpret_cast<const u4*>(static_cast<const char*>(c.set.src[t]) + pair.x * c.set.src_stride[t] + at);
+      x[i] = CACHED ? *from : __builtin_nontemporal_load(from);
       to[i] = reinterpret_cast<u4*>(static_cast<char*>(c.set.dst[t]) + pair.y * c.set.dst_stride[t] + at);
     }
 #pragma unroll
@@ -89,12 +96,15 @@ __device__ __forceinline__ void copy_run(const CopyPlan& c, int64_t items, int g
   }
 }
 
-// The first `count` of a plan's pairs.
-__device__ __forceinline__ void copy_pairs(const CopyPlan& c, const int2* pairs, int count, int group, int groups) {
+// The first `count` of a plan's pairs, which read `sources` pages.
+__device__ __forceinline__ void copy_pairs(const CopyPlan& c, const int2* pairs, int count, int sources, int group,
+                                           int groups) {
   const int64_t items = (int64_t)count * c.slices;
   auto pair_of = [&](int p) { return pairs[p]; };
-  if (count * c.bytes >= kLongCopy) copy_run<kRun>(c, items, group, groups, pair_of);
-  else copy_run<1>(c, items, group, groups, pair_of);
+  const bool shared = count >= 3 * sources;
+  if (count * c.bytes < kLongCopy) copy_run<1, false>(c, items, group, groups, pair_of);
+  else if (shared) copy_run<kSharedRun, true>(c, items, group, groups, pair_of);
+  else copy_run<kRun, false>(c, items, group, groups, pair_of);
 }
 
 // tkv_copy_pages_args without its set.
@@ -116,7 +126,7 @@ __device__ __forceinline__ bool is_pair(const PairLists& a, int s, int d) {
 // inline below 32 MiB.  A pair is carried out unless an earlier one has its
 // destination or, within one set of pools, any one reads it.
 __global__ void __launch_bounds__(kCopy) copy_few_kernel(CopyPlan c, PairLists a) {
-  copy_run<1>(c, (int64_t)a.n * c.slices, blockIdx.x, gridDim.x, [&](int p) {
+  copy_run<1, false>(c, (int64_t)a.n * c.slices, blockIdx.x, gridDim.x, [&](int p) {
     const int s = a.src[p], d = a.dst[p];
     bool bad = !is_pair(a, s, d);
     for (int x = threadIdx.x; x < a.n; x += kCopy) {
@@ -128,38 +138,57 @@ __global__ void __launch_bounds__(kCopy) copy_few_kernel(CopyPlan c, PairLists a
 }
 
 // Many pairs: the same rule in three passes of one workgroup over the pages
-// that the pairs name (owner: the first pair of a destination; read: a source).
+// that the pairs name (owner: the first pair of a destination; read: a source).  A
+// thread's first pairs stay in registers.
+constexpr int kKept = 4;
+
 __global__ void __launch_bounds__(kPlan) copy_check_kernel(PairLists a) {
   int* owner = a.work;
   int* read = owner + a.dst_pages;
   const int64_t pages = (int64_t)a.dst_pages + a.src_pages;
   int2* pairs = reinterpret_cast<int2*>(a.work + pages + (pages & 1));
-  for (int i = threadIdx.x; i < a.n; i += kPlan) {
-    const int s = a.src[i], d = a.dst[i];
-    if (is_pair(a, s, d)) {
-      owner[d] = a.n;
-      if (a.same) read[d] = 0;
-    }
+  int2 kept[kKept];
+#pragma unroll
+  for (int k = 0; k < kKept; ++k) {
+    const int i = threadIdx.x + k * kPlan;
+    kept[k] = i < a.n ? make_int2(a.src[i], a.dst[i]) : make_int2(-1, -1);
   }
-  settle();
-  for (int i = threadIdx.x; i < a.n; i += kPlan) {
-    const int s = a.src[i], d = a.dst[i];
-    if (is_pair(a, s, d)) {
-      atomicMin(owner + d, i);
-      if (a.same) atomicExch(read + s, 1);
+  auto each = [&](auto take) {
+#pragma unroll
+    for (int k = 0; k < kKept; ++k) {
+      const int i = threadIdx.x + k * kPlan;
+      if (i < a.n) take(i, kept[k].x, kept[k].y, is_pair(a, kept[k].x, kept[k].y));
     }
-  }
+    for (int i = threadIdx.x + kKept * kPlan; i < a.n; i += kPlan) {
+      const int s = a.src[i], d = a.dst[i];
+      take(i, s, d, is_pair(a, s, d));
+    }
+  };
+  each([&](int, int, int d, bool ok) {
+    if (!ok) return;
+    owner[d] = a.n;
+    if (a.same) read[d] = 0;
+  });
   settle();
-  for (int i = threadIdx.x; i < a.n; i += kPlan) {
-    const int s = a.src[i], d = a.dst[i];
-    bool ok = is_pair(a, s, d);
-    if (ok) ok = atomicAdd(owner + d, 0) == i && !(a.same && atomicAdd(read + d, 0) != 0);
+  each([&](int i, int s, int d, bool ok) {
+    if (!ok) return;
+    atomicMin(owner + d, i);
+    if (a.same) atomicExch(read + s, 1);
+  });
+  settle();
+  each([&](int i, int s, int d, bool ok) {
+    if (ok) {
+      const int first = __hip_atomic_load(owner + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int taken = a.same ? __hip_atomic_load(read + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+      ok = first == i && taken == 0;
+    }
     pairs[i] = make_int2(ok ? s : -1, d);
-  }
+  });
 }
 
-__global__ void __launch_bounds__(kCopy) copy_pairs_kernel(CopyPlan c, const int2* pairs, const int* count, int n) {
-  copy_pairs(c, pairs, count ? *count : n, blockIdx.x, gridDim.x);
+// head: a plan's (below), or null for n pairs of as many pages.
+__global__ void __launch_bounds__(kCopy) copy_pairs_kernel(CopyPlan c, const int2* pairs, const int* head, int n) {
+  copy_pairs(c, pairs, head ? head[1] : n, head ? head[2] : n, blockIdx.x, gridDim.x);
 }
 
 // ---------------------------------------------------------------------------
@@ -242,7 +271,7 @@ struct RowsParams {
 };
 
 struct RowsWork {  // a.work, in int32
-  int* head;       // status, copies, new pages
+  int* head;       // status, copies, pages that they read
   int *old_len, *kept, *first, *pages;
   int2* pairs;
   int *fresh, *staged;
@@ -301,10 +330,11 @@ __global__ void __launch_bounds__(T) rows_plan_kernel(RowsParams a) {
     }
     return;
   }
-  int *most = lds, *best = lds + B;
+  int *most = lds, *best = lds + B, *copied = lds + 2 * B;
   for (int b = tid; b < B; b += T) {
     most[b] = -1;
     best[b] = B;
+    copied[b] = 0;
   }
   if (tid == 0) past = 0;
   // This thread's first row and first pages stay in registers: most plans need no others.
@@ -333,7 +363,10 @@ __global__ void __launch_bounds__(T) rows_plan_kernel(RowsParams a) {
   }
   __syncthreads();
   const bool too_long = past != 0;
-  int2 done = make_int2(0, 0);  // new pages and copies of the rows before this round's
+  // New pages and copies (below 2^16 of them) of the rows before this round's, and in
+  // the copies' upper half the parents that they read from.
+  int2 done = make_int2(0, 0);
+  constexpr int kCopies = 0xffff;
   for (int b0 = 0; b0 < B; b0 += T) {
     const int b = b0 + tid;
     Row r;
@@ -348,13 +381,14 @@ __global__ void __launch_bounds__(T) rows_plan_kernel(RowsParams a) {
       copy = !too_long && r.rest && !heir;
     }
     int2 total;
-    const int2 at = block_scan(scan, need, copy ? 1 : 0, total);
+    const int first_copy = copy && atomicExch(copied + r.a, 1) == 0 ? kCopies + 1 : 0;
+    const int2 at = block_scan(scan, need, copy ? 1 + first_copy : 0, total);
     if (b < B) {
       w.old_len[b] = max(0, min(a.seq_lens[b], table_tokens(a)));
       w.kept[b] = r.f + (heir ? 1 : 0);
       w.first[b] = done.x + at.x;
       w.pages[b] = pages;
-      if (copy) w.pairs[done.y + at.y] = make_int2(r.last, done.x + at.x);
+      if (copy) w.pairs[(done.y + at.y) & kCopies] = make_int2(r.last, done.x + at.x);
     }
     done.x += total.x;
     done.y += total.y;
@@ -371,7 +405,7 @@ __global__ void __launch_bounds__(T) rows_plan_kernel(RowsParams a) {
   }
   const int status = too_long ? TKV_ROWS_PAST_TABLE : found < done.x ? TKV_ROWS_NO_PAGES : TKV_ROWS_DONE;
   settle();
-  const int copies = status ? 0 : done.y;
+  const int copies = status ? 0 : done.y & kCopies;
   for (int i = tid; i < copies; i += T) {
     int2 p = w.pairs[i];
     p.y = w.fresh[p.y];
@@ -381,6 +415,7 @@ __global__ void __launch_bounds__(T) rows_plan_kernel(RowsParams a) {
   if (tid == 0) {
     w.head[0] = status;
     w.head[1] = copies;
+    w.head[2] = done.y >> 16;
     *a.status = status;
   }
 }
@@ -390,7 +425,7 @@ __global__ void __launch_bounds__(kCopy) rows_apply_kernel(RowsParams a, CopyPla
   const RowsWork w = rows_work(a);
   if (w.head[0] != TKV_ROWS_DONE) return;
   if ((int)blockIdx.x >= tables) {
-    copy_pairs(c, w.pairs, w.head[1], blockIdx.x - tables, gridDim.x - tables);
+    copy_pairs(c, w.pairs, w.head[1], w.head[2], blockIdx.x - tables, gridDim.x - tables);
     return;
   }
   const int P = a.max_pages, N = a.num_pages;
@@ -441,24 +476,24 @@ struct PageBlock {
 };
 
 struct CompactWork {
-  int* head;          // live pages, moves
+  int* head;          // live pages, moves, pages that they read
   int2* pairs;        // at most N / 2 moves
-  int* count;         // references of the i-th page that moves
+  int* refs;          // the counts before the call
   PageBlock* blocks;  // of per >= 4 pages each
 };
 
+__host__ __device__ inline int64_t compact_refs_at(int64_t N) { return 16 + (N + 4) / 4 * 4; }
+__host__ __device__ inline int64_t compact_blocks_at(int64_t N) { return compact_refs_at(N) + (N + 4) / 4 * 4; }
 __host__ __device__ inline int64_t compact_work_ints(int64_t N) {
-  const int64_t pairs = 16 + (N + 2) / 2 * 2, counts = (N / 2 + 4) / 4 * 4;
-  return (pairs + counts + 3) / 4 * 4 + 4 * (N / 4 + kPlan);
+  return compact_blocks_at(N) + 4 * (N / 4 + kPlan);
 }
 
 __device__ __forceinline__ CompactWork compact_work(const CompactParams& a) {
   CompactWork w;
-  const int64_t N = a.num_pages, pairs = 16 + (N + 2) / 2 * 2, counts = (N / 2 + 4) / 4 * 4;
   w.head = a.work;
   w.pairs = reinterpret_cast<int2*>(a.work + 16);
-  w.count = a.work + pairs;
-  w.blocks = reinterpret_cast<PageBlock*>(a.work + (pairs + counts + 3) / 4 * 4);
+  w.refs = a.work + compact_refs_at(a.num_pages);
+  w.blocks = reinterpret_cast<PageBlock*>(a.work + compact_blocks_at(a.num_pages));
   return w;
 }
 
@@ -467,6 +502,11 @@ __global__ void __launch_bounds__(T) compact_plan_kernel(CompactParams a) {
   __shared__ ScanLds<T> scan;
   const CompactWork w = compact_work(a);
   const int tid = threadIdx.x, N = a.num_pages, per = a.per;
+  if (blockIdx.x > 0) {
+    // The second launch reads the counts while it writes them.
+    for (int64_t i = (int64_t)(blockIdx.x - 1) * T + tid; i < N; i += (int64_t)(gridDim.x - 1) * T) w.refs[i] = a.refs[i];
+    return;
+  }
   const int64_t round = (int64_t)per * T;
   int live = 0;
   uint64_t m = 0;
@@ -486,18 +526,14 @@ __global__ void __launch_bounds__(T) compact_plan_kernel(CompactParams a) {
     const int2 at = block_scan(scan, __popcll(from), __popcll(to), total);
     int s = done.x + at.x, d = done.y + at.y;
     if (mine < N) w.blocks[p0 / per + tid] = PageBlock{m, s, d};
-    for (; from; from &= from - 1, ++s) {
-      const int page = (int)mine + __builtin_ctzll(from);
-      w.pairs[s].x = page;
-      w.count[s] = a.refs[page];
-    }
+    for (; from; from &= from - 1, ++s) w.pairs[s].x = (int)mine + __builtin_ctzll(from);
     for (; to; to &= to - 1, ++d) w.pairs[d].y = (int)mine + __builtin_ctzll(to);
     done.x += total.x;
     done.y += total.y;
   }
   if (tid == 0) {
     w.head[0] = live;
-    w.head[1] = done.x;
+    w.head[1] = w.head[2] = done.x;
     if (a.live) *a.live = live;
   }
 }
@@ -518,7 +554,7 @@ __global__ void __launch_bounds__(kCopy) compact_apply_kernel(CompactParams a, C
   const CompactWork w = compact_work(a);
   const int live = w.head[0];
   if ((int)blockIdx.x >= tables) {
-    copy_pairs(c, w.pairs, w.head[1], blockIdx.x - tables, gridDim.x - tables);
+    copy_pairs(c, w.pairs, w.head[1], w.head[2], blockIdx.x - tables, gridDim.x - tables);
     return;
   }
   const int P = a.max_pages, N = a.num_pages, per = a.per;
@@ -533,7 +569,7 @@ __global__ void __launch_bounds__(kCopy) compact_apply_kernel(CompactParams a, C
     } else {
       const int p = (int)(i - entries);
       const int move = p < live ? move_of(w, p, per, live) : -1;
-      a.out_refs[p] = p >= live ? 0 : move >= 0 ? w.count[move] : a.refs[p];
+      a.out_refs[p] = p >= live ? 0 : w.refs[move >= 0 ? w.pairs[move].x : p];
     }
   }
 }
@@ -634,7 +670,7 @@ extern "C" int tkv_fork_rows(const tkv_fork_rows_args* a, tkv_stream_t stream) {
   const RowsParams p{a->block_table, a->seq_lens, a->refs, a->parents, a->new_lens, a->status, a->work,
                      a->table_stride, a->B, a->max_pages, a->page_size, a->num_pages};
   const int bad = launch(small ? rows_plan_kernel<kSmallPlan> : rows_plan_kernel<kPlan>,
-                         dim3(1 + (staging < 512 ? staging : 512)), dim3(threads), 2 * sizeof(int) * a->B, st, p);
+                         dim3(1 + (staging < 512 ? staging : 512)), dim3(threads), 3 * sizeof(int) * a->B, st, p);
   if (bad) return bad;
   const int64_t tables = (entries + kCopy - 1) / kCopy;
   const int t = (int)(tables < 512 ? tables : 512);
@@ -662,8 +698,9 @@ extern "C" int tkv_compact_pages(const tkv_compact_pages_args* a, tkv_stream_t s
   const CompactParams p{a->block_table, a->refs, a->out_table, a->out_refs, a->live, a->work,
                         a->table_stride, a->out_stride, a->B, a->max_pages, a->num_pages,
                         pages_per_thread(a->num_pages, threads)};
-  const int bad = launch(small ? compact_plan_kernel<kSmallPlan> : compact_plan_kernel<kPlan>, dim3(1), dim3(threads),
-                         0, st, p);
+  const int staging = (a->num_pages + 4 * threads - 1) / (4 * threads);
+  const int bad = launch(small ? compact_plan_kernel<kSmallPlan> : compact_plan_kernel<kPlan>,
+                         dim3(1 + (staging < 512 ? staging : 512)), dim3(threads), 0, st, p);
   if (bad) return bad;
   const int64_t tables = ((int64_t)a->B * a->max_pages + a->num_pages + kCopy - 1) / kCopy;
   const int t = (int)(tables < 512 ? tables : 512);
@@ -680,5 +717,5 @@ extern "C" int tkv_copy_planned(const tkv_page_set* set, const int32_t* work, in
   const unsigned groups = copy_groups(most, c);
   if (!groups) return TKV_OK;
   return launch(copy_pairs_kernel, dim3(groups), dim3(kCopy), 0, reinterpret_cast<hipStream_t>(stream), c,
-                reinterpret_cast<const int2*>(work + 16), (const int*)(work + 1), 0);
+                reinterpret_cast<const int2*>(work + 16), (const int*)work, 0);
 }
