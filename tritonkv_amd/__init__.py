@@ -11,6 +11,11 @@ surface:
   pack/scale/zero layout (reference ``quantize.py``), plus ``append_kv``;
 * ``tritonkv_amd.paged``: the same cache format in page pools addressed
   through a block table (``paged_append``, ``paged_decode_attention``);
+* ``tritonkv_amd.paged16``: unquantized fp16 and bf16 page pools
+  (``paged16_append``, ``paged16_decode_attention``);
+* ``tritonkv_amd.pages``: the pages of either kind, copied, forked, handed out,
+  taken back and compacted on the device (``copy_pages``, ``fork_rows``,
+  ``resize_rows``, ``compact_pages``);
 * ``tritonkv_amd.channel``: per-channel (KIVI-style) keys with an fp16
   residual window, the key format the reference plans
   (``ChannelKVCache``, ``channel_decode_attention``);

@@ -19,7 +19,8 @@ the buffer base changes at page boundaries.  ``page_size`` must be a multiple
 of 32 (the kernel's token chunk), so a chunk never straddles two pages.
 
 Codes, metadata and results are bit-identical to the contiguous cache holding
-the same logical tokens.  The fp16 control has no paged form.
+the same logical tokens.  The fp16 control has no paged form; unquantized pages are
+:mod:`tritonkv_amd.paged16`'s.
 """
 
 from __future__ import annotations
