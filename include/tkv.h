@@ -342,13 +342,12 @@ int tkv_dequantize(const uint8_t *packed, const uint16_t *scale, const uint16_t 
  * The rows are cut on the device, from their lengths: their chunks of 32 tokens
  * (an empty row counts as one), laid end to end, are shared out evenly over at
  * most `workgroups` workgroups (1 to 65535) per KV head and 16 query heads (32 where
- * a KV head has more than 16), of at
- * least least_chunks chunks each -- or over long_workgroups (at most workgroups;
- * 0: never) where the batch has no more rows and each gets at least long_chunks --
- * and a second launch joins the rows that were
- * cut: partials holds 2 * workgroups * HQ * (D + 2) floats (16-byte aligned),
- * row_pieces 2 * B int32 (8-byte aligned).  workgroups == 0 keeps every row
- * whole, in one launch (at most 65535 rows).  No counterpart in the reference (its caches are contiguous). */
+ * a KV head has more than 16), of at least least_chunks chunks each -- or over
+ * long_workgroups (at most workgroups; 0: never) where the batch has no more rows and
+ * each gets at least long_chunks -- and a second launch joins the rows that were cut:
+ * partials holds 2 * workgroups * HQ * (D + 2) floats (16-byte aligned), row_pieces
+ * 2 * B int32 (8-byte aligned).  workgroups == 0 keeps every row whole, in one launch
+ * (at most 65535 rows).  No counterpart in the reference (its caches are contiguous). */
 typedef struct tkv_paged16_args {
   const void *q;
   int64_t q_strides[2];
@@ -401,8 +400,9 @@ typedef struct tkv_page_set {
  * with one destination the first is carried out.  Within one set of pools (same)
  * a page that the call reads is never written: a pair whose destination is a
  * pair's source is skipped, and (p, p) is no pair.  work: tkv_copy_pages_work(args)
- * int32, 8-byte aligned (0: none, NULL will do; below 0: wrong arguments).  No counterpart in the reference, nor have the next two
- * (its caches have no pages). */
+ * int32, 8-byte aligned (0: none, NULL will do; below 0: wrong arguments).  At most 2^30
+ * pages and pairs.  No counterpart in the reference, nor have the next two (its caches have
+ * no pages). */
 typedef struct tkv_copy_pages_args {
   tkv_page_set set;
   const int32_t *src, *dst;
@@ -424,7 +424,7 @@ int tkv_copy_pages(const tkv_copy_pages_args *args, tkv_stream_t stream);
  * the row's pages are -1, and refs follow.  *status is TKV_ROWS_DONE, or says why
  * nothing was changed.  set: the pools (src == dst), whose copies go with the
  * table; work: tkv_fork_rows_work() int32, 8-byte aligned.  Two launches; at most
- * 8192 rows. */
+ * 8192 rows and 2^30 pages. */
 enum { TKV_ROWS_DONE = 0, TKV_ROWS_NO_PAGES = 1, TKV_ROWS_PAST_TABLE = 2 };
 typedef struct tkv_fork_rows_args {
   tkv_page_set set;
@@ -441,7 +441,7 @@ int tkv_fork_rows(const tkv_fork_rows_args *args, tkv_stream_t stream);
  * out_table is block_table with the moved pages' new numbers, out_refs refs with
  * their counts at the new places, and *live (NULL: not wanted) n.  out_table and
  * out_refs may be block_table and refs.  The old places keep their bytes.  work:
- * tkv_compact_pages_work() int32, 16-byte aligned.  Two launches. */
+ * tkv_compact_pages_work() int32, 16-byte aligned.  Two launches; at most 2^30 pages. */
 typedef struct tkv_compact_pages_args {
   tkv_page_set set;
   const int32_t *block_table, *refs;

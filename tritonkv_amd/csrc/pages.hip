@@ -363,8 +363,8 @@ __global__ void __launch_bounds__(T) rows_plan_kernel(RowsParams a) {
   }
   __syncthreads();
   const bool too_long = past != 0;
-  // New pages and copies (below 2^16 of them) of the rows before this round's, and in
-  // the copies' upper half the parents that they read from.
+  // New pages and copies (below 2^16 of them) of the rows taken so far, and in the
+  // copies' upper half the parents that they read from.
   int2 done = make_int2(0, 0);
   constexpr int kCopies = 0xffff;
   for (int b0 = 0; b0 < B; b0 += T) {
