@@ -50,18 +50,27 @@ constexpr int kRun = 4;
 constexpr int kSharedRun = 3;
 constexpr int64_t kLongCopy = 32 << 20;
 
+// M: the most tensors.  Where a set has no more than kFewTensors the kernels take a
+// smaller plan: 1.2 KB less of arguments save 0.3 us of every launch (8 pages of 512 KiB
+// 3.6 -> 3.3 us captured, 5.2 -> 4.9 eager; a compaction of 1024 pages 8.8 -> 8.3 eager).
+constexpr int kFewTensors = 4;
+
+template <int M>
 struct CopyPlan {
-  tkv_page_set set;
-  int32_t first[TKV_PAGE_TENSORS];  // slices of a page before tensor t
-  int32_t slices;                   // of a page, in all tensors
-  int64_t bytes;                    // of a page, in all tensors
+  static constexpr int kMost = M;
+  const void* src[M];
+  void* dst[M];
+  int64_t src_stride[M], dst_stride[M], size[M];
+  int32_t first[M];       // slices of a page before tensor t
+  int32_t count, slices;  // tensors; slices of a page, in all of them
+  int64_t bytes;          // of a page, in all tensors
 };
 
 // Pair p of the copies as (source, destination); a negative source is no pair.
 // pair_of(p) may hold barriers: it is called by all threads alike.  CACHED: the loads
 // keep what they read.
-template <int RUN, bool CACHED, class PairOf>
-__device__ __forceinline__ void copy_run(const CopyPlan& c, int64_t items, int group, int groups, PairOf pair_of) {
+template <int RUN, bool CACHED, int M, class PairOf>
+__device__ __forceinline__ void copy_run(const CopyPlan<M>& c, int64_t items, int group, int groups, PairOf pair_of) {
   for (int64_t base = (int64_t)group * RUN; base < items; base += (int64_t)groups * RUN) {
     int p = items <= UINT32_MAX ? (int)((uint32_t)base / (uint32_t)c.slices) : (int)(base / c.slices);
     int s = (int)(base - (int64_t)p * c.slices);
@@ -81,14 +90,14 @@ __device__ __forceinline__ void copy_run(const CopyPlan& c, int64_t items, int g
       if (pair.x < 0) continue;
       int t = 0;
 #pragma unroll
-      for (int step = TKV_PAGE_TENSORS / 2; step; step /= 2)
-        if (t + step < c.set.count && c.first[t + step] <= s) t += step;
+      for (int step = M / 2; step; step /= 2)
+        if (t + step < c.count && c.first[t + step] <= s) t += step;
       const int64_t at = (int64_t)(s - c.first[t]) * kSlice + threadIdx.x * 16;
-      if (at >= c.set.bytes[t]) continue;
+      if (at >= c.size[t]) continue;
       const u4* from =
-          reinterpret_cast<const u4*>(static_cast<const char*>(c.set.src[t]) + pair.x * c.set.src_stride[t] + at);
+          reinterpret_cast<const u4*>(static_cast<const char*>(c.src[t]) + pair.x * c.src_stride[t] + at);
       x[i] = CACHED ? *from : __builtin_nontemporal_load(from);
-      to[i] = reinterpret_cast<u4*>(static_cast<char*>(c.set.dst[t]) + pair.y * c.set.dst_stride[t] + at);
+      to[i] = reinterpret_cast<u4*>(static_cast<char*>(c.dst[t]) + pair.y * c.dst_stride[t] + at);
     }
 #pragma unroll
     for (int i = 0; i < RUN; ++i)
@@ -97,7 +106,8 @@ __device__ __forceinline__ void copy_run(const CopyPlan& c, int64_t items, int g
 }
 
 // The first `count` of a plan's pairs, which read `sources` pages.
-__device__ __forceinline__ void copy_pairs(const CopyPlan& c, const int2* pairs, int count, int sources, int group,
+template <int M>
+__device__ __forceinline__ void copy_pairs(const CopyPlan<M>& c, const int2* pairs, int count, int sources, int group,
                                            int groups) {
   const int64_t items = (int64_t)count * c.slices;
   auto pair_of = [&](int p) { return pairs[p]; };
@@ -125,7 +135,8 @@ __device__ __forceinline__ bool is_pair(const PairLists& a, int s, int d) {
 // 64 / 65; of 512 KiB: 8 4.4 / 6.6, 64 17.2 / 17.1, 256 60 / 56, 1024 213 / 196.  So
 // inline below 32 MiB.  A pair is carried out unless an earlier one has its
 // destination or, within one set of pools, any one reads it.
-__global__ void __launch_bounds__(kCopy) copy_few_kernel(CopyPlan c, PairLists a) {
+template <int M>
+__global__ void __launch_bounds__(kCopy) copy_few_kernel(CopyPlan<M> c, PairLists a) {
   copy_run<1, false>(c, (int64_t)a.n * c.slices, blockIdx.x, gridDim.x, [&](int p) {
     const int s = a.src[p], d = a.dst[p];
     bool bad = !is_pair(a, s, d);
@@ -187,7 +198,8 @@ __global__ void __launch_bounds__(kPlan) copy_check_kernel(PairLists a) {
 }
 
 // head: a plan's (below), or null for n pairs of as many pages.
-__global__ void __launch_bounds__(kCopy) copy_pairs_kernel(CopyPlan c, const int2* pairs, const int* head, int n) {
+template <int M>
+__global__ void __launch_bounds__(kCopy) copy_pairs_kernel(CopyPlan<M> c, const int2* pairs, const int* head, int n) {
   copy_pairs(c, pairs, head ? head[1] : n, head ? head[2] : n, blockIdx.x, gridDim.x);
 }
 
@@ -421,7 +433,8 @@ __global__ void __launch_bounds__(T) rows_plan_kernel(RowsParams a) {
 }
 
 // Workgroups [0, tables): the table, lengths and counts; the others: the copies.
-__global__ void __launch_bounds__(kCopy) rows_apply_kernel(RowsParams a, CopyPlan c, int tables) {
+template <int M>
+__global__ void __launch_bounds__(kCopy) rows_apply_kernel(RowsParams a, CopyPlan<M> c, int tables) {
   const RowsWork w = rows_work(a);
   if (w.head[0] != TKV_ROWS_DONE) return;
   if ((int)blockIdx.x >= tables) {
@@ -550,7 +563,8 @@ __device__ __forceinline__ int move_of(const CompactWork& w, int page, int per, 
 }
 
 // Workgroups [0, tables): the table and the counts; the others: the copies.
-__global__ void __launch_bounds__(kCopy) compact_apply_kernel(CompactParams a, CopyPlan c, int tables) {
+template <int M>
+__global__ void __launch_bounds__(kCopy) compact_apply_kernel(CompactParams a, CopyPlan<M> c, int tables) {
   const CompactWork w = compact_work(a);
   const int live = w.head[0];
   if ((int)blockIdx.x >= tables) {
@@ -577,9 +591,11 @@ __global__ void __launch_bounds__(kCopy) compact_apply_kernel(CompactParams a, C
 // ---------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------
-static int make_plan(const tkv_page_set& s, CopyPlan& c) {
+using FullPlan = CopyPlan<TKV_PAGE_TENSORS>;
+
+static int make_plan(const tkv_page_set& s, FullPlan& c) {
   if (s.count < 0 || s.count > TKV_PAGE_TENSORS) return TKV_EINVAL;
-  c.set = s;
+  c.count = s.count;
   c.bytes = 0;
   int64_t slices = 0;
   for (int t = 0; t < s.count; ++t) {
@@ -588,32 +604,55 @@ static int make_plan(const tkv_page_set& s, CopyPlan& c) {
          (uint64_t)s.dst_stride[t]) & 15)
       return TKV_EINVAL;
     if (s.src_stride[t] < s.bytes[t] || s.dst_stride[t] < s.bytes[t]) return TKV_EINVAL;
+    c.src[t] = s.src[t];
+    c.dst[t] = s.dst[t];
+    c.src_stride[t] = s.src_stride[t];
+    c.dst_stride[t] = s.dst_stride[t];
+    c.size[t] = s.bytes[t];
     c.first[t] = (int32_t)slices;
     slices += (s.bytes[t] + kSlice - 1) / kSlice;
     if (slices > INT32_MAX) return TKV_EUNSUPPORTED;
     c.bytes += s.bytes[t];
   }
-  for (int t = s.count; t < TKV_PAGE_TENSORS; ++t) c.first[t] = INT32_MAX;
   c.slices = (int32_t)slices;
   return TKV_OK;
+}
+
+// start(plan) with the plan that the kernels take.
+template <class Start>
+static int with_plan(const FullPlan& c, Start start) {
+  if (c.count > kFewTensors) return start(c);
+  CopyPlan<kFewTensors> few;
+  for (int t = 0; t < c.count; ++t) {
+    few.src[t] = c.src[t];
+    few.dst[t] = c.dst[t];
+    few.src_stride[t] = c.src_stride[t];
+    few.dst_stride[t] = c.dst_stride[t];
+    few.size[t] = c.size[t];
+    few.first[t] = c.first[t];
+  }
+  few.count = c.count;
+  few.slices = c.slices;
+  few.bytes = c.bytes;
+  return start(few);
 }
 
 constexpr int kCopyGroups = 8192;  // workgroups that stride over the copies
 
 // Workgroups for at most `pairs` copies.
-static unsigned copy_groups(int64_t pairs, const CopyPlan& c) {
+static unsigned copy_groups(int64_t pairs, const FullPlan& c) {
   const int64_t items = pairs * c.slices;
   return (unsigned)(items < kCopyGroups ? items : kCopyGroups);
 }
 
-static int check_copy(const tkv_copy_pages_args* a, CopyPlan& c) {
+static int check_copy(const tkv_copy_pages_args* a, FullPlan& c) {
   if (!a || !a->src || !a->dst || a->n <= 0 || a->src_pages <= 0 || a->dst_pages <= 0) return TKV_EINVAL;
   if (a->n > kMaxPages || a->src_pages > kMaxPages || a->dst_pages > kMaxPages) return TKV_EUNSUPPORTED;
   if (a->same && a->src_pages != a->dst_pages) return TKV_EINVAL;
   return make_plan(a->set, c);
 }
 
-static bool checked_inline(const tkv_copy_pages_args* a, const CopyPlan& c) {
+static bool checked_inline(const tkv_copy_pages_args* a, const FullPlan& c) {
   return a->n <= kInlinePairs && a->n * c.bytes < kLongCopy;
 }
 
@@ -621,7 +660,7 @@ static bool checked_inline(const tkv_copy_pages_args* a, const CopyPlan& c) {
 
 extern "C" int64_t tkv_copy_pages_work(const tkv_copy_pages_args* a) {
   using namespace tkv;
-  CopyPlan c;
+  FullPlan c;
   const int rc = check_copy(a, c);
   if (rc) return rc;
   return checked_inline(a, c) ? 0 : (int64_t)a->src_pages + a->dst_pages + 1 + 2 * (int64_t)a->n;
@@ -629,7 +668,7 @@ extern "C" int64_t tkv_copy_pages_work(const tkv_copy_pages_args* a) {
 
 extern "C" int tkv_copy_pages(const tkv_copy_pages_args* a, tkv_stream_t stream) {
   using namespace tkv;
-  CopyPlan c;
+  FullPlan c;
   const int rc = check_copy(a, c);
   if (rc) return rc;
   const bool in_line = checked_inline(a, c);
@@ -638,11 +677,15 @@ extern "C" int tkv_copy_pages(const tkv_copy_pages_args* a, tkv_stream_t stream)
   const PairLists p{a->src, a->dst, a->work, a->n, a->src_pages, a->dst_pages, a->same};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(copy_groups(a->n, c)), block(kCopy);
-  if (in_line) return launch(copy_few_kernel, grid, block, 0, st, c, p);
+  if (in_line)
+    return with_plan(c, [&](auto plan) { return launch(copy_few_kernel<plan.kMost>, grid, block, 0, st, plan, p); });
   const int64_t pages = (int64_t)a->dst_pages + a->src_pages;
   const int2* pairs = reinterpret_cast<const int2*>(a->work + pages + (pages & 1));
   const int bad = launch(copy_check_kernel, dim3(1), dim3(kPlan), 0, st, p);
-  return bad ? bad : launch(copy_pairs_kernel, grid, block, 0, st, c, pairs, (const int*)nullptr, (int)a->n);
+  if (bad) return bad;
+  return with_plan(c, [&](auto plan) {
+    return launch(copy_pairs_kernel<plan.kMost>, grid, block, 0, st, plan, pairs, (const int*)nullptr, (int)a->n);
+  });
 }
 
 extern "C" int64_t tkv_fork_rows_work(int32_t B, int32_t max_pages, int32_t num_pages, int32_t parents) {
@@ -658,7 +701,7 @@ extern "C" int tkv_fork_rows(const tkv_fork_rows_args* a, tkv_stream_t stream) {
     return TKV_EINVAL;
   if (a->B > kMaxRows || a->num_pages > kMaxPages) return TKV_EUNSUPPORTED;
   if ((int64_t)a->max_pages * a->page_size > INT32_MAX || (int64_t)a->B * a->max_pages > INT32_MAX) return TKV_EINVAL;
-  CopyPlan c;
+  FullPlan c;
   const int rc = make_plan(a->set, c);
   if (rc) return rc;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -674,7 +717,9 @@ extern "C" int tkv_fork_rows(const tkv_fork_rows_args* a, tkv_stream_t stream) {
   if (bad) return bad;
   const int64_t tables = (entries + kCopy - 1) / kCopy;
   const int t = (int)(tables < 512 ? tables : 512);
-  return launch(rows_apply_kernel, dim3(t + copy_groups(a->B, c)), dim3(kCopy), 0, st, p, c, t);
+  return with_plan(c, [&](auto plan) {
+    return launch(rows_apply_kernel<plan.kMost>, dim3(t + copy_groups(a->B, c)), dim3(kCopy), 0, st, p, plan, t);
+  });
 }
 
 extern "C" int64_t tkv_compact_pages_work(int32_t num_pages) {
@@ -689,7 +734,7 @@ extern "C" int tkv_compact_pages(const tkv_compact_pages_args* a, tkv_stream_t s
       a->out_stride < a->max_pages)
     return TKV_EINVAL;
   if (a->num_pages > kMaxPages) return TKV_EUNSUPPORTED;
-  CopyPlan c;
+  FullPlan c;
   const int rc = make_plan(a->set, c);
   if (rc) return rc;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -704,18 +749,23 @@ extern "C" int tkv_compact_pages(const tkv_compact_pages_args* a, tkv_stream_t s
   if (bad) return bad;
   const int64_t tables = ((int64_t)a->B * a->max_pages + a->num_pages + kCopy - 1) / kCopy;
   const int t = (int)(tables < 512 ? tables : 512);
-  return launch(compact_apply_kernel, dim3(t + copy_groups(a->num_pages / 2, c)), dim3(kCopy), 0, st, p, c, t);
+  return with_plan(c, [&](auto plan) {
+    return launch(compact_apply_kernel<plan.kMost>, dim3(t + copy_groups(a->num_pages / 2, c)), dim3(kCopy), 0, st, p,
+                  plan, t);
+  });
 }
 
 // The copies of a plan in further tensors: pairs and their count as the plan left them.
 extern "C" int tkv_copy_planned(const tkv_page_set* set, const int32_t* work, int32_t most, tkv_stream_t stream) {
   using namespace tkv;
   if (!set || !work || (uintptr_t)work & 7 || most < 0) return TKV_EINVAL;
-  CopyPlan c;
+  FullPlan c;
   const int rc = make_plan(*set, c);
   if (rc) return rc;
   const unsigned groups = copy_groups(most, c);
   if (!groups) return TKV_OK;
-  return launch(copy_pairs_kernel, dim3(groups), dim3(kCopy), 0, reinterpret_cast<hipStream_t>(stream), c,
-                reinterpret_cast<const int2*>(work + 16), (const int*)work, 0);
+  return with_plan(c, [&](auto plan) {
+    return launch(copy_pairs_kernel<plan.kMost>, dim3(groups), dim3(kCopy), 0, reinterpret_cast<hipStream_t>(stream),
+                  plan, reinterpret_cast<const int2*>(work + 16), (const int*)work, 0);
+  });
 }
