@@ -353,6 +353,65 @@ def test_more_tensors_than_a_launch_takes():
         assert torch.equal(p, w)
 
 
+@pytest.mark.parametrize("each", [1, 2, 3, 39])
+@pytest.mark.parametrize("extra", [0, 1, 33])
+def test_long_forks_and_compactions(each, extra):
+    """Over 32 MiB of copies, of 1 to 39 copies of a page, in pages of no whole slices, in as
+    many tensors as the smaller argument block takes, one more, and more than a launch takes."""
+    from tritonkv_amd.pages import compact_pages, fork_rows
+
+    groups, page = 40 // each, 48
+    B = groups * (each + 1)
+    N = 2 * B + 7
+    m = Model(B, 2, N, page)
+    pools = [_pool(N, HKV=1, page=page, D=8, seed=x) for x in range(extra + 1)] + \
+        [_pool(N, HKV=12, page=page, D=264, seed=50 + x) for x in range(3)]
+    assert groups * each * sum(p[0].numel() * 2 for p in pools) > 32 << 20
+    want = [p.clone() for p in pools]
+    # the parents among the others; their pages at the upper end
+    parents = [b - b % (each + 1) + each // 2 for b in range(B)]
+    for g, b in enumerate(sorted(set(parents))):
+        m.lens[b], m.table[b][0], m.refs[N - 1 - g] = 20, N - 1 - g, 1
+    table, lens, refs = _state(m)
+    status, copies = m.fork(parents)
+    assert status == 0 and len(copies) == groups * each
+    assert fork_rows(pools, table, lens, refs, _i32(parents)).tolist() == [0]
+    assert m.same_as(table, lens, refs)
+    kept = [b if b % 2 else -1 for b in range(B)]
+    assert m.fork(kept) == (0, [])
+    assert fork_rows(pools, table, lens, refs, _i32(kept)).tolist() == [0]
+    moves = _compacted(m)
+    compact_pages(pools, table, refs)
+    assert m.same_as(table, lens, refs)
+    for w, p in zip(want, pools):
+        for pairs in filter(None, (copies, moves)):
+            s, d = (torch.tensor(x, device=DEV) for x in zip(*pairs))
+            w[d] = w[s]
+        assert torch.equal(_bits(p), _bits(w))
+
+
+def test_a_long_compaction():
+    from tritonkv_amd.pages import compact_pages
+
+    N = 150
+    pools = [_pool(N, HKV=3, page=48, D=264, seed=x) for x in range(10)]
+    want = [p.clone() for p in pools]
+    live = list(range(40)) + list(range(90, 150))
+    m = Model(4, 25, N, 48)
+    for i, p in enumerate(live):
+        m.table[i // 25][i % 25], m.refs[p] = p, 1
+    m.lens = [25 * 48] * 4
+    table, lens, refs = _state(m)
+    moves = _compacted(m)
+    assert len(moves) == 50 and len(moves) * sum(p[0].numel() * 2 for p in pools) > 32 << 20
+    compact_pages(pools, table, refs)
+    assert m.same_as(table, lens, refs)
+    s, d = (torch.tensor(x, device=DEV) for x in zip(*moves))
+    for w, p in zip(want, pools):
+        w[d] = w[s]
+        assert torch.equal(_bits(p), _bits(w))
+
+
 def test_broken_tables_stay_inside():
     """Entries and lengths that no call leaves are not followed out of the pools."""
     from tritonkv_amd.pages import compact_pages, fork_rows
