@@ -424,7 +424,13 @@ int tkv_copy_pages(const tkv_copy_pages_args *args, tkv_stream_t stream);
  * the row's pages are -1, and refs follow.  *status is TKV_ROWS_DONE, or says why
  * nothing was changed.  set: the pools (src == dst), whose copies go with the
  * table; work: tkv_fork_rows_work() int32, 8-byte aligned.  Two launches; at most
- * 8192 rows and 2^30 pages. */
+ * 8192 rows and 2^30 pages.
+ * All seq_lens tokens of an old row count as written: where rows hold room made ahead
+ * (n_b above L_a, say) tkv_fork_rows would share its pages, and two rows would write
+ * their next tokens into one place.  tkv_fork_rows_written takes the tokens that every
+ * old row holds (written, B entries; NULL: seq_lens): full pages of these alone are
+ * shared, and pages of room stay with the row that keeps the partial page, as far as
+ * they are nobody else's; every other row gets new ones. */
 enum { TKV_ROWS_DONE = 0, TKV_ROWS_NO_PAGES = 1, TKV_ROWS_PAST_TABLE = 2 };
 typedef struct tkv_fork_rows_args {
   tkv_page_set set;
@@ -435,6 +441,11 @@ typedef struct tkv_fork_rows_args {
 } tkv_fork_rows_args;
 int64_t tkv_fork_rows_work(int32_t B, int32_t max_pages, int32_t num_pages, int32_t parents);
 int tkv_fork_rows(const tkv_fork_rows_args *args, tkv_stream_t stream);
+typedef struct tkv_fork_written_args {
+  tkv_fork_rows_args rows;
+  const int32_t *written;
+} tkv_fork_written_args;
+int tkv_fork_rows_written(const tkv_fork_written_args *args, tkv_stream_t stream);
 
 /* Live pages (refs > 0) to the low end: with n of them, the i-th live page at or
  * past n is copied to the i-th free page below n in every tensor of the set;
@@ -451,7 +462,7 @@ typedef struct tkv_compact_pages_args {
 int64_t tkv_compact_pages_work(int32_t num_pages);
 int tkv_compact_pages(const tkv_compact_pages_args *args, tkv_stream_t stream);
 
-/* The copies of the tkv_fork_rows or tkv_compact_pages call that last used `work`,
+/* The copies of the tkv_fork_rows (or _written) or tkv_compact_pages call that last used `work`,
  * in the tensors of another set (a set holds 32).  most: the most pairs there can
  * be, the call's B or num_pages / 2. */
 int tkv_copy_planned(const tkv_page_set *set, const int32_t *work, int32_t most, tkv_stream_t stream);

@@ -188,6 +188,12 @@ class ForkRowsArgs(ctypes.Structure):
     ]
 
 
+class ForkWrittenArgs(ForkRowsArgs):
+    """Mirror of ``tkv_fork_written_args``: a ``tkv_fork_rows_args`` and one more field."""
+
+    _fields_ = [("written", ctypes.c_void_p)]
+
+
 class CompactPagesArgs(ctypes.Structure):
     """Mirror of ``tkv_compact_pages_args``."""
 
@@ -255,6 +261,7 @@ SIGNATURES = {
     "tkv_copy_pages": ([ctypes.POINTER(CopyPagesArgs), _P], ctypes.c_int),
     "tkv_fork_rows_work": ([_I32, _I32, _I32, _I32], _I64),
     "tkv_fork_rows": ([ctypes.POINTER(ForkRowsArgs), _P], ctypes.c_int),
+    "tkv_fork_rows_written": ([ctypes.POINTER(ForkWrittenArgs), _P], ctypes.c_int),
     "tkv_compact_pages_work": ([_I32], _I64),
     "tkv_compact_pages": ([ctypes.POINTER(CompactPagesArgs), _P], ctypes.c_int),
     "tkv_copy_planned": ([ctypes.POINTER(PageSet), _P, _I32, _P], ctypes.c_int),

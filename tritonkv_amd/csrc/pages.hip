@@ -268,16 +268,18 @@ __host__ __device__ inline int pages_per_thread(int N, int threads) {
 
 // ---------------------------------------------------------------------------
 // Rows: row b becomes the first min(want_b, L_a) tokens of old row a =
-// parents[b], with pages for want_b.  keep = min(want_b, L_a) has f = keep /
-// page full pages, which are shared, and perhaps a partial one.  That page stays
-// with one row (`heir`) if nobody else keeps it: it was a's alone, no other
-// child of a keeps it as a full page, and of the children that end in it the heir
-// is a itself or the lowest; every other child copies it to its first new page.
+// parents[b], with pages for want_b.  Of these keep = min(want_b, L_a, written_a)
+// hold something: f = keep / page full pages, which are shared, and perhaps a
+// partial one.  That page, and the room that a has after it, stays with one row
+// (`heir`) if nobody else keeps it: it was a's alone, no other child of a keeps it as
+// a full page, and of the children that end before it or in it the heir is a itself or
+// the lowest; every other child copies the partial page to its first new page.  A page
+// of unwritten room is never shared: two rows would write their own tokens into it.
 // ---------------------------------------------------------------------------
-// tkv_fork_rows_args without its set.
+// tkv_fork_written_args without its set.
 struct RowsParams {
   int32_t *block_table, *seq_lens, *refs;
-  const int32_t *parents, *new_lens;
+  const int32_t *parents, *new_lens, *written;
   int32_t *status, *work;
   int32_t table_stride, B, max_pages, page_size, num_pages;
 };
@@ -308,26 +310,44 @@ __device__ __forceinline__ RowsWork rows_work(const RowsParams& a) {
 }
 
 struct Row {
-  int a, want, f, last;  // parent (-1: none), tokens, full pages kept, pool page after them
-  bool rest;             // ... of which some tokens are kept
+  int a, want, f;  // parent (-1: none), tokens, full pages kept
+  int tail, last;  // old pages after them, as far as the row reaches, and the first of them in the pools
+  bool rest;       // ... of which some tokens are kept
 };
 
 __device__ __forceinline__ int table_tokens(const RowsParams& a) { return a.max_pages * a.page_size; }
 
+// WRITTEN: a.written is given.  (Without it the plan of a beam step is 0.3 us shorter for not
+// looking.)
+template <bool WRITTEN>
 __device__ __forceinline__ Row row_of(const RowsParams& a, int b) {
   Row r;
   r.a = a.parents ? a.parents[b] : b;
   if (r.a < 0 || r.a >= a.B) r.a = -1;
   const int have = r.a < 0 ? 0 : max(0, min(a.seq_lens[r.a], table_tokens(a)));
   r.want = r.a < 0 ? 0 : a.new_lens ? max(0, a.new_lens[b]) : have;
-  const int keep = min(have, r.want);
+  const int reach = min(have, r.want);
+  const int keep = WRITTEN && r.a >= 0 ? min(reach, max(0, a.written[r.a])) : reach;
   r.f = keep / a.page_size;
   r.rest = keep % a.page_size != 0;
-  r.last = r.rest ? a.block_table[(int64_t)r.a * a.table_stride + r.f] : -1;
+  r.tail = r.rest;
+  if (WRITTEN) r.tail = reach / a.page_size + (reach % a.page_size != 0) - r.f;
+  r.last = r.tail ? a.block_table[(int64_t)r.a * a.table_stride + r.f] : -1;
   return r;
 }
 
-template <int T>
+// Pages of its parent's tail that an heir keeps: those that are nobody else's.
+__device__ __forceinline__ int tail_of_heir(const RowsParams& a, const Row& r) {
+  const int32_t* entry = a.block_table + (int64_t)r.a * a.table_stride + r.f;
+  int n = 1;  // (the first was looked at: may_inherit)
+  for (; n < r.tail; ++n) {
+    const int page = entry[n];
+    if (page < 0 || page >= a.num_pages || a.refs[page] != 1) break;
+  }
+  return n;
+}
+
+template <int T, bool WRITTEN>
 __global__ void __launch_bounds__(T) rows_plan_kernel(RowsParams a) {
   extern __shared__ int lds[];
   __shared__ ScanLds<T> scan;
@@ -352,25 +372,25 @@ __global__ void __launch_bounds__(T) rows_plan_kernel(RowsParams a) {
   // This thread's first row and first pages stay in registers: most plans need no others.
   const int per = pages_per_thread(N, T);
   const uint64_t mask0 = used_mask(a.refs, (int64_t)tid * per, per, N);
-  Row row0{-1, 0, 0, -1, false};
-  int owners0 = 0;  // references of the page that it ends in
+  Row row0{-1, 0, 0, 0, -1, false};
+  int owners0 = 0;  // references of the first page of its tail
   if (tid < B) {
-    row0 = row_of(a, tid);
+    row0 = row_of<WRITTEN>(a, tid);
     if (row0.last >= 0 && row0.last < N) owners0 = a.refs[row0.last];
   }
   __syncthreads();
   for (int b = tid; b < B; b += T) {
-    const Row r = b == tid ? row0 : row_of(a, b);
+    const Row r = b == tid ? row0 : row_of<WRITTEN>(a, b);
     if (r.a >= 0) atomicMax(most + r.a, r.f);
     if (r.want > table_tokens(a)) past = 1;
   }
   __syncthreads();
   auto may_inherit = [&](const Row& r, int b) {
-    if (!r.rest || r.f != most[r.a] || r.last < 0 || r.last >= N) return false;
+    if (!r.tail || r.f != most[r.a] || r.last < 0 || r.last >= N) return false;
     return (b == tid ? owners0 : a.refs[r.last]) == 1;
   };
   for (int b = tid; b < B; b += T) {
-    const Row r = b == tid ? row0 : row_of(a, b);
+    const Row r = b == tid ? row0 : row_of<WRITTEN>(a, b);
     if (may_inherit(r, b)) atomicMin(best + r.a, r.a == b ? -1 : b);
   }
   __syncthreads();
@@ -382,22 +402,22 @@ __global__ void __launch_bounds__(T) rows_plan_kernel(RowsParams a) {
   for (int b0 = 0; b0 < B; b0 += T) {
     const int b = b0 + tid;
     Row r;
-    int need = 0, pages = 0;
-    bool heir = false, copy = false;
+    int need = 0, pages = 0, inherited = 0;
+    bool copy = false;
     if (b < B) {
-      r = b == tid ? row0 : row_of(a, b);
-      heir = may_inherit(r, b) && best[r.a] == (r.a == b ? -1 : b);
+      r = b == tid ? row0 : row_of<WRITTEN>(a, b);
+      if (may_inherit(r, b) && best[r.a] == (r.a == b ? -1 : b)) inherited = WRITTEN ? tail_of_heir(a, r) : 1;
       pages = (int)(((int64_t)r.want + a.page_size - 1) / a.page_size);
       // (a row that does not fit its table asks for nothing: the call fails)
-      need = too_long ? 0 : pages - r.f - (heir ? 1 : 0);
-      copy = !too_long && r.rest && !heir;
+      need = too_long ? 0 : pages - r.f - inherited;
+      copy = !too_long && r.rest && !inherited;
     }
     int2 total;
     const int first_copy = copy && atomicExch(copied + r.a, 1) == 0 ? kCopies + 1 : 0;
     const int2 at = block_scan(scan, need, copy ? 1 + first_copy : 0, total);
     if (b < B) {
       w.old_len[b] = max(0, min(a.seq_lens[b], table_tokens(a)));
-      w.kept[b] = r.f + (heir ? 1 : 0);
+      w.kept[b] = r.f + inherited;
       w.first[b] = done.x + at.x;
       w.pages[b] = pages;
       if (copy) w.pairs[(done.y + at.y) & kCopies] = make_int2(r.last, done.x + at.x);
@@ -693,7 +713,7 @@ extern "C" int64_t tkv_fork_rows_work(int32_t B, int32_t max_pages, int32_t num_
   return tkv::rows_work_ints(B, max_pages, num_pages, parents != 0);
 }
 
-extern "C" int tkv_fork_rows(const tkv_fork_rows_args* a, tkv_stream_t stream) {
+static int fork_rows(const tkv_fork_rows_args* a, const int32_t* written, tkv_stream_t stream) {
   using namespace tkv;
   if (!a || !a->block_table || !a->seq_lens || !a->refs || !a->status || !a->work || (uintptr_t)a->work & 7)
     return TKV_EINVAL;
@@ -710,16 +730,23 @@ extern "C" int tkv_fork_rows(const tkv_fork_rows_args* a, tkv_stream_t stream) {
   const bool small = a->B <= kSmallPlan && a->num_pages <= 16 * kSmallPlan;
   const int threads = small ? kSmallPlan : kPlan;
   const unsigned staging = a->parents ? (unsigned)((entries + 4 * threads - 1) / (4 * threads)) : 0;
-  const RowsParams p{a->block_table, a->seq_lens, a->refs, a->parents, a->new_lens, a->status, a->work,
+  const RowsParams p{a->block_table, a->seq_lens, a->refs, a->parents, a->new_lens, written, a->status, a->work,
                      a->table_stride, a->B, a->max_pages, a->page_size, a->num_pages};
-  const int bad = launch(small ? rows_plan_kernel<kSmallPlan> : rows_plan_kernel<kPlan>,
-                         dim3(1 + (staging < 512 ? staging : 512)), dim3(threads), 3 * sizeof(int) * a->B, st, p);
+  const auto plan_kernel = small ? (written ? rows_plan_kernel<kSmallPlan, true> : rows_plan_kernel<kSmallPlan, false>)
+                                 : (written ? rows_plan_kernel<kPlan, true> : rows_plan_kernel<kPlan, false>);
+  const int bad = launch(plan_kernel, dim3(1 + (staging < 512 ? staging : 512)), dim3(threads), 3 * sizeof(int) * a->B, st, p);
   if (bad) return bad;
   const int64_t tables = (entries + kCopy - 1) / kCopy;
   const int t = (int)(tables < 512 ? tables : 512);
   return with_plan(c, [&](auto plan) {
     return launch(rows_apply_kernel<plan.kMost>, dim3(t + copy_groups(a->B, c)), dim3(kCopy), 0, st, p, plan, t);
   });
+}
+
+extern "C" int tkv_fork_rows(const tkv_fork_rows_args* a, tkv_stream_t stream) { return fork_rows(a, nullptr, stream); }
+
+extern "C" int tkv_fork_rows_written(const tkv_fork_written_args* a, tkv_stream_t stream) {
+  return a ? fork_rows(&a->rows, a->written, stream) : TKV_EINVAL;
 }
 
 extern "C" int64_t tkv_compact_pages_work(int32_t num_pages) {

@@ -6,7 +6,8 @@ A paged cache is page pools (of any layer, K and V; 2/4-bit
 that share page numbers, and three int32 tensors that say which row owns what:
 
 * ``block_table`` ``(B, max_pages)``: row b's pages in order, -1 after them;
-* ``seq_lens`` ``(B,)``: its tokens; it uses ``ceil(seq_lens[b] / page_size)`` pages;
+* ``seq_lens`` ``(B,)``: its tokens, or as many as it has room for; it uses
+  ``ceil(seq_lens[b] / page_size)`` pages;
 * ``refs`` ``(num_pages,)``: how many used table entries name each page, 0 for
   a free one.  (A caller may add counts of its own to keep pages alive.)
 
@@ -16,7 +17,9 @@ rows out of other rows (parallel samples, beams, a shared prefix), sharing
 their full pages, and :func:`compact_pages` moves the live pages to the low end
 of the pools.  A page that is not full belongs to one row alone, so the appends
 (:func:`~tritonkv_amd.paged.paged_append`, ``paged16_append`` and the decodes'
-fused ones) never write into another row's tokens.
+fused ones) never write into another row's tokens.  Where rows hold room made ahead,
+whose pages are full only by ``seq_lens``, this takes ``written``, the tokens that
+they really hold: :func:`fork_rows`.
 
 Everything runs on the current stream, in two launches, from device tensors
 alone: nothing is copied to the host and no call synchronises.  Calls that may
@@ -142,7 +145,7 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 _C = {f: _offset(_lib.CopyPagesArgs, f) for f in ("src", "dst")}
-_F = {f: _offset(_lib.ForkRowsArgs, f) for f in ("parents", "new_lens", "status")}
+_F = {f: _offset(_lib.ForkWrittenArgs, f) for f in ("parents", "new_lens", "status", "written")}
 _P = {f: _offset(_lib.CompactPagesArgs, f) for f in ("live",)}
 _APART, _WRITTEN = 2, 4  # flags of a kept call's tensors: apart from written ones; written
 
@@ -212,7 +215,8 @@ def copy_pages(pools, src: torch.Tensor, dst: torch.Tensor, dst_pools=None, _wor
 
 def fork_rows(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor,
               parents: torch.Tensor | None, new_lens: torch.Tensor | None = None,
-              status: torch.Tensor | None = None, _workspace: dict | None = None) -> torch.Tensor:
+              status: torch.Tensor | None = None, _workspace: dict | None = None, *,
+              written: torch.Tensor | None = None) -> torch.Tensor:
     """Make every row of a block table out of an old row, in place.
 
     Row b becomes the first ``min(new_lens[b], seq_lens[a])`` tokens of old
@@ -225,6 +229,14 @@ def fork_rows(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, refs: to
     * a smaller ``new_lens`` truncates, 0 or a parent of -1 frees;
     * a larger one makes room: tokens from the old length on are whatever the
       new pages hold until they are written.
+
+    ``written``, an int32 ``(B,)`` tensor, says how many of its ``seq_lens`` tokens
+    every old row holds (None: all of them).  It is needed where an old row has room
+    that was made ahead and is not written yet: without it the full pages of that room
+    would be shared, and the rows would write their next tokens over each other's.
+    With it only full pages of written tokens are shared; the pages of room stay with
+    the row that keeps the partial page, and other rows get new ones.  (The rows made
+    hold ``min(written[parents[b]], new_lens[b])`` tokens.)
 
     Full pages are shared (``refs`` counts the rows).  The page that a row ends
     in, if not full, stays with one row -- the parent itself, else its first
@@ -246,7 +258,7 @@ def fork_rows(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, refs: to
             got = status
             if got is None and isinstance(refs, torch.Tensor):
                 got = torch.empty(1, dtype=torch.int32, device=refs.device)
-            if prep.run(block_table, seq_lens, refs, parents, new_lens, got, *tensors):
+            if prep.run(block_table, seq_lens, refs, parents, new_lens, written, got, *tensors):
                 return got
     B, max_pages = _check_rows(block_table, refs)
     device, num_pages = refs.device, refs.numel()
@@ -263,47 +275,51 @@ def fork_rows(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, refs: to
     _int32_arg(seq_lens, B, device, "seq_lens", "B lengths")
     par = None if parents is None else _int32_arg(parents, B, device, "parents", "B rows")
     new = None if new_lens is None else _int32_arg(new_lens, B, device, "new_lens", "B lengths")
-    written = [block_table, seq_lens, refs]
+    held = None if written is None else _int32_arg(written, B, device, "written", "B token counts")
+    outputs = [block_table, seq_lens, refs]
     if status is None:
         status_given = torch.empty(1, dtype=torch.int32, device=device)
     else:
         status_given = _int32_arg(status, 1, device, "status", "one entry")
-        written.append(status)
-    for i, a in enumerate(written):
-        if any(_overlap(a, b) for b in written[i + 1:] + [x for x in (parents, new_lens) if x is not None]):
+        outputs.append(status)
+    inputs = [x for x in (parents, new_lens, written) if x is not None]
+    for i, a in enumerate(outputs):
+        if any(_overlap(a, b) for b in outputs[i + 1:] + inputs):
             raise ValueError("block_table, seq_lens, refs and status are written: they must not share memory "
-                             "with each other, parents or new_lens")
+                             "with each other, parents, new_lens or written")
     _require_gpu(refs, "fork_rows")
     words = _lib.load().tkv_fork_rows_work(B, max_pages, num_pages, int(par is not None))
     work = _work(_workspace, "fork_rows", words, device)
     sets = _page_sets(pages, pages)
-    args = _lib.ForkRowsArgs(
+    args = _lib.ForkWrittenArgs(
         set=sets[0], block_table=block_table.data_ptr(), seq_lens=seq_lens.data_ptr(), refs=refs.data_ptr(),
-        parents=_lib.ptr(par), new_lens=_lib.ptr(new), status=status_given.data_ptr(), work=work.data_ptr(),
+        parents=_lib.ptr(par), new_lens=_lib.ptr(new), written=_lib.ptr(held), status=status_given.data_ptr(),
+        work=work.data_ptr(),
         table_stride=_row_stride(block_table), B=B, max_pages=max_pages, page_size=page_size, num_pages=num_pages)
-    _lib.check(_lib.launch(device, "tkv_fork_rows", args), "fork_rows")
+    _lib.check(_lib.launch(device, "tkv_fork_rows_written", args), "fork_rows")
     for one in sets[1:]:
         _lib.check(_lib.launch(device, "tkv_copy_planned", one, work.data_ptr(), B), "fork_rows")
     if key is not None and len(sets) == 1:
-        _keep16(_workspace, key, args, "tkv_fork_rows", "fork_rows", device, (work,),
+        _keep16(_workspace, key, args, "tkv_fork_rows_written", "fork_rows", device, (work,),
                 ((block_table, -1, 4, 1 | _WRITTEN), (seq_lens, -1, 4, _WRITTEN), (refs, -1, 4, _WRITTEN),
                  (parents, _F["parents"], 4, _APART), (new_lens, _F["new_lens"], 4, _APART),
+                 (written, _F["written"], 4, _APART),
                  (status_given, _F["status"], 4, _WRITTEN), *((t, -1, 16, 1) for t in tensors)))
     return status_given
 
 
 def resize_rows(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor,
                 new_lens: torch.Tensor, status: torch.Tensor | None = None,
-                _workspace: dict | None = None) -> torch.Tensor:
+                _workspace: dict | None = None, *, written: torch.Tensor | None = None) -> torch.Tensor:
     """Give every row ``new_lens[b]`` tokens: :func:`fork_rows` with every row its own parent.
 
     Rows that grow get pages, rows that shrink return theirs, a length of 0
     frees the row.  A row cut inside a page that it shares gets its own
-    copy of that page.
+    copy of that page.  ``written`` as there; rows keep the room that is their own.
     """
     if new_lens is None:
         raise ValueError("new_lens must be an int32 tensor of B lengths")
-    return fork_rows(pools, block_table, seq_lens, refs, None, new_lens, status, _workspace)
+    return fork_rows(pools, block_table, seq_lens, refs, None, new_lens, status, _workspace, written=written)
 
 
 def compact_pages(pools, block_table: torch.Tensor, refs: torch.Tensor, out=None,
