@@ -15,7 +15,10 @@
 // Precision: out is fp32, and P enters the matrix cores as a sum of 16-bit
 // terms, two for fp16 (22 bits) and three for bf16 (24): with P rounded once
 // the output would be 2e-4 (fp16) or 2e-3 (bf16) off, and the extra MFMAs
-// run in the shadow of the loads.
+// run in the shadow of the loads.  Its lower terms may be 0 or below, which times an
+// infinite V would be NaN where p * V is infinite: a wave that finds NaN among its
+// results goes over its chunks again, with V's infinities in a product of their own
+// against p > 0.  Looking for NaN costs 0.1 us of a step.
 //
 // Measured, at steps of the sizes that a serving loop has (bytes of K, V, q and out
 // over the time of both launches): 32 rows of 32768, HKV 8, G 4, fp16, pages of 256:
@@ -36,6 +39,7 @@ typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 
 struct Half {
   static constexpr int kTerms = 2;
+  static constexpr uint32_t kInf = 0x7c00;
   // P is scaled by 2^14: the low term of a small p would else fall below
   // fp16's smallest step (2^-24), e.g. 3e-5 of a p of 2^-10.
   static constexpr float kShift = 14.0f;
@@ -47,6 +51,7 @@ struct Half {
 
 struct Bf16 {
   static constexpr int kTerms = 3;
+  static constexpr uint32_t kInf = 0x7f80;
   static constexpr float kShift = 0.0f;
   static __device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c,
@@ -59,6 +64,14 @@ struct Bf16 {
   static __device__ __forceinline__ float lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
   static __device__ __forceinline__ float hi(uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
 };
+
+// The infinities among two values, zeros in the others' place.
+template <class T>
+__device__ __forceinline__ uint32_t infinities(uint32_t w) {
+  const uint32_t lo = (w & 0x7fffu) == T::kInf ? 0x0000ffffu : 0u;
+  const uint32_t hi = (w >> 16 & 0x7fffu) == T::kInf ? 0xffff0000u : 0u;
+  return w & (lo | hi);
+}
 
 // ---------------------------------------------------------------------------
 // The split, made on the device from the rows' lengths.
@@ -379,16 +392,19 @@ paged16_split_kernel(const int32_t* lens, int B, int S, int workgroups, int leas
     const int last = hi - 1;
     f4 accv[HT][EPL];
     float m_run[HT], l_run[HT];
+    auto start = [&] {
 #pragma unroll
-    for (int ht = 0; ht < HT; ++ht) {
+      for (int ht = 0; ht < HT; ++ht) {
 #pragma unroll
-      for (int mv = 0; mv < EPL; ++mv) accv[ht][mv] = f4{0.f, 0.f, 0.f, 0.f};
-      m_run[ht] = -INFINITY;
-      l_run[ht] = 0.0f;
-    }
+        for (int mv = 0; mv < EPL; ++mv) accv[ht][mv] = f4{0.f, 0.f, 0.f, 0.f};
+        m_run[ht] = -INFINITY;
+        l_run[ht] = 0.0f;
+      }
+    };
+    start();
 
-    auto step = [&](int c, int cb, auto tail) {
-      constexpr bool TAIL = decltype(tail)::value;
+    auto step = [&](int c, int cb, int r, int j, auto tail, auto infinite) {
+      constexpr bool TAIL = decltype(tail)::value, INF = decltype(infinite)::value;
       const bool more = cb + 32 * NW < hi;
       if constexpr (TAIL && APPEND) {
         if (owner) {
@@ -437,7 +453,7 @@ paged16_split_kernel(const int32_t* lens, int B, int S, int workgroups, int leas
       }
       // Online softmax in base 2; the accumulators are rescaled only in chunks
       // where a head's maximum rose.
-      u4 pt[HT][T::kTerms];
+      u4 pt[HT][T::kTerms], some[HT];  // some (INF): 1 where p > 0
 #pragma unroll
       for (int ht = 0; ht < HT; ++ht) {
         float top = x[ht][0];
@@ -459,6 +475,10 @@ paged16_split_kernel(const int32_t* lens, int B, int S, int workgroups, int leas
           p[i] = __builtin_amdgcn_exp2f(x[ht][i] + off);
           l_run[ht] += p[i];
         }
+        if constexpr (INF)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            some[ht][i] = T::pack(p[2 * i] > 0.0f ? 1.0f : 0.0f, p[2 * i + 1] > 0.0f ? 1.0f : 0.0f);
 #pragma unroll
         for (int n = 0; n < T::kTerms; ++n)
 #pragma unroll
@@ -478,12 +498,26 @@ paged16_split_kernel(const int32_t* lens, int B, int S, int workgroups, int leas
 #pragma unroll
             for (int e = 0; e < VW; ++e) vx[i][e] = 0u;
       }
+      // V is waited for behind the softmax: left to itself the compiler may ask for it, and with
+      // it for the next K, ahead of the exponentials (32 rows of 8000-16384, head dim 64: 134 us
+      // against 129).
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int mv = 0; mv < EPL; ++mv) {
         const uint32_t sel = (mv & 1) ? 0x07060302u : 0x05040100u;
         u4 av;
 #pragma unroll
         for (int i = 0; i < 4; ++i) av[i] = perm(vx[2 * i + 1][mv / 2], vx[2 * i][mv / 2], sel);
+        if constexpr (INF) {
+          u4 iv;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            iv[i] = infinities<T>(av[i]);
+            av[i] ^= iv[i];
+          }
+#pragma unroll
+          for (int ht = 0; ht < HT; ++ht) accv[ht][mv] = T::mfma(iv, some[ht], accv[ht][mv]);
+        }
 #pragma unroll
         for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
@@ -495,8 +529,24 @@ paged16_split_kernel(const int32_t* lens, int B, int S, int workgroups, int leas
     // Full chunks, then the row's partial last one, or the one that takes the new token.
     const int full = app ? last : hi;
     int c = 0, cb = lo + 32 * w;
-    for (; cb + 32 <= full; cb += 32 * NW, ++c) step(c, cb, std::false_type{});
-    if (cb < hi) step(c, cb, std::true_type{});
+    for (; cb + 32 <= full; cb += 32 * NW, ++c) step(c, cb, r, j, std::false_type{}, std::false_type{});
+    if (cb < hi) step(c, cb, r, j, std::true_type{}, std::false_type{});
+
+    f4 all = f4{0.f, 0.f, 0.f, 0.f};  // NaN if one of them is
+#pragma unroll
+    for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+      for (int mv = 0; mv < EPL; ++mv) all += accv[ht][mv];
+    const float sum = (all[0] + all[1]) + (all[2] + all[3]);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum != sum) != 0, 0)) {
+      start();
+      for (c = 0, cb = lo + 32 * w; cb < hi; cb += 32 * NW, ++c) {
+        if ((c & 31) == 0) tiles(c);
+        load_k(c);
+        load_v(c);
+        step(c, cb, (int)opaque(r), (int)opaque(j), std::true_type{}, std::true_type{});
+      }
+    }
 
     if (APPEND && owner && hb0 == 0) {
       const uint32_t t16 = (uint32_t)last / 16, pg = t16 / (uint32_t)prm.page_tiles;

@@ -272,8 +272,9 @@ def paged16_decode_attention(
     of no tokens gives zeros.  ``lse``: a contiguous ``(B, HQ)`` float32 tensor
     that receives the natural logarithm of each row's sum of exp(score), -inf
     for a row of no tokens, so that the results over two caches can be joined.
-    Nothing past a row's length reaches them, NaN and infinities included; an
-    infinite V value of a live token gives an infinity or NaN.
+    Nothing past a row's length reaches them, NaN and infinities included; those
+    of live tokens show as in softmax (a weight below 2**-126 of the largest counts as 0,
+    and 0 times infinity is NaN).
 
     ``k_new`` / ``v_new``, ``(B, HKV, D)`` or ``(B, HKV, 1, D)`` in the pools'
     type, fuse the step's append into the call: the token takes position
