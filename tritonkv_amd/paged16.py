@@ -90,22 +90,31 @@ def plan_shares(B: int, HKV: int, G: int, S: int, D: int = 128, device=None,
                 piece_tokens: int | None = None) -> tuple[int, int, int, int]:
     """``(least_chunks, workgroups, long_workgroups, long_chunks)`` of a decode (``include/tkv.h``).
 
-    ``S`` is the tables' capacity; the rows' lengths are the device's business.
+    ``S`` is the tables' capacity, all that the host knows of the lengths: it decides whether
+    rows stay whole, the least share and the number of workgroups; the cut itself follows the
+    lengths, on the device.
     ``piece_tokens`` fixes a workgroup's tokens instead.  The rules, with
     what was measured on MI355X (us of a captured step; U = HKV times the
     blocks of query heads, 16 or for more 32, the workgroups that attend to the same tokens):
 
-    * Rows stay whole, in one launch, where that is faster than cutting them
+    * Rows stay whole, in one launch, where that was faster than cutting them
       and joining (a second launch, 2.4 us and more): one CU reads at most
       38 GB/s, so only in narrow tables, or with many rows.  Up to 256 tokens of 128 dims
       (250 tokens, D 128: B * U = 2 5.8 whole, 6.8 cut; 32 6.3, 7.1; D 256 10.7,
-      7.9), twice that from 64 row units on (505 tokens: B * U = 2 10.1, 7.0; 32 10.5,
-      7.6; 128 11.3, 11.0), four times from 512 (up to 512 of 1024: 512 units
-      19.9, 23.7).
+      7.9).  Twice that where B * U * D is 16384 or more (whole / cut, 505 tokens of 128
+      dims: B * U = 32 10.3 / 7.6, 64 10.7 / 8.9, 128 11.2 / 11.1, 256 12.9 / 15.8, 504 22.6 /
+      26.5; 1-505 tokens: 64 10.2 / 9.9, 128 10.6 / 11.6; 1000 of 64 dims: 64 11.5 / 9.1, 128
+      12.0 / 10.8, 256 13.2 / 15.8; 250 of 256 dims: 32 11.7 / 8.5, 64 12.3 / 13.7).  Four times
+      from 512 units on (up to 512 of 1024: 512 units 19.9 / 23.7; all 1000: 512 44.0 / 46.0,
+      1024 85 / 87; but 1-1000: 512 32.3 / 28.8, 1024 54.8 / 51.5: long and short rows mixed lose
+      by whole rows, equal ones gain).
     * Otherwise two workgroups per CU (four at head dim 64, whose chunks are half
       as large: 8 rows of up to 2999, 16 KV heads, w = 1 / 2 / 4 16.9 / 15.7 /
       15.5), of at least 128 tokens of 128 dims, half of that in tables of
-      at most 512 tokens (one row of 505: 6.7, with 128 7.2; of 4000: 8.8, 8.0).
+      at most 512 tokens.  The better one hangs on the lengths, which the table only bounds (64 /
+      128 tokens, 2 KV heads: one row of 505 6.9 / 7.4, of 1000 7.3 / 7.5, of 2000 7.3 / 8.0, of
+      4000 8.8 / 8.0; 8 KV heads: one row of 4000 10.6 / 8.7, 4 rows of 505 7.6 / 8.2, of 1000 9.4 /
+      8.7, 8 rows of 505 9.1 / 8.7): a short row in a wide table takes 0.5 us more.
     * One per CU where the batch has no more rows than that and every workgroup
       gets a long stream, 16 chunks (2 per CU, 1, in turn: 32 rows of 32768 648, 637; of
       8192 169, 165; one of 32768 26.8, 25.9; 16 of 8000-16384 at D 256 143, 138;
@@ -128,7 +137,7 @@ def plan_shares(B: int, HKV: int, G: int, S: int, D: int = 128, device=None,
                              f"more than {MAX_WORKGROUPS} pieces")
         return least, most, 0, 0
     row = S * D
-    if row <= 32768 * (4 if B * units >= 512 else 2 if B * units >= 64 else 1):
+    if row <= 32768 * (4 if B * units >= 512 else 2 if B * units * D >= 16384 else 1):
         return 1, 0, 0, 0
     least = (256 if S <= 512 else 512) // D or 1
     cu = compute_units(device) or 256
