@@ -336,9 +336,10 @@ int tkv_dequantize(const uint8_t *packed, const uint16_t *scale, const uint16_t 
  *   out        (B, HQ, D);  lse (B, HQ) or NULL: the natural logarithm of the
  *              row's sum of exp(score)
  *   k_new/v_new  NULL, or (B, HKV, D) in the pools' type, strides batch, head:
- *              the token at L_b - 1 of every row, attended to and put into its
- *              page by this call (not stored where the table entry lies outside
- *              [0, num_pages); rows of no tokens take none)
+ *              the token at seq_lens[b] - 1 of every row, attended to and put into
+ *              its page by this call (not stored where the table entry lies outside
+ *              [0, num_pages); rows of no tokens, or of more than the table holds,
+ *              take none)
  * The rows are cut on the device, from their lengths: their chunks of 32 tokens
  * (an empty row counts as one), laid end to end, are shared out evenly over at
  * most `workgroups` workgroups (1 to 65535) per KV head and 16 query heads (32 where

@@ -351,7 +351,7 @@ paged16_split_kernel(const int32_t* lens, int B, int S, int workgroups, int leas
     const int bt = (int)opaque(tid), bl = bt & 63;
     lo = 32 * (int)g.begin;
     hi = min(g.L, 32 * (int)g.end);
-    app = APPEND && hi == g.L && hi > lo;
+    app = APPEND && hi == g.L && hi > lo && !(hi == S && lens && lens[g.b] > S);  // (a place past the table: none)
     owner = app && w == ((hi - 1 - lo) / 32) % NW;
     u4 new8 = {0u, 0u, 0u, 0u};  // lanes 0 .. D / 8 - 1: 8 dims of the new key; then of the value
     const bool mine = APPEND && owner && bl < D / 4;

@@ -277,8 +277,8 @@ def paged16_decode_attention(
     q: ``(B, HQ, D)`` in the pools' type, D 64, 128 or 256; pools as
     :func:`empty_paged16_pool`; block_table: ``(B, max_pages)`` int32;
     seq_lens: ``(B,)`` int32 (None: every row holds ``max_pages * page_size``
-    tokens).  Returns ``(B, HQ, D)`` float32, in ``out`` if it is given.  A row
-    of no tokens gives zeros.  ``lse``: a contiguous ``(B, HQ)`` float32 tensor
+    tokens; lengths past that are clamped to it).  Returns ``(B, HQ, D)`` float32, in
+    ``out`` if it is given.  A row of no tokens gives zeros.  ``lse``: a contiguous ``(B, HQ)`` float32 tensor
     that receives the natural logarithm of each row's sum of exp(score), -inf
     for a row of no tokens, so that the results over two caches can be joined.
     Nothing past a row's length reaches them, NaN and infinities included; those
@@ -288,7 +288,8 @@ def paged16_decode_attention(
     ``k_new`` / ``v_new``, ``(B, HKV, D)`` or ``(B, HKV, 1, D)`` in the pools'
     type, fuse the step's append into the call: the token takes position
     ``seq_lens[b] - 1`` of its row, in the page (unless the table entry lies
-    outside the pool) and in the attention.
+    outside the pool) and in the attention.  A row of no tokens takes none, nor does one
+    whose length is past its table, as in :func:`paged16_append`.
 
     ``piece_tokens`` fixes how many tokens a workgroup takes of a row; by
     default the device chooses, from the lengths.  With ``_workspace`` the
