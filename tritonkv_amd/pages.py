@@ -140,8 +140,18 @@ def _span(t: torch.Tensor) -> tuple:
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether a and b share memory.  Two that lie in turn at one stride, such as the halves of a
+    pool of paired pages or columns of one table, do not; at different strides, meeting
+    address ranges count as shared."""
     (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 <= b1 and b0 <= a1
+    if a0 > b1 or b0 > a1:
+        return False
+    stride = a.stride(0) * a.element_size()
+    if a.dim() < 2 or b.dim() < 2 or stride <= 0 or stride != b.stride(0) * b.element_size():
+        return True
+    size = [_span(t[0]) for t in (a, b)]
+    between = (b0 - a0) % stride
+    return between <= size[0][1] - size[0][0] or between + size[1][1] - size[1][0] >= stride
 
 
 _C = {f: _offset(_lib.CopyPagesArgs, f) for f in ("src", "dst")}
