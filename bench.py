@@ -19,10 +19,11 @@ of a HIP graph holding exactly K steps, after W untimed warmup steps.
 to its own average duration (a graph of split-kernel launches only) and
 MI355X's 8 TB/s HBM peak.  ``cpu_baseline`` times the oracle's scalar C
 restatement of the reference's CPU path on a bounded sample of the same step.
-Unless ``--quick``, the line also carries the 2-bit and fp16-control numbers of
-the same shape, the same 4-bit step over shuffled page pools (page sizes 32
+Unless ``--quick``, the line also carries the 2-bit and fp16-control times of
+the same shape, of the same 4-bit step over shuffled page pools (page sizes 32
 and 256), and the Qwen2.5-1.5B table of BASELINE.json configs 2-3
-(cache-resident and DRAM-resident, ctx 512..16384).
+(cache-resident and DRAM-resident, ctx 512..16384).  The line stays short enough
+to be read from the end of a log; ``--record FILE`` writes the complete record.
 
 A background sampler reads the GPU's clocks, power and temperatures while the
 Llama-shape legs run (``clocks``: per-leg windows and the quotable gate).
@@ -75,8 +76,11 @@ def _args():
     ap.add_argument("--rows", type=int, default=8, help="kernels listed in the summary")
     ap.add_argument("--no-clocks", action="store_true",
                     help="do not sample clocks/power/temperature during the timed legs")
+    ap.add_argument("--record", metavar="FILE", default=None,
+                    help="also write the complete record (every leg's details, clocks and checks) "
+                         "to FILE as one JSON line")
     ap.add_argument("--compare", nargs="+", metavar="RUN_JSON", default=None,
-                    help="no timing: compare the bench JSON lines of complete runs row by row")
+                    help="no timing: compare the records (--record) of complete runs row by row")
     ap.add_argument("--kernel-probe", choices=sorted(KERNEL_PROBES), default=None,
                     help="no timing: a few eager launches of one split kernel at its benchmark "
                          "shape, for rocprofv3 --pmc counter runs")
@@ -1789,8 +1793,39 @@ def main() -> int:
     }
     if _CLOCKS is not None:
         _CLOCKS.stop()
-    print(json.dumps(line))
+    if a.record:
+        with open(a.record, "w") as f:
+            f.write(json.dumps(line) + "\n")
+    print(json.dumps(short_line(line)))
     return 0
+
+
+def short_line(line: dict) -> dict:
+    """The record with its legs' times (us, in ``legs``) in place of their details, and the
+    checks counted: a few KB where the whole is 37, of which a log's reader may get the end alone."""
+    out = {k: v for k, v in line.items() if k not in ("detail", "check", "clocks")}
+    if out.get("cpu_baseline"):
+        out["cpu_baseline"] = {k: v for k, v in out["cpu_baseline"].items() if not isinstance(v, dict)}
+    records = list(_check_leaves(line["check"] or {}))
+    out["checks"] = {"records": len(records), "failed": sum(not c["ok"] for c in records)} if records else None
+    if line["clocks"]:
+        out["clocks"] = {k: line["clocks"][k] for k in ("gfx_mhz_mean", "power_w_mean", "quotable")
+                         if k in line["clocks"]}
+    d = line["detail"]
+    legs = {k: v["us_per_step"] for k, v in d.items() if isinstance(v, dict) and "us_per_step" in v}
+    for k in ("paged4", "channel_keys"):
+        legs.update({f"{k}_{n}": v["us_per_step"] for n, v in d.get(k, {}).items()})
+    out["legs"] = legs
+    qwen = {}
+    for r in d.get("qwen2.5-1.5b", {}).get("rows", []):  # ctx -> method -> [hot, cold]
+        qwen.setdefault(str(r["ctx"]), {})[r["method"]] = [r["hot_us"], r["cold_us"]]
+    if qwen:
+        out["qwen2.5-1.5b_hot_cold"] = qwen
+    e2e = {ctx: {m: v.get("graph_us", v.get("eager_us")) for m, v in row.items() if isinstance(v, dict)}
+           for ctx, row in d.get("qwen2.5-1.5b_e2e_decode", {}).get("ctx", {}).items()}
+    if e2e:
+        out["qwen2.5-1.5b_e2e"] = e2e
+    return out
 
 
 def _check_leaves(checks):
