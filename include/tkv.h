@@ -368,11 +368,12 @@ int tkv_paged16_decode_attention(const tkv_paged16_args *args, tkv_stream_t stre
 
 /* K and V of N tokens per row into such pools, one launch: token n of row b, for
  * n < counts[b] (NULL: N), goes to position positions[b] + n.  k_new, v_new
- * (B, HKV, N, D), strides batch, head, token, in the pools' type or fp32
- * (new_is_fp32), rounded to nearest even; bases and strides are multiples of 16
+ * (B, HKV, N, D), strides batch, head, token, in the pools' type, in fp32 or in the
+ * other 16-bit type (new_is_fp32: 0, 1, 2), rounded to nearest even; bases and strides are multiples of 16
  * bytes.  Positions outside [0, max_pages * page_size) and table entries
  * outside [0, num_pages) are not written.  Any page_size; D a multiple of 8; at most
  * 65535 rows and 2^31 - 1 groups of 8 values in each (N * HKV * D / 8). */
+enum { TKV_NEW_SAME = 0, TKV_NEW_FP32 = 1, TKV_NEW_OTHER = 2 };
 typedef struct tkv_paged16_append_args {
   const void *k_new, *v_new;
   int64_t k_new_strides[3], v_new_strides[3];

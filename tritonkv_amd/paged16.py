@@ -191,11 +191,9 @@ _A = {f: _offset(_lib.Paged16AppendArgs, f) for f in ("k", "v", "k_new", "v_new"
                                                       "counts")}
 
 
-def _new_rows(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """New tokens as the kernels read them: in the pools' type or fp32, rows on 16 bytes."""
-    if x.dtype != dtype and x.dtype != torch.float32:
-        x = x.float()
-    return x if _dense_rows(x, 8 if x.dtype == dtype else 4) else x.contiguous().clone()
+def _new_rows(x: torch.Tensor) -> torch.Tensor:
+    """New tokens as the kernel reads them: rows on 16 bytes."""
+    return x if _dense_rows(x, 16 // x.element_size()) else x.contiguous().clone()
 
 
 def paged16_append(k_pool: torch.Tensor, v_pool: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
@@ -239,13 +237,14 @@ def paged16_append(k_pool: torch.Tensor, v_pool: torch.Tensor, k_new: torch.Tens
     _require_gpu(k_pool, "paged16_append")
     if B == 0 or N == 0:
         return
-    kn, vn = _new_rows(k_new, k_pool.dtype), _new_rows(v_new, k_pool.dtype)
-    align = 8 if kn.dtype == k_pool.dtype else 4
+    kn, vn = _new_rows(k_new), _new_rows(v_new)
+    align = 16 // kn.element_size()
+    kind = 0 if kn.dtype == k_pool.dtype else 1 if kn.dtype == torch.float32 else 2
     args = _lib.Paged16AppendArgs(
         k_new=kn.data_ptr(), v_new=vn.data_ptr(), k_new_strides=_strides(kn, align),
         v_new_strides=_strides(vn, align), k=k_pool.data_ptr(), v=v_pool.data_ptr(),
         k_strides=_strides(k_pool, 8), v_strides=_strides(v_pool, 8), block_table=table.data_ptr(),
-        positions=pos.data_ptr(), counts=_lib.ptr(num), new_is_fp32=int(kn.dtype == torch.float32),
+        positions=pos.data_ptr(), counts=_lib.ptr(num), new_is_fp32=kind,
         is_bf16=int(k_pool.dtype == torch.bfloat16), B=B, HKV=HKV, N=N, D=D,
         block_table_stride=table.shape[1], max_pages=table.shape[1], page_size=page_size,
         num_pages=num_pages)
