@@ -4,9 +4,11 @@
 //   out[b, h] = sum_t p_t v_t / sum_t p_t,  p_t = exp(sm_scale q[b, h] . k_t - max),
 //   lse[b, h] = max + log sum_t p_t,        t < L_b
 //
-// The decode reads every live token's K and V row once (2 * D * 2 bytes per
-// token and KV head) for 4 * D * G flops: it is bound by HBM for every GQA
-// group.  One workgroup = a share of the batch's tokens for one KV head and up to
+// The decode reads every live token's K and V row (2 * D * 2 bytes per token and KV
+// head) once for every block of up to 32 query heads of a KV head, for 4 * D * G flops: G
+// per byte where G <= 32, so HBM bounds it there.  Wider groups repeat the reads and the
+// chunks' work per block (8 rows of 8192, 2 KV heads, bf16: G 32 20.6 us, 33 29.0, 64 29.7, 128
+// 50.3).  One workgroup = a share of the batch's tokens for one KV head and up to
 // 32 of its query heads; each of its four waves walks 32-token chunks, two 16-row
 // MFMA tiles.  Scores are S^T = K Q^T (tokens as rows, heads as columns), whose
 // accumulator layout is the B operand layout of O^T = V^T P^T, so the
@@ -22,10 +24,11 @@
 //
 // Measured, at steps of the sizes that a serving loop has (bytes of K, V, q and out
 // over the time of both launches): 32 rows of 32768, HKV 8, G 4, fp16, pages of 256:
-// 607 us, 7.1 TB/s; 32 rows of 1000-16384, HKV 8, G 8, bf16, pages of 64, with the
-// append: 175 us, 6.5 TB/s.  32 rows of 8192 in pages of 256, 64 and 16: 165, 166 and
-// 172 us.  Small steps are bound by the two launches and the chain of lengths, table, K
-// and V: one row of 505 tokens (12 / 2 heads) takes 6.7 us.
+// 607 us one call after the other and 641 in a graph, 7.1 and 6.7 TB/s; 32 rows of
+// 1000-16384, HKV 8, G 8, bf16, pages of 64, with the append: 177 us, 6.5 TB/s.  32 rows of
+// 8192 in pages of 256, 64 and 16: 165, 166 and 172 us.  Small steps are bound by the two
+// launches and the chain of lengths, table, K and V: one row of 505 tokens (12 / 2 heads)
+// takes 6.8 us.
 #include "decode_common.h"
 #include "launch.h"
 
@@ -94,7 +97,7 @@ __device__ __forceinline__ uint32_t infinities(uint32_t w) {
 // workgroups == 0: one workgroup per row.
 //
 // Measured on 32 rows of 200-16184 tokens (HKV 8, G 4 / 8, D 128): pieces of one row
-// each, cut evenly, 184-194 us; shares 172 / 176.  8 rows of 300-4000 take 18.9 us in
+// each, cut evenly, 184-194 us; shares 172 / 176; of 1000-16384 (G 8) 193 and 178.  8 rows of 300-4000 take 18.9 us in
 // tables of 131072 tokens and of 4032.
 // ---------------------------------------------------------------------------
 // What finds a workgroup's first segment: scalar arguments of the kernel, which are in
