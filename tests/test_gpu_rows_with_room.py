@@ -194,3 +194,46 @@ def test_quantized_pools_and_more_tensors_than_a_launch_takes():
         rows = [p.packed[m.table[b][1]] for b in range(3)]
         assert all(torch.equal(r[:, :8], first[1][:, :8]) for r in rows)
         assert not torch.equal(rows[0][:, 8], rows[1][:, 8]) and not torch.equal(rows[1][:, 8], rows[2][:, 8])
+
+
+@pytest.mark.parametrize("B", [1, 3, 5, 70, 300])
+def test_long_rooms_with_pages_that_others_hold(B):
+    """The heir keeps its parent's room up to the first page that is not the parent's alone."""
+    from tritonkv_amd.pages import fork_rows
+
+    rng = random.Random(B)
+    P = 700 if B < 10 else 90
+    m = Rows(B, P, B * P + 50, 16)
+    m.fork(None, [rng.randint(0, P * 16) if b % 2 == 0 else 0 for b in range(B)])
+    for b in range(0, B, 2):
+        for _ in range(min(m.lens[b], rng.choice([0, 16, 20, 100]))):
+            m.append(b)
+    for b in range(0, B, 4):  # a count of the caller's own on some page of the room
+        used = -(-m.lens[b] // 16)
+        held = len(m.tokens[b]) // 16
+        if used > held:
+            m.refs[m.table[b][rng.randint(held, used - 1)]] += 1
+    pools = [torch.zeros(m.N, 1, 16, 8, dtype=F16, device=DEV)]
+    state = _i32(m.table), _i32(m.lens), _i32(m.refs)
+    parents = [b - b % 2 if rng.random() < 0.5 else b for b in range(B)]
+    rng.shuffle(parents)
+    written = _i32(m.written)
+    want, _ = m.fork(parents)
+    assert fork_rows(pools, *state, _i32(parents), written=written).tolist() == [want]
+    assert state[0].tolist() == m.table and state[1].tolist() == m.lens and state[2].tolist() == m.refs
+
+
+def test_the_most_rows():
+    from tritonkv_amd.pages import fork_rows
+
+    m = Rows(8192, 3, 8192 * 4, 16)
+    m.fork(None, [48 if b % 2 == 0 else 0 for b in range(8192)])
+    for b in range(0, 8192, 2):
+        m.tokens[b] = [1] * (b % 33)
+    pools = [torch.zeros(m.N, 1, 16, 8, dtype=F16, device=DEV)]
+    state = _i32(m.table), _i32(m.lens), _i32(m.refs)
+    parents = [b - b % 2 for b in range(8192)]
+    written = _i32(m.written)
+    want, _ = m.fork(parents)
+    assert want == 0 and fork_rows(pools, *state, _i32(parents), written=written).tolist() == [0]
+    assert state[0].tolist() == m.table and state[1].tolist() == m.lens and state[2].tolist() == m.refs
