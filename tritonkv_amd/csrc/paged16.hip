@@ -29,8 +29,7 @@
 // 8192 in pages of 256, 64 and 16: 165, 166 and 172 us.  Small steps are bound by the two
 // launches and the chain of lengths, table, K and V: one row of 505 tokens (12 / 2 heads)
 // takes 6.8 us.
-#include "decode_common.h"
-#include "launch.h"
+#include "page_shares.h"
 
 namespace tkv {
 
@@ -79,181 +78,12 @@ __device__ __forceinline__ uint32_t infinities(uint32_t w) {
   return w & (lo | hi);
 }
 
-// ---------------------------------------------------------------------------
-// The split, made on the device from the rows' lengths.
-//
-// A serving loop's table is as wide as its longest request may get, and the
-// lengths live on the device, so a split of the table's capacity would leave
-// most pieces empty and the others uneven.  Instead the rows' chunks (32 tokens;
-// an empty row counts as one, which writes its zeros) are laid end to end, and the
-// W = min(workgroups, ceil(chunks / least_chunks)) workgroups of a KV head
-// take equal shares of that line, workgroup i the chunks from Shares::start(i) on.
-// (long_workgroups of them where that gives each long_chunks at least, in batches of
-// no more rows: fewer, longer streams then read faster; paged16.py has the figures.)
-// A share covers the end of one row, whole rows, and the start of another; each
-// such segment is attended by itself.  Whole rows are written out; the others
-// leave a partial in slot 2i (the row began in an earlier share) or 2i + 1, and
-// the join kernel merges a row's partials, which lie in consecutive shares.
-// workgroups == 0: one workgroup per row.
-//
-// Measured on 32 rows of 200-16184 tokens (HKV 8, G 4 / 8, D 128): pieces of one row
-// each, cut evenly, 184-194 us; shares 172 / 176; of 1000-16384 (G 8) 193 and 178.  8 rows of 300-4000 take 18.9 us in
-// tables of 131072 tokens and of 4032.
-// ---------------------------------------------------------------------------
-// What finds a workgroup's first segment: scalar arguments of the kernel, which are in
-// registers when a wave starts (a struct is not), so that the lengths are asked for at once.
-struct SharePlan {
-  const int32_t* lens;
-  int B, S, workgroups, least_chunks, long_workgroups, long_chunks;
-};
-
 struct Paged16Params {
   tkv_paged16_args a;
   int G, page_tiles;
   float qk_scale;  // sm_scale * log2(e)
   uint32_t k16[3], v16[3];  // the pools' strides in 16 bytes: products of 32 bits by 32
 };
-
-__device__ __forceinline__ int clamp_len(int L, int S) { return max(0, min(L, S)); }
-__device__ __forceinline__ uint32_t chunks_of(int L) { return max(1u, ((uint32_t)L + 31) / 32); }
-
-// Inclusive sum over the wave's lanes, on the VALU: four shifts within rows of 16
-// lanes, then the rows' totals passed on.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t add_dpp(uint32_t v) {
-  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-  v = add_dpp<0x111, 0xF>(v);  // row_shr:1
-  v = add_dpp<0x112, 0xF>(v);
-  v = add_dpp<0x114, 0xF>(v);
-  v = add_dpp<0x118, 0xF>(v);
-  v = add_dpp<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
-  return add_dpp<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
-}
-
-struct Shares {
-  uint32_t each, more;  // the first `more` shares hold each + 1 chunks
-  __device__ __forceinline__ uint32_t start(uint32_t i) const { return i * each + min(i, more); }
-  __device__ __forceinline__ uint32_t of(uint32_t chunk) const {
-    const uint32_t big = more * (each + 1);
-    return chunk < big ? chunk / (each + 1) : more + (chunk - big) / each;
-  }
-};
-
-// The rows' lengths, 64 of them in a wave's lanes at a time.
-struct RowLens {
-  const int32_t* lens;
-  int B, S, lane, first, L;
-  __device__ __forceinline__ void load(int b0) {
-    first = b0;
-    L = lens ? (b0 + lane < B ? clamp_len(lens[b0 + lane], S) : 0) : S;
-  }
-  __device__ __forceinline__ int of(int b) {  // b uniform
-    if (b >= first + 64) load(b);
-    return __builtin_amdgcn_readlane(L, b - first);
-  }
-};
-
-struct Segment {
-  int b, L;             // a row and its length
-  uint32_t begin, end;  // its chunks of this segment
-  uint32_t at;          // the row's first chunk on the line
-};
-
-// Chunks from which on every workgroup has its least (saturated).
-__device__ __forceinline__ uint32_t full_at(const SharePlan& a) {
-  const uint64_t n = (uint64_t)(uint32_t)a.workgroups * (uint32_t)a.least_chunks;
-  return n > 0xffffffffu ? 0xffffffffu : (uint32_t)n;
-}
-
-__device__ __forceinline__ Shares make_shares(uint32_t total, const SharePlan& a, uint32_t& W) {
-  W = a.workgroups;
-  if (a.B <= a.long_workgroups && total >= (uint32_t)a.long_workgroups * (uint32_t)a.long_chunks) W = a.long_workgroups;
-  else if (total < full_at(a)) W = min(W, (total + a.least_chunks - 1) / (uint32_t)a.least_chunks);
-  Shares s;
-  s.each = total / W;
-  s.more = total - s.each * W;
-  return s;
-}
-
-// This workgroup's first segment and the end of its share; false: it has none.
-__device__ __forceinline__ bool first_segment(const SharePlan& plan, int i, RowLens& rows, Shares& sh,
-                                              Segment& g, uint32_t& share_end) {
-  const int B = plan.B, lane = rows.lane;
-  if (plan.workgroups == 0) {
-    rows.load(i & ~63);
-    g.b = i;
-    g.L = rows.of(i);
-    g.begin = g.at = 0;
-    g.end = share_end = chunks_of(g.L);
-    sh.each = sh.more = 0;
-    return true;
-  }
-  rows.load(0);
-  uint32_t W;
-  if (!rows.lens || B == 1) {  // every row alike
-    const int L = rows.of(0);
-    const uint32_t l = chunks_of(L);
-    sh = make_shares(l * B, plan, W);
-    if ((uint32_t)i >= W) return false;
-    const uint32_t from = sh.start(i);
-    share_end = sh.start(i + 1);
-    g.b = from / l;
-    g.L = L;
-    g.at = g.b * l;
-    g.begin = from - g.at;
-    g.end = min(share_end - g.at, l);
-    return true;
-  }
-  // Up to 64 rows, which is most batches, one scan serves the sum and the search.
-  uint32_t l = lane < B ? chunks_of(rows.L) : 0, past = wave_scan(l);
-  uint32_t sum = __builtin_amdgcn_readlane((int)past, 63);
-  for (int b0 = 64; b0 < B; b0 += 64) {
-    rows.load(b0);
-    sum += __builtin_amdgcn_readlane((int)wave_scan(b0 + lane < B ? chunks_of(rows.L) : 0), 63);
-  }
-  sh = make_shares(sum, plan, W);
-  if ((uint32_t)i >= W) return false;
-  const uint32_t from = sh.start(i);
-  share_end = sh.start(i + 1);
-  uint32_t before = 0;
-  for (int b0 = 0; b0 < B; b0 += 64) {
-    if (B > 64) {
-      rows.load(b0);
-      l = b0 + lane < B ? chunks_of(rows.L) : 0;
-      past = wave_scan(l);
-    }
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(before + past > from);
-    if (hit) {
-      const int at = __builtin_ctzll(hit);
-      const uint32_t n = __builtin_amdgcn_readlane((int)l, at);
-      g.b = b0 + at;
-      g.L = __builtin_amdgcn_readlane(rows.L, at);
-      g.at = before + __builtin_amdgcn_readlane((int)past, at) - n;
-      g.begin = from - g.at;
-      g.end = min(share_end - g.at, n);
-      return true;
-    }
-    before += __builtin_amdgcn_readlane((int)past, 63);
-  }
-  return false;  // not reached: from < sum
-}
-
-// Where the partial of head h in a slot lives; maxima and sums after all rows.
-__device__ __forceinline__ int64_t partial_row(int HQ, uint32_t slot, int h) { return (int64_t)slot * HQ + h; }
-__device__ __forceinline__ float* partial_ml(float* partials, int workgroups, int HQ, int D) {
-  return partials + (int64_t)2 * workgroups * HQ * D;
-}
-
-__device__ __forceinline__ void store_row4(float* out, float* lse, int D, float shift, int64_t row, int d, f4 o,
-                                           float m, float l) {
-  // A row that saw nothing (no tokens, or scores of -inf alone) is zero.
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  *reinterpret_cast<f4*>(out + row * D + d) = o * inv;
-  if (lse && d == 0)
-    lse[row] = l == 0.0f ? -INFINITY : (m - shift + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
-}
 
 // ---------------------------------------------------------------------------
 // The split kernel.
@@ -641,61 +471,6 @@ paged16_split_kernel(const int32_t* lens, int B, int S, int workgroups, int leas
 }
 
 // ---------------------------------------------------------------------------
-// The join of rows that several workgroups shared; whole rows were written by the
-// split kernel.  LANES lanes take a (b, h): lane (g, dq) merges float4 column dq of
-// pieces g, g + SG, ..., and the SG groups meet in LDS.
-// Few rows have many pieces and take 256 lanes each; many rows have one to three
-// pieces each, and four of them share a workgroup.
-// ---------------------------------------------------------------------------
-template <int D, int LANES>
-__global__ void __launch_bounds__(256) paged16_join_kernel(const int2* row_pieces, float* partials, float* out,
-                                                           float* lse, int HQ, int rows, int workgroups, float shift) {
-  constexpr int DQ = D / 4, SG = LANES / DQ, ROWS = 256 / LANES;
-  __shared__ float sm_m[ROWS][SG], sm_l[ROWS][SG];
-  __shared__ f4 sm_a[ROWS][SG][DQ];
-  const int in = threadIdx.x / LANES, row0 = blockIdx.x * ROWS + in;
-  const bool live = row0 < rows;
-  const int b = live ? row0 / HQ : 0, h = row0 - b * HQ;
-  const int2 pieces = live ? row_pieces[b] : make_int2(0, 0);
-  if (ROWS == 1 && pieces.y <= 1) return;
-  const int t = threadIdx.x % LANES, dq = t % DQ, g = t / DQ;
-  const float* ml = partial_ml(partials, workgroups, HQ, D);
-  float m = -INFINITY, l = 0.0f;
-  f4 o = f4{0.f, 0.f, 0.f, 0.f};
-  const int n = pieces.y > 1 ? pieces.y : 0;
-#pragma unroll 4
-  for (int s = g; s < n; s += SG) {
-    const int64_t row = partial_row(HQ, 2 * (pieces.x + s) + (s == 0 ? 1 : 0), h);
-    const float2 x = *reinterpret_cast<const float2*>(ml + 2 * row);
-    const f4 os = *reinterpret_cast<const f4*>(partials + row * D + 4 * dq);
-    const float mn = fmaxf(m, x.x);
-    const float al = safe_exp2_diff(m, mn), be = safe_exp2_diff(x.x, mn);
-    o = o * al + os * be;
-    l = l * al + x.y * be;
-    m = mn;
-  }
-  if (dq == 0) {
-    sm_m[in][g] = m;
-    sm_l[in][g] = l;
-  }
-  sm_a[in][g][dq] = o;
-  __syncthreads();
-  if (g == 0 && n) {
-    float mstar = -INFINITY, lt = 0.0f;
-#pragma unroll
-    for (int x = 0; x < SG; ++x) mstar = fmaxf(mstar, sm_m[in][x]);
-    f4 ot = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int x = 0; x < SG; ++x) {
-      const float f = safe_exp2_diff(sm_m[in][x], mstar);
-      ot += sm_a[in][x][dq] * f;
-      lt += sm_l[in][x] * f;
-    }
-    store_row4(out, lse, D, shift, row0, 4 * dq, ot, mstar, lt);
-  }
-}
-
-// ---------------------------------------------------------------------------
 // Append: token n < counts[b] of row b's N goes to logical position
 // positions[b] + n, rounded to the pools' type once.  Thread = 8 dims of a (token,
 // head), two at a time, of K (even blockIdx.x) or V (odd) of row blockIdx.y; heads
@@ -761,23 +536,6 @@ __global__ void __launch_bounds__(256) paged16_append_kernel(tkv_paged16_append_
 // ---------------------------------------------------------------------------
 // Host side: validation and dispatch.
 // ---------------------------------------------------------------------------
-constexpr int kMaxPageTokens = 1 << 24;
-constexpr int kJoinRows = 512;  // (b, h) rows from which on the join takes a wave for each
-
-// Pool rows are read and written 16 bytes at a time; one 16-row tile spans 32 bits.
-static bool pool_ok(const void* p, const int64_t* strides) {
-  if (!p || (uintptr_t)p & 15) return false;
-  for (int i = 0; i < 3; ++i)
-    if (strides[i] < 0 || strides[i] % 8 || strides[i] / 8 > UINT32_MAX) return false;
-  return strides[2] > 0 && strides[2] < (int64_t(1) << 26);
-}
-static bool rows_ok(const void* p, const int64_t* strides, int n, int align) {
-  if ((uintptr_t)p & 15) return false;
-  for (int i = 0; i < n; ++i)
-    if (strides[i] % align) return false;
-  return true;
-}
-
 static int check_paged16(const tkv_paged16_args* a) {
   if (!a || !a->q || !a->out || !a->block_table) return TKV_EINVAL;
   if (a->B <= 0 || a->HQ <= 0 || a->HKV <= 0 || a->D <= 0 || a->HQ % a->HKV) return TKV_EINVAL;
@@ -785,10 +543,10 @@ static int check_paged16(const tkv_paged16_args* a) {
   if (a->page_size <= 0 || a->page_size % 16 || a->page_size > kMaxPageTokens || a->max_pages <= 0 ||
       a->num_pages <= 0 || a->block_table_stride < a->max_pages)
     return TKV_EINVAL;
-  if ((int64_t)a->max_pages * a->page_size > INT32_MAX - 65536) return TKV_EINVAL;
-  // the rows' chunks are summed in 32 bits
-  if ((int64_t)a->B * ((int64_t)a->max_pages * a->page_size / 32 + 1) > INT32_MAX) return TKV_EINVAL;
-  if (!pool_ok(a->k, a->k_strides) || !pool_ok(a->v, a->v_strides)) return TKV_EINVAL;
+  if (!shares_ok(a->B, a->max_pages, a->page_size, a->least_chunks, a->workgroups, a->long_workgroups, a->long_chunks,
+                 a->partials, a->row_pieces))
+    return TKV_EINVAL;
+  if (!pool_ok(a->k, a->k_strides, 8) || !pool_ok(a->v, a->v_strides, 8)) return TKV_EINVAL;
   if (!rows_ok(a->q, a->q_strides, 2, 8)) return TKV_EINVAL;
   if ((uintptr_t)a->out & 15) return TKV_EINVAL;
   if (a->k_new || a->v_new) {
@@ -796,14 +554,6 @@ static int check_paged16(const tkv_paged16_args* a) {
         !rows_ok(a->v_new, a->v_new_strides, 2, 8))
       return TKV_EINVAL;
   }
-  if (a->least_chunks <= 0 || a->workgroups < 0 || a->workgroups > 65535) return TKV_EINVAL;
-  if (a->long_workgroups < 0 || a->long_workgroups > a->workgroups || a->long_chunks < 0 ||
-      (int64_t)a->long_workgroups * a->long_chunks > INT32_MAX || (a->long_workgroups && !a->long_chunks))
-    return TKV_EINVAL;
-  if (!a->workgroups && a->B > 65535) return TKV_EINVAL;
-  if (a->workgroups && (!a->partials || (uintptr_t)a->partials & 15 || !a->row_pieces ||
-                        (uintptr_t)a->row_pieces & 7))
-    return TKV_EINVAL;
   if (a->D != 64 && a->D != 128 && a->D != 256) return TKV_EUNSUPPORTED;
   return TKV_OK;
 }
@@ -820,20 +570,11 @@ static int launch_paged16(const Paged16Params& p, hipStream_t st) {
                 p.a.max_pages * p.a.page_size, p.a.workgroups, p.a.least_chunks, p.a.long_workgroups, p.a.long_chunks, p);
 }
 
-template <int D>
-static int launch_join(const Paged16Params& p, float shift, hipStream_t st) {
-  const int rows = p.a.B * p.a.HQ;
-  const bool many = rows >= kJoinRows;
-  return launch(many ? paged16_join_kernel<D, 64> : paged16_join_kernel<D, 256>,
-                dim3((unsigned)(many ? (rows + 3) / 4 : rows)), dim3(256), 0, st,
-                reinterpret_cast<const int2*>(p.a.row_pieces), p.a.partials, p.a.out, p.a.lse, p.a.HQ, rows,
-                p.a.workgroups, shift);
-}
-
 template <class T, int D>
 static int dispatch_paged16(const Paged16Params& p, hipStream_t st) {
   const int rc = p.G <= 16 ? launch_paged16<T, D, 1>(p, st) : launch_paged16<T, D, 2>(p, st);
-  return rc || !p.a.workgroups ? rc : launch_join<D>(p, T::kShift, st);
+  if (rc || !p.a.workgroups) return rc;
+  return join_shares(D, p.a.B, p.a.HQ, p.a.workgroups, p.a.row_pieces, p.a.partials, p.a.out, p.a.lse, T::kShift, st);
 }
 
 template <class T>
@@ -868,7 +609,7 @@ extern "C" int tkv_paged16_append(const tkv_paged16_append_args* a, tkv_stream_t
   if (a->B <= 0 || a->HKV <= 0 || a->N <= 0 || a->D <= 0 || a->D % 8) return TKV_EINVAL;
   if (a->page_size <= 0 || a->max_pages <= 0 || a->num_pages <= 0 || a->block_table_stride < a->max_pages)
     return TKV_EINVAL;
-  if (!pool_ok(a->k, a->k_strides) || !pool_ok(a->v, a->v_strides)) return TKV_EINVAL;
+  if (!pool_ok(a->k, a->k_strides, 8) || !pool_ok(a->v, a->v_strides, 8)) return TKV_EINVAL;
   if (a->new_is_fp32 < TKV_NEW_SAME || a->new_is_fp32 > TKV_NEW_OTHER) return TKV_EINVAL;
   const int align = a->new_is_fp32 == TKV_NEW_FP32 ? 4 : 8;
   if (!rows_ok(a->k_new, a->k_new_strides, 3, align) || !rows_ok(a->v_new, a->v_new_strides, 3, align))
