@@ -385,6 +385,110 @@ typedef struct tkv_paged16_append_args {
 } tkv_paged16_append_args;
 int tkv_paged16_append(const tkv_paged16_append_args *args, tkv_stream_t stream);
 
+/* An 8-bit paged cache.  A pool is codes (num_pages, HKV, page_size, D), e4m3fn (largest 448)
+ * or int8 (largest 127), and fp32 scales (num_pages, HKV, page_size / block): token t of a
+ * page is code * scale[t / block].  block is 32, 64 or 128 and divides page_size; D is 64, 128
+ * or 256.  Code strides are in bytes, of page, head and token, multiples of 16 with D dense
+ * bytes a token; scale strides in floats, of page, head and block.  No counterpart in the
+ * reference, nor has tkv_rotary (it has 2 and 4 bits in contiguous caches, and leaves
+ * positions to the model). */
+enum { TKV_F16 = 0, TKV_BF16 = 1, TKV_F32 = 2 };
+
+/* Attention of the last tokens of every row over such pools; out and lse fp32.
+ *   q          (B, HQ, M, D) fp16, or bf16 with q_is_bf16, strides batch, head, query in
+ *              elements, multiples of 8; M at most 32
+ *   seq_lens   as in tkv_paged16_args
+ *   counts     NULL, or how many of row b's M queries there are, c_b (NULL: M): query m <
+ *              c_b is the row's token L_b - c_b + m and attends to itself and what is before
+ *              it; others get out = 0 and lse = -inf, as does one that attends to nothing
+ *   out        (B, HQ, M, D);  lse (B, HQ, M) or NULL
+ * A KV head's HQ / HKV * M queries are taken 16 at a time (32 where there are more than
+ * 16) by a workgroup.  The split is that of tkv_paged16_args, HQ * M in the place of HQ:
+ * partials holds 2 * workgroups * HQ * M * (D + 2) floats. */
+typedef struct tkv_paged8_args {
+  const void *q;
+  int64_t q_strides[3];
+  const void *k, *v;
+  int64_t k_strides[3], v_strides[3];
+  const float *k_scale, *v_scale;
+  int64_t k_scale_strides[3], v_scale_strides[3];
+  const int32_t *block_table, *seq_lens, *counts;
+  float *out, *lse, *partials;
+  int32_t *row_pieces;
+  int32_t is_int8, q_is_bf16, B, HQ, HKV, M, D;
+  int32_t block, block_table_stride, max_pages, page_size, num_pages;
+  float sm_scale;
+  int32_t least_chunks, workgroups, long_workgroups, long_chunks;
+} tkv_paged8_args;
+int tkv_paged8_decode_attention(const tkv_paged8_args *args, tkv_stream_t stream);
+
+/* K and V of N tokens per row, (B, HKV, N, D) in x_type (strides batch, head, token,
+ * multiples of 16 bytes), quantized into such pools: token n < counts[b] (NULL: N) of
+ * row b goes to position positions[b] + n, unless that lies outside [0, max_pages *
+ * page_size) or its table entry outside [0, num_pages).  A block whose first slot is written
+ * gets the least power of two s >= 2^-64 with |x| <= top * s over its new values (448 or 127;
+ * magnitudes above 2^64 count as 2^64, NaN does not count); one that is entered further in keeps
+ * its scale where that is larger (if it is positive and finite), and else the codes before the
+ * new ones are rounded again under s.  Codes are x / s to nearest even; int8 stores NaN as 0.
+ * inv_freq (NULL: none): radians per position of the dims / 2 pairs of a key's first dims values
+ * (a multiple of 16), which are turned before they are quantized, as by tkv_rotary at the
+ * tokens' positions; and with q, (B, HQ, N, D) in x_type, so are the queries, into q_out (rows
+ * past counts[b] are left alone; q_out may be q). */
+typedef struct tkv_paged8_append_args {
+  const void *k_new, *v_new;
+  int64_t k_new_strides[3], v_new_strides[3];
+  void *k, *v;
+  int64_t k_strides[3], v_strides[3];
+  float *k_scale, *v_scale;
+  int64_t k_scale_strides[3], v_scale_strides[3];
+  const int32_t *block_table, *positions, *counts;
+  const double *inv_freq;
+  const void *q;
+  void *q_out;
+  int64_t q_strides[3], q_out_strides[3];
+  float factor;
+  int32_t interleaved, dims, HQ;
+  int32_t is_int8, x_type, B, HKV, N, D;
+  int32_t block, block_table_stride, max_pages, page_size, num_pages;
+} tkv_paged8_append_args;
+int tkv_paged8_append(const tkv_paged8_append_args *args, tkv_stream_t stream);
+
+/* Tokens positions[b] (NULL: 0) to positions[b] + counts[b] - 1 (NULL: N of them) of row b as
+ * values of x_type, into k_out and v_out (B, HKV, N, D), strides batch, head, token in
+ * elements, multiples of 16 bytes.  Rows of the outputs past counts[b], and those of tokens
+ * outside the table or of entries outside the pool, are left alone. */
+typedef struct tkv_paged8_read_args {
+  const void *k, *v;
+  int64_t k_strides[3], v_strides[3];
+  const float *k_scale, *v_scale;
+  int64_t k_scale_strides[3], v_scale_strides[3];
+  void *k_out, *v_out;
+  int64_t k_out_strides[3], v_out_strides[3];
+  const int32_t *block_table, *positions, *counts;
+  int32_t is_int8, x_type, B, HKV, N, D;
+  int32_t block, block_table_stride, max_pages, page_size, num_pages;
+} tkv_paged8_read_args;
+int tkv_paged8_read(const tkv_paged8_read_args *args, tkv_stream_t stream);
+
+/* Rotary positions: the pairs (a, b) of a head's first dims values, (i, i + dims / 2) or,
+ * interleaved, (2i, 2i + 1), become factor * (a cos t - b sin t, a sin t + b cos t), t =
+ * inv_freq[i] times the token's position, in 64 bits; with adjoint they turn back
+ * (-t), which is the gradient's way.  q (B, HQ, N, D) and k (B, HKV, N, D; NULL: none) in x_type,
+ * strides batch, head, token in elements, multiples of 16 bytes; the outputs may be the inputs.
+ * Token n of row b has the position positions[b * position_strides[0] + n *
+ * position_strides[1]] + n * position_step.  D is a multiple of 16 and at most 256, dims even. */
+typedef struct tkv_rotary_args {
+  const void *q, *k;
+  void *q_out, *k_out;
+  int64_t q_strides[3], k_strides[3], q_out_strides[3], k_out_strides[3];
+  const int32_t *positions;
+  int64_t position_strides[2];
+  const double *inv_freq;
+  float factor;
+  int32_t position_step, x_type, interleaved, adjoint, B, HQ, HKV, N, D, dims;
+} tkv_rotary_args;
+int tkv_rotary(const tkv_rotary_args *args, tkv_stream_t stream);
+
 /* Page tensors that share page numbers: page p of tensor t is the `bytes[t]`
  * bytes at src[t] + p * src_stride[t], and a copy writes them at dst[t] + q *
  * dst_stride[t] (the same pointers and strides within one set of pools).

@@ -13,7 +13,10 @@ surface:
   through a block table (``paged_append``, ``paged_decode_attention``);
 * ``tritonkv_amd.paged16``: unquantized fp16 and bf16 page pools
   (``paged16_append``, ``paged16_decode_attention``);
-* ``tritonkv_amd.pages``: the pages of either kind, copied, forked, handed out,
+* ``tritonkv_amd.paged8``: 8-bit pages (e4m3 or int8) with a scale for each block of
+  tokens and head (``paged8_append``, ``paged8_read``, ``paged8_decode_attention``);
+* ``tritonkv_amd.rotary``: rotary positions of queries and keys (``apply_rotary``);
+* ``tritonkv_amd.pages``: the pages of any kind, copied, forked, handed out,
   taken back and compacted on the device (``copy_pages``, ``fork_rows``,
   ``resize_rows``, ``compact_pages``);
 * ``tritonkv_amd.channel``: per-channel (KIVI-style) keys with an fp16

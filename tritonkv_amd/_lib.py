@@ -137,6 +137,151 @@ class Paged16AppendArgs(ctypes.Structure):
     ]
 
 
+class Paged8Args(ctypes.Structure):
+    """Mirror of ``tkv_paged8_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_strides", ctypes.c_int64 * 3),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("k_scale_strides", ctypes.c_int64 * 3),
+        ("v_scale_strides", ctypes.c_int64 * 3),
+        ("block_table", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("partials", ctypes.c_void_p),
+        ("row_pieces", ctypes.c_void_p),
+        ("is_int8", ctypes.c_int32),
+        ("q_is_bf16", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("HQ", ctypes.c_int32),
+        ("HKV", ctypes.c_int32),
+        ("M", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("block", ctypes.c_int32),
+        ("block_table_stride", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("sm_scale", ctypes.c_float),
+        ("least_chunks", ctypes.c_int32),
+        ("workgroups", ctypes.c_int32),
+        ("long_workgroups", ctypes.c_int32),
+        ("long_chunks", ctypes.c_int32),
+    ]
+
+
+class Paged8AppendArgs(ctypes.Structure):
+    """Mirror of ``tkv_paged8_append_args``."""
+
+    _fields_ = [
+        ("k_new", ctypes.c_void_p),
+        ("v_new", ctypes.c_void_p),
+        ("k_new_strides", ctypes.c_int64 * 3),
+        ("v_new_strides", ctypes.c_int64 * 3),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("k_scale_strides", ctypes.c_int64 * 3),
+        ("v_scale_strides", ctypes.c_int64 * 3),
+        ("block_table", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("inv_freq", ctypes.c_void_p),
+        ("q", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("q_strides", ctypes.c_int64 * 3),
+        ("q_out_strides", ctypes.c_int64 * 3),
+        ("factor", ctypes.c_float),
+        ("interleaved", ctypes.c_int32),
+        ("dims", ctypes.c_int32),
+        ("HQ", ctypes.c_int32),
+        ("is_int8", ctypes.c_int32),
+        ("x_type", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("HKV", ctypes.c_int32),
+        ("N", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("block", ctypes.c_int32),
+        ("block_table_stride", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+    ]
+
+
+class Paged8ReadArgs(ctypes.Structure):
+    """Mirror of ``tkv_paged8_read_args``."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("k_scale_strides", ctypes.c_int64 * 3),
+        ("v_scale_strides", ctypes.c_int64 * 3),
+        ("k_out", ctypes.c_void_p),
+        ("v_out", ctypes.c_void_p),
+        ("k_out_strides", ctypes.c_int64 * 3),
+        ("v_out_strides", ctypes.c_int64 * 3),
+        ("block_table", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("is_int8", ctypes.c_int32),
+        ("x_type", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("HKV", ctypes.c_int32),
+        ("N", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("block", ctypes.c_int32),
+        ("block_table_stride", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    """Mirror of ``tkv_rotary_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        ("q_strides", ctypes.c_int64 * 3),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("q_out_strides", ctypes.c_int64 * 3),
+        ("k_out_strides", ctypes.c_int64 * 3),
+        ("positions", ctypes.c_void_p),
+        ("position_strides", ctypes.c_int64 * 2),
+        ("inv_freq", ctypes.c_void_p),
+        ("factor", ctypes.c_float),
+        ("position_step", ctypes.c_int32),
+        ("x_type", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("adjoint", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("HQ", ctypes.c_int32),
+        ("HKV", ctypes.c_int32),
+        ("N", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("dims", ctypes.c_int32),
+    ]
+
+
 PAGE_TENSORS = 32  # TKV_PAGE_TENSORS
 
 
@@ -257,6 +402,10 @@ SIGNATURES = {
     "tkv_dequantize": ([_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P], ctypes.c_int),
     "tkv_paged16_decode_attention": ([ctypes.POINTER(Paged16Args), _P], ctypes.c_int),
     "tkv_paged16_append": ([ctypes.POINTER(Paged16AppendArgs), _P], ctypes.c_int),
+    "tkv_paged8_decode_attention": ([ctypes.POINTER(Paged8Args), _P], ctypes.c_int),
+    "tkv_paged8_append": ([ctypes.POINTER(Paged8AppendArgs), _P], ctypes.c_int),
+    "tkv_paged8_read": ([ctypes.POINTER(Paged8ReadArgs), _P], ctypes.c_int),
+    "tkv_rotary": ([ctypes.POINTER(RotaryArgs), _P], ctypes.c_int),
     "tkv_copy_pages_work": ([ctypes.POINTER(CopyPagesArgs)], _I64),
     "tkv_copy_pages": ([ctypes.POINTER(CopyPagesArgs), _P], ctypes.c_int),
     "tkv_fork_rows_work": ([_I32, _I32, _I32, _I32], _I64),

@@ -1,0 +1,63 @@
+// Rotary positions of queries and keys, for gfx950.
+//
+// Every value is read and written once, for 6 flops a pair: bound by HBM.  A
+// workgroup takes a few tokens with all their heads, so that the angles, in 64 bits,
+// are worked out once a token and not once a head.
+#include "../../include/tkv.h"
+#include "launch.h"
+#include "rotary.h"
+
+namespace tkv {
+
+constexpr int kTurnThreads = 256;
+
+template <int T, bool VEC>
+__global__ void __launch_bounds__(kTurnThreads) rotary_kernel(TurnPlan p, TurnRows q, TurnRows k, int tile) {
+  extern __shared__ float2 turns[];
+  const uint32_t from = blockIdx.x * (uint32_t)tile;
+  const int tokens = (int)min((uint32_t)tile, (uint32_t)p.B * (uint32_t)p.N - from);
+  make_turns<kTurnThreads>(p, from, tokens, turns);
+  __syncthreads();
+  turn_tokens<T, VEC, kTurnThreads>(p, q, from, tokens, turns);
+  if (k.x) turn_tokens<T, VEC, kTurnThreads>(p, k, from, tokens, turns);
+}
+
+static bool rows_aligned(const void* p, const int64_t* strides, int align) {
+  return !((uintptr_t)p & 15) && !(strides[0] % align) && !(strides[1] % align) && !(strides[2] % align);
+}
+
+}  // namespace tkv
+
+extern "C" int tkv_rotary(const tkv_rotary_args* a, tkv_stream_t stream) {
+  using namespace tkv;
+  if (!a || !a->q || !a->q_out || !a->positions || !a->inv_freq || !a->k != !a->k_out) return TKV_EINVAL;
+  if (a->B <= 0 || a->HQ <= 0 || (a->k && a->HKV <= 0) || a->N <= 0 || a->D <= 0 || a->D % 16 || a->D > 256)
+    return TKV_EINVAL;
+  if (a->dims <= 0 || a->dims % 2 || a->dims > a->D || a->x_type < TKV_F16 || a->x_type > TKV_F32) return TKV_EINVAL;
+  if ((int64_t)a->B * a->N > INT32_MAX || a->HQ > 65535 || (a->k && a->HKV > 65535)) return TKV_EINVAL;
+  const int align = a->x_type == TKV_F32 ? 4 : 8;
+  if (!rows_aligned(a->q, a->q_strides, align) || !rows_aligned(a->q_out, a->q_out_strides, align)) return TKV_EINVAL;
+  if (a->k && (!rows_aligned(a->k, a->k_strides, align) || !rows_aligned(a->k_out, a->k_out_strides, align)))
+    return TKV_EINVAL;
+  TurnPlan p{a->positions, {a->position_strides[0], a->position_strides[1]}, a->position_step, nullptr, a->inv_freq,
+             a->factor, a->adjoint ? -a->factor : a->factor, a->interleaved, a->dims, a->D, a->N, a->B};
+  auto rows = [&](const void* x, void* out, const int64_t* xs, const int64_t* os, int H) {
+    return TurnRows{x, out, {xs[0], xs[1], xs[2]}, {os[0], os[1], os[2]}, H, xs[1] < xs[2]};
+  };
+  const TurnRows q = rows(a->q, a->q_out, a->q_strides, a->q_out_strides, a->HQ),
+                 k = rows(a->k, a->k_out, a->k_strides, a->k_out_strides, a->k ? a->HKV : 0);
+  const int64_t total = (int64_t)a->B * a->N;
+  const int tile = total >= 8192 ? 8 : 1;
+  const bool vec = a->interleaved || a->dims % 16 == 0;
+  const dim3 grid((unsigned)((total + tile - 1) / tile));
+  const size_t lds = sizeof(float2) * tile * (a->dims / 2);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  auto start = [&](auto type) {
+    constexpr int T = decltype(type)::value;
+    return launch(vec ? rotary_kernel<T, true> : rotary_kernel<T, false>, grid, dim3(kTurnThreads), lds, st, p, q, k,
+                  tile);
+  };
+  return a->x_type == TKV_F16    ? start(std::integral_constant<int, kF16>{})
+         : a->x_type == TKV_BF16 ? start(std::integral_constant<int, kBf16>{})
+                                 : start(std::integral_constant<int, kF32>{});
+}

@@ -2,7 +2,8 @@
 
 A paged cache is page pools (of any layer, K and V; 2/4-bit
 :class:`~tritonkv_amd.quantize.QuantizedTensor` pools of
-:mod:`tritonkv_amd.paged` or 16-bit tensors of :mod:`tritonkv_amd.paged16`)
+:mod:`tritonkv_amd.paged`, 8-bit ones of :mod:`tritonkv_amd.paged8` or 16-bit tensors of
+:mod:`tritonkv_amd.paged16`)
 that share page numbers, and three int32 tensors that say which row owns what:
 
 * ``block_table`` ``(B, max_pages)``: row b's pages in order, -1 after them;
@@ -31,6 +32,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from .paged8 import Paged8Pool
 from .paged16 import _buffer, _int32_arg, _keep16, _offset
 from .kernels.fused_decode_attn import _prepared
 from .quantize import QuantizedTensor, _require_gpu
@@ -41,22 +43,24 @@ MAX_PAGES = 2 ** 30
 
 def _tensors(pools) -> list:
     """The page tensors of pools, in order."""
-    if isinstance(pools, (QuantizedTensor, torch.Tensor)):
+    if isinstance(pools, (QuantizedTensor, Paged8Pool, torch.Tensor)):
         raise TypeError("pools must be a list or tuple of page pools")
     found = []
     for p in pools:
         if isinstance(p, QuantizedTensor):
             found += [p.packed, p.scale, p.zero]
+        elif isinstance(p, Paged8Pool):
+            found += p.page_tensors()
         elif isinstance(p, torch.Tensor):
             found.append(p)
         else:
-            raise TypeError(f"a page pool is a QuantizedTensor or a tensor, got {type(p).__name__}")
+            raise TypeError(f"a page pool is a QuantizedTensor, a Paged8Pool or a tensor, got {type(p).__name__}")
     return found
 
 
 def _page_size(pools) -> int:
-    sizes = {(p.packed if isinstance(p, QuantizedTensor) else p).shape[2] for p in pools
-             if (p.packed if isinstance(p, QuantizedTensor) else p).dim() == 4}
+    pages = [p.packed if isinstance(p, QuantizedTensor) else p.codes if isinstance(p, Paged8Pool) else p for p in pools]
+    sizes = {p.shape[2] for p in pages if p.dim() == 4}
     if len(sizes) != 1:
         raise ValueError(f"the pools must be (num_pages, HKV, page_size, ...) of one page_size, got {sorted(sizes)}")
     return sizes.pop()
