@@ -19,6 +19,8 @@
 // scaled by a power of two each, so that their largest value lies in [2^14, 2^15):
 // exact for what is over 2^-30 of it.  P enters as two fp16 terms (22 bits).  A block's
 // scale of V multiplies its chunks' product in fp32, one of K the scores.
+#include <algorithm>
+
 #include "page_shares.h"
 #include "rotary.h"
 
@@ -261,7 +263,10 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
     auto step = [&](int c, int cb, auto tail) {
       constexpr bool TAIL = decltype(tail)::value;
       const bool more = cb + 32 * NW < hi;
-      float x[HT][8];
+      float x[HT][8], f[HT];  // scores, and what they are in powers of two
+      auto hidden = [&](int ht, int i) {
+        return TAIL && cb + slot_token(j, i) > (MULTI ? min(last, seen[ht] - 1) : last);
+      };
       {
         // (opaque: read again in every chunk, not kept in registers)
         const uint16_t* ql = lds_q + (int)opaque((uint32_t)(r * QROW + 16 * j));
@@ -288,17 +293,10 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
           }
 #pragma unroll
         for (int ht = 0; ht < HT; ++ht) {
-          const float f = ks * qs[ht];
+          f[ht] = ks * qs[ht];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[ht][i] = s[ht][i / 4][i % 4] * f;
+          for (int i = 0; i < 8; ++i) x[ht][i] = s[ht][i / 4][i % 4];
         }
-      }
-      if constexpr (TAIL) {
-#pragma unroll
-        for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (cb + slot_token(j, i) > (MULTI ? min(last, seen[ht] - 1) : last)) x[ht][i] = -INFINITY;
       }
       if (!TAIL && more) {
         if (((c + 1) & 63) == 0) chunks(c + 1);  // V of chunk c is on its way already, its scale in vs
@@ -309,9 +307,9 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
       u4 pt[HT][2];
 #pragma unroll
       for (int ht = 0; ht < HT; ++ht) {
-        float top = x[ht][0];
+        float top = -INFINITY;
 #pragma unroll
-        for (int i = 1; i < 8; ++i) top = fmaxf(top, x[ht][i]);
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, hidden(ht, i) ? -INFINITY : x[ht][i] * f[ht]);
         if (__builtin_amdgcn_ballot_w64(top > m_run[ht]) != 0) {
           const float mn = vmax(m_run[ht], xor_max16_32(top));
           const float alpha = safe_exp2_diff(m_run[ht], mn);
@@ -320,12 +318,13 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
 #pragma unroll
           for (int mv = 0; mv < EPL; ++mv) accv[ht][mv] *= alpha;
         }
-        // scores of -inf under a maximum of -inf give p = 0, not NaN
+        // Scores of -inf under a maximum of -inf give p = 0, not NaN.  The product is not rounded
+        // before the maximum is off: at scores of 32 and more that alone was 1.3e-6 of p.
         const float off = kShift8 - (m_run[ht] == -INFINITY ? 0.0f : m_run[ht]);
         float p[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(x[ht][i] + off);
+          p[i] = hidden(ht, i) ? 0.0f : __builtin_amdgcn_exp2f(fmaf(x[ht][i], f[ht], off));
           l_run[ht] += p[i];
         }
 #pragma unroll
@@ -485,9 +484,10 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
 // ---------------------------------------------------------------------------
 // Append: token n < counts[b] of row b goes to position positions[b] + n.
 //
-// A workgroup takes a KV head's tokens of one block of the row, of K or V: their values stay
-// in registers from the load over the block's largest magnitude to the codes, so each is
-// read and written once.  The scale is the least power of two s with |x| <= top * s, or the block's
+// A workgroup takes the tokens of one block of the row, of K or V, of a few KV heads in
+// turn: a head's values stay in registers from the load over the block's largest magnitude to the
+// codes, so each is read and written once, and the turns of its keys are worked out once for
+// the heads.  The scale is the least power of two s with |x| <= top * s, or the block's
 // own where that is larger: by powers of two nothing is rounded twice in e4m3 (but what
 // falls under its smallest normal code), and a scale rises seldom.  Where it rises, the
 // codes of the block's earlier tokens are rounded again under the new one.
@@ -496,6 +496,9 @@ struct Append8Params {
   tkv_paged8_append_args a;
   TurnPlan turn;
   TurnRows q;
+  uint32_t kv_groups;    // workgroups of K and V per row; those of the queries follow
+  int heads;             // of a workgroup of K or V
+  int q_tile, q_parts;   // tokens of a workgroup of queries, and the workgroups that share their heads
 };
 
 constexpr float kLargest = 18446744073709551616.0f;  // 2^64
@@ -524,148 +527,218 @@ __device__ __forceinline__ void over_scale(float* y, float s) {
 // Whether a scale can be a block's: positive and finite.
 __device__ __forceinline__ bool is_scale(float s) { return s > 0.0f && s < INFINITY; }
 
-template <class C, int T, int D, int ITEMS>
+// The largest of the wave's values, in every lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t max_dpp(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = max_dpp<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+  v = max_dpp<0x112, 0xF>(v);
+  v = max_dpp<0x114, 0xF>(v);
+  v = max_dpp<0x118, 0xF>(v);
+  v = max_dpp<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  v = max_dpp<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+template <class C, int T, int D, int ITEMS, bool ROT>
 __global__ void __launch_bounds__(1024) paged8_append_kernel(Append8Params prm) {
   const tkv_paged8_append_args& a = prm.a;
   constexpr int PER = D / 16;
+  extern __shared__ float2 lds_turns[];
+  __shared__ uint32_t tops[2][16];
   const int b = blockIdx.y, tid = threadIdx.x;
+  if constexpr (ROT)
+    if (blockIdx.x >= prm.kv_groups) {
+      const int at = (int)(blockIdx.x - prm.kv_groups), n0 = at / prm.q_parts * prm.q_tile;
+      const auto token = [&](int i) { return make_int2(b, n0 + i); };
+      const int tokens = min(prm.q_tile, a.N - n0), part = at % prm.q_parts;
+      if (prm.q_tile > 1) turn_tokens<T, true, true>(prm.turn, prm.q, TurnRows{}, tokens, part, prm.q_parts, lds_turns, token);
+      else turn_tokens<T, true, false>(prm.turn, prm.q, TurnRows{}, tokens, part, prm.q_parts, lds_turns, token);
+      return;
+    }
   const int64_t pos = a.positions[b], room = (int64_t)a.max_pages * a.page_size;
   const int count = a.counts ? min(a.counts[b], a.N) : a.N;
-  const uint32_t of = blockIdx.x / (2 * (uint32_t)a.HKV), hv = blockIdx.x - of * (2 * (uint32_t)a.HKV);
+  const uint32_t sets = (uint32_t)((a.HKV + prm.heads - 1) / prm.heads), of = blockIdx.x / (2 * sets),
+                 hv = blockIdx.x - of * (2 * sets);
   const bool isv = hv & 1;
-  const int h = (int)(hv >> 1);
+  const int h0 = (int)(hv >> 1) * prm.heads, h1 = min(h0 + prm.heads, a.HKV);
   const int64_t begin = max(pos, (int64_t)0), end = min(pos + count, room);
   const int64_t base = (begin / a.block + of) * a.block;  // the block's first position
   const int64_t t0 = max(begin, base), t1 = min(end, base + a.block);
   if (t0 >= t1) return;
+  const int rows = (int)(t1 - t0), first = (int)(t0 - base);
+  const int64_t* const xs = isv ? a.v_new_strides : a.k_new_strides;
+  const char* x = static_cast<const char*>(isv ? a.v_new : a.k_new) +
+                  (b * xs[0] + h0 * xs[1] + (t0 - pos) * xs[2]) * kBytes<T>;
+  const bool turned = ROT && !isv;
+  const bool interleaved = prm.turn.interleaved;
+  const int dims = turned ? prm.turn.dims : 0;
+  Raw8<T> raw[ITEMS][2];
+  auto load = [&](const char* x) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int u = tid + i * (int)blockDim.x, row = u / PER, e = u % PER;
+      if (row >= rows) continue;
+      const Places pl(e, dims, interleaved, D);
+      raw[i][0].template load<true>(x + (row * xs[2] + pl.first) * kBytes<T>);
+      raw[i][1].template load<true>(x + (row * xs[2] + pl.second) * kBytes<T>);
+    }
+  };
+  load(x);  // (under way before the table is known)
   const uint32_t pg = (uint32_t)((uint64_t)base / (uint32_t)a.page_size);
   const int page = a.block_table[(int64_t)b * a.block_table_stride + pg];
   if (page < 0 || page >= a.num_pages) return;
-  const int rows = (int)(t1 - t0), first = (int)(t0 - base), at = (int)(base - (int64_t)pg * a.page_size);
-  float* const sp = (isv ? a.v_scale : a.k_scale) + page * (isv ? a.v_scale_strides : a.k_scale_strides)[0] +
-                    h * (isv ? a.v_scale_strides : a.k_scale_strides)[1] +
-                    at / a.block * (isv ? a.v_scale_strides : a.k_scale_strides)[2];
-  const float held = *sp;
-  const int64_t* const xs = isv ? a.v_new_strides : a.k_new_strides;
+  const int at = (int)(base - (int64_t)pg * a.page_size);
+  const int64_t* const ss = isv ? a.v_scale_strides : a.k_scale_strides;
   const int64_t* const ps = isv ? a.v_strides : a.k_strides;
-  const char* const x = static_cast<const char*>(isv ? a.v_new : a.k_new) +
-                        (b * xs[0] + h * xs[1] + (t0 - pos) * xs[2]) * kBytes<T>;
-  uint8_t* const to = static_cast<uint8_t*>(isv ? a.v : a.k) + page * ps[0] + h * ps[1] + at * ps[2];
-  const int dims = isv ? 0 : prm.turn.dims;
-  const bool interleaved = prm.turn.interleaved;
-
-  float y[ITEMS][16];
-  float top = 0.0f;
+  float* sp = (isv ? a.v_scale : a.k_scale) + page * ss[0] + h0 * ss[1] + at / a.block * ss[2];
+  uint8_t* to = static_cast<uint8_t*>(isv ? a.v : a.k) + page * ps[0] + h0 * ps[1] + at * ps[2];
+  Turns my[ITEMS];
+  if (turned)
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const int u = tid + i * (int)blockDim.x, row = u / PER, e = u % PER;
-    if (row >= rows) continue;
-    const Places pl(e, dims, interleaved);
-    load8<T>(x + (row * xs[2] + pl.first) * kBytes<T>, y[i]);
-    load8<T>(x + (row * xs[2] + pl.second) * kBytes<T>, y[i] + 8);
-    if (dims)
-      turn16(y[i], e, dims, interleaved, [&](int pair) {
-        const float2 t = turn_of((double)(t0 + row), prm.turn.inv_freq[pair]);
-        return make_float2(t.x * prm.turn.factor, t.y * prm.turn.sin_factor);
+    for (int i = 0; i < ITEMS; ++i) {
+      const int u = tid + i * (int)blockDim.x, row = u / PER, e = u % PER;
+      my[i].set(e, row < rows ? dims : 0, interleaved, D, [&](const int* pair, float2* t) {
+        double w[8];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) w[n] = prm.turn.inv_freq[pair[n]];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          t[n] = turn_of((double)(t0 + row), w[n]);
+          t[n] = make_float2(t[n].x * prm.turn.factor, t[n].y * prm.turn.sin_factor);
+        }
       });
-#pragma unroll
-    for (int d = 0; d < 16; ++d) {
-      // (comparisons, which leave a NaN as it is; it does not count for the scale)
-      y[i][d] = y[i][d] > kLargest ? kLargest : y[i][d] < -kLargest ? -kLargest : y[i][d];
-      top = fmaxf(top, fabsf(y[i][d]));
     }
-  }
-  __shared__ float tops[16];
+
+  for (int h = h0; h < h1; ++h, sp += ss[1], to += ps[1]) {
+    const float held = first ? *sp : 0.0f;
+    float y[ITEMS][16];
+    float top = 0.0f;
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-  if (blockDim.x > 64) {
-    if ((tid & 63) == 0) tops[tid >> 6] = top;
-    __syncthreads();
-    for (int i = 0; i < (int)blockDim.x / 64; ++i) top = fmaxf(top, tops[i]);
-  }
-  const bool known = first > 0 && is_scale(held);
-  const float need = least_scale<C>(top), scale = known ? fmaxf(held, need) : need;
-  if (tid == 0) *sp = scale;
-  if (known && scale > held) {
-    const float ratio = held / scale;
-    for (int u = tid; u < first * PER; u += blockDim.x) {
-      u4* const p = reinterpret_cast<u4*>(to + (u / PER) * ps[2] + 16 * (u % PER));
-      u4 c = *p;
+    for (int i = 0; i < ITEMS; ++i) {
+      if ((tid + i * (int)blockDim.x) / PER >= rows) continue;
+      raw[i][0].values(y[i]);
+      raw[i][1].values(y[i] + 8);
+      if (turned) my[i].turn(y[i], interleaved);
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        float z[4];
-        C::values(c[d], z);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) z[n] *= ratio;
-        c[d] = C::codes(z);
+      for (int d = 0; d < 16; ++d) {
+        // (comparisons, which leave a NaN as it is; it does not count for the scale)
+        if (T != kF16) y[i][d] = y[i][d] > kLargest ? kLargest : y[i][d] < -kLargest ? -kLargest : y[i][d];
+        top = fmaxf(top, fabsf(y[i][d]));
       }
-      *p = c;
+    }
+    if (h + 1 < h1) load(x += xs[1] * kBytes<T>);
+    uint32_t most = wave_max(__builtin_bit_cast(uint32_t, top));
+    if (blockDim.x > 64) {
+      uint32_t* const all = tops[h & 1];  // (of two heads in turn: one barrier a head)
+      if ((tid & 63) == 0) all[tid >> 6] = most;
+      __syncthreads();
+      for (int i = 0; i < (int)blockDim.x / 64; ++i) most = max(most, all[i]);
+    }
+    const bool known = first > 0 && is_scale(held);
+    const float need = least_scale<C>(__builtin_bit_cast(float, most)), scale = known ? fmaxf(held, need) : need;
+    if (tid == 0) *sp = scale;
+    if (known && scale > held) {
+      const float ratio = held / scale;
+      for (int u = tid; u < first * PER; u += blockDim.x) {
+        u4* const p = reinterpret_cast<u4*>(to + (u / PER) * ps[2] + 16 * (u % PER));
+        u4 c = *p;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          float z[4];
+          C::values(c[d], z);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) z[n] *= ratio;
+          c[d] = C::codes(z);
+        }
+        *p = c;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int u = tid + i * (int)blockDim.x, row = u / PER, e = u % PER;
+      if (row >= rows) continue;
+      const Places pl(e, dims, interleaved, D);
+      over_scale<16>(y[i], scale);
+      uint8_t* const p = to + (first + row) * ps[2];
+      __builtin_nontemporal_store(u2{C::codes(y[i]), C::codes(y[i] + 4)}, reinterpret_cast<u2*>(p + pl.first));
+      __builtin_nontemporal_store(u2{C::codes(y[i] + 8), C::codes(y[i] + 12)}, reinterpret_cast<u2*>(p + pl.second));
     }
   }
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const int u = tid + i * (int)blockDim.x, row = u / PER, e = u % PER;
-    if (row >= rows) continue;
-    const Places pl(e, dims, interleaved);
-    over_scale<16>(y[i], scale);
-    uint8_t* const p = to + (first + row) * ps[2];
-    const u2 c0 = u2{C::codes(y[i]), C::codes(y[i] + 4)}, c1 = u2{C::codes(y[i] + 8), C::codes(y[i] + 12)};
-    *reinterpret_cast<u2*>(p + pl.first) = c0;
-    *reinterpret_cast<u2*>(p + pl.second) = c1;
-  }
-}
-
-// The queries of an append with rotary positions.
-template <int T>
-__global__ void __launch_bounds__(256) paged8_turn_queries_kernel(TurnPlan p, TurnRows q, int tile) {
-  extern __shared__ float2 turns[];
-  const uint32_t from = blockIdx.x * (uint32_t)tile;
-  const int tokens = (int)min((uint32_t)tile, (uint32_t)p.B * (uint32_t)p.N - from);
-  make_turns<256>(p, from, tokens, turns);
-  __syncthreads();
-  turn_tokens<T, true, 256>(p, q, from, tokens, turns);
 }
 
 // ---------------------------------------------------------------------------
-// Read: tokens positions[b] .. positions[b] + counts[b] - 1 of row b as values, 16 dims of K
-// (even blockIdx.x) or V (odd) per thread.
+// Read: tokens positions[b] .. positions[b] + counts[b] - 1 of row b as values.
+//
+// A workgroup takes 32 slots of a page (one block, so that page and scale are the same for all of
+// its threads) of K or V, of one or two heads; an item is 16 bytes of output, and a thread asks for
+// eight before it writes any.  Workgroups follow each other along the tokens of a head.
 // ---------------------------------------------------------------------------
-template <class C, int T>
-__global__ void __launch_bounds__(256) paged8_read_kernel(tkv_paged8_read_args a, uint32_t items, int heads_first) {
-  const bool isv = blockIdx.x & 1;
+template <class C, int T, int D>
+__global__ void __launch_bounds__(256) paged8_read_kernel(tkv_paged8_read_args a, int heads) {
+  constexpr int DIMS = 16 / kBytes<T>, PER = D / DIMS, ITEMS = 32 * PER / 256;
+  constexpr int HEADS = ITEMS >= 8 ? 1 : 8 / ITEMS;  // under way at once
   const int b = blockIdx.y;
-  const uint32_t u = (blockIdx.x >> 1) * 256 + threadIdx.x;
-  if (u >= items) return;
-  const uint32_t per = (uint32_t)a.D / 16, rest = u / per, e = u - rest * per;
-  uint32_t n, h;
-  if (heads_first) {
-    n = rest / (uint32_t)a.HKV;
-    h = rest - n * (uint32_t)a.HKV;
-  } else {
-    h = rest / (uint32_t)a.N;
-    n = rest - h * (uint32_t)a.N;
-  }
-  if (a.counts && (int)n >= a.counts[b]) return;
-  const int64_t t = (a.positions ? (int64_t)a.positions[b] : 0) + n;
-  if (t < 0 || t >= (int64_t)a.max_pages * a.page_size) return;
-  const uint32_t pg = (uint32_t)t / (uint32_t)a.page_size, at = (uint32_t)t - pg * (uint32_t)a.page_size;
+  const uint32_t sets = (uint32_t)((a.HKV + heads - 1) / heads), blocks = gridDim.x / (2 * sets),
+                 hv = blockIdx.x / blocks, of = blockIdx.x - hv * blocks;
+  const bool isv = hv & 1;
+  const int h0 = (int)(hv >> 1) * heads, h1 = min(h0 + heads, a.HKV);
+  const int64_t pos = a.positions ? (int64_t)a.positions[b] : 0, begin = max(pos, (int64_t)0);
+  const int64_t end = min(pos + (a.counts ? min(a.counts[b], a.N) : a.N), (int64_t)a.max_pages * a.page_size);
+  const int64_t base = (begin / 32 + of) * 32, t0 = max(begin, base), t1 = min(end, base + 32);
+  if (t0 >= t1) return;
+  const uint32_t pg = (uint32_t)((uint64_t)base / (uint32_t)a.page_size);
   const int page = a.block_table[(int64_t)b * a.block_table_stride + pg];
   if (page < 0 || page >= a.num_pages) return;
+  const int at = (int)(base - (int64_t)pg * a.page_size), first = (int)(t0 - base), last = (int)(t1 - base);
   const int64_t* const ps = isv ? a.v_strides : a.k_strides;
   const int64_t* const ss = isv ? a.v_scale_strides : a.k_scale_strides;
   const int64_t* const os = isv ? a.v_out_strides : a.k_out_strides;
-  const float s = (isv ? a.v_scale : a.k_scale)[page * ss[0] + h * ss[1] + (int64_t)(at / (uint32_t)a.block) * ss[2]];
-  const u4 c = *reinterpret_cast<const u4*>(static_cast<const uint8_t*>(isv ? a.v : a.k) + page * ps[0] + h * ps[1] +
-                                            at * ps[2] + 16 * e);
-  float y[16];
+  const float* const s = (isv ? a.v_scale : a.k_scale) + page * ss[0] + at / a.block * ss[2];
+  const uint8_t* const p = static_cast<const uint8_t*>(isv ? a.v : a.k) + page * ps[0] + at * ps[2];
+  char* const o = static_cast<char*>(isv ? a.v_out : a.k_out) + (b * os[0] + (base - pos) * os[2]) * kBytes<T>;
+  for (int h = h0; h < h1; h += HEADS) {
+    u2 c[HEADS][ITEMS];
+    float f[HEADS];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) C::values(c[i], y + 4 * i);
+    for (int n = 0; n < HEADS; ++n) {
+      if (h + n >= h1) break;
+      f[n] = s[(h + n) * ss[1]];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) y[i] *= s;
-  char* const o = static_cast<char*>(isv ? a.v_out : a.k_out) +
-                  (b * os[0] + h * os[1] + n * os[2] + 16 * e) * kBytes<T>;
-  store8<T>(o, y);
-  store8<T>(o + 8 * kBytes<T>, y + 8);
+      for (int i = 0; i < ITEMS; ++i) {
+        const int u = (int)threadIdx.x + 256 * i, slot = u / PER, e = u % PER;
+        if (slot < first || slot >= last) continue;
+        const uint8_t* const q = p + (h + n) * ps[1] + slot * ps[2] + DIMS * e;
+        if constexpr (DIMS == 8) c[n][i] = __builtin_nontemporal_load(reinterpret_cast<const u2*>(q));
+        else c[n][i][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(q));
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < HEADS; ++n) {
+      if (h + n >= h1) break;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const int u = (int)threadIdx.x + 256 * i, slot = u / PER, e = u % PER;
+        if (slot < first || slot >= last) continue;
+        float y[8];
+        u4 w;
+        C::values(c[n][i][0], y);
+        if constexpr (DIMS == 8) {
+          C::values(c[n][i][1], y + 4);
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            w[x] = T == kF16 ? pack_h2(y[2 * x] * f[n], y[2 * x + 1] * f[n])
+                             : pack_bf2(y[2 * x] * f[n], y[2 * x + 1] * f[n]);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) w[x] = __builtin_bit_cast(uint32_t, y[x] * f[n]);
+        }
+        __builtin_nontemporal_store(w, reinterpret_cast<u4*>(o + ((h + n) * os[1] + slot * os[2] + DIMS * e) * kBytes<T>));
+      }
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -711,29 +784,41 @@ static int dispatch_paged8(const Paged8Params& p, hipStream_t st) {
   return dispatch_paged8<C, 256>(p, st);
 }
 
-template <class C, int T, int D>
-static int launch_append8(const Append8Params& p, hipStream_t st) {
+template <class C, int T, int D, bool ROT>
+static int launch_append8(Append8Params p, hipStream_t st) {
   const tkv_paged8_append_args& a = p.a;
+  constexpr int PER = D / 16;
   // Few tokens: a wave holds them all.  Else a thread for 16 values of a block, or for 32 of the
   // largest block of the largest heads.
-  const bool few = a.N * (D / 16) <= 64;
-  const int items = a.block * (D / 16), threads = few ? 64 : items < 1024 ? items : 1024;
+  const bool few = a.N * (int64_t)PER <= 64;
+  const int items = a.block * PER, threads = few ? 64 : items < 1024 ? items : 1024;
   const int64_t blocks = ((int64_t)a.N + a.block - 2) / a.block + 1;  // that N tokens may touch
-  const dim3 grid((unsigned)(blocks * 2 * a.HKV), (unsigned)a.B);
-  const auto kernel = !few && items > 1024 ? paged8_append_kernel<C, T, D, 2> : paged8_append_kernel<C, T, D, 1>;
-  const int rc = launch(kernel, grid, dim3((unsigned)threads), 0, st, p);
-  if (rc || !p.q.x) return rc;
-  const int64_t total = (int64_t)a.B * a.N;
-  const int tile = total >= 8192 ? 8 : 1;
-  return launch(paged8_turn_queries_kernel<T>, dim3((unsigned)((total + tile - 1) / tile)), dim3(256),
-                sizeof(float2) * tile * (p.turn.dims / 2), st, p.turn, p.q, tile);
+  p.heads = a.HKV > 1 && blocks * a.B * a.HKV > 1024 ? 2 : 1;
+  const int sets = (a.HKV + p.heads - 1) / p.heads;
+  int64_t groups = blocks * 2 * sets;
+  p.kv_groups = (uint32_t)groups;
+  size_t lds = 0;
+  if (p.q.x) {
+    const int64_t total = (int64_t)a.B * a.N;
+    p.q_tile = total >= kTurnMany ? std::min(kTurnTile * std::max(1, threads / 256), threads / PER) : 1;
+    const int lanes = threads / (p.q_tile * PER);
+    p.q_parts = total < kTurnFew ? (p.q.H + lanes - 1) / lanes : 1;
+    groups += ((int64_t)a.N + p.q_tile - 1) / p.q_tile * p.q_parts;
+    lds = sizeof(float2) * p.q_tile * (p.turn.dims / 2);
+  }
+  if (groups > INT32_MAX) return TKV_EINVAL;
+  auto kernel = paged8_append_kernel<C, T, D, 1, ROT>;
+  if constexpr (D == 256)
+    if (!few && items > 1024) kernel = paged8_append_kernel<C, T, D, 2, ROT>;
+  return launch(kernel, dim3((unsigned)groups, (unsigned)a.B), dim3((unsigned)threads), lds, st, p);
 }
 
 template <class C, int T>
 static int dispatch_append8(const Append8Params& p, hipStream_t st) {
-  if (p.a.D == 64) return launch_append8<C, T, 64>(p, st);
-  if (p.a.D == 128) return launch_append8<C, T, 128>(p, st);
-  return launch_append8<C, T, 256>(p, st);
+  const bool turn = p.a.inv_freq;
+  if (p.a.D == 64) return turn ? launch_append8<C, T, 64, true>(p, st) : launch_append8<C, T, 64, false>(p, st);
+  if (p.a.D == 128) return turn ? launch_append8<C, T, 128, true>(p, st) : launch_append8<C, T, 128, false>(p, st);
+  return turn ? launch_append8<C, T, 256, true>(p, st) : launch_append8<C, T, 256, false>(p, st);
 }
 
 template <class F>
@@ -792,15 +877,13 @@ extern "C" int tkv_paged8_append(const tkv_paged8_append_args* a, tkv_stream_t s
   p.a = *a;
   if (a->inv_freq) {
     if (a->dims <= 0 || a->dims > a->D || a->dims % 16) return TKV_EINVAL;
-    p.turn = TurnPlan{a->positions, {1, 0}, 1, a->counts, a->inv_freq, a->factor, a->factor, a->interleaved, a->dims, a->D,
-                      a->N, a->B};
+    p.turn = TurnPlan{a->positions, {1, 0}, 1, a->counts, a->inv_freq, a->factor, a->factor, a->interleaved, a->dims, a->D};
     if (a->q) {
       if (a->HQ <= 0 || a->HQ > 65535 || (int64_t)a->B * a->N > INT32_MAX || !rows_ok(a->q, a->q_strides, 3, align) ||
           !rows_ok(a->q_out, a->q_out_strides, 3, align))
         return TKV_EINVAL;
       p.q = TurnRows{a->q, a->q_out, {a->q_strides[0], a->q_strides[1], a->q_strides[2]},
-                     {a->q_out_strides[0], a->q_out_strides[1], a->q_out_strides[2]}, a->HQ,
-                     a->q_strides[1] < a->q_strides[2]};
+                     {a->q_out_strides[0], a->q_out_strides[1], a->q_out_strides[2]}, a->HQ};
     }
   }
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -813,9 +896,9 @@ extern "C" int tkv_paged8_append(const tkv_paged8_append_args* a, tkv_stream_t s
 extern "C" int tkv_paged8_read(const tkv_paged8_read_args* a, tkv_stream_t stream) {
   using namespace tkv;
   if (!a || !a->k_out || !a->v_out || !a->block_table) return TKV_EINVAL;
-  if (a->B <= 0 || a->B > 65535 || a->HKV <= 0 || a->N <= 0 || a->D <= 0 || a->D % 16 || a->max_pages <= 0 ||
-      a->block_table_stride < a->max_pages)
+  if (a->B <= 0 || a->B > 65535 || a->HKV <= 0 || a->N <= 0 || a->max_pages <= 0 || a->block_table_stride < a->max_pages)
     return TKV_EINVAL;
+  if (a->D != 64 && a->D != 128 && a->D != 256) return TKV_EUNSUPPORTED;
   if (!format_ok(a->k, a->v, a->k_scale, a->v_scale, a->k_strides, a->v_strides, a->k_scale_strides, a->v_scale_strides,
                  a->block, a->page_size, a->num_pages))
     return TKV_EINVAL;
@@ -823,14 +906,18 @@ extern "C" int tkv_paged8_read(const tkv_paged8_read_args* a, tkv_stream_t strea
   if (a->x_type < TKV_F16 || a->x_type > TKV_F32) return TKV_EINVAL;
   const int align = a->x_type == TKV_F32 ? 4 : 8;
   if (!rows_ok(a->k_out, a->k_out_strides, 3, align) || !rows_ok(a->v_out, a->v_out_strides, 3, align)) return TKV_EINVAL;
-  const int64_t items = (int64_t)a->N * a->HKV * (a->D / 16);
-  if (items > INT32_MAX) return TKV_EINVAL;
-  const dim3 grid((unsigned)(2 * ((items + 255) / 256)), (unsigned)a->B);
-  const int heads_first = a->k_out_strides[1] < a->k_out_strides[2];
+  const int64_t blocks = ((int64_t)a->N + 30) / 32 + 1;  // of 32 slots that N tokens may touch
+  const int heads = a->HKV > 1 && blocks * a->B * a->HKV > 2048 ? 2 : 1;
+  const int64_t groups = blocks * 2 * ((a->HKV + heads - 1) / heads);
+  if (groups > INT32_MAX) return TKV_EINVAL;
+  const dim3 grid((unsigned)groups, (unsigned)a->B);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   return by_type(a->x_type, [&](auto type) {
     constexpr int T = decltype(type)::value;
-    return launch(a->is_int8 ? paged8_read_kernel<Int8, T> : paged8_read_kernel<E4m3, T>, grid, dim3(256), 0, st, *a,
-                  (uint32_t)items, heads_first);
+    auto kernel = [&](auto code) {
+      using C = decltype(code);
+      return a->D == 64 ? paged8_read_kernel<C, T, 64> : a->D == 128 ? paged8_read_kernel<C, T, 128> : paged8_read_kernel<C, T, 256>;
+    };
+    return launch(a->is_int8 ? kernel(Int8{}) : kernel(E4m3{}), grid, dim3(256), 0, st, *a, heads);
   });
 }

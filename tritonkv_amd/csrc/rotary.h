@@ -50,33 +50,50 @@ __device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, v);
 }
 
-// Eight values at p, which is on 16 bytes.
+// Eight values as they lie at an address on 16 bytes.  NT: past the caches, for streams.
 template <int T>
-__device__ __forceinline__ void load8(const void* p, float* y) {
-  if constexpr (T == kF32) {
-    const f4 a = *static_cast<const f4*>(p), b = *(static_cast<const f4*>(p) + 1);
+struct Raw8 {
+  u4 w[kBytes<T> / 2];
+  template <bool NT>
+  __device__ __forceinline__ void load(const void* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = a[i], y[4 + i] = b[i];
-  } else {
-    const u4 w = *static_cast<const u4*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      y[2 * i] = T == kF16 ? half_lo(w[i]) : __builtin_bit_cast(float, w[i] << 16);
-      y[2 * i + 1] = T == kF16 ? half_hi(w[i]) : __builtin_bit_cast(float, w[i] & 0xffff0000u);
+    for (int i = 0; i < kBytes<T> / 2; ++i) {
+      const u4* const at = static_cast<const u4*>(p) + i;
+      w[i] = NT ? __builtin_nontemporal_load(at) : *at;
     }
   }
+  __device__ __forceinline__ void values(float* y) const {
+    if constexpr (T == kF32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t v = w[i / 4][i % 4];
+        y[i] = __builtin_bit_cast(float, v);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        y[2 * i] = T == kF16 ? half_lo(w[0][i]) : __builtin_bit_cast(float, w[0][i] << 16);
+        y[2 * i + 1] = T == kF16 ? half_hi(w[0][i]) : __builtin_bit_cast(float, w[0][i] & 0xffff0000u);
+      }
+    }
+  }
+};
+template <bool NT, class V>
+__device__ __forceinline__ void put(void* p, V v) {
+  if constexpr (NT) __builtin_nontemporal_store(v, static_cast<V*>(p));
+  else *static_cast<V*>(p) = v;
 }
-template <int T>
+template <int T, bool NT>
 __device__ __forceinline__ void store8(void* p, const float* y) {
   if constexpr (T == kF32) {
-    *static_cast<f4*>(p) = f4{y[0], y[1], y[2], y[3]};
-    *(static_cast<f4*>(p) + 1) = f4{y[4], y[5], y[6], y[7]};
+    put<NT>(p, f4{y[0], y[1], y[2], y[3]});
+    put<NT>(static_cast<char*>(p) + 16, f4{y[4], y[5], y[6], y[7]});
   } else {
     u4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       w[i] = T == kF16 ? pack_h2(y[2 * i], y[2 * i + 1]) : pack_bf2(y[2 * i], y[2 * i + 1]);
-    *static_cast<u4*>(p) = w;
+    put<NT>(p, w);
   }
 }
 template <int T>
@@ -98,46 +115,62 @@ __device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) 
   b = x * s + b * c;
 }
 
-// How a head's 16 values of item e (of D / 16) lie: at two places of 8, `first` and `second`.
-// Item e of the halves' layout holds 8 pairs, the others 16 neighbours.
+// Item e of a head's D / 16 is the values from place(e) on and those from place(e) + far on, 8 each:
+// neighbouring items read neighbouring 16 bytes.  far is half of what turns, whose pairs then
+// lie in one item (the halves' layout, dims a multiple of 16), half of the rest, or half of the head
+// (interleaved pairs).
 struct Places {
   int first, second;
-  __device__ __forceinline__ Places(int e, int dims, bool interleaved) {
-    const bool halves = !interleaved && 16 * e < dims;
-    first = halves ? 8 * e : 16 * e;
-    second = halves ? 8 * e + dims / 2 : 16 * e + 8;
+  __device__ __forceinline__ Places(int e, int dims, bool interleaved, int D) {
+    if (interleaved) dims = 0;
+    const bool turned = 16 * e < dims;
+    const int rest = D - dims;
+    first = turned ? 8 * e : dims + 8 * (e - dims / 16);
+    second = first + (turned ? dims / 2 : rest / 2);
   }
 };
 
-// Turns the 16 values of an item, whose turns come from at(pair) (factor and direction included).
-template <class At>
-__device__ __forceinline__ void turn16(float* y, int e, int dims, bool interleaved, At at) {
-  if (interleaved) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (8 * e + i < dims / 2) {
-        const float2 t = at(8 * e + i);
-        turn_pair(y[2 * i], y[2 * i + 1], t.x, t.y);
-      }
-  } else if (16 * e < dims) {
+// The turns of an item's 8 pairs, and the item turned by them.  Interleaved: 4 pairs of the
+// first place, 4 of the second.  Pairs past `dims` are left alone.
+struct Turns {
+  float2 of[8];
+  uint32_t mask;  // a bit for each pair that turns
+  // at(pairs, of): the turns of 8 pairs.  (All are asked for at once, those that do not turn as pair 0.)
+  template <class At>
+  __device__ __forceinline__ void set(int e, int dims, bool interleaved, int D, At at) {
+    int pairs[8];
+    mask = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 t = at(8 * e + i);
-      turn_pair(y[i], y[8 + i], t.x, t.y);
+      const int pair = interleaved ? 4 * e + (i & 3) + (i >> 2) * (D / 4) : 8 * e + i;
+      const bool turns = pair < dims / 2;
+      mask |= turns ? 1u << i : 0u;
+      pairs[i] = turns ? pair : 0;
+    }
+    if (mask) at(pairs, of);
+  }
+  __device__ __forceinline__ void turn(float* y, bool interleaved) const {
+    if (mask == 0) return;
+    if (!interleaved) {  // all of the item's pairs turn
+#pragma unroll
+      for (int i = 0; i < 8; ++i) turn_pair(y[i], y[8 + i], of[i].x, of[i].y);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (mask >> i & 1) turn_pair(y[2 * i], y[2 * i + 1], of[i].x, of[i].y);
     }
   }
-}
+};
 
 // ---------------------------------------------------------------------------
-// Tokens turned by a workgroup of THREADS: `tokens` of them from flat token `from` (row
-// token / N, token % N) on, all H heads.  lds: tokens * dims / 2 turns.
+// Tokens turned by a workgroup: its turns go to LDS once, then a thread takes an item of a
+// token and walks over heads, with the item's turns in registers.
 // ---------------------------------------------------------------------------
 struct TurnRows {
   const void* x;
   void* out;
   int64_t xs[3], outs[3];  // strides in elements: batch, head, token
   int H;
-  bool heads_first;        // a token's heads lie nearer than a head's tokens
 };
 
 struct TurnPlan {
@@ -148,59 +181,97 @@ struct TurnPlan {
   const double* inv_freq;
   float factor;                 // of cos; of sin with the direction's sign:
   float sin_factor;
-  int interleaved, dims, D, N, B;
+  int interleaved, dims, D;
 };
 
-template <int THREADS>
-__device__ __forceinline__ void make_turns(const TurnPlan& p, uint32_t from, int tokens, float2* lds) {
-  const uint32_t pairs = (uint32_t)p.dims / 2, total = (uint32_t)tokens * pairs;
-  for (uint32_t u = threadIdx.x; u < total; u += THREADS) {
-    const uint32_t i = u / pairs, pair = u - i * pairs, token = from + i, b = token / (uint32_t)p.N,
-                   n = token - b * (uint32_t)p.N;
-    const int64_t pos = (int64_t)p.positions[b * p.position_strides[0] + n * p.position_strides[1]] +
-                        (int64_t)p.position_step * n;
-    const float2 t = turn_of((double)pos, p.inv_freq[pair]);
-    lds[u] = make_float2(t.x * p.factor, t.y * p.sin_factor);
-  }
+// The position of a row's token n.
+__device__ __forceinline__ double position_of(const TurnPlan& p, int b, int n) {
+  return (double)((int64_t)p.positions[b * p.position_strides[0] + n * p.position_strides[1]] +
+                  (int64_t)p.position_step * n);
 }
 
-// VEC: halves of whole groups of 8 (or interleaved pairs); else a thread takes a pair.
-template <int T, bool VEC, int THREADS>
-__device__ __forceinline__ void turn_tokens(const TurnPlan& p, const TurnRows& r, uint32_t from, int tokens,
-                                            const float2* lds) {
-  const uint32_t pairs = (uint32_t)p.dims / 2, per = (uint32_t)p.D / (VEC ? 16 : 2), H = r.H, total = per * H * tokens;
-  for (uint32_t u = threadIdx.x; u < total; u += THREADS) {
-    const uint32_t rest = u / per, e = u - rest * per;
-    uint32_t i, h;
-    if (r.heads_first) {
-      i = rest / H;
-      h = rest - i * H;
-    } else {
-      h = rest / (uint32_t)tokens;
-      i = rest - h * (uint32_t)tokens;
+// Tokens of 256 threads: few, so that it reads a token's heads together, but not one, whose
+// turns would be all of a thread's start (4 x 8213 tokens, 32 + 8 heads, bf16, us at 1 / 2 / 4 / 8 /
+// 16 / 32 tokens: 145 / 115 / 114 / 118 / 135 / 171).
+constexpr int kTurnTile = 4;
+constexpr int64_t kTurnMany = 4096;  // tokens from which on there are workgroups enough for that
+constexpr int64_t kTurnFew = 2048;   // up to here heads are shared out over workgroups too
+
+// Heads that a thread has under way at once.  (Four: 113 us for 115 of the case above, but more
+// registers than the append's own work needs: 4 x 2049 tokens with rotary 42.7 us against 36.5.)
+constexpr int kTurnHeads = 2;
+
+// Tokens i < tokens, which lie at (row, token) = token(i), of the heads part, part + parts, ... (in
+// strides of the heads that the workgroup's threads hold at once) of q and then k.
+// lds: tokens * dims / 2 turns.  tokens times the items of a head is at most the threads.
+// VEC: halves of whole groups of 8 (or interleaved pairs); else an item is a pair.
+template <int T, bool VEC, bool NT, class Token>
+__device__ __forceinline__ void turn_tokens(const TurnPlan& p, const TurnRows& q, const TurnRows& k, int tokens,
+                                            int part, int parts, float2* lds, Token token) {
+  const int threads = (int)blockDim.x, tid = (int)threadIdx.x;
+  const int pairs = p.dims / 2, per = p.D / (VEC ? 16 : 2), slots = tokens * per, lanes = threads / slots;
+  for (int u = tid; u < tokens * pairs; u += threads) {
+    const int i = u / pairs, pair = u - i * pairs;
+    const int2 at = token(i);
+    const float2 t = turn_of(position_of(p, at.x, at.y), p.inv_freq[pair]);
+    lds[u] = make_float2(t.x * p.factor, t.y * p.sin_factor);
+  }
+  __syncthreads();
+  const int lane = tid / slots, slot = tid - lane * slots, i = slot / per, e = slot - i * per;
+  if (lane >= lanes) return;
+  const int2 at = token(i);
+  if (p.counts && at.y >= p.counts[at.x]) return;
+  const float2* const turns = lds + i * pairs;
+  const int heads = q.H + k.H, step = lanes * parts;
+  auto rows = [&](int h, const char*& x, char*& o) {
+    const TurnRows& r = h < q.H ? q : k;
+    const int g = h < q.H ? h : h - q.H;
+    x = static_cast<const char*>(r.x) + (at.x * r.xs[0] + g * r.xs[1] + at.y * r.xs[2]) * kBytes<T>;
+    o = static_cast<char*>(r.out) + (at.x * r.outs[0] + g * r.outs[1] + at.y * r.outs[2]) * kBytes<T>;
+  };
+  if constexpr (VEC) {
+    const Places pl(e, p.dims, p.interleaved, p.D);
+    Turns my;
+    my.set(e, p.dims, p.interleaved, p.D, [&](const int* pair, float2* t) {
+#pragma unroll
+      for (int n = 0; n < 8; ++n) t[n] = turns[pair[n]];
+    });
+    constexpr int HEADS = kTurnHeads;
+    for (int h0 = lane + lanes * part; h0 < heads; h0 += step * HEADS) {
+      Raw8<T> a[HEADS], b[HEADS];
+      char* o[HEADS];
+#pragma unroll
+      for (int n = 0; n < HEADS; ++n) {
+        const int h = h0 + n * step;
+        if (h >= heads) break;
+        const char* x;
+        rows(h, x, o[n]);
+        a[n].template load<NT>(x + pl.first * kBytes<T>);
+        b[n].template load<NT>(x + pl.second * kBytes<T>);
+      }
+#pragma unroll
+      for (int n = 0; n < HEADS; ++n) {
+        if (h0 + n * step >= heads) break;
+        float y[16];
+        a[n].values(y);
+        b[n].values(y + 8);
+        my.turn(y, p.interleaved);
+        store8<T, NT>(o[n] + pl.first * kBytes<T>, y);
+        store8<T, NT>(o[n] + pl.second * kBytes<T>, y + 8);
+      }
     }
-    const uint32_t token = from + i, b = token / (uint32_t)p.N, n = token - b * (uint32_t)p.N;
-    if (p.counts && (int)n >= p.counts[b]) continue;
-    const int64_t in = b * r.xs[0] + h * r.xs[1] + n * r.xs[2], out = b * r.outs[0] + h * r.outs[1] + n * r.outs[2];
-    const float2* turns = lds + i * pairs;
-    if constexpr (VEC) {
-      float y[16];
-      const Places at((int)e, p.dims, p.interleaved);
-      const char* x = static_cast<const char*>(r.x) + in * kBytes<T>;
-      char* o = static_cast<char*>(r.out) + out * kBytes<T>;
-      load8<T>(x + at.first * kBytes<T>, y);
-      load8<T>(x + at.second * kBytes<T>, y + 8);
-      turn16(y, (int)e, p.dims, p.interleaved, [&](int pair) { return turns[pair]; });
-      store8<T>(o + at.first * kBytes<T>, y);
-      store8<T>(o + at.second * kBytes<T>, y + 8);
-    } else {
-      const bool turned = e < pairs;
-      const int first = turned && !p.interleaved ? (int)e : (int)(2 * e),
-                second = turned && !p.interleaved ? (int)(e + pairs) : (int)(2 * e + 1);
-      float a = load1<T>(r.x, in + first), c = load1<T>(r.x, in + second);
-      if (turned) turn_pair(a, c, turns[e].x, turns[e].y);
-      store1<T>(r.out, out + first, a);
-      store1<T>(r.out, out + second, c);
+  } else {
+    const bool turned = e < pairs;
+    const int first = turned && !p.interleaved ? e : 2 * e, second = turned && !p.interleaved ? e + pairs : 2 * e + 1;
+    const float2 t = turned ? turns[e] : make_float2(1.0f, 0.0f);
+    for (int h = lane + lanes * part; h < heads; h += step) {
+      const char* x;
+      char* o;
+      rows(h, x, o);
+      float a = load1<T>(x, first), c = load1<T>(x, second);
+      if (turned) turn_pair(a, c, t.x, t.y);
+      store1<T>(o, first, a);
+      store1<T>(o, second, c);
     }
   }
 }

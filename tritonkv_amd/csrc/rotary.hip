@@ -3,6 +3,8 @@
 // Every value is read and written once, for 6 flops a pair: bound by HBM.  A
 // workgroup takes a few tokens with all their heads, so that the angles, in 64 bits,
 // are worked out once a token and not once a head.
+#include <algorithm>
+
 #include "../../include/tkv.h"
 #include "launch.h"
 #include "rotary.h"
@@ -11,15 +13,15 @@ namespace tkv {
 
 constexpr int kTurnThreads = 256;
 
-template <int T, bool VEC>
-__global__ void __launch_bounds__(kTurnThreads) rotary_kernel(TurnPlan p, TurnRows q, TurnRows k, int tile) {
+template <int T, bool VEC, bool NT>
+__global__ void __launch_bounds__(kTurnThreads) rotary_kernel(TurnPlan p, TurnRows q, TurnRows k, int N, uint32_t total,
+                                                              int tile) {
   extern __shared__ float2 turns[];
   const uint32_t from = blockIdx.x * (uint32_t)tile;
-  const int tokens = (int)min((uint32_t)tile, (uint32_t)p.B * (uint32_t)p.N - from);
-  make_turns<kTurnThreads>(p, from, tokens, turns);
-  __syncthreads();
-  turn_tokens<T, VEC, kTurnThreads>(p, q, from, tokens, turns);
-  if (k.x) turn_tokens<T, VEC, kTurnThreads>(p, k, from, tokens, turns);
+  turn_tokens<T, VEC, NT>(p, q, k, (int)min((uint32_t)tile, total - from), blockIdx.y, gridDim.y, turns, [&](int i) {
+    const uint32_t token = from + (uint32_t)i, b = token / (uint32_t)N;
+    return make_int2((int)b, (int)(token - b * (uint32_t)N));
+  });
 }
 
 static bool rows_aligned(const void* p, const int64_t* strides, int align) {
@@ -39,23 +41,30 @@ extern "C" int tkv_rotary(const tkv_rotary_args* a, tkv_stream_t stream) {
   if (!rows_aligned(a->q, a->q_strides, align) || !rows_aligned(a->q_out, a->q_out_strides, align)) return TKV_EINVAL;
   if (a->k && (!rows_aligned(a->k, a->k_strides, align) || !rows_aligned(a->k_out, a->k_out_strides, align)))
     return TKV_EINVAL;
-  TurnPlan p{a->positions, {a->position_strides[0], a->position_strides[1]}, a->position_step, nullptr, a->inv_freq,
-             a->factor, a->adjoint ? -a->factor : a->factor, a->interleaved, a->dims, a->D, a->N, a->B};
+  const TurnPlan p{a->positions, {a->position_strides[0], a->position_strides[1]}, a->position_step, nullptr, a->inv_freq,
+                   a->factor, a->adjoint ? -a->factor : a->factor, a->interleaved, a->dims, a->D};
   auto rows = [&](const void* x, void* out, const int64_t* xs, const int64_t* os, int H) {
-    return TurnRows{x, out, {xs[0], xs[1], xs[2]}, {os[0], os[1], os[2]}, H, xs[1] < xs[2]};
+    return TurnRows{x, out, {xs[0], xs[1], xs[2]}, {os[0], os[1], os[2]}, H};
   };
   const TurnRows q = rows(a->q, a->q_out, a->q_strides, a->q_out_strides, a->HQ),
                  k = rows(a->k, a->k_out, a->k_strides, a->k_out_strides, a->k ? a->HKV : 0);
-  const int64_t total = (int64_t)a->B * a->N;
-  const int tile = total >= 8192 ? 8 : 1;
+  const uint32_t total = (uint32_t)(a->B * (int64_t)a->N);
   const bool vec = a->interleaved || a->dims % 16 == 0;
-  const dim3 grid((unsigned)((total + tile - 1) / tile));
+  const int per = a->D / (vec ? 16 : 2);
+  const bool many = total >= kTurnMany;
+  const int tile = many ? std::min(kTurnTile, kTurnThreads / per) : 1;
+  // Few tokens: heads over more workgroups, a walk of one step each.
+  const int heads = q.H + k.H, lanes = kTurnThreads / (tile * per), walk = (heads + lanes - 1) / lanes;
+  const dim3 grid((total + tile - 1) / tile, total < kTurnFew ? (unsigned)walk : 1);
   const size_t lds = sizeof(float2) * tile * (a->dims / 2);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   auto start = [&](auto type) {
     constexpr int T = decltype(type)::value;
-    return launch(vec ? rotary_kernel<T, true> : rotary_kernel<T, false>, grid, dim3(kTurnThreads), lds, st, p, q, k,
-                  tile);
+    return launch(!vec   ? rotary_kernel<T, false, false>
+                  : many ? rotary_kernel<T, true, true>
+                         : rotary_kernel<T, true, false>,
+                  grid, dim3(kTurnThreads), lds, st, p, q, k,
+                  a->N, total, tile);
   };
   return a->x_type == TKV_F16    ? start(std::integral_constant<int, kF16>{})
          : a->x_type == TKV_BF16 ? start(std::integral_constant<int, kBf16>{})

@@ -312,8 +312,8 @@ def paged8_read(k_pool: Paged8Pool, v_pool: Paged8Pool, block_table: torch.Tenso
             raise ValueError(f"out has {N} tokens, not {tokens}")
         if not _apart(out[0], out[1]) or not all(_apart(x, t) for x in out for t in _pool_tensors(k_pool, v_pool)):
             raise ValueError("out must not share memory with itself or the pools")
-    if B > MAX_ROWS or N * HKV * (D // 16) > 2 ** 31 - 1:
-        raise ValueError(f"at most {MAX_ROWS} rows and 2**31 - 1 groups of 16 values in each, got {B} of {N} tokens")
+    if B > MAX_ROWS or N * HKV * (D // 4) > 2 ** 31 - 1:
+        raise ValueError(f"at most {MAX_ROWS} rows and 2**31 - 1 groups of 4 values in each, got {B} of {N} tokens")
     table = _check_table(block_table, B, device)
     if table.shape[1] * page_size > 2 ** 32 - 1:
         raise ValueError(f"{table.shape[1]} pages of {page_size} tokens a row: at most 2**32 - 1 tokens")
