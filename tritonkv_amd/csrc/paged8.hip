@@ -91,7 +91,7 @@ constexpr float kShift8 = 14.0f;  // P is scaled by 2^14, clear of fp16's smalle
 
 // HT: tiles of 16 columns (a KV head's queries) per workgroup.  MULTI: more than one query per row.
 template <class C, int D, int HT, int NW, bool MULTI>
-__global__ void __launch_bounds__(NW * 64, D == 256 ? 1 : 4 - HT)
+__global__ void __launch_bounds__(NW * 64, D == 256 ? 3 - HT : 4 - HT)
 paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least_chunks, int long_workgroups,
                     int long_chunks, Paged8Params prm) {
   constexpr int NKL = D / 64;  // 16-byte loads of a K row's lane
@@ -133,19 +133,25 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
   uint64_t kt = 0, vt = 0;      // this lane's chunk
   float kscale = 0, vscale = 0;
   int lo, hi;                   // tokens of the segment
-  auto chunks = [&](int c) {
+  int entry = 0;
+  uint32_t at = 0;
+  auto look_up = [&](int c) {   // asks for the table entries from the wave's chunk c on
     const int t = lo + 32 * (w + NW * (c + lane));
-    uint32_t page = 0, at = 0;  // past the segment: never used
+    at = 0;
+    entry = -1;                 // past the segment: the pool's first chunk, never used
     if (t < hi) {
       const uint32_t pg = (uint32_t)t / (uint32_t)a.page_size;
       at = (uint32_t)t - pg * (uint32_t)a.page_size;
-      page = min(max(a.block_table[(int64_t)g.b * a.block_table_stride + pg], 0), a.num_pages - 1);
-      const int64_t i = at / (uint32_t)a.block;
-      kscale = a.k_scale[page * a.k_scale_strides[0] + hk * a.k_scale_strides[1] + i * a.k_scale_strides[2]];
-      vscale = a.v_scale[page * a.v_scale_strides[0] + hk * a.v_scale_strides[1] + i * a.v_scale_strides[2]];
+      entry = a.block_table[(int64_t)g.b * a.block_table_stride + pg];
     }
+  };
+  auto place = [&] {            // and turns them into addresses
+    const uint32_t page = min(max(entry, 0), a.num_pages - 1);
     kt = khead + 16 * ((uint64_t)page * prm.k16[0] + (uint64_t)at * prm.k16[2]);
     vt = vhead + 16 * ((uint64_t)page * prm.v16[0] + (uint64_t)at * prm.v16[2]);
+    const int64_t i = at / (uint32_t)a.block;
+    kscale = a.k_scale[page * a.k_scale_strides[0] + hk * a.k_scale_strides[1] + i * a.k_scale_strides[2]];
+    vscale = a.v_scale[page * a.v_scale_strides[0] + hk * a.v_scale_strides[1] + i * a.v_scale_strides[2]];
   };
   auto lane_ptr = [&](uint64_t x, int l) {
     const uint32_t x0 = __builtin_amdgcn_readlane((int)(uint32_t)x, l);
@@ -157,10 +163,8 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
   };
   u4 kx[2][NKL];
   uint32_t vx[8][VW];
-  float ks, vs;  // the scales of the chunk whose K, V are in kx, vx
   auto load_k = [&](int c) {
     const rsrc_t rk = make_rsrc(lane_ptr(kt, c & 63), kspan);
-    ks = lane_float(kscale, c & 63);
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -168,7 +172,6 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
   };
   auto load_v = [&](int c) {
     const rsrc_t rv = make_rsrc(lane_ptr(vt, c & 63), vspan);
-    vs = lane_float(vscale, c & 63);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if constexpr (VW == 4) {
@@ -207,7 +210,7 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
                                              8 * (u % (D / 8)));
       }
     }
-    chunks(0);
+    look_up(0);
     ask = a.counts ? min(max(a.counts[g.b], 0), a.M) : a.M;
 #pragma unroll
     for (int i = 0; i < QR; ++i) {
@@ -234,6 +237,7 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
       }
       if (u < QV) *reinterpret_cast<u4*>(lds_q + col * QROW + 8 * (u % (D / 8))) = q8[i];
     }
+    place();  // (the queries were made ready while the table was on its way)
     if (lo + 32 * w < hi) {
       load_k(0);
       load_v(0);
@@ -263,6 +267,7 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
     auto step = [&](int c, int cb, auto tail) {
       constexpr bool TAIL = decltype(tail)::value;
       const bool more = cb + 32 * NW < hi;
+      const float ks = lane_float(kscale, c & 63), vs = lane_float(vscale, c & 63);
       float x[HT][8], f[HT];  // scores, and what they are in powers of two
       auto hidden = [&](int ht, int i) {
         return TAIL && cb + slot_token(j, i) > (MULTI ? min(last, seen[ht] - 1) : last);
@@ -299,7 +304,10 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
         }
       }
       if (!TAIL && more) {
-        if (((c + 1) & 63) == 0) chunks(c + 1);  // V of chunk c is on its way already, its scale in vs
+        if (((c + 1) & 63) == 0) {  // V of chunk c is on its way already, its scale in vs
+          look_up(c + 1);
+          place();
+        }
         load_k(c + 1);
       }
       // Online softmax in base 2; the accumulators are rescaled only in chunks
@@ -327,15 +335,13 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
           p[i] = hidden(ht, i) ? 0.0f : __builtin_amdgcn_exp2f(fmaf(x[ht][i], f[ht], off));
           l_run[ht] += p[i];
         }
+        // The first term cut (one instruction a pair), what is left of p, exact, rounded: 2^-22 of p at most.
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t wd = pack_h2(p[2 * i], p[2 * i + 1]);
-            pt[ht][n][i] = wd;
-            p[2 * i] -= half_lo(wd);
-            p[2 * i + 1] -= half_hi(wd);
-          }
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p[2 * i], p[2 * i + 1]));
+          pt[ht][0][i] = hi;
+          pt[ht][1][i] = pack_h2(fma_mix_h<false>(hi, -1.0f, p[2 * i]), fma_mix_h<true>(hi, -1.0f, p[2 * i + 1]));
+        }
       }
       if constexpr (TAIL) {
         // Rows past the sequence are whatever the page holds there (possibly

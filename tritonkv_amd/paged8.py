@@ -34,7 +34,7 @@ import torch
 from . import _lib
 from .kernels.fused_decode_attn import _backend, _prepared, compute_units
 from .paged import _check_table
-from .paged16 import (HEAD_DIMS, MAX_ROWS, _buffer, _dense_rows, _int32_arg, _keep16, _new_rows, _offset, _strides,
+from .paged16 import (HEAD_DIMS, MAX_ROWS, MAX_WORKGROUPS, _buffer, _dense_rows, _int32_arg, _keep16, _new_rows, _offset, _strides,
                       plan_shares)
 from .quantize import _require_gpu
 from .rotary import _APART, _WRITTEN, DTYPES, Rotary, _apart, _check_rotary, _no_grad, _same_place
@@ -44,6 +44,37 @@ BLOCKS = (32, 64, 128)
 MAX_QUERIES = 32
 ROTARY_MULTIPLE = 16
 MAX_PAGE_SIZE = 2 ** 24
+
+
+def plan_shares8(B: int, HKV: int, columns: int, S: int, D: int, device=None,
+                 piece_tokens: int | None = None) -> tuple[int, int, int, int]:
+    """:func:`~tritonkv_amd.paged16.plan_shares` for 8-bit pages, whose chunks hold half the bytes;
+    ``columns`` are a KV head's queries.  Measured on MI355X (us; U = HKV times the blocks of
+    16 or 32 columns):
+
+    * Rows stay whole up to 512 tokens of 128 dims, 256 of 256 and 512 of 64 (whole / cut, one row: 507
+      of 128 8.9 / 9.2, 1019 13.5 / 8.5; 251 of 256 9.3 / 9.9, 507 13.5 / 9.9; 1019 of 64 10.0 / 8.4; 16
+      rows of 1-507, 8 KV heads, 9.8 / 13.4), and where B * U is 512 or more, twice or four times that
+      (64 rows of 1-1019, 8 KV heads, 22.7 / 26.2, all 1019 26.8 / 28.8; of 64 dims 13.4 / 17.1 and 15.0
+      / 18.5; 507 of 256 27.4 / 29.9; but 1-2043 of 128 36.5 / 34.3).
+    * Otherwise two workgroups per CU, four of 64 dims and one of 256 with more than 16 columns (1 / 2 /
+      3 / 4: 32 rows of 32768 376 / 325 / 338 / 341, of 8000-16384 with 64 dims 100 / 70 / 70 / 71, 8 of 1-2999
+      with 64 dims, 16 KV heads, 18.1 / 16.1 / 15.8 / 14.8; 16 rows of 4 queries and 64 heads 55 / 47 / 61 / 58;
+      one row of 32768 20.1 / 18.4 / 19.9 / 23.7; 32 of 16384 with 256 dims 185 / 176 / 212, one with 24
+      columns 22 / 37 / 23), of at least 128 tokens of 128 dims, half of that in tables of at most 512
+      tokens (64 / 128 / 256: 16 rows of 1-1000 14.1 / 14.0 / 15.9).
+    """
+    if piece_tokens is not None:
+        return plan_shares(B, HKV, columns, S, D, device, piece_tokens)
+    if B > MAX_ROWS:
+        raise ValueError(f"at most {MAX_ROWS} rows, got {B}")
+    units = HKV * -(-columns // (16 if columns <= 16 else 32))
+    if S * D <= (131072 if B * units >= 512 else 32768 if D == 64 else 65536):
+        return 1, 0, 0, 0
+    least = (256 if S <= 512 else 512) // D or 1
+    per_cu = 4 if D == 64 else 1 if D == 256 and columns > 16 else 2
+    cu = compute_units(device) or 256
+    return least, min(max(1, per_cu * cu // units), -(-B * -(-S // 32) // least), MAX_WORKGROUPS), 0, 0
 
 
 @dataclass(frozen=True)
@@ -403,7 +434,7 @@ def paged8_decode_attention(
             raise ValueError(f"{name} must be a contiguous float32 {tuple(shape)} tensor on {device}")
     if out is not None and out.data_ptr() % 16:
         raise ValueError("out must start on a 16-byte boundary")
-    least, groups, few, long = plan_shares(B, HKV, HQ // HKV * M, S, D, device, piece_tokens)
+    least, groups, few, long = plan_shares8(B, HKV, HQ // HKV * M, S, D, device, piece_tokens)
     ok, why = _backend(q)
     if not ok:
         raise RuntimeError(f"paged8_decode_attention requires the tritonkv_amd HIP backend: {why}")
