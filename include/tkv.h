@@ -430,7 +430,7 @@ int tkv_paged8_decode_attention(const tkv_paged8_args *args, tkv_stream_t stream
  * magnitudes above 2^64 count as 2^64, NaN does not count); one that is entered further in keeps
  * its scale where that is larger (if it is positive and finite), and else the codes before the
  * new ones are rounded again under s.  Codes are x / s to nearest even; int8 stores NaN as 0.
- * inv_freq (NULL: none): radians per position of the dims / 2 pairs of a key's first dims values
+ * turns (NULL: none): as in tkv_rotary_args, for the dims / 2 pairs of a key's first dims values
  * (a multiple of 16), which are turned before they are quantized, as by tkv_rotary at the
  * tokens' positions; and with q, (B, HQ, N, D) in x_type, so are the queries, into q_out (rows
  * past counts[b] are left alone; q_out may be q). */
@@ -442,7 +442,7 @@ typedef struct tkv_paged8_append_args {
   float *k_scale, *v_scale;
   int64_t k_scale_strides[3], v_scale_strides[3];
   const int32_t *block_table, *positions, *counts;
-  const double *inv_freq;
+  const uint64_t *turns;
   const void *q;
   void *q_out;
   int64_t q_strides[3], q_out_strides[3];
@@ -472,8 +472,8 @@ int tkv_paged8_read(const tkv_paged8_read_args *args, tkv_stream_t stream);
 
 /* Rotary positions: the pairs (a, b) of a head's first dims values, (i, i + dims / 2) or,
  * interleaved, (2i, 2i + 1), become factor * (a cos t - b sin t, a sin t + b cos t), t =
- * inv_freq[i] times the token's position, in 64 bits; with adjoint they turn back
- * (-t), which is the gradient's way.  q (B, HQ, N, D) and k (B, HKV, N, D; NULL: none) in x_type,
+ * turns[i] times the token's position, turns in units of 2^-64 of a whole turn (the product
+ * wraps at whole turns); with adjoint they turn back (-t), which is the gradient's way.  q (B, HQ, N, D) and k (B, HKV, N, D; NULL: none) in x_type,
  * strides batch, head, token in elements, multiples of 16 bytes; the outputs may be the inputs.
  * Token n of row b has the position positions[b * position_strides[0] + n *
  * position_strides[1]] + n * position_step.  D is a multiple of 16 and at most 256, dims even. */
@@ -483,7 +483,7 @@ typedef struct tkv_rotary_args {
   int64_t q_strides[3], k_strides[3], q_out_strides[3], k_out_strides[3];
   const int32_t *positions;
   int64_t position_strides[2];
-  const double *inv_freq;
+  const uint64_t *turns;
   float factor;
   int32_t position_step, x_type, interleaved, adjoint, B, HQ, HKV, N, D, dims;
 } tkv_rotary_args;

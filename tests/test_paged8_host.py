@@ -210,6 +210,27 @@ def test_frequencies():
             assert math.isclose(x, w / 16)
 
 
+def test_turns():
+    """Frequencies as turns in 2**-64, against exact fractions."""
+    from fractions import Fraction
+
+    def arctan(n, one):  # of 1 / n
+        x = total = one // n
+        for k in range(3, 400, 2):
+            x //= -n * n
+            total += x // k
+        return total
+
+    one = 1 << 300
+    inv_2pi = Fraction(one, 8 * (4 * arctan(5, one) - arctan(239, one)))
+    g = torch.Generator().manual_seed(1)
+    w = torch.cat([torch.tensor([1.0, 0.0, -0.25, 7.5, 1e-6, 1e-30, 3e5], dtype=torch.float64),
+                   torch.rand(200, generator=g, dtype=torch.float64) * 3 - 1])
+    for x, t in zip(w.tolist(), ro._turns(w).tolist()):
+        off = (t - int(Fraction(x) * inv_2pi * 2 ** 64)) % 2 ** 64
+        assert min(off, 2 ** 64 - off) <= (16 if abs(x) < 10 else 2 ** 20)  # 8 products, each cut
+
+
 def test_apart():
     x = torch.zeros(2, 7, 10, 8)  # (B, N, heads, D)
     q, k, v = (x[:, :, a:b].transpose(1, 2) for a, b in ((0, 6), (6, 8), (8, 10)))

@@ -197,7 +197,7 @@ class Paged8AppendArgs(ctypes.Structure):
         ("block_table", ctypes.c_void_p),
         ("positions", ctypes.c_void_p),
         ("counts", ctypes.c_void_p),
-        ("inv_freq", ctypes.c_void_p),
+        ("turns", ctypes.c_void_p),
         ("q", ctypes.c_void_p),
         ("q_out", ctypes.c_void_p),
         ("q_strides", ctypes.c_int64 * 3),
@@ -267,7 +267,7 @@ class RotaryArgs(ctypes.Structure):
         ("k_out_strides", ctypes.c_int64 * 3),
         ("positions", ctypes.c_void_p),
         ("position_strides", ctypes.c_int64 * 2),
-        ("inv_freq", ctypes.c_void_p),
+        ("turns", ctypes.c_void_p),
         ("factor", ctypes.c_float),
         ("position_step", ctypes.c_int32),
         ("x_type", ctypes.c_int32),

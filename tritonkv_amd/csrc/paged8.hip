@@ -19,6 +19,11 @@
 // scaled by a power of two each, so that their largest value lies in [2^14, 2^15):
 // exact for what is over 2^-30 of it.  P enters as two fp16 terms (22 bits).  A block's
 // scale of V multiplies its chunks' product in fp32, one of K the scores.
+//
+// Measured (split kernel, us): 32 rows of 32768, HKV 8, G 4, e4m3 319, 6.7 TB/s; 32 rows of
+// 1000-16384, HKV 8, G 8, e4m3 93, 6.1 TB/s; 16 rows of 500-8000 with four queries of 64 heads, int8,
+// 42: 32 columns a workgroup, bound by the vector units (about 600 instructions a chunk); one row of
+// 505 5.5.  The join takes 2-5 us more.
 #include <algorithm>
 
 #include "page_shares.h"
@@ -497,6 +502,10 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
 // own where that is larger: by powers of two nothing is rounded twice in e4m3 (but what
 // falls under its smallest normal code), and a scale rises seldom.  Where it rises, the
 // codes of the block's earlier tokens are rounded again under the new one.
+//
+// Bound by HBM (4 x 8213 tokens, counts of half to all, 8 heads, fp16: 151 MB in 29.6 us, 5.1 TB/s; with
+// each head's loads behind the one's before 30.4, with 16 neighbouring values to a thread 52), short
+// ones by the chain of position, value, scale: 64 rows of a token with rotary 6.3 us.
 // ---------------------------------------------------------------------------
 struct Append8Params {
   tkv_paged8_append_args a;
@@ -506,6 +515,8 @@ struct Append8Params {
   int heads;             // of a workgroup of K or V
   int q_tile, q_parts;   // tokens of a workgroup of queries, and the workgroups that share their heads
 };
+
+constexpr int kAppendHeads = 2;
 
 constexpr float kLargest = 18446744073709551616.0f;  // 2^64
 
@@ -548,20 +559,19 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
-template <class C, int T, int D, int ITEMS, bool ROT>
+// ROT: 0 no rotary positions, 1 by halves, 2 interleaved.
+template <class C, int T, int ITEMS, int ROT>
 __global__ void __launch_bounds__(1024) paged8_append_kernel(Append8Params prm) {
   const tkv_paged8_append_args& a = prm.a;
-  constexpr int PER = D / 16;
+  const int D = a.D, PER = D / 16, shift = D == 64 ? 2 : D == 128 ? 3 : 4;  // items of a token's head
   extern __shared__ float2 lds_turns[];
-  __shared__ uint32_t tops[2][16];
+  __shared__ uint32_t tops[kAppendHeads][16];
   const int b = blockIdx.y, tid = threadIdx.x;
-  if constexpr (ROT)
+  if constexpr (ROT != 0)
     if (blockIdx.x >= prm.kv_groups) {
       const int at = (int)(blockIdx.x - prm.kv_groups), n0 = at / prm.q_parts * prm.q_tile;
-      const auto token = [&](int i) { return make_int2(b, n0 + i); };
-      const int tokens = min(prm.q_tile, a.N - n0), part = at % prm.q_parts;
-      if (prm.q_tile > 1) turn_tokens<T, true, true>(prm.turn, prm.q, TurnRows{}, tokens, part, prm.q_parts, lds_turns, token);
-      else turn_tokens<T, true, false>(prm.turn, prm.q, TurnRows{}, tokens, part, prm.q_parts, lds_turns, token);
+      turn_tokens<T, true, ROT == 2, true>(prm.turn, prm.q, TurnRows{}, min(prm.q_tile, a.N - n0), at % prm.q_parts,
+                                           prm.q_parts, lds_turns, [&](int i) { return make_int2(b, n0 + i); });
       return;
     }
   const int64_t pos = a.positions[b], room = (int64_t)a.max_pages * a.page_size;
@@ -579,55 +589,74 @@ __global__ void __launch_bounds__(1024) paged8_append_kernel(Append8Params prm) 
   const char* x = static_cast<const char*>(isv ? a.v_new : a.k_new) +
                   (b * xs[0] + h0 * xs[1] + (t0 - pos) * xs[2]) * kBytes<T>;
   const bool turned = ROT && !isv;
-  const bool interleaved = prm.turn.interleaved;
+  constexpr bool interleaved = ROT == 2;
   const int dims = turned ? prm.turn.dims : 0;
-  Raw8<T> raw[ITEMS][2];
-  auto load = [&](const char* x) {
+  // The turns of the thread's items: the frequencies are asked for first, the values next, and while
+  // those are on their way the angles are worked out.
+  Turns my[ITEMS];
+  uint64_t w[ITEMS][8];
+  const bool few = blockDim.x == 64;  // few tokens: the angles by all threads, into LDS
+  const int pairs = dims / 2;
+  if (turned && !few)
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const int u = tid + i * (int)blockDim.x, row = u / PER, e = u % PER;
+      const int u = tid + i * (int)blockDim.x;
+      int pair[8];
+      my[i].pick(u & (PER - 1), u >> shift < rows ? dims : 0, interleaved, D, pair);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) w[i][n] = prm.turn.turns[pair[n]];
+    }
+  Raw8<T> raw[kAppendHeads][ITEMS][2];
+#pragma unroll
+  for (int n = 0; n < kAppendHeads; ++n) {  // (under way before the table is known)
+    if (h0 + n >= h1) continue;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int u = tid + i * (int)blockDim.x, row = u >> shift, e = u & (PER - 1);
       if (row >= rows) continue;
       const Places pl(e, dims, interleaved, D);
-      raw[i][0].template load<true>(x + (row * xs[2] + pl.first) * kBytes<T>);
-      raw[i][1].template load<true>(x + (row * xs[2] + pl.second) * kBytes<T>);
+      const char* const at = x + (n * xs[1] + row * xs[2]) * kBytes<T>;
+      raw[n][i][0].template load<true>(at + pl.first * kBytes<T>);
+      raw[n][i][1].template load<true>(at + pl.second * kBytes<T>);
     }
-  };
-  load(x);  // (under way before the table is known)
+  }
   const uint32_t pg = (uint32_t)((uint64_t)base / (uint32_t)a.page_size);
   const int page = a.block_table[(int64_t)b * a.block_table_stride + pg];
+  const auto turn = [&](int row, uint64_t freq) {
+    const float2 t = turn_of(t0 + row, freq);
+    return make_float2(t.x * prm.turn.factor, t.y * prm.turn.sin_factor);
+  };
+  if (turned && few) {
+    for (int u = tid; u < rows * pairs; u += 64) lds_turns[u] = turn(u / pairs, prm.turn.turns[u % pairs]);
+    __syncthreads();
+    int pair[8];
+    my[0].pick(tid & (PER - 1), tid >> shift < rows ? dims : 0, interleaved, D, pair);
+#pragma unroll
+    for (int n = 0; n < 8; ++n) my[0].of[n] = lds_turns[min(tid >> shift, rows - 1) * pairs + pair[n]];
+  } else if (turned) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+      for (int n = 0; n < 8; ++n) my[i].of[n] = turn((tid + i * (int)blockDim.x) >> shift, w[i][n]);
+  }
   if (page < 0 || page >= a.num_pages) return;
   const int at = (int)(base - (int64_t)pg * a.page_size);
   const int64_t* const ss = isv ? a.v_scale_strides : a.k_scale_strides;
   const int64_t* const ps = isv ? a.v_strides : a.k_strides;
   float* sp = (isv ? a.v_scale : a.k_scale) + page * ss[0] + h0 * ss[1] + at / a.block * ss[2];
   uint8_t* to = static_cast<uint8_t*>(isv ? a.v : a.k) + page * ps[0] + h0 * ps[1] + at * ps[2];
-  Turns my[ITEMS];
-  if (turned)
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const int u = tid + i * (int)blockDim.x, row = u / PER, e = u % PER;
-      my[i].set(e, row < rows ? dims : 0, interleaved, D, [&](const int* pair, float2* t) {
-        double w[8];
-#pragma unroll
-        for (int n = 0; n < 8; ++n) w[n] = prm.turn.inv_freq[pair[n]];
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          t[n] = turn_of((double)(t0 + row), w[n]);
-          t[n] = make_float2(t[n].x * prm.turn.factor, t[n].y * prm.turn.sin_factor);
-        }
-      });
-    }
-
-  for (int h = h0; h < h1; ++h, sp += ss[1], to += ps[1]) {
+  for (int n = 0; n < kAppendHeads; ++n, sp += ss[1], to += ps[1]) {
+    if (h0 + n >= h1) continue;
     const float held = first ? *sp : 0.0f;
     float y[ITEMS][16];
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      if ((tid + i * (int)blockDim.x) / PER >= rows) continue;
-      raw[i][0].values(y[i]);
-      raw[i][1].values(y[i] + 8);
-      if (turned) my[i].turn(y[i], interleaved);
+      if ((tid + i * (int)blockDim.x) >> shift >= rows) continue;
+      raw[n][i][0].values(y[i]);
+      raw[n][i][1].values(y[i] + 8);
+      if (turned) my[i].template turn<interleaved>(y[i]);
 #pragma unroll
       for (int d = 0; d < 16; ++d) {
         // (comparisons, which leave a NaN as it is; it does not count for the scale)
@@ -635,10 +664,9 @@ __global__ void __launch_bounds__(1024) paged8_append_kernel(Append8Params prm) 
         top = fmaxf(top, fabsf(y[i][d]));
       }
     }
-    if (h + 1 < h1) load(x += xs[1] * kBytes<T>);
     uint32_t most = wave_max(__builtin_bit_cast(uint32_t, top));
     if (blockDim.x > 64) {
-      uint32_t* const all = tops[h & 1];  // (of two heads in turn: one barrier a head)
+      uint32_t* const all = tops[n];
       if ((tid & 63) == 0) all[tid >> 6] = most;
       __syncthreads();
       for (int i = 0; i < (int)blockDim.x / 64; ++i) most = max(most, all[i]);
@@ -648,8 +676,8 @@ __global__ void __launch_bounds__(1024) paged8_append_kernel(Append8Params prm) 
     if (tid == 0) *sp = scale;
     if (known && scale > held) {
       const float ratio = held / scale;
-      for (int u = tid; u < first * PER; u += blockDim.x) {
-        u4* const p = reinterpret_cast<u4*>(to + (u / PER) * ps[2] + 16 * (u % PER));
+      for (int u = tid; u < first << shift; u += blockDim.x) {
+        u4* const p = reinterpret_cast<u4*>(to + (u >> shift) * ps[2] + 16 * (u & (PER - 1)));
         u4 c = *p;
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
@@ -664,7 +692,7 @@ __global__ void __launch_bounds__(1024) paged8_append_kernel(Append8Params prm) 
     }
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const int u = tid + i * (int)blockDim.x, row = u / PER, e = u % PER;
+      const int u = tid + i * (int)blockDim.x, row = u >> shift, e = u & (PER - 1);
       if (row >= rows) continue;
       const Places pl(e, dims, interleaved, D);
       over_scale<16>(y[i], scale);
@@ -680,7 +708,10 @@ __global__ void __launch_bounds__(1024) paged8_append_kernel(Append8Params prm) 
 //
 // A workgroup takes 32 slots of a page (one block, so that page and scale are the same for all of
 // its threads) of K or V, of one or two heads; an item is 16 bytes of output, and a thread asks for
-// eight before it writes any.  Workgroups follow each other along the tokens of a head.
+// eight before it writes any.  Workgroups follow each other along the tokens of a head.  Bound by
+// HBM: 8 rows of 2000-16384 tokens, 8 heads, bf16, 451 MB in 85.8 us, 5.3 TB/s (heads before
+// tokens in the order of workgroups 89, a thread for a token's dims of all heads 87; a place for
+// every item 125).
 // ---------------------------------------------------------------------------
 template <class C, int T, int D>
 __global__ void __launch_bounds__(256) paged8_read_kernel(tkv_paged8_read_args a, int heads) {
@@ -790,21 +821,24 @@ static int dispatch_paged8(const Paged8Params& p, hipStream_t st) {
   return dispatch_paged8<C, 256>(p, st);
 }
 
-template <class C, int T, int D, bool ROT>
+template <class C, int T, int ROT>
 static int launch_append8(Append8Params p, hipStream_t st) {
   const tkv_paged8_append_args& a = p.a;
-  constexpr int PER = D / 16;
+  const int PER = a.D / 16;
   // Few tokens: a wave holds them all.  Else a thread for 16 values of a block, or for 32 of the
   // largest block of the largest heads.
   const bool few = a.N * (int64_t)PER <= 64;
   const int items = a.block * PER, threads = few ? 64 : items < 1024 ? items : 1024;
   const int64_t blocks = ((int64_t)a.N + a.block - 2) / a.block + 1;  // that N tokens may touch
-  p.heads = a.HKV > 1 && blocks * a.B * a.HKV > 1024 ? 2 : 1;
+  // Two heads to a workgroup, whose turns are then worked out once for both, where that leaves
+  // workgroups enough.
+  p.heads = a.HKV > 1 && blocks * a.B * a.HKV > 1024 ? kAppendHeads : 1;
   const int sets = (a.HKV + p.heads - 1) / p.heads;
   int64_t groups = blocks * 2 * sets;
   p.kv_groups = (uint32_t)groups;
   size_t lds = 0;
-  if (p.q.x) {
+  if (p.q.x) {  // (in one launch with the keys: 4 x 2049 tokens, 32 + 8
+                // heads, 33.8 us; in two 41)
     const int64_t total = (int64_t)a.B * a.N;
     p.q_tile = total >= kTurnMany ? std::min(kTurnTile * std::max(1, threads / 256), threads / PER) : 1;
     const int lanes = threads / (p.q_tile * PER);
@@ -812,19 +846,17 @@ static int launch_append8(Append8Params p, hipStream_t st) {
     groups += ((int64_t)a.N + p.q_tile - 1) / p.q_tile * p.q_parts;
     lds = sizeof(float2) * p.q_tile * (p.turn.dims / 2);
   }
-  if (groups > INT32_MAX) return TKV_EINVAL;
-  auto kernel = paged8_append_kernel<C, T, D, 1, ROT>;
-  if constexpr (D == 256)
-    if (!few && items > 1024) kernel = paged8_append_kernel<C, T, D, 2, ROT>;
-  return launch(kernel, dim3((unsigned)groups, (unsigned)a.B), dim3((unsigned)threads), lds, st, p);
+  if (ROT && few) lds = std::max(lds, sizeof(float2) * a.N * (p.turn.dims / 2));
+  if (groups * threads > UINT32_MAX) return TKV_EINVAL;
+  return launch(!few && items > 1024 ? paged8_append_kernel<C, T, 2, ROT> : paged8_append_kernel<C, T, 1, ROT>,
+                dim3((unsigned)groups, (unsigned)a.B), dim3((unsigned)threads), lds, st, p);
 }
 
 template <class C, int T>
 static int dispatch_append8(const Append8Params& p, hipStream_t st) {
-  const bool turn = p.a.inv_freq;
-  if (p.a.D == 64) return turn ? launch_append8<C, T, 64, true>(p, st) : launch_append8<C, T, 64, false>(p, st);
-  if (p.a.D == 128) return turn ? launch_append8<C, T, 128, true>(p, st) : launch_append8<C, T, 128, false>(p, st);
-  return turn ? launch_append8<C, T, 256, true>(p, st) : launch_append8<C, T, 256, false>(p, st);
+  return !p.a.turns        ? launch_append8<C, T, 0>(p, st)
+         : p.a.interleaved ? launch_append8<C, T, 2>(p, st)
+                           : launch_append8<C, T, 1>(p, st);
 }
 
 template <class F>
@@ -878,12 +910,12 @@ extern "C" int tkv_paged8_append(const tkv_paged8_append_args* a, tkv_stream_t s
   if (!rows_ok(a->k_new, a->k_new_strides, 3, align) || !rows_ok(a->v_new, a->v_new_strides, 3, align)) return TKV_EINVAL;
   if (a->D != 64 && a->D != 128 && a->D != 256) return TKV_EUNSUPPORTED;
   if (((int64_t)a->N / a->block + 2) * 2 * a->HKV > INT32_MAX) return TKV_EINVAL;
-  if (!a->q != !a->q_out || (a->q && !a->inv_freq)) return TKV_EINVAL;
+  if (!a->q != !a->q_out || (a->q && !a->turns)) return TKV_EINVAL;
   Append8Params p{};
   p.a = *a;
-  if (a->inv_freq) {
+  if (a->turns) {
     if (a->dims <= 0 || a->dims > a->D || a->dims % 16) return TKV_EINVAL;
-    p.turn = TurnPlan{a->positions, {1, 0}, 1, a->counts, a->inv_freq, a->factor, a->factor, a->interleaved, a->dims, a->D};
+    p.turn = TurnPlan{a->positions, {1, 0}, 1, a->counts, a->turns, a->factor, a->factor, a->interleaved, a->dims, a->D};
     if (a->q) {
       if (a->HQ <= 0 || a->HQ > 65535 || (int64_t)a->B * a->N > INT32_MAX || !rows_ok(a->q, a->q_strides, 3, align) ||
           !rows_ok(a->q_out, a->q_out_strides, 3, align))
@@ -915,7 +947,7 @@ extern "C" int tkv_paged8_read(const tkv_paged8_read_args* a, tkv_stream_t strea
   const int64_t blocks = ((int64_t)a->N + 30) / 32 + 1;  // of 32 slots that N tokens may touch
   const int heads = a->HKV > 1 && blocks * a->B * a->HKV > 2048 ? 2 : 1;
   const int64_t groups = blocks * 2 * ((a->HKV + heads - 1) / heads);
-  if (groups > INT32_MAX) return TKV_EINVAL;
+  if (groups * 256 > UINT32_MAX) return TKV_EINVAL;
   const dim3 grid((unsigned)groups, (unsigned)a->B);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   return by_type(a->x_type, [&](auto type) {

@@ -1,5 +1,5 @@
 // Rotary positions: pairs (a, b) of a head's first `dims` values turn by an angle
-// theta = position * inv_freq[pair],
+// theta = position * frequency[pair],
 //
 //   (a, b) -> factor * (a cos(theta) - b sin(theta), a sin(theta) + b cos(theta)),
 //
@@ -11,14 +11,15 @@
 
 namespace tkv {
 
-// The angle is taken in 64 bits, as quarter turns less whole turns: a position of 2^20 times a
-// frequency of 1 would be 0.06 radians off in 32.  What remains, at most a
-// half of a quarter turn, is exact to 2^-25 of itself in 32 bits.
-__device__ __forceinline__ float2 turn_of(double position, double inv_freq) {
-  double v = position * inv_freq * 0.15915494309189535;  // turns
-  v = 4.0 * (v - __builtin_rint(v));
-  const double k = __builtin_rint(v);
-  const float x = (float)(v - k) * 1.5707963267948966f;  // within pi / 4
+// A frequency is turns per position in units of 2^-64, so that the product with a position,
+// which wraps at whole turns, is exact to 2^-32 of a turn at any position: in 32-bit floats the
+// angle of position 2^20 at a frequency of 1 would be 0.06 radians off.  (64-bit floats were the
+// first form, as fast where the loads bound the kernel: 22 us for the keys of 4 x 2049 tokens either way.)
+__device__ __forceinline__ float2 turn_of(int64_t position, uint64_t frequency) {
+  const uint32_t p = (uint32_t)position, w0 = (uint32_t)frequency, w1 = (uint32_t)(frequency >> 32);
+  const uint32_t t = p * w1 + __umulhi(p, w0) + (uint32_t)((uint64_t)position >> 32) * w0;
+  const uint32_t quarter = (t + 0x20000000u) >> 30;
+  const float x = (float)(int)(t - (quarter << 30)) * 1.4629180792671596e-9f;  // 2 pi / 2^32: within pi / 4
   // Taylor's series: the first terms left out are x^11 / 11! and x^12 / 12!, under 2e-9.
   const float z = x * x;
   float s = fmaf(z, 2.7557319e-6f, -1.9841270e-4f);
@@ -30,9 +31,8 @@ __device__ __forceinline__ float2 turn_of(double position, double inv_freq) {
   c = fmaf(z, c, 4.1666667e-2f);
   c = fmaf(z, c, -0.5f);
   c = fmaf(z, c, 1.0f);
-  const int quarter = (int)k & 3;
   const float sn = quarter & 1 ? c : s, cs = quarter & 1 ? s : c;
-  return make_float2(quarter == 1 || quarter == 2 ? -cs : cs, quarter & 2 ? -sn : sn);
+  return make_float2((quarter + 1) & 2 ? -cs : cs, quarter & 2 ? -sn : sn);
 }
 
 // ---------------------------------------------------------------------------
@@ -135,10 +135,8 @@ struct Places {
 struct Turns {
   float2 of[8];
   uint32_t mask;  // a bit for each pair that turns
-  // at(pairs, of): the turns of 8 pairs.  (All are asked for at once, those that do not turn as pair 0.)
-  template <class At>
-  __device__ __forceinline__ void set(int e, int dims, bool interleaved, int D, At at) {
-    int pairs[8];
+  // The item's pairs, those that do not turn as pair 0.
+  __device__ __forceinline__ void pick(int e, int dims, bool interleaved, int D, int* pairs) {
     mask = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -147,17 +145,20 @@ struct Turns {
       mask |= turns ? 1u << i : 0u;
       pairs[i] = turns ? pair : 0;
     }
-    if (mask) at(pairs, of);
   }
-  __device__ __forceinline__ void turn(float* y, bool interleaved) const {
-    if (mask == 0) return;
-    if (!interleaved) {  // all of the item's pairs turn
+  template <bool INTER>
+  __device__ __forceinline__ void turn(float* y) const {
+    if constexpr (INTER) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float a = y[2 * i], b = y[2 * i + 1];
+        turn_pair(a, b, of[i].x, of[i].y);
+        y[2 * i] = mask >> i & 1 ? a : y[2 * i];
+        y[2 * i + 1] = mask >> i & 1 ? b : y[2 * i + 1];
+      }
+    } else if (mask) {  // all of the item's pairs turn
 #pragma unroll
       for (int i = 0; i < 8; ++i) turn_pair(y[i], y[8 + i], of[i].x, of[i].y);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (mask >> i & 1) turn_pair(y[2 * i], y[2 * i + 1], of[i].x, of[i].y);
     }
   }
 };
@@ -178,16 +179,15 @@ struct TurnPlan {
   int64_t position_strides[2];  // batch, token
   int position_step;            // added per token
   const int32_t* counts;        // a row's live tokens, or null
-  const double* inv_freq;
+  const uint64_t* turns;        // of a position, for each pair, in 2^-64
   float factor;                 // of cos; of sin with the direction's sign:
   float sin_factor;
   int interleaved, dims, D;
 };
 
 // The position of a row's token n.
-__device__ __forceinline__ double position_of(const TurnPlan& p, int b, int n) {
-  return (double)((int64_t)p.positions[b * p.position_strides[0] + n * p.position_strides[1]] +
-                  (int64_t)p.position_step * n);
+__device__ __forceinline__ int64_t position_of(const TurnPlan& p, int b, int n) {
+  return (int64_t)p.positions[b * p.position_strides[0] + n * p.position_strides[1]] + (int64_t)p.position_step * n;
 }
 
 // Tokens of 256 threads: few, so that it reads a token's heads together, but not one, whose
@@ -204,8 +204,8 @@ constexpr int kTurnHeads = 2;
 // Tokens i < tokens, which lie at (row, token) = token(i), of the heads part, part + parts, ... (in
 // strides of the heads that the workgroup's threads hold at once) of q and then k.
 // lds: tokens * dims / 2 turns.  tokens times the items of a head is at most the threads.
-// VEC: halves of whole groups of 8 (or interleaved pairs); else an item is a pair.
-template <int T, bool VEC, bool NT, class Token>
+// VEC: halves of whole groups of 8 (or INTERleaved pairs); else an item is a pair (of halves).
+template <int T, bool VEC, bool INTER, bool NT, class Token>
 __device__ __forceinline__ void turn_tokens(const TurnPlan& p, const TurnRows& q, const TurnRows& k, int tokens,
                                             int part, int parts, float2* lds, Token token) {
   const int threads = (int)blockDim.x, tid = (int)threadIdx.x;
@@ -213,7 +213,7 @@ __device__ __forceinline__ void turn_tokens(const TurnPlan& p, const TurnRows& q
   for (int u = tid; u < tokens * pairs; u += threads) {
     const int i = u / pairs, pair = u - i * pairs;
     const int2 at = token(i);
-    const float2 t = turn_of(position_of(p, at.x, at.y), p.inv_freq[pair]);
+    const float2 t = turn_of(position_of(p, at.x, at.y), p.turns[pair]);
     lds[u] = make_float2(t.x * p.factor, t.y * p.sin_factor);
   }
   __syncthreads();
@@ -230,12 +230,12 @@ __device__ __forceinline__ void turn_tokens(const TurnPlan& p, const TurnRows& q
     o = static_cast<char*>(r.out) + (at.x * r.outs[0] + g * r.outs[1] + at.y * r.outs[2]) * kBytes<T>;
   };
   if constexpr (VEC) {
-    const Places pl(e, p.dims, p.interleaved, p.D);
+    const Places pl(e, p.dims, INTER, p.D);
     Turns my;
-    my.set(e, p.dims, p.interleaved, p.D, [&](const int* pair, float2* t) {
+    int pair[8];
+    my.pick(e, p.dims, INTER, p.D, pair);
 #pragma unroll
-      for (int n = 0; n < 8; ++n) t[n] = turns[pair[n]];
-    });
+    for (int n = 0; n < 8; ++n) my.of[n] = turns[pair[n]];
     constexpr int HEADS = kTurnHeads;
     for (int h0 = lane + lanes * part; h0 < heads; h0 += step * HEADS) {
       Raw8<T> a[HEADS], b[HEADS];
@@ -255,14 +255,14 @@ __device__ __forceinline__ void turn_tokens(const TurnPlan& p, const TurnRows& q
         float y[16];
         a[n].values(y);
         b[n].values(y + 8);
-        my.turn(y, p.interleaved);
+        my.turn<INTER>(y);
         store8<T, NT>(o[n] + pl.first * kBytes<T>, y);
         store8<T, NT>(o[n] + pl.second * kBytes<T>, y + 8);
       }
     }
   } else {
     const bool turned = e < pairs;
-    const int first = turned && !p.interleaved ? e : 2 * e, second = turned && !p.interleaved ? e + pairs : 2 * e + 1;
+    const int first = turned ? e : 2 * e, second = turned ? e + pairs : 2 * e + 1;
     const float2 t = turned ? turns[e] : make_float2(1.0f, 0.0f);
     for (int h = lane + lanes * part; h < heads; h += step) {
       const char* x;

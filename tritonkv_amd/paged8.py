@@ -37,7 +37,7 @@ from .paged import _check_table
 from .paged16 import (HEAD_DIMS, MAX_ROWS, MAX_WORKGROUPS, _buffer, _dense_rows, _int32_arg, _keep16, _new_rows, _offset, _strides,
                       plan_shares)
 from .quantize import _require_gpu
-from .rotary import _APART, _WRITTEN, DTYPES, Rotary, _apart, _check_rotary, _no_grad, _same_place
+from .rotary import _APART, _WRITTEN, DTYPES, MAX_TOKENS, Rotary, _apart, _check_rotary, _no_grad, _same_place
 
 CODES = (torch.float8_e4m3fn, torch.int8)
 BLOCKS = (32, 64, 128)
@@ -77,7 +77,7 @@ def plan_shares8(B: int, HKV: int, columns: int, S: int, D: int, device=None,
     return least, min(max(1, per_cu * cu // units), -(-B * -(-S // 32) // least), MAX_WORKGROUPS), 0, 0
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class Paged8Pool:
     """Codes of a page pool and their scales (see the module).
 
@@ -184,7 +184,7 @@ def _pool_tensors(k_pool, v_pool) -> tuple:
 _POOL = ("k", "k_scale", "v", "v_scale")
 _D = {f: _offset(_lib.Paged8Args, f) for f in (*_POOL, "q", "block_table", "seq_lens", "counts", "out", "lse")}
 _A = {f: _offset(_lib.Paged8AppendArgs, f) for f in (*_POOL, "k_new", "v_new", "block_table", "positions", "counts",
-                                                     "inv_freq", "q", "q_out")}
+                                                     "turns", "q", "q_out")}
 _R = {f: _offset(_lib.Paged8ReadArgs, f) for f in (*_POOL, "k_out", "v_out", "block_table", "positions", "counts")}
 
 
@@ -225,7 +225,7 @@ def paged8_append(k_pool: Paged8Pool, v_pool: Paged8Pool, k_new: torch.Tensor, v
         key = ("append8",) if rotary is None else ("append8", rotary.factor, rotary.interleaved, q_out is q)
         prep = _prepared(_workspace, key)
         if prep is not None and prep.run(*_pool_tensors(k_pool, v_pool), k_new, v_new, block_table, positions, counts,
-                                         None if rotary is None else rotary.inv_freq, q, q_out):
+                                         None if rotary is None else rotary.turns, q, q_out):
             return q_out
     num_pages, HKV, page_size, D = _check_pools8(k_pool, v_pool)
     device = k_pool.codes.device
@@ -240,8 +240,8 @@ def paged8_append(k_pool: Paged8Pool, v_pool: Paged8Pool, k_new: torch.Tensor, v
     if k_new.shape != v_new.shape or k_new.dtype != v_new.dtype:
         raise ValueError("k_new and v_new must have the same shape and dtype")
     B, _, N, _ = k_new.shape
-    if B > MAX_ROWS or (N // 32 + 2) * 2 * HKV > 2 ** 31 - 1 or B * N > 2 ** 31 - 1:
-        raise ValueError(f"k_new and v_new: at most {MAX_ROWS} rows and 2**31 - 1 tokens, got {tuple(k_new.shape)}")
+    if B > MAX_ROWS or N * HKV * D > 2 ** 33:
+        raise ValueError(f"k_new and v_new: at most {MAX_ROWS} rows of 2**33 values, got {tuple(k_new.shape)}")
     table = _check_table(block_table, B, device)
     if table.shape[1] * page_size > 2 ** 32 - 1:
         raise ValueError(f"{table.shape[1]} pages of {page_size} tokens a row: at most 2**32 - 1 tokens")
@@ -260,8 +260,8 @@ def paged8_append(k_pool: Paged8Pool, v_pool: Paged8Pool, k_new: torch.Tensor, v
             raise ValueError("q_out without q")
     if q is not None:
         if not isinstance(q, torch.Tensor) or q.dim() != 4 or (q.shape[0], q.shape[2], q.shape[3]) != (B, N, D) \
-                or not 0 < q.shape[1] <= 65535:
-            raise ValueError(f"q must be a ({B}, HQ, {N}, {D}) tensor")
+                or not 0 < q.shape[1] <= 65535 or N > MAX_TOKENS:
+            raise ValueError(f"q must be a ({B}, HQ, {N}, {D}) tensor of at most {MAX_TOKENS} tokens a row")
         if q.dtype != k_new.dtype or q.device != device:
             raise ValueError(f"q must be {k_new.dtype} on {device}, got {q.dtype} on {q.device}")
         if q_out is not None:
@@ -282,7 +282,7 @@ def paged8_append(k_pool: Paged8Pool, v_pool: Paged8Pool, k_new: torch.Tensor, v
     args = _lib.Paged8AppendArgs(
         **_pool_fields(k_pool, v_pool), k_new=kn.data_ptr(), v_new=vn.data_ptr(), k_new_strides=_strides(kn, align),
         v_new_strides=_strides(vn, align), block_table=table.data_ptr(), positions=pos.data_ptr(), counts=_lib.ptr(num),
-        inv_freq=None if rotary is None else rotary.inv_freq.data_ptr(), q=_lib.ptr(qn), q_out=_lib.ptr(q_out),
+        turns=None if rotary is None else rotary.turns.data_ptr(), q=_lib.ptr(qn), q_out=_lib.ptr(q_out),
         q_strides=(0, 0, 0) if qn is None else _strides(qn, align),
         q_out_strides=(0, 0, 0) if q_out is None else _strides(q_out, align),
         factor=1.0 if rotary is None else rotary.factor, interleaved=int(rotary is not None and rotary.interleaved),
@@ -294,7 +294,7 @@ def paged8_append(k_pool: Paged8Pool, v_pool: Paged8Pool, k_new: torch.Tensor, v
         _keep16(_workspace, key, args, "tkv_paged8_append", "paged8_append", device, (),
                 (*_pool_slots(_A, k_pool, v_pool), (k_new, _A["k_new"], 16, 1 | read), (v_new, _A["v_new"], 16, 1 | read),
                  (block_table, _A["block_table"], 4), (positions, _A["positions"], 4), (counts, _A["counts"], 4),
-                 (None if rotary is None else rotary.inv_freq, _A["inv_freq"], 8), (q, _A["q"], 16, 1 | read),
+                 (None if rotary is None else rotary.turns, _A["turns"], 8), (q, _A["q"], 16, 1 | read),
                  (q_out, _A["q_out"], 16, 1 | written)))
     return q_out
 
@@ -343,8 +343,8 @@ def paged8_read(k_pool: Paged8Pool, v_pool: Paged8Pool, block_table: torch.Tenso
             raise ValueError(f"out has {N} tokens, not {tokens}")
         if not _apart(out[0], out[1]) or not all(_apart(x, t) for x in out for t in _pool_tensors(k_pool, v_pool)):
             raise ValueError("out must not share memory with itself or the pools")
-    if B > MAX_ROWS or N * HKV * (D // 4) > 2 ** 31 - 1:
-        raise ValueError(f"at most {MAX_ROWS} rows and 2**31 - 1 groups of 4 values in each, got {B} of {N} tokens")
+    if B > MAX_ROWS or N * HKV * D > 2 ** 33:
+        raise ValueError(f"at most {MAX_ROWS} rows of 2**33 values, got {B} of {N} tokens")
     table = _check_table(block_table, B, device)
     if table.shape[1] * page_size > 2 ** 32 - 1:
         raise ValueError(f"{table.shape[1]} pages of {page_size} tokens a row: at most 2**32 - 1 tokens")

@@ -10,8 +10,8 @@ inv_freq[i]``:
     (a, b) -> factor * (a cos t - b sin t, a sin t + b cos t)
 
 Pair i is the values ``(i, i + dims / 2)``, or ``(2i, 2i + 1)`` with
-``interleaved``; values past ``dims`` stay as they are.  Angles are worked out in 64
-bits for any int32 position, so there is no table and no longest context.
+``interleaved``; values past ``dims`` stay as they are.  Angles are worked out modulo whole
+turns, in 64-bit integers, for any int32 position, so there is no table and no longest context.
 """
 
 from __future__ import annotations
@@ -27,6 +27,7 @@ from .quantize import _require_gpu
 
 DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 MAX_HEAD_DIM = 256
+MAX_TOKENS = 2 ** 25 - 1  # of a call: its workgroups' threads are counted in 32 bits
 
 
 def _number(d: dict, name: str, default=None) -> float:
@@ -92,6 +93,21 @@ def rotary_frequencies(dims: int, base: float = 10000.0, scaling: dict | None = 
             _number(scaling, "attention_factor", max(1.0, 0.1 * math.log(factor) + 1.0)))
 
 
+# 1 / (2 pi) as a sum of four numbers of 24 bits, whose products with 26 bits are exact in float64.
+_INV_2PI = (0x28be60 * 2.0 ** -24, 0xdb9391 * 2.0 ** -48, 0x054a7f * 2.0 ** -72, 0x09d5f4 * 2.0 ** -96)
+
+
+def _turns(inv_freq: torch.Tensor) -> torch.Tensor:
+    """float64 radians per position as turns in 2**-64, modulo 2**64: where they lie, without a wait."""
+    far = inv_freq * 134217729.0  # 2**27 + 1
+    high = far - (far - inv_freq)  # the upper 26 bits; the rest has no more
+    pieces = torch.stack([high, inv_freq - high])
+    parts = torch.stack([pieces * c for c in _INV_2PI])
+    upper = (parts - parts.trunc()) * 2.0 ** 32
+    lower = (upper - upper.trunc()) * 2.0 ** 32
+    return ((upper.to(torch.int64) << 32) + lower.to(torch.int64)).sum((0, 1))
+
+
 class Rotary:
     """The frequencies of a model's rotary positions, on a device.
 
@@ -117,6 +133,7 @@ class Rotary:
                 raise ValueError("inv_freq must be a floating-point tensor of radians per position, one for each pair")
             inv_freq, scaled = inv_freq.detach().to(torch.float64).contiguous(), 1.0
         self.inv_freq = inv_freq
+        self.turns = _turns(inv_freq)
         self.dims = 2 * inv_freq.numel()
         self.interleaved = bool(interleaved)
         self.factor = float(scaled if factor is None else factor)
@@ -153,7 +170,7 @@ def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     return False
 
 
-_R = {f: _offset(_lib.RotaryArgs, f) for f in ("q", "k", "q_out", "k_out", "positions", "inv_freq")}
+_R = {f: _offset(_lib.RotaryArgs, f) for f in ("q", "k", "q_out", "k_out", "positions", "turns")}
 _APART, _WRITTEN = 2, 4  # flags of a kept call's tensors: apart from written ones; written
 
 
@@ -206,7 +223,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         inside = out[0] is q and out[1] is k
         key = ("rotary", bool(adjoint), rotary.factor, rotary.interleaved, inside)
         prep = _prepared(_workspace, key)
-        if prep is not None and prep.run(q, k, *out, positions, rotary.inv_freq):
+        if prep is not None and prep.run(q, k, *out, positions, rotary.turns):
             return out[0], out[1]
     if not isinstance(q, torch.Tensor) or q.dim() not in (3, 4):
         raise ValueError("q must be a (B, HQ, N, D) or (B, HQ, D) tensor")
@@ -233,8 +250,8 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     if not isinstance(positions, torch.Tensor) or positions.dtype != torch.int32 or positions.device != device \
             or tuple(positions.shape) not in ((B,), (B, N)):
         raise ValueError(f"positions must be an int32 ({B},) or ({B}, {N}) tensor on {device}")
-    if B * N > 2 ** 31 - 1 or any(x is not None and x.shape[1] > 65535 for x in (q, k)):
-        raise ValueError("at most 2**31 - 1 tokens and 65535 heads")
+    if B * N > MAX_TOKENS or any(x is not None and x.shape[1] > 65535 for x in (q, k)):
+        raise ValueError(f"at most {MAX_TOKENS} tokens and 65535 heads")
     align = 16 // q.element_size()
     outs = [_out_like(x, o, name, align) if x is not None else None
             for x, o, name in ((q, outs[0], "out[0]"), (k, outs[1], "out[1]"))]
@@ -263,7 +280,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         q_strides=strides(read[0]), k_strides=strides(read[1]), q_out_strides=strides(outs[0]),
         k_out_strides=strides(outs[1]), positions=positions.data_ptr(),
         position_strides=(positions.stride(0), positions.stride(1) if positions.dim() == 2 else 0),
-        inv_freq=rotary.inv_freq.data_ptr(), factor=rotary.factor, position_step=int(positions.dim() == 1),
+        turns=rotary.turns.data_ptr(), factor=rotary.factor, position_step=int(positions.dim() == 1),
         x_type=DTYPES.index(q.dtype), interleaved=int(rotary.interleaved), adjoint=int(adjoint), B=B, HQ=q.shape[1],
         HKV=0 if k is None else k.shape[1], N=N, D=D, dims=rotary.dims)
     _lib.check(_lib.launch(device, "tkv_rotary", args), "apply_rotary")
@@ -272,7 +289,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         _keep16(_workspace, key, args, "tkv_rotary", "apply_rotary", device, (),
                 ((q, _R["q"], 16, 1 | apart), (k, _R["k"], 16, 1 | apart), (outs[0], _R["q_out"], 16, 1 | written),
                  (outs[1], _R["k_out"], 16, 1 | written), (positions, _R["positions"], 4, 1 | apart),
-                 (rotary.inv_freq, _R["inv_freq"], 8)))
+                 (rotary.turns, _R["turns"], 8)))
     return outs[0], outs[1]
 
 
