@@ -505,7 +505,7 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
 //
 // Bound by HBM (4 x 8213 tokens, counts of half to all, 8 heads, fp16: 151 MB in 29.6 us, 5.1 TB/s; with
 // each head's loads behind the one's before 30.4, with 16 neighbouring values to a thread 52), short
-// ones by the chain of position, value, scale: 64 rows of a token with rotary 6.3 us.
+// ones by the chain of position, value, scale: 64 rows of a token with rotary 6.3 us (5.8 back to back).
 // ---------------------------------------------------------------------------
 struct Append8Params {
   tkv_paged8_append_args a;
