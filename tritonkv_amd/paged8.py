@@ -219,6 +219,7 @@ def paged8_append(k_pool: Paged8Pool, v_pool: Paged8Pool, k_new: torch.Tensor, v
 
     Does not synchronise, and with ``q_out`` allocates nothing where the tensors are used as they lie.
     """
+    _no_grad(k_new, v_new, q)
     key = None
     if _workspace is not None and (q is None or q_out is not None) and _both_pools(k_pool, v_pool) \
             and (rotary is None or isinstance(rotary, Rotary)):
@@ -229,7 +230,6 @@ def paged8_append(k_pool: Paged8Pool, v_pool: Paged8Pool, k_new: torch.Tensor, v
             return q_out
     num_pages, HKV, page_size, D = _check_pools8(k_pool, v_pool)
     device = k_pool.codes.device
-    _no_grad(k_new, v_new, q)
     for name, x in (("k_new", k_new), ("v_new", v_new)):
         if not isinstance(x, torch.Tensor) or x.dim() != 4 or (x.shape[1], x.shape[3]) != (HKV, D):
             raise ValueError(f"{name} must be a (B, {HKV}, N, {D}) tensor")
