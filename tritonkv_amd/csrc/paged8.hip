@@ -659,8 +659,9 @@ __global__ void __launch_bounds__(1024) paged8_append_kernel(Append8Params prm) 
       if (turned) my[i].template turn<interleaved>(y[i]);
 #pragma unroll
       for (int d = 0; d < 16; ++d) {
-        // (comparisons, which leave a NaN as it is; it does not count for the scale)
-        if (T != kF16) y[i][d] = y[i][d] > kLargest ? kLargest : y[i][d] < -kLargest ? -kLargest : y[i][d];
+        // (comparisons, which leave a NaN as it is; it does not count for the scale.  In every type: fp16
+        // holds infinities, and a turn's factor may take its keys as far.)
+        y[i][d] = y[i][d] > kLargest ? kLargest : y[i][d] < -kLargest ? -kLargest : y[i][d];
         top = fmaxf(top, fabsf(y[i][d]));
       }
     }
