@@ -623,8 +623,7 @@ __global__ void __launch_bounds__(1024) paged8_append_kernel(Append8Params prm) 
   const uint32_t pg = (uint32_t)((uint64_t)base / (uint32_t)a.page_size);
   const int page = a.block_table[(int64_t)b * a.block_table_stride + pg];
   const auto turn = [&](int row, uint64_t freq) {
-    const float2 t = turn_of(t0 + row, freq);
-    return make_float2(t.x * prm.turn.factor, t.y * prm.turn.sin_factor);
+    return turn_of(t0 + row, freq, prm.turn.factor, prm.turn.sin_factor);
   };
   if (turned && few) {
     for (int u = tid; u < rows * pairs; u += 64) lds_turns[u] = turn(u / pairs, prm.turn.turns[u % pairs]);

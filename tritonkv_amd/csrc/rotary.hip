@@ -1,7 +1,7 @@
 // Rotary positions of queries and keys, for gfx950.
 //
 // Every value is read and written once, for 6 flops a pair: bound by HBM.  A
-// workgroup takes a few tokens with all their heads, so that the angles, in 64 bits,
+// workgroup takes a few tokens with all their heads, so that the angles, modulo whole turns,
 // are worked out once a token and not once a head.  4 x 8213 tokens, 32 + 8 heads, bf16: 673 MB in
 // 111 us, 6.1 TB/s (a copy's rate is 4.8); one token of 64 rows 3.3 us.
 #include <algorithm>
