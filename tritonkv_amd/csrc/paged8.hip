@@ -657,12 +657,7 @@ __global__ void __launch_bounds__(1024) paged8_append_kernel(Append8Params prm) 
       raw[n][i][1].values(y[i] + 8);
       if (turned) my[i].template turn<interleaved>(y[i]);
 #pragma unroll
-      for (int d = 0; d < 16; ++d) {
-        // (comparisons, which leave a NaN as it is; it does not count for the scale.  In every type: fp16
-        // holds infinities, and a turn's factor may take its keys as far.)
-        y[i][d] = y[i][d] > kLargest ? kLargest : y[i][d] < -kLargest ? -kLargest : y[i][d];
-        top = fmaxf(top, fabsf(y[i][d]));
-      }
+      for (int d = 0; d < 16; ++d) top = fmaxf(top, fabsf(y[i][d]));  // (a NaN does not count)
     }
     uint32_t most = wave_max(__builtin_bit_cast(uint32_t, top));
     if (blockDim.x > 64) {
@@ -670,6 +665,18 @@ __global__ void __launch_bounds__(1024) paged8_append_kernel(Append8Params prm) 
       if ((tid & 63) == 0) all[tid >> 6] = most;
       __syncthreads();
       for (int i = 0; i < (int)blockDim.x / 64; ++i) most = max(most, all[i]);
+    }
+    // Magnitudes past 2^64: in every type, since fp16 holds infinities and a turn's factor may take its
+    // keys as far; looked for only where the block's largest is one (for every value of an fp16 prompt
+    // 32.2 us against 30.1).
+    constexpr uint32_t kMost = __builtin_bit_cast(uint32_t, kLargest);
+    if (most > kMost) {
+      most = kMost;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int d = 0; d < 16; ++d)  // (comparisons, which leave a NaN as it is)
+          y[i][d] = y[i][d] > kLargest ? kLargest : y[i][d] < -kLargest ? -kLargest : y[i][d];
     }
     const bool known = first > 0 && is_scale(held);
     const float need = least_scale<C>(__builtin_bit_cast(float, most)), scale = known ? fmaxf(held, need) : need;
