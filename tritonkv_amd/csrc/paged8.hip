@@ -357,6 +357,9 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
 #pragma unroll
             for (int e = 0; e < VW; ++e) vx[i][e] = 0u;
       }
+      float vf[HT];  // V's scale, 0 for a column that sees none of the chunk (a scale of NaN would reach it)
+#pragma unroll
+      for (int ht = 0; ht < HT; ++ht) vf[ht] = TAIL && MULTI && seen[ht] <= cb ? 0.0f : vs;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int y = 0; y < VW; ++y)
@@ -388,7 +391,7 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
               f4 o = mfma_k32(av[e], pt[ht][1], f4{0.f, 0.f, 0.f, 0.f});
               o = mfma_k32(av[e], pt[ht][0], o);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) accv[ht][mv][i] = fmaf(o[i], vs, accv[ht][mv][i]);
+              for (int i = 0; i < 4; ++i) accv[ht][mv][i] = fmaf(o[i], vf[ht], accv[ht][mv][i]);
               if constexpr (TAIL && MULTI && C::kHasNan) {
                 u4 sees;
 #pragma unroll
