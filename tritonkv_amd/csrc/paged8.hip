@@ -340,7 +340,9 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
           p[i] = hidden(ht, i) ? 0.0f : __builtin_amdgcn_exp2f(fmaf(x[ht][i], f[ht], off));
           l_run[ht] += p[i];
         }
-        // The first term cut (one instruction a pair), what is left of p, exact, rounded: 2^-22 of p at most.
+        // The first term cut, what is left of p, exact, rounded: 2^-22 of p at most, under what the sums in 32
+        // bits add.  (Both rounded: 2^-23, outputs as far from 64 bits, 3.16e-7 of the norm for 3.18e-7 at one
+        // row of 505, 7.7e-8 for 7.5e-8 at D 64; 16 rows of four queries 48.8 us for 47.7.)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p[2 * i], p[2 * i + 1]));
