@@ -1,0 +1,56 @@
+"""What the 8-bit page calls and apply_rotary refuse: outputs over the tensors that say where tokens lie, and more."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tritonkv_amd import paged8 as p8
+from tritonkv_amd import rotary as ro
+
+I32 = torch.int32
+
+
+def pool():
+    return p8.empty_paged8_pool(4, 2, 64, 64, torch.int8, 32, device="cpu")
+
+
+def over(t, like):
+    """A tensor of like's form over t's memory."""
+    return torch.empty(0, dtype=like.dtype).set_(t.untyped_storage(), 0, like.shape, like.stride())
+
+
+def test_read_refuses_outputs_over_its_other_tensors():
+    k, v, table, n = pool(), pool(), torch.zeros(1, 64, dtype=I32), torch.zeros(1, dtype=I32)
+    out = tuple(torch.zeros(1, 2, 8, 64) for _ in range(2))
+    for kw in (dict(block_table=over(out[0], table)), dict(positions=over(out[1], n)), dict(counts=over(out[0], n))):
+        with pytest.raises(ValueError, match="share"):
+            p8.paged8_read(k, v, **{**dict(block_table=table), **kw}, out=out)
+
+
+def append(q_out):
+    return dict(k_pool=pool(), v_pool=pool(), k_new=torch.zeros(2, 2, 3, 64), v_new=torch.zeros(2, 2, 3, 64),
+                block_table=torch.zeros(2, 2, dtype=I32), positions=torch.zeros(2, dtype=I32),
+                counts=torch.zeros(2, dtype=I32), rotary=ro.Rotary(64, device="cpu"), q=torch.zeros(2, 4, 3, 64),
+                q_out=q_out)
+
+
+def test_append_refuses_queries_over_its_other_tensors():
+    q_out = torch.zeros(2, 4, 3, 64)
+    for name in ("block_table", "positions", "counts"):
+        a = append(q_out)
+        a[name] = over(q_out, a[name])
+        with pytest.raises(ValueError, match="share"):
+            p8.paged8_append(**a)
+    a = append(q_out)
+    a["rotary"].turns = over(q_out, a["rotary"].turns)
+    with pytest.raises(ValueError, match="share"):
+        p8.paged8_append(**a)
+
+
+def test_rotary_refuses_outputs_over_its_turns():
+    q, pos, rot = torch.zeros(2, 4, 3, 64), torch.zeros(2, dtype=I32), ro.Rotary(64, device="cpu")
+    out = torch.zeros_like(q)
+    rot.turns = over(out, rot.turns)
+    with pytest.raises(ValueError, match="share"):
+        ro.apply_rotary(q, None, pos, rot, out=(out, None))

@@ -269,8 +269,9 @@ def paged8_append(k_pool: Paged8Pool, v_pool: Paged8Pool, k_new: torch.Tensor, v
                     or q_out.device != device or not _dense_rows(q_out, align) \
                     or any(s <= 0 for s in _strides(q_out, align)):
                 raise ValueError("q_out must be a tensor of q's shape, dtype and device with dense rows on 16 bytes")
+            others = [t for t in (k_new, v_new, table, pos, num, rotary.turns) if t is not None]
             if not (_same_place(q, q_out) or _apart(q, q_out)) or \
-                    not all(_apart(q_out, t) for t in (k_new, v_new, *_pool_tensors(k_pool, v_pool))):
+                    not all(_apart(q_out, t) for t in (*others, *_pool_tensors(k_pool, v_pool))):
                 raise ValueError("q_out must be q itself or share no memory with the other tensors")
     _require_gpu(k_pool.codes, "paged8_append")
     if q is not None and q_out is None:
@@ -341,8 +342,6 @@ def paged8_read(k_pool: Paged8Pool, v_pool: Paged8Pool, block_table: torch.Tenso
         N, dtype = out[0].shape[2], out[0].dtype
         if tokens is not None and tokens != N:
             raise ValueError(f"out has {N} tokens, not {tokens}")
-        if not _apart(out[0], out[1]) or not all(_apart(x, t) for x in out for t in _pool_tensors(k_pool, v_pool)):
-            raise ValueError("out must not share memory with itself or the pools")
     if B > MAX_ROWS or N * HKV * D > 2 ** 33:
         raise ValueError(f"at most {MAX_ROWS} rows of 2**33 values, got {B} of {N} tokens")
     table = _check_table(block_table, B, device)
@@ -350,6 +349,10 @@ def paged8_read(k_pool: Paged8Pool, v_pool: Paged8Pool, block_table: torch.Tenso
         raise ValueError(f"{table.shape[1]} pages of {page_size} tokens a row: at most 2**32 - 1 tokens")
     pos = None if positions is None else _int32_arg(positions, B, device, "positions", "B start positions")
     num = None if counts is None else _int32_arg(counts, B, device, "counts", "B token counts")
+    if out is not None:
+        others = [t for t in (table, pos, num, *_pool_tensors(k_pool, v_pool)) if t is not None]
+        if not _apart(out[0], out[1]) or not all(_apart(x, t) for x in out for t in others):
+            raise ValueError("out must not share memory with itself or the other tensors")
     _require_gpu(k_pool.codes, "paged8_read")
     if out is None:
         out = tuple(torch.zeros(B, HKV, N, D, dtype=dtype, device=device) for _ in range(2))

@@ -260,7 +260,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         if not _same_place(x, o) and not _apart(x, o):
             raise ValueError("an output must be its input itself or share no memory with it")
         if not all(_apart(o, t) for t in (*(t for pair in given[i + 1:] for t in pair), positions,
-                                          *(y for y, _ in given[:i]))):
+                                          rotary.turns, *(y for y, _ in given[:i]))):
             raise ValueError("an output must not share memory with the other tensors")
     _require_gpu(q, "apply_rotary")
     if q.numel() == 0 and (k is None or k.numel() == 0):
