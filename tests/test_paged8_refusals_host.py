@@ -54,3 +54,27 @@ def test_rotary_refuses_outputs_over_its_turns():
     rot.turns = over(out, rot.turns)
     with pytest.raises(ValueError, match="share"):
         ro.apply_rotary(q, None, pos, rot, out=(out, None))
+
+
+def test_a_kept_read_still_checks_its_tokens(monkeypatch):
+    """``tokens`` must be the outputs', in the call that is kept and in those after it."""
+    from tritonkv_amd import _lib
+
+    class Kept:
+        def __init__(self, key):
+            self.key = key
+
+        def run(self, *tensors):
+            return True
+
+    monkeypatch.setattr(p8, "_require_gpu", lambda *a: None)
+    monkeypatch.setattr(p8, "_keep16", lambda ws, key, *a: ws.update(call=Kept(key)))
+    monkeypatch.setattr(_lib, "launch", lambda *a: 0)
+    table, out = torch.zeros(1, 2, dtype=I32), tuple(torch.zeros(1, 2, 8, 64) for _ in range(2))
+    for first in (None, 8):
+        ws: dict = {}
+        p8.paged8_read(pool(), pool(), table, tokens=first, out=out, _workspace=ws)
+        assert "call" in ws
+        with pytest.raises(ValueError, match="tokens"):
+            p8.paged8_read(pool(), pool(), table, tokens=9, out=out, _workspace=ws)
+        assert p8.paged8_read(pool(), pool(), table, tokens=8, out=out, _workspace=ws)[0] is out[0]

@@ -313,7 +313,7 @@ def paged8_read(k_pool: Paged8Pool, v_pool: Paged8Pool, block_table: torch.Tenso
     """
     key = None
     if _workspace is not None and isinstance(out, (tuple, list)) and len(out) == 2 and _both_pools(k_pool, v_pool):
-        key = ("read8",)
+        key = ("read8", tokens)
         prep = _prepared(_workspace, key)
         if prep is not None and prep.run(*_pool_tensors(k_pool, v_pool), block_table, positions, counts, *out):
             return out[0], out[1]
