@@ -45,6 +45,8 @@ struct Slot {
   c10::Device device{c10::kCPU};
   std::vector<int64_t> sizes;
   std::vector<int64_t> strides;  // of a tensor that is used as it is strided; else empty: contiguous
+  std::vector<int64_t> layout;   // its strides in bytes, whichever form it has
+  int64_t entry;                 // bytes of an entry
   uintptr_t span;                // bytes from its first entry to the end of its last
   bool apart, written;           // shares no memory with other such slots if one of the two is written
 };
@@ -76,6 +78,35 @@ void* plain_pointer(const at::Tensor& t, const std::vector<int64_t>& strides) {
       !(strides.empty() ? t.is_contiguous() : t.strides() == c10::IntArrayRef(strides)))
     return nullptr;
   return t.mutable_data_ptr();
+}
+
+// Bytes from a slot's first entry to the end of its last over the axes of smaller strides than `below`.
+int64_t extent(const Slot& s, int64_t below) {
+  int64_t n = s.entry;
+  for (size_t d = 0; d < s.sizes.size(); ++d)
+    if (s.layout[d] < below) n += (s.sizes[d] - 1) * s.layout[d];
+  return n;
+}
+
+// Whether two slots' tensors, `between` bytes apart, lie in turn over a stride that both have (queries and
+// keys of one projection's output), and so share nothing although their spans do.
+bool in_turn(const Slot& a, const Slot& b, int64_t between) {
+  auto steps = [](const Slot& s, int64_t period) {  // every wider stride is a multiple of the period
+    for (size_t d = 0; d < s.sizes.size(); ++d)
+      if (s.sizes[d] > 1 && s.layout[d] > period && s.layout[d] % period) return false;
+    return true;
+  };
+  for (size_t d = 0; d < a.sizes.size(); ++d) {
+    const int64_t period = a.layout[d];
+    if (a.sizes[d] < 2 || period <= 0) continue;
+    for (size_t x = 0; x < b.sizes.size(); ++x) {
+      if (b.sizes[x] < 2 || b.layout[x] != period || !steps(a, period) || !steps(b, period)) continue;
+      const int64_t at = (between % period + period) % period;
+      if (extent(a, period) <= at && at + extent(b, period) <= period) return true;
+      break;
+    }
+  }
+  return false;
 }
 
 void free_call(PyObject* capsule) {
@@ -127,8 +158,9 @@ PyObject* prepare(PyObject*, PyObject* const* a, Py_ssize_t n) {
         s.sizes = v.sizes().vec();
         s.written = flags & kWritten;
         s.apart = s.written || flags & kApart;
-        s.span = v.element_size();
-        for (int64_t d = 0; d < v.dim(); ++d) s.span += v.element_size() * (v.size(d) - 1) * v.stride(d);
+        s.entry = v.element_size();
+        for (int64_t d = 0; d < v.dim(); ++d) s.layout.push_back(s.entry * v.stride(d));
+        s.span = extent(s, INT64_MAX);
         if (s.apart && ++apart > kMaxApart) {
           PyErr_SetString(PyExc_ValueError, "prepare: too many slots that must lie apart");
           return nullptr;
@@ -169,7 +201,7 @@ PyObject* run(PyObject*, PyObject* const* a, Py_ssize_t n) {
     std::memcpy(args, call->args, call->size);
     struct {
       uintptr_t begin, end;
-      bool written;
+      const Slot* slot;
     } apart[kMaxApart];
     size_t spans = 0;
     for (size_t i = 0; i < call->slots.size(); ++i) {
@@ -189,8 +221,10 @@ PyObject* run(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (s.apart) {
         const uintptr_t begin = (uintptr_t)p, end = begin + s.span;
         for (size_t x = 0; x < spans; ++x)
-          if ((s.written || apart[x].written) && begin < apart[x].end && apart[x].begin < end) Py_RETURN_NONE;
-        apart[spans++] = {begin, end, s.written};
+          if ((s.written || apart[x].slot->written) && begin < apart[x].end && apart[x].begin < end &&
+              !in_turn(*apart[x].slot, s, (int64_t)(begin - apart[x].begin)))
+            Py_RETURN_NONE;
+        apart[spans++] = {begin, end, &s};
       }
     }
     c10::hip::OptionalHIPGuard guard;

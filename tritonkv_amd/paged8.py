@@ -172,9 +172,9 @@ def _pool_fields(k_pool: Paged8Pool, v_pool: Paged8Pool) -> dict:
                 block=k_pool.block, page_size=k_pool.page_size, num_pages=k_pool.codes.shape[0])
 
 
-def _pool_slots(offsets: dict, k_pool: Paged8Pool, v_pool: Paged8Pool) -> tuple:
-    return ((k_pool.codes, offsets["k"], 16, 1), (k_pool.scale, offsets["k_scale"], 4, 1),
-            (v_pool.codes, offsets["v"], 16, 1), (v_pool.scale, offsets["v_scale"], 4, 1))
+def _pool_slots(offsets: dict, k_pool: Paged8Pool, v_pool: Paged8Pool, flags: int = 0) -> tuple:
+    return ((k_pool.codes, offsets["k"], 16, 1 | flags), (k_pool.scale, offsets["k_scale"], 4, 1 | flags),
+            (v_pool.codes, offsets["v"], 16, 1 | flags), (v_pool.scale, offsets["v_scale"], 4, 1 | flags))
 
 
 def _pool_tensors(k_pool, v_pool) -> tuple:
@@ -291,11 +291,13 @@ def paged8_append(k_pool: Paged8Pool, v_pool: Paged8Pool, k_new: torch.Tensor, v
         B=B, HKV=HKV, N=N, D=D, block_table_stride=table.shape[1], max_pages=table.shape[1])
     _lib.check(_lib.launch(device, "tkv_paged8_append", args), "paged8_append")
     if key is not None and kn is k_new and vn is v_new and qn is q:
-        read, written = (0, 0) if q_out is q else (_APART, _WRITTEN)
+        # In place q is what is written, as q_out, the same tensor, which need not lie apart from it.
+        read, written = (_WRITTEN, 0) if q_out is q else (_APART, _WRITTEN)
         _keep16(_workspace, key, args, "tkv_paged8_append", "paged8_append", device, (),
-                (*_pool_slots(_A, k_pool, v_pool), (k_new, _A["k_new"], 16, 1 | read), (v_new, _A["v_new"], 16, 1 | read),
-                 (block_table, _A["block_table"], 4), (positions, _A["positions"], 4), (counts, _A["counts"], 4),
-                 (None if rotary is None else rotary.turns, _A["turns"], 8), (q, _A["q"], 16, 1 | read),
+                (*_pool_slots(_A, k_pool, v_pool, _APART), (k_new, _A["k_new"], 16, 1 | _APART),
+                 (v_new, _A["v_new"], 16, 1 | _APART), (block_table, _A["block_table"], 4, _APART),
+                 (positions, _A["positions"], 4, _APART), (counts, _A["counts"], 4, _APART),
+                 (None if rotary is None else rotary.turns, _A["turns"], 8, _APART), (q, _A["q"], 16, 1 | read),
                  (q_out, _A["q_out"], 16, 1 | written)))
     return q_out
 
@@ -367,8 +369,9 @@ def paged8_read(k_pool: Paged8Pool, v_pool: Paged8Pool, block_table: torch.Tenso
     _lib.check(_lib.launch(device, "tkv_paged8_read", args), "paged8_read")
     if key is not None:
         _keep16(_workspace, key, args, "tkv_paged8_read", "paged8_read", device, (),
-                (*_pool_slots(_R, k_pool, v_pool), (block_table, _R["block_table"], 4), (positions, _R["positions"], 4),
-                 (counts, _R["counts"], 4), (out[0], _R["k_out"], 16, 1), (out[1], _R["v_out"], 16, 1)))
+                (*_pool_slots(_R, k_pool, v_pool, _APART), (block_table, _R["block_table"], 4, _APART),
+                 (positions, _R["positions"], 4, _APART), (counts, _R["counts"], 4, _APART),
+                 (out[0], _R["k_out"], 16, 1 | _WRITTEN), (out[1], _R["v_out"], 16, 1 | _WRITTEN)))
     return out[0], out[1]
 
 

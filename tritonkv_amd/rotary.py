@@ -285,11 +285,12 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         HKV=0 if k is None else k.shape[1], N=N, D=D, dims=rotary.dims)
     _lib.check(_lib.launch(device, "tkv_rotary", args), "apply_rotary")
     if key is not None and read[0] is q and read[1] is k:
-        written, apart = (0, 0) if inside else (_WRITTEN, _APART)
+        # In place q and k are what is written; the outputs, the same tensors, need not lie apart from them.
+        read, written = (_WRITTEN, 0) if inside else (_APART, _WRITTEN)
         _keep16(_workspace, key, args, "tkv_rotary", "apply_rotary", device, (),
-                ((q, _R["q"], 16, 1 | apart), (k, _R["k"], 16, 1 | apart), (outs[0], _R["q_out"], 16, 1 | written),
-                 (outs[1], _R["k_out"], 16, 1 | written), (positions, _R["positions"], 4, 1 | apart),
-                 (rotary.turns, _R["turns"], 8)))
+                ((q, _R["q"], 16, 1 | read), (k, _R["k"], 16, 1 | read), (outs[0], _R["q_out"], 16, 1 | written),
+                 (outs[1], _R["k_out"], 16, 1 | written), (positions, _R["positions"], 4, 1 | _APART),
+                 (rotary.turns, _R["turns"], 8, _APART)))
     return outs[0], outs[1]
 
 
