@@ -115,6 +115,9 @@ class Rotary:
     or ``inv_freq``, a tensor of radians per position of each pair, says them outright
     (per-pair factors of a long context are divided into it).  ``factor`` multiplies cos
     and sin (default: what ``scaling`` says, else 1).
+
+    The frequencies are copied and turned into integers here, by some twenty launches: make one per model, and
+    where they follow the length, one per length that is met, not one per step.
     """
 
     def __init__(self, dims: int | None = None, base: float = 10000.0, *, interleaved: bool = False,
@@ -131,7 +134,7 @@ class Rotary:
             if not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1 or inv_freq.numel() == 0 \
                     or not inv_freq.is_floating_point():
                 raise ValueError("inv_freq must be a floating-point tensor of radians per position, one for each pair")
-            inv_freq, scaled = inv_freq.detach().to(torch.float64).contiguous(), 1.0
+            inv_freq, scaled = inv_freq.detach().to(torch.float64, copy=True).contiguous(), 1.0
         self.inv_freq = inv_freq
         self.turns = _turns(inv_freq)
         self.dims = 2 * inv_freq.numel()
