@@ -18,3 +18,22 @@ def test_a_rotary_keeps_frequencies_of_its_own(dtype):
     before = rot.inv_freq.clone()
     w.mul_(2)
     assert torch.equal(rot.inv_freq, before) and torch.equal(rot.turns, ro._turns(before))
+
+
+LLAMA3 = dict(factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0, original_max_position_embeddings=8192)
+YARN = dict(factor=16.0, original_max_position_embeddings=4096)
+
+
+@pytest.mark.parametrize("kind,rest", [("linear", dict(factor=4.0)), ("ntk", dict(factor=4.0)), ("llama3", LLAMA3),
+                                       ("yarn", YARN)])
+def test_a_scaling_may_name_its_type_as_models_do(kind, rest):
+    want = ro.rotary_frequencies(64, 1e4, dict(type=kind, **rest))
+    assert ro.rotary_frequencies(64, 1e4, dict(rope_type=kind, **rest)) == want
+    assert ro.rotary_frequencies(64, 1e4, dict(rope_type=kind, type=kind, **rest)) == want
+    with pytest.raises(ValueError, match="type"):
+        ro.rotary_frequencies(64, 1e4, dict(rope_type=kind, type="other", **rest))
+    for missing in ({}, dict(type=None), dict(rope_type="other")):
+        with pytest.raises(ValueError, match="type"):
+            ro.rotary_frequencies(64, 1e4, dict(**missing, **rest))
+    with pytest.raises(ValueError, match=f"'{kind}'.*'factor'"):
+        ro.rotary_frequencies(64, 1e4, dict(rope_type=kind))

@@ -30,9 +30,9 @@ MAX_HEAD_DIM = 256
 MAX_TOKENS = 2 ** 25 - 1  # of a call: its workgroups' threads are counted in 32 bits
 
 
-def _number(d: dict, name: str, default=None) -> float:
+def _number(d: dict, kind: str, name: str, default=None) -> float:
     if name not in d and default is None:
-        raise ValueError(f"scaling of type {d['type']!r} needs {name!r}")
+        raise ValueError(f"scaling of type {kind!r} needs {name!r}")
     x = float(d.get(name, default))
     if not x > 0 or math.isinf(x):
         raise ValueError(f"scaling: {name} must be positive, got {x}")
@@ -44,7 +44,7 @@ def rotary_frequencies(dims: int, base: float = 10000.0, scaling: dict | None = 
     multiplies cos and sin.
 
     Pair i turns by ``base ** (-2 i / dims)``.  ``scaling`` stretches that for contexts longer
-    than a model was trained on, by its ``"factor"``:
+    than a model was trained on, by its ``"factor"`` and its ``"type"`` (or ``"rope_type"``):
 
     * ``{"type": "linear"}``: every frequency divided by the factor;
     * ``{"type": "ntk"}``: ``base * factor ** (dims / (dims - 2))`` as the base, which
@@ -64,10 +64,12 @@ def rotary_frequencies(dims: int, base: float = 10000.0, scaling: dict | None = 
     plain = [base ** (-2.0 * i / dims) for i in range(dims // 2)]
     if scaling is None:
         return plain, 1.0
-    kind = scaling.get("type")
+    kind = scaling.get("rope_type", scaling.get("type"))
+    if scaling.get("type", kind) != kind:
+        raise ValueError(f"scaling: type {scaling['type']!r} and rope_type {kind!r}")
     if kind not in ("linear", "ntk", "llama3", "yarn"):
         raise ValueError(f"scaling type must be 'linear', 'ntk', 'llama3' or 'yarn', got {kind!r}")
-    factor = _number(scaling, "factor")
+    factor = _number(scaling, kind, "factor")
     if kind == "linear":
         return [w / factor for w in plain], 1.0
     if kind == "ntk":
@@ -75,9 +77,9 @@ def rotary_frequencies(dims: int, base: float = 10000.0, scaling: dict | None = 
             raise ValueError("scaling of type 'ntk' needs more than 2 dims")
         wide = base * factor ** (dims / (dims - 2))
         return [wide ** (-2.0 * i / dims) for i in range(dims // 2)], 1.0
-    original = _number(scaling, "original_max_position_embeddings")
+    original = _number(scaling, kind, "original_max_position_embeddings")
     if kind == "llama3":
-        low, high = _number(scaling, "low_freq_factor"), _number(scaling, "high_freq_factor")
+        low, high = _number(scaling, kind, "low_freq_factor"), _number(scaling, kind, "high_freq_factor")
         if high <= low:
             raise ValueError(f"scaling: high_freq_factor must be over low_freq_factor, got {high} and {low}")
         kept = [min(1.0, max(0.0, (original * w / (2 * math.pi) - low) / (high - low))) for w in plain]
@@ -86,11 +88,11 @@ def rotary_frequencies(dims: int, base: float = 10000.0, scaling: dict | None = 
     def pair(turns: float) -> float:  # the pair that makes so many turns over the original context
         return dims * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-    first = max(0, math.floor(pair(_number(scaling, "beta_fast", 32.0))))
-    last = min(dims - 1, math.ceil(pair(_number(scaling, "beta_slow", 1.0))))
+    first = max(0, math.floor(pair(_number(scaling, kind, "beta_fast", 32.0))))
+    last = min(dims - 1, math.ceil(pair(_number(scaling, kind, "beta_slow", 1.0))))
     ramp = [min(1.0, max(0.0, (i - first) / max(last - first, 1e-3))) for i in range(dims // 2)]
     return ([w * ((1 - x) + x / factor) for w, x in zip(plain, ramp)],
-            _number(scaling, "attention_factor", max(1.0, 0.1 * math.log(factor) + 1.0)))
+            _number(scaling, kind, "attention_factor", max(1.0, 0.1 * math.log(factor) + 1.0)))
 
 
 # 1 / (2 pi) as a sum of four numbers of 24 bits, whose products with 26 bits are exact in float64.
