@@ -37,3 +37,22 @@ def test_a_scaling_may_name_its_type_as_models_do(kind, rest):
             ro.rotary_frequencies(64, 1e4, dict(**missing, **rest))
     with pytest.raises(ValueError, match=f"'{kind}'.*'factor'"):
         ro.rotary_frequencies(64, 1e4, dict(rope_type=kind))
+
+
+@pytest.mark.parametrize("scaling,name", [
+    (dict(type="yarn", mscale=0.707, **YARN), "mscale"), (dict(type="yarn", truncate=False, **YARN), "truncate"),
+    (dict(type="linear", factor=4.0, attention_factor=1.2), "attention_factor"),
+    (dict(type="ntk", factor=4.0, beta_fast=32), "beta_fast"), (dict(type="llama3", mscale=1.0, **LLAMA3), "mscale"),
+    (dict(type="yarn", long_factor=[1.0], **YARN), "long_factor")])
+def test_entries_that_a_scaling_does_not_know_are_refused(scaling, name):
+    """They would change the angles, and were passed over."""
+    with pytest.raises(ValueError, match=name):
+        ro.rotary_frequencies(64, 1e4, scaling)
+    del scaling[name]
+    ro.rotary_frequencies(64, 1e4, scaling)
+
+
+def test_entries_that_a_scaling_knows_are_taken():
+    ro.rotary_frequencies(64, 1e4, dict(type="linear", factor=4.0, original_max_position_embeddings=4096))
+    f, a = ro.rotary_frequencies(64, 1e4, dict(type="yarn", beta_fast=16, beta_slow=2, attention_factor=1.0, **YARN))
+    assert a == 1.0 and not any(math.isnan(w) for w in f)

@@ -39,6 +39,10 @@ def _number(d: dict, kind: str, name: str, default=None) -> float:
     return x
 
 
+_SCALINGS = {"linear": (), "ntk": (), "llama3": ("low_freq_factor", "high_freq_factor"),
+             "yarn": ("beta_fast", "beta_slow", "attention_factor")}
+
+
 def rotary_frequencies(dims: int, base: float = 10000.0, scaling: dict | None = None) -> tuple:
     """``(frequencies, factor)``: radians per position of the ``dims / 2`` pairs, and what
     multiplies cos and sin.
@@ -56,6 +60,8 @@ def rotary_frequencies(dims: int, base: float = 10000.0, scaling: dict | None = 
       and ``"beta_slow"`` (1): pairs that turn more often than beta_fast over the original
       context stay, those that turn less than beta_slow are divided, a ramp over the
       pairs between, and cos and sin take ``"attention_factor"`` (0.1 ln factor + 1).
+
+    Other entries, which would change the angles in ways that these do not know, are refused.
     """
     if dims <= 0 or dims % 2:
         raise ValueError(f"dims must be positive and even, got {dims}")
@@ -67,8 +73,11 @@ def rotary_frequencies(dims: int, base: float = 10000.0, scaling: dict | None = 
     kind = scaling.get("rope_type", scaling.get("type"))
     if scaling.get("type", kind) != kind:
         raise ValueError(f"scaling: type {scaling['type']!r} and rope_type {kind!r}")
-    if kind not in ("linear", "ntk", "llama3", "yarn"):
+    if kind not in _SCALINGS:
         raise ValueError(f"scaling type must be 'linear', 'ntk', 'llama3' or 'yarn', got {kind!r}")
+    known = ("type", "rope_type", "factor", "original_max_position_embeddings", *_SCALINGS[kind])
+    if any(name not in known for name in scaling):
+        raise ValueError(f"scaling of type {kind!r} does not know {[name for name in scaling if name not in known]}")
     factor = _number(scaling, kind, "factor")
     if kind == "linear":
         return [w / factor for w in plain], 1.0
