@@ -78,3 +78,16 @@ def test_a_kept_read_still_checks_its_tokens(monkeypatch):
         with pytest.raises(ValueError, match="tokens"):
             p8.paged8_read(pool(), pool(), table, tokens=9, out=out, _workspace=ws)
         assert p8.paged8_read(pool(), pool(), table, tokens=8, out=out, _workspace=ws)[0] is out[0]
+
+
+def test_decode_refuses_queries_that_require_grad():
+    """It records no gradient, and says so, also where a call is kept."""
+    q = torch.zeros(1, 4, 64).half().requires_grad_()
+    args = q, pool(), pool(), torch.zeros(1, 2, dtype=I32)
+    for kw in (dict(), dict(_workspace={})):
+        with pytest.raises(ValueError, match="requires grad"):
+            p8.paged8_decode_attention(*args, **kw)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="GPU|HIP"):
+            p8.paged8_decode_attention(*args, **kw)
+        with pytest.raises(RuntimeError, match="GPU|HIP"):
+            p8.paged8_decode_attention(q.detach(), *args[1:], **kw)

@@ -402,11 +402,14 @@ def paged8_decode_attention(
     Returns ``out``, float32 of q's shape; ``lse``, a contiguous float32 tensor of its shape without D,
     receives the natural logarithm of each sum of exp(score).  A query that attends to nothing,
     or that there is not, gives zeros and -inf.  Nothing past a query's token reaches its
-    result, NaN included; those of the tokens it sees show as in softmax.
+    result, NaN included; those of the tokens it sees show as in softmax in 32 bits (a query
+    whose scores pass 2**128 gives NaN; scores below -2**128 count as -inf).  Records no gradient: a
+    query that requires grad is refused.
 
     ``piece_tokens`` and ``_workspace`` as in
     :func:`~tritonkv_amd.paged16.paged16_decode_attention`.
     """
+    _no_grad(q)
     key = None
     if _workspace is not None and _both_pools(k_pool, v_pool):
         key = ("paged8", sm_scale, piece_tokens)

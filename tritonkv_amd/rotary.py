@@ -200,7 +200,7 @@ def _check_rotary(rotary, D: int, device) -> None:
 def _no_grad(*tensors) -> None:
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
         raise ValueError("a tensor requires grad, which this call does not record: run it under torch.no_grad() "
-                         "(the gradient is the same call on the output's gradient with adjoint=True)")
+                         "(apply_rotary's gradient is the same call on the output's gradient with adjoint=True)")
 
 
 def _out_like(x: torch.Tensor, out, name: str, align: int) -> torch.Tensor:
