@@ -843,7 +843,9 @@ static int launch_append8(Append8Params p, hipStream_t st) {
   const int items = a.block * PER, threads = few ? 64 : items < 1024 ? items : 1024;
   const int64_t blocks = ((int64_t)a.N + a.block - 2) / a.block + 1;  // that N tokens may touch
   // Two heads to a workgroup, whose turns are then worked out once for both, where that leaves
-  // workgroups enough.
+  // workgroups enough (blocks of 32 tokens of 128 dims times heads, one / two, us: prompts of 288 5.2 / 5.4, 544
+  // 6.5 / 6.2, 1088 9.3 / 8.5, 4128 25.2 / 21.2, with rotary 1088 25.7 / 23.5, 4128 86 / 77; steps of 512 4.0 /
+  // 4.6, 1024 4.5 / 4.5, 4096 8.2 / 6.9; blocks of 128 tokens of 256 dims 320 14.7 / 15.1, 1056 44.4 / 44.7).
   p.heads = a.HKV > 1 && blocks * a.B * a.HKV > 1024 ? kAppendHeads : 1;
   const int sets = (a.HKV + p.heads - 1) / p.heads;
   int64_t groups = blocks * 2 * sets;
@@ -957,7 +959,9 @@ extern "C" int tkv_paged8_read(const tkv_paged8_read_args* a, tkv_stream_t strea
   const int align = a->x_type == TKV_F32 ? 4 : 8;
   if (!rows_ok(a->k_out, a->k_out_strides, 3, align) || !rows_ok(a->v_out, a->v_out_strides, 3, align)) return TKV_EINVAL;
   const int64_t blocks = ((int64_t)a->N + 30) / 32 + 1;  // of 32 slots that N tokens may touch
-  const int heads = a->HKV > 1 && blocks * a->B * a->HKV > 2048 ? 2 : 1;
+  // Two heads to a workgroup where that leaves workgroups enough (blocks times heads, one / two, us: bf16 544 7.1 /
+  // 7.3, 1088 10.1 / 9.9, 1632 12.9 / 11.9, 4352 26.3 / 23.5; fp32 1088 13.3 / 14.1, 1632 18.8 / 16.0).
+  const int heads = a->HKV > 1 && blocks * a->B * a->HKV > 1280 ? 2 : 1;
   const int64_t groups = blocks * 2 * ((a->HKV + heads - 1) / heads);
   if (groups * 256 > UINT32_MAX) return TKV_EINVAL;
   const dim3 grid((unsigned)groups, (unsigned)a->B);

@@ -203,8 +203,14 @@ __device__ __forceinline__ int64_t position_of(const TurnPlan& p, int b, int n) 
 // turns would be all of a thread's start (4 x 8213 tokens, 32 + 8 heads, bf16, us at 1 / 2 / 4 / 8 /
 // 16 / 32 tokens: 145 / 115 / 114 / 118 / 135 / 171).
 constexpr int kTurnTile = 4;
-constexpr int64_t kTurnMany = 4096;  // tokens from which on there are workgroups enough for that
-constexpr int64_t kTurnFew = 2048;   // up to here heads are shared out over workgroups too
+// Tokens from which on there are workgroups enough for that (one / several tokens a workgroup, 32 + 8 heads of
+// 128 dims, us: 2048 tokens 10.2 / 10.0, 4096 16.4 / 17.1, 6144 27.2 / 24.2, 16384 63 / 58; 1024 of one token
+// 6.9 / 7.6; an append of 1024-token prompts gains from 1024 tokens on, 12.6 / 11.1).
+constexpr int64_t kTurnMany = 4096;
+// Up to here the heads are shared out over workgroups too (shared / not, us: 1 to 16 tokens of 128 + 16 heads 3.4 /
+// 4.5, 64 4.0 / 4.8, 256 6.5 / 6.9, 500 10.2 / 8.8; of 32 + 8 heads 16 3.4 / 3.6, 256 4.1 / 3.9, 500 4.8 / 4.6,
+// 1024 8.2 / 6.9).
+constexpr int64_t kTurnFew = 384;
 
 // Heads that a thread has under way at once.  (Four: 113 us for 115 of the case above, but more
 // registers than the append's own work needs: 4 x 2049 tokens with rotary 42.7 us against 36.5.)
