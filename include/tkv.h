@@ -454,7 +454,7 @@ typedef struct tkv_paged8_append_args {
 int tkv_paged8_append(const tkv_paged8_append_args *args, tkv_stream_t stream);
 
 /* Tokens positions[b] (NULL: 0) to positions[b] + counts[b] - 1 (NULL: N of them) of row b as
- * values of x_type, into k_out and v_out (B, HKV, N, D), strides batch, head, token in
+ * values of x_type (code * scale in fp32, rounded), into k_out and v_out (B, HKV, N, D), strides batch, head, token in
  * elements, multiples of 16 bytes.  Rows of the outputs past counts[b], and those of tokens
  * outside the table or of entries outside the pool, are left alone. */
 typedef struct tkv_paged8_read_args {

@@ -20,10 +20,11 @@
 // exact for what is over 2^-30 of it.  P enters as two fp16 terms (22 bits).  A block's
 // scale of V multiplies its chunks' product in fp32, one of K the scores.
 //
-// Measured (split kernel, us): 32 rows of 32768, HKV 8, G 4, e4m3 319, 6.7 TB/s; 32 rows of
-// 1000-16384, HKV 8, G 8, e4m3 93, 6.1 TB/s; 16 rows of 500-8000 with four queries of 64 heads, int8,
-// 42: 32 columns a workgroup, bound by the vector units (about 600 instructions a chunk); one row of
-// 505 5.5.  The join takes 2-5 us more.
+// Measured (split kernel, us): 32 rows of 32768, HKV 8, G 4, e4m3 317-325, 6.7 TB/s; 32 rows of
+// 1000-16384, HKV 8, G 8, e4m3 94, 6.1 TB/s; 16 rows of 500-8000 with four queries of 64 heads, int8,
+// 42: 32 columns a workgroup, bound by the vector units (about 600 instructions a chunk; e4m3 48 in all for
+// int8's 49, of 16 columns 43 for 36: its chunk of NaN places holds 13 registers in scratch); one row of
+// 505 7.4, four chunks in turn per wave.  The join takes 2-5 us more.
 #include <algorithm>
 
 #include "page_shares.h"
@@ -332,7 +333,9 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
           for (int mv = 0; mv < EPL; ++mv) accv[ht][mv] *= alpha;
         }
         // Scores of -inf under a maximum of -inf give p = 0, not NaN.  The product is not rounded
-        // before the maximum is off: at scores of 32 and more that alone was 1.3e-6 of p.
+        // before the maximum is off: at scores of 32 and more that alone was 1.3e-6 of p.  (With the shift in the
+        // exponent that is rounded to 2^-21 at most, 3.3e-7 of p; a product behind the power, 8 more instructions
+        // a tile, would be exact.)
         const float off = kShift8 - (m_run[ht] == -INFINITY ? 0.0f : m_run[ht]);
         float p[8];
 #pragma unroll
@@ -508,9 +511,9 @@ paged8_split_kernel(const int32_t* lens, int B, int S, int workgroups, int least
 // falls under its smallest normal code), and a scale rises seldom.  Where it rises, the
 // codes of the block's earlier tokens are rounded again under the new one.
 //
-// Bound by HBM (4 x 8213 tokens, counts of half to all, 8 heads, fp16: 151 MB in 29.6 us, 5.1 TB/s; with
+// Bound by HBM (4 x 8213 tokens, counts of half to all, 8 heads, fp16: 151 MB in 29.8 us, 5.1 TB/s; with
 // each head's loads behind the one's before 30.4, with 16 neighbouring values to a thread 52), short
-// ones by the chain of position, value, scale: 64 rows of a token with rotary 6.3 us (5.8 back to back).
+// ones by the chain of position, value, scale: 64 rows of a token with rotary 5.5 us.
 // ---------------------------------------------------------------------------
 struct Append8Params {
   tkv_paged8_append_args a;

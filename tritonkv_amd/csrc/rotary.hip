@@ -3,7 +3,9 @@
 // Every value is read and written once, for 6 flops a pair: bound by HBM.  A
 // workgroup takes a few tokens with all their heads, so that the angles, modulo whole turns,
 // are worked out once a token and not once a head.  4 x 8213 tokens, 32 + 8 heads, bf16: 673 MB in
-// 111 us, 6.1 TB/s (a copy's rate is 4.8); one token of 64 rows 3.3 us.
+// 111 us, 6.1 TB/s (a copy's rate is 4.8); one token of 64 rows 3.4 us.  Halves of
+// 64 of 128 dims take 141 us, halves that are no groups of 8, which go one value at a time, 198 (20 of 128
+// dims; of 80 156).
 #include <algorithm>
 #include <type_traits>
 

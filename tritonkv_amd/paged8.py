@@ -49,20 +49,20 @@ MAX_PAGE_SIZE = 2 ** 24
 def plan_shares8(B: int, HKV: int, columns: int, S: int, D: int, device=None,
                  piece_tokens: int | None = None) -> tuple[int, int, int, int]:
     """:func:`~tritonkv_amd.paged16.plan_shares` for 8-bit pages, whose chunks hold half the bytes;
-    ``columns`` are a KV head's queries.  Measured on MI355X (us; U = HKV times the blocks of
-    16 or 32 columns):
+    ``columns`` are a KV head's queries.  Measured on MI355X (us, each pair in one session; U = HKV times the
+    blocks of 16 or 32 columns):
 
-    * Rows stay whole up to 512 tokens of 128 dims, 256 of 256 and 512 of 64 (whole / cut, one row: 507
-      of 128 8.9 / 9.2, 1019 13.5 / 8.5; 251 of 256 9.3 / 9.9, 507 13.5 / 9.9; 1019 of 64 10.0 / 8.4; 16
-      rows of 1-507, 8 KV heads, 9.8 / 13.4), and where B * U is 512 or more, twice or four times that
-      (64 rows of 1-1019, 8 KV heads, 22.7 / 26.2, all 1019 26.8 / 28.8; of 64 dims 13.4 / 17.1 and 15.0
-      / 18.5; 507 of 256 27.4 / 29.9; but 1-2043 of 128 36.5 / 34.3).
+    * Rows stay whole up to 512 tokens of 128 dims, 256 of 256 and 512 of 64 (whole / cut, one row, steps of
+      a graph: 507 of 128 7.8 / 8.0, 1019 10.9 / 8.1; 251 of 256 8.9 / 9.9, 507 11.8 / 9.8; 1019 of 64 8.3 /
+      8.1; 16 rows of 1-507, 8 KV heads, 9.4 / 12.8), and where B * U is 512 or more, twice or four times that
+      (64 rows of 1-1019, 8 KV heads, 21.9 / 24.1, all 1019 27.8 / 32.1; of 64 dims 13.6 / 16.5 and 15.7 /
+      19.0; 507 of 256 29.1 / 33.0; but 1-2043 of 128 38.6 / 36.9).
     * Otherwise two workgroups per CU, four of 64 dims and one of 256 with more than 16 columns (1 / 2 /
-      3 / 4: 32 rows of 32768 376 / 325 / 338 / 341, of 8000-16384 with 64 dims 100 / 70 / 70 / 71, 8 of 1-2999
-      with 64 dims, 16 KV heads, 18.1 / 16.1 / 15.8 / 14.8; 16 rows of 4 queries and 64 heads 55 / 47 / 61 / 58;
-      one row of 32768 20.1 / 18.4 / 19.9 / 23.7; 32 of 16384 with 256 dims 185 / 176 / 212, one with 24
-      columns 22 / 37 / 23), of at least 128 tokens of 128 dims, half of that in tables of at most 512
-      tokens (64 / 128 / 256: 16 rows of 1-1000 14.1 / 14.0 / 15.9).
+      3 / 4: 32 rows of 32768 422 / 353 / 362 / 361, of 8000-16384 with 64 dims 105 / 71 / 71 / 71, 8 of 1-2999
+      with 64 dims, 16 KV heads, 16.7 / 15.4 / 14.9 / 15.1; 16 rows of 4 queries and 64 heads 58 / 49 / 63 / 60;
+      one row of 32768 21.4 / 19.5 / 20.9 / 22.6; 32 of 16384 with 256 dims 372 / 349 / 360, one with 24
+      columns 29 / 41 / 55), of at least 128 tokens of 128 dims, half of that in tables of at most 512
+      tokens (64 / 128 / 256: 16 rows of 1-1000 13.6 / 13.9 / 15.0).
     """
     if piece_tokens is not None:
         return plan_shares(B, HKV, columns, S, D, device, piece_tokens)
@@ -207,7 +207,9 @@ def paged8_append(k_pool: Paged8Pool, v_pool: Paged8Pool, k_new: torch.Tensor, v
     both under the scale of either: give every row pages of its own to write into, as
     :mod:`tritonkv_amd.pages` does.
 
-    How blocks get their scales stands in the module's documentation.  Magnitudes above 2**64,
+    How blocks get their scales stands in the module's documentation.  Codes behind the new tokens in
+    their last block are left as they are, under the scale that it then has: what is written over is written
+    over up to the row's end.  Magnitudes above 2**64,
     infinities among them, count as 2**64.  NaN does not count for a scale; e4m3 keeps it, int8
     stores 0.
 
@@ -308,7 +310,8 @@ def paged8_read(k_pool: Paged8Pool, v_pool: Paged8Pool, block_table: torch.Tenso
     """Tokens of 8-bit pages as values: ``(k, v)``, each ``(B, HKV, tokens, D)``.
 
     Row b's are the ``counts[b]`` tokens (None: all of ``tokens``) from ``positions[b]`` on
-    (None: 0), code times scale rounded once to ``dtype`` (float16, bfloat16 or float32).
+    (None: 0), code times scale in 32 bits, rounded to ``dtype`` (float16, bfloat16 or float32): once, where
+    the scale is a power of two, as the append's are.
     ``out``: a pair of tensors for them, in any strides with dense rows (``tokens`` and ``dtype``
     are then theirs).  Rows past a row's count, and tokens outside the table or in entries outside
     the pool, are left as they were; in new tensors they are zero.
